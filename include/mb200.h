@@ -216,6 +216,96 @@ int mb_attention_prefill_bf16(const uint16_t* q, int ldq, const uint16_t* k_cach
                               const int* start_pos, const int* kv_len, int B, int S, int Hq,
                               int Hkv, int Dh, int causal, uint16_t* out, int ldo, void* stream);
 
+/* ---- 4-bit paged KV cache ---------------------------------------------------
+ * The 4-bit counterpart of the bf16 cache above (attention semantics of
+ * mlx/kernels/full/llama_decoder_layer.py:30-37), head dim 128, pages of 64
+ * tokens: cache = uint8 [num_pages][Hkv][8704]. The bytes of one page and head:
+ *   [0, 4096)     key codes: token t at byte 64 t, byte j = dim 2j (low four
+ *                 bits) and dim 2j + 1 (high four bits)
+ *   [4096, 8192)  value codes, the same, but the 16-byte piece c of token t
+ *                 stands at piece c ^ ((t >> 1) & 3)
+ *   [8192, 8448)  per token: bf16 scale, bf16 minimum of the key
+ *   [8448, 8704)  per token: bf16 scale, bf16 minimum of the value
+ * Over the 128 dims x of a token and head: minimum = min(x), scale =
+ * bf16((max(x) - min(x)) / 15), code = (x - minimum) / scale rounded to the
+ * nearest whole number (ties to even), clamped to 0..15, and 0 where scale is 0;
+ * a code stands for minimum + scale * code. A token with a NaN or an infinity
+ * reads back as NaN (the others of its page do not change).
+ *
+ * block_table [B][max_pages], kv_len, start_pos, new_len [B] are int32 in
+ * device memory. A position outside the table, or a table entry outside
+ * 0..num_pages-1, is never accessed: it is skipped (not stored; read back as
+ * zeros; not attended) and recorded in the device status word (0x8). */
+
+/* Bytes of one page of all Hkv heads. */
+size_t mb_kv4_page_bytes(int Hkv);
+
+/* Store the keys and values of S tokens a sequence: token s < new_len[b] (null:
+ * S) goes to position start_pos[b] + s. k, v: bf16 [B][S][Hkv][128] with the
+ * element strides {batch, token, head} (multiples of 8; the 128 dims
+ * contiguous), 16-byte aligned. Nothing else of the cache is written. */
+int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, const int64_t* k_strides,
+                       const int64_t* v_strides, uint8_t* cache, int num_pages, int Hkv,
+                       const int* block_table, int max_pages, const int* start_pos,
+                       const int* new_len, int B, int S, void* stream);
+
+/* Read positions start_pos[b] .. start_pos[b] + S - 1 back as fp32
+ * [B][S][Hkv][128]; zeros at positions >= kv_len[b]. */
+int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv, const int* block_table,
+                      int max_pages, const int* start_pos, const int* kv_len, int B, int S,
+                      float* k_out, float* v_out, void* stream);
+
+/* out = softmax(scale * q k^T) v for S query rows a sequence over keys
+ * 0..kv_len[b]-1; with start_pos, row s sees the keys at positions <=
+ * start_pos[b] + s only (causal), else all. q, out: bf16 [B][S][Hq][128] with ldq /
+ * ldo elements between two positions' rows (multiples of 8), the heads
+ * contiguous. A row that sees no key becomes zeros. B <= 4096; every length is
+ * read on the device, so ragged batches balance and the call can be captured. */
+size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages);
+int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache, int num_pages,
+                          const int* block_table, int max_pages, const int* kv_len,
+                          const int* start_pos, int B, int S, int Hq, int Hkv, int Dh, float scale,
+                          uint16_t* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* ---- page operations of a paged cache -----------------------------------------
+ * For any cache of 64-token pages (bf16 or 4-bit): block_table [B][max_pages],
+ * seq_len [B], page_refs [num_pages], all int32 in device memory and changed in
+ * place. A sequence owns the first ceil(seq_len / 64) entries of its row (what
+ * stands behind them is left as it was); page_refs[p] counts the rows that name
+ * page p, 0 = free. New pages are the lowest-numbered free ones, given out in
+ * row order. A call that cannot be served changes nothing and says so in its
+ * int32 status in device memory: the number of pages that were lacking, or -1
+ * for a length, parent or table entry out of range. Nothing returns to the host.
+ * pools: npools device pointers (16-byte aligned) to [num_pages] pages of
+ * page_bytes[i] bytes (multiples of 16); the two arrays are read during the call.
+ * Workspace: mb_kv_pages_workspace_bytes, 16-byte aligned, caller owned. */
+size_t mb_kv_pages_workspace_bytes(int B, int max_pages, int num_pages);
+
+/* Room for new_len[b] more tokens of every sequence; start_pos[b] receives the
+ * length before, seq_len[b] becomes the length after. */
+int mb_kv_pages_extend(int* block_table, int* seq_len, int* page_refs, int B, int max_pages,
+                       int num_pages, const int* new_len, int* start_pos, int* status,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row b becomes a fork of row parent[b] as it was before the call (parent[b] ==
+ * b: stays; -1: is freed, length 0). A fork shares its parent's full pages and
+ * gets a copy, in a page that was free before the call, of a partly filled
+ * last one. What row b held before is released. */
+int mb_kv_pages_fork(void* const* pools, const int64_t* page_bytes, int npools, int* block_table,
+                     int* seq_len, int* page_refs, int B, int max_pages, int num_pages,
+                     const int* parent, int* status, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Move the pages in use into 0..live-1 with the fewest moves: the pages in use
+ * from `live` on go, in order, into the free ones below it. The block table and
+ * page_refs follow; remap [num_pages] receives every page's new number (-1: was
+ * free), live (or -1) the number of pages in use. */
+int mb_kv_pages_compact(void* const* pools, const int64_t* page_bytes, int npools, int* block_table,
+                        const int* seq_len, int* page_refs, int B, int max_pages, int num_pages,
+                        int* remap, int* live, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /* ---- LLaMA decoder layer (hook mlx/kernels/full/llama_decoder_layer.py:17-64;
  *      registry mlx/kernels/full/registry.py:87-104; Metal kernel
  *      metal/kernels/full/llama_decoder_layer/default.metal:16-206) ------- */

@@ -96,6 +96,18 @@ SIGNATURES = {
                                            _P, C.c_size_t, _P]),
     "mb_attention_prefill_bf16": (C.c_int, [_P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I,
                                             _P, _I, _P]),
+    "mb_kv4_page_bytes": (C.c_size_t, [_I]),
+    "mb_kv4_append_bf16": (C.c_int, [_P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _P]),
+    "mb_kv4_gather_f32": (C.c_int, [_P, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "mb_attention_kv4_workspace_bytes": (C.c_size_t, [_I] * 5),
+    "mb_attention_kv4_bf16": (C.c_int, [_P, _I64, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I,
+                                        C.c_float, _P, _I64, _P, C.c_size_t, _P]),
+    "mb_kv_pages_workspace_bytes": (C.c_size_t, [_I] * 3),
+    "mb_kv_pages_extend": (C.c_int, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, C.c_size_t, _P]),
+    "mb_kv_pages_fork": (C.c_int, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, C.c_size_t,
+                                   _P]),
+    "mb_kv_pages_compact": (C.c_int, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, C.c_size_t,
+                                      _P]),
     "mb_decoder_layer_create": (C.c_int, [C.POINTER(MbDecoderConfig), _P, _P, _P, _P, _I, _I,
                                           C.POINTER(C.c_void_p)]),
     "mb_decoder_layer_destroy": (None, [_P]),

@@ -1,0 +1,715 @@
+// GQA attention over the 4-bit paged KV cache (layout in kv4.cuh); the 4-bit
+// counterpart of mb_attention_decode_bf16 (reference semantics:
+// mlx/kernels/full/llama_decoder_layer.py:30-37).
+//
+// Mathematics. Key j of a page stands for mk_j + sk_j * u_j (u_j its 128 whole
+// codes), value j for mv_j + sv_j * w_j. So
+//   score_j = c * (sk_j * (q . u_j) + mk_j * sum(q)),      c = log2(e) * scale
+//   out     = (sum_j p_j sv_j w_j + sum_j p_j mv_j) / sum_j p_j,  p_j = 2^score_j
+// and the tensor cores multiply the codes themselves: a code's four bits, left
+// where they stand in the low bits of a 16-bit half, ARE the fp16 number
+// u * 2^-24 (u * 2^-20 for the odd code of a byte), a subnormal that mma.sync
+// multiplies exactly. Eight codes become four operand registers in five
+// logic operations; the powers of two are taken out of q (2^-4) and of the
+// sums. q is scaled by a power of two into fp16's range, which loses nothing
+// of a bf16 number down to 2^-22 of the row's largest.
+// The value scale goes into the exponent: P_j = 2^(score_j + log2(sv_j) - R)
+// with a running reference R per query row, so that P_j sv-weighted is what is
+// rounded to fp16 (11 bits, and 2^-24 absolute at a range up to 2^15), and the
+// denominator is sum_j P_j / sv_j in fp32. R only moves when a weight would
+// pass 2^15, so most pages rescale nothing.
+//
+// Orientation: keys are the 16 MMA rows, query rows the 8 columns (S^T = K
+// Q^T, O^T = V^T P^T), so a decode step's 8 query heads of a kv head fill a
+// column tile and no row is wasted; P^T moves from the accumulator layout to
+// the operand layout by movmatrix. Query rows are the S * G pairs (position,
+// head of the group); NT column tiles of 8 per pass over the cache.
+//
+// Schedule: the flat list of (sequence, kv head, row tile, page) is cut into
+// equal shares, one a CTA, planned on the device from kv_len, so that ragged
+// batches balance. Each warp takes every NW-th page of its CTA's share through
+// its own ring of whole-page bulk copies (8704 bytes, one mbarrier each); the
+// warps meet only when a (sequence, kv head, row tile) ends. One that lies
+// within a share is written at once, the others as partials (at most two a
+// CTA) which attn_kv4_combine_kernel joins.
+#include <cuda_fp16.h>
+
+#include "kv4.cuh"
+#include "kernels.h"
+
+namespace {
+using namespace kv4;
+
+constexpr int NW = 4;  // warps per CTA
+constexpr int ST = 3;  // pages in a warp's ring
+
+struct Args {
+  const uint16_t* q;
+  const uint8_t* cache;
+  const int* table;
+  const int* kv_len;
+  const int* start_pos;  // null: every key below kv_len is seen
+  uint16_t* out;
+  float* part_o;   // [grid][2][cols][DH]
+  float* part_ml;  // [grid][2][cols][2]
+  int4* desc;      // [grid]: first slot, number of partials (0: none), b, unit
+  uint32_t* status;
+  int64_t ldq, ldo;  // elements between two positions' rows
+  int num_pages, max_pages, B, S, Hkv, G, RT;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The codes of one 32-bit word as four fp16 pairs: codes 0|4, 1|5 (x16), 2|6, 3|7 (x16).
+__device__ __forceinline__ void spread(uint32_t w, uint32_t (&e)[4]) {
+  e[0] = w & 0x000F000Fu;
+  e[1] = w & 0x00F000F0u;
+  w >>= 8;
+  e[2] = w & 0x000F000Fu;
+  e[3] = w & 0x00F000F0u;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Attended pages of sequence b.
+__device__ __forceinline__ int seq_len(const Args& a, int b) {
+  return max(0, min(a.kv_len[b], a.max_pages * PAGE));
+}
+
+// pre[b] = flat index of the first page of sequence b, pre[B] = their number.
+__device__ void plan(const Args& a, int* pre, int* wsum) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.B + NW * 32 - 1) / (NW * 32);
+  const int b0 = tid * per, b1 = min(a.B, b0 + per);
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) sum += (seq_len(a, b) + PAGE - 1) / PAGE;
+  sum *= a.Hkv * a.RT;
+  int inc = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += y;
+  }
+  if (lane == 31) wsum[warp] = inc;
+  __syncthreads();
+  int run = inc - sum;
+  for (int w = 0; w < warp; ++w) run += wsum[w];
+  for (int b = b0; b < b1; ++b) {
+    pre[b] = run;
+    run += (seq_len(a, b) + PAGE - 1) / PAGE * a.Hkv * a.RT;
+  }
+  if (tid == NW * 32 - 1) {
+    int all = 0;
+    for (int w = 0; w < NW; ++w) all += wsum[w];
+    pre[a.B] = all;
+  }
+  __syncthreads();
+}
+
+// Sequence of flat page f: pre[b] <= f < pre[b + 1].
+__device__ __forceinline__ int find_seq(const int* pre, int B, int f) {
+  int lo = 0, hi = B;  // pre[lo] <= f < pre[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= f) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// A warp's running state over the pages of one unit: NT column tiles.
+template <int NT>
+struct State {
+  float o[NT][4][2][4];   // [32-dim piece][dim pair][accumulator]
+  float R[NT][2], l[NT][2], om[NT][2];
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][c][h][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        R[t][e] = -INFINITY;
+        l[t][e] = om[t][e] = 0.f;
+      }
+    }
+  }
+};
+
+// Floats of one warp's state in shared memory.
+template <int NT>
+constexpr int area_floats() { return NT * 38 * 32; }
+
+template <int NT>
+__global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  constexpr int COLS = NT * 8;
+  extern __shared__ __align__(128) uint8_t sm[];
+  uint8_t* ring = sm + (threadIdx.x >> 5) * ST * BLOB;
+  float* area = reinterpret_cast<float*>(sm + NW * ST * BLOB);  // [NW/2][area_floats]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(area + (NW / 2) * area_floats<NT>());  // [NW][ST]
+  int* wsum = reinterpret_cast<int*>(bars + NW * ST);          // [NW]
+  int* page_ok = wsum + NW;                                    // [NW][ST]
+  int* pre = page_ok + NW * ST;                                // [B + 1]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, tig = lane & 3;
+  uint64_t* bar = bars + warp * ST;
+  int* ok_flag = page_ok + warp * ST;
+  if (lane == 0)
+    for (int i = 0; i < ST; ++i) mbd::mbar_init(bar + i, 1);
+  mbd::fence_mbar_init();
+  plan(a, pre, wsum);
+
+  // sequences without keys: their rows are zeros
+  const int row_elems = a.Hkv * a.G * DH;
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (pre[b] == pre[b + 1])
+      for (int s = 0; s < a.S; ++s)
+        for (int i = threadIdx.x * 8; i < row_elems; i += NW * 32 * 8)
+          *reinterpret_cast<uint4*>(a.out + ((int64_t)b * a.S + s) * a.ldo + i) = make_uint4(0, 0, 0, 0);
+
+  const int total = pre[a.B];
+  const int per = (total + gridDim.x - 1) / gridDim.x;
+  const int begin = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+  const int end = min(begin + per, total);
+  const int units = a.Hkv * a.RT;
+  if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+
+  // ---- this warp's loads: pages begin + warp, + NW, ... ----
+  const int mine = end - begin > warp ? (end - begin - warp + NW - 1) / NW : 0;
+  int issued = 0;
+  int win_pid = 0, win_ok = 0, win_kvh = 0;  // lane i: page (issued / 32) * 32 + i of this warp
+  auto issue = [&]() {
+    if ((issued & 31) == 0) {
+      const int f = begin + warp + NW * (issued + lane);
+      if (f < end) {
+        const int b = find_seq(pre, a.B, f);
+        const int rem = f - pre[b], pages = (pre[b + 1] - pre[b]) / units;
+        const int unit = rem / pages;
+        win_kvh = unit / a.RT;
+        const int pid = a.table[(int64_t)b * a.max_pages + (rem - unit * pages)];
+        win_ok = pid >= 0 && pid < a.num_pages;
+        win_pid = win_ok ? pid : 0;
+        if (!win_ok) atomicOr(a.status, MB_DEV_BAD_PAGE);
+      }
+    }
+    const int src = issued & 31;
+    const int pid = __shfl_sync(0xffffffffu, win_pid, src);
+    const int kvh = __shfl_sync(0xffffffffu, win_kvh, src);
+    const int good = __shfl_sync(0xffffffffu, win_ok, src);
+    const int st = issued % ST;
+    if (lane == 0) {
+      ok_flag[st] = good;
+      mbd::mbar_expect_tx(bar + st, BLOB);
+      mbd::bulk_load(ring + st * BLOB, a.cache + ((int64_t)pid * a.Hkv + kvh) * BLOB, BLOB, bar + st);
+    }
+    ++issued;
+  };
+  for (int i = 0; i < ST && i < mine; ++i) issue();
+  int used = 0;       // pages consumed
+  bool dead = false;  // a copy never arrived: consume and load nothing more
+  int dead_at = 0;
+
+  State<NT> z;
+  int f0 = begin;
+  while (f0 < end) {
+    // one segment: the pages of one (sequence, kv head, row tile) in this share
+    const int b = find_seq(pre, a.B, f0);
+    const int pages = (pre[b + 1] - pre[b]) / units;
+    const int unit = (f0 - pre[b]) / pages;
+    const int ub = pre[b] + unit * pages;  // flat index of the unit's first page
+    const int f1 = min(end, ub + pages);
+    const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
+    const int L = seq_len(a, b);
+    // row s sees the keys up to position first + s
+    const int first = a.start_pos ? min(a.start_pos[b], L) : L;
+    z.reset();
+
+    int f = begin + warp + NW * used;
+    if (f < f1) {
+      // ---- q of this unit as B fragments ----
+      uint32_t qf[NT][16];
+      float cq[NT][2], qs[NT][2];
+      int lim[NT][2];  // keys below lim are seen by column 2 tig + e
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int r = rt * COLS + t * 8 + gid;
+        const bool have = r < a.S * a.G;
+        const int s = r / a.G;
+        float x[32];
+        if (have) {
+          const uint4* p = reinterpret_cast<const uint4*>(
+              a.q + ((int64_t)b * a.S + s) * a.ldq + (kvh * a.G + (r - s * a.G)) * DH + 32 * tig);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 w = p[i];
+            x[8 * i] = lo_bf(w.x), x[8 * i + 1] = hi_bf(w.x), x[8 * i + 2] = lo_bf(w.y);
+            x[8 * i + 3] = hi_bf(w.y), x[8 * i + 4] = lo_bf(w.z), x[8 * i + 5] = hi_bf(w.z);
+            x[8 * i + 6] = lo_bf(w.w), x[8 * i + 7] = hi_bf(w.w);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = 0.f;
+        }
+        float mx = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          mx = fmaxf(mx, fabsf(x[i]));
+          sum += x[i];
+        }
+#pragma unroll
+        for (int off = 1; off <= 2; off <<= 1) {
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        }
+        // 2^e brings the row's largest to [2^11, 2^12)
+        int e = 11 - ((int)(__float_as_uint(mx) >> 23) - 127);
+        e = max(-100, min(100, e));
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float up16 = up * 0.0625f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          qf[t][4 * w] = pack_h2(x[8 * w] * up, x[8 * w + 4] * up);
+          qf[t][4 * w + 1] = pack_h2(x[8 * w + 1] * up16, x[8 * w + 5] * up16);
+          qf[t][4 * w + 2] = pack_h2(x[8 * w + 2] * up, x[8 * w + 6] * up);
+          qf[t][4 * w + 3] = pack_h2(x[8 * w + 3] * up16, x[8 * w + 7] * up16);
+        }
+        const float down = a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - max(e, -100)) << 23);
+        const float sq = a.scale_log2 * sum;
+        const int mylim = min(L, first + s + 1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int from = (2 * tig + c) * 4;  // a lane whose fragment row is column 2 tig + c
+          cq[t][c] = __shfl_sync(0xffffffffu, down, from);
+          qs[t][c] = __shfl_sync(0xffffffffu, sq, from);
+          lim[t][c] = __shfl_sync(0xffffffffu, mylim, from);
+        }
+      }
+      const int all_seen = min(L, first + (rt * COLS) / a.G + 1);  // keys that every column sees
+
+      for (; f < f1; f += NW) {
+        const int st = used % ST;
+        if (!dead) {
+          dead = !mbd::mbar_wait(bar + st, (used / ST) & 1, a.status, MB_DEV_TIMEOUT_TMA);
+          dead = __any_sync(0xffffffffu, dead);
+          dead_at = used;
+        }
+        if (!dead && ok_flag[st]) {
+          const uint8_t* pg = ring + st * BLOB;
+          const uint32_t pg_s = mbd::smem_u32(pg);
+          const int key0 = (f - ub) * PAGE;
+          const bool masked = key0 + PAGE > all_seen;
+          // ---- scores of 64 keys: t = log2 of the value-weighted softmax term ----
+          float sc[NT][4][4];
+          float rv[4][2], mv[4][2];  // 1 / sv and mv / sv of keys 16 mt + gid (+ 8)
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[t][mt][e] = 0.f;
+            const uint4 ka = *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid) * ROW + tig * 16);
+            const uint4 kb =
+                *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid + 8) * ROW + tig * 16);
+            const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t ea[4], eb[4];
+              spread(wa[w], ea);
+              spread(wb[w], eb);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                mma_f16_16816(sc[t][mt], ea[0], eb[0], ea[1], eb[1], qf[t][4 * w], qf[t][4 * w + 1]);
+                mma_f16_16816(sc[t][mt], ea[2], eb[2], ea[3], eb[3], qf[t][4 * w + 2],
+                              qf[t][4 * w + 3]);
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int t0 = mt * 16 + gid + 8 * r;
+              const uint32_t kp = *reinterpret_cast<const uint32_t*>(pg + K_PARAMS + t0 * 4);
+              uint32_t vp = *reinterpret_cast<const uint32_t*>(pg + V_PARAMS + t0 * 4);
+              if (masked && key0 + t0 >= L) vp = 0;  // what stands past the end may be anything
+              const float sv = lo_bf(vp);
+              // scale 0 (all dims alike, codes 0) must not enter the logarithm
+              const float svc = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p90f);
+              const float lg = __log2f(svc);
+              rv[mt][r] = __frcp_rn(svc);
+              mv[mt][r] = hi_bf(vp) * rv[mt][r];
+              const float sk = lo_bf(kp), mk = hi_bf(kp);
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  float x = fmaf(mk, qs[t][c], fmaf(sk, sc[t][mt][2 * r + c] * cq[t][c], lg));
+                  if (masked && key0 + t0 >= lim[t][c]) x = -INFINITY;
+                  sc[t][mt][2 * r + c] = x;
+                }
+            }
+          }
+          // ---- reference, weights ----
+          uint32_t pf[NT][4][2];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float mx[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              mx[c] = sc[t][0][c];
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt) {
+                mx[c] = fmaxf(mx[c], sc[t][mt][c]);
+                mx[c] = fmaxf(mx[c], sc[t][mt][2 + c]);
+              }
+#pragma unroll
+              for (int off = 4; off <= 16; off <<= 1)
+                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], off));
+            }
+            const bool raise = mx[0] > z.R[t][0] + 15.f || mx[1] > z.R[t][1] + 15.f;
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float Rn = mx[c] > z.R[t][c] + 15.f ? mx[c] - 8.f : z.R[t][c];
+                const float f = z.R[t][c] == Rn ? 1.f : fast_exp2(z.R[t][c] - Rn);
+                z.R[t][c] = Rn;
+                z.l[t][c] *= f;
+                z.om[t][c] *= f;
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    z.o[t][p][h][c] *= f;
+                    z.o[t][p][h][2 + c] *= f;
+                  }
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float R = z.R[t][c] == -INFINITY ? 0.f : z.R[t][c];  // nothing seen so far
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const float p = fast_exp2(sc[t][mt][2 * r + c] - R);
+                  sc[t][mt][2 * r + c] = p;
+                  z.l[t][c] = fmaf(p, rv[mt][r], z.l[t][c]);
+                  z.om[t][c] = fmaf(p, mv[mt][r], z.om[t][c]);
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+              pf[t][mt][0] = transpose8x8(pack_h2(sc[t][mt][0], sc[t][mt][1]));
+              pf[t][mt][1] = transpose8x8(pack_h2(sc[t][mt][2], sc[t][mt][3]));
+            }
+          }
+          // ---- O^T += V^T P^T ----
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            const int key = mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+            const uint32_t rowp = pg_s + V_CODES + key * ROW;
+            const int sw = (key >> 1) & 3;
+#pragma unroll
+            for (int p = 0; p < 4; p += 2) {
+              uint32_t v[4];  // octets 0, 1 of piece p, then of piece p + 1
+              ldsm_x4_t(v, rowp + (((p + (lane >> 4)) ^ sw) << 4));
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                uint32_t e0[4], e1[4];
+                spread(v[2 * j], e0);
+                spread(v[2 * j + 1], e1);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  mma_f16_16816(z.o[t][p + j][0], e0[0], e0[1], e1[0], e1[1], pf[t][mt][0],
+                                pf[t][mt][1]);
+                  mma_f16_16816(z.o[t][p + j][1], e0[2], e0[3], e1[2], e1[3], pf[t][mt][0],
+                                pf[t][mt][1]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();  // all lanes are done with this page
+        ++used;
+        if (issued < mine && !dead) issue();
+      }
+    }
+
+    // ---- the warps' states of this segment, joined pairwise ----
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) {
+          z.l[t][c] += __shfl_xor_sync(0xffffffffu, z.l[t][c], off);
+          z.om[t][c] += __shfl_xor_sync(0xffffffffu, z.om[t][c], off);
+        }
+#pragma unroll
+    for (int half = NW / 2; half >= 1; half >>= 1) {
+      if (warp >= half && warp < 2 * half) {
+        float* dst = area + (warp - half) * area_floats<NT>() + lane;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            dst[(t * 38 + i) * 32] = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            dst[(t * 38 + 32 + c) * 32] = z.R[t][c];
+            dst[(t * 38 + 34 + c) * 32] = z.l[t][c];
+            dst[(t * 38 + 36 + c) * 32] = z.om[t][c];
+          }
+        }
+      }
+      __syncthreads();
+      if (warp < half) {
+        const float* src = area + warp * area_floats<NT>() + lane;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float fa[2], fb[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float Ro = src[(t * 38 + 32 + c) * 32];
+            const float Rn = fmaxf(z.R[t][c], Ro);
+            fa[c] = z.R[t][c] == -INFINITY ? 0.f : fast_exp2(z.R[t][c] - Rn);
+            fb[c] = Ro == -INFINITY ? 0.f : fast_exp2(Ro - Rn);
+            z.R[t][c] = Rn;
+            z.l[t][c] = z.l[t][c] * fa[c] + src[(t * 38 + 34 + c) * 32] * fb[c];
+            z.om[t][c] = z.om[t][c] * fa[c] + src[(t * 38 + 36 + c) * 32] * fb[c];
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float& o = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
+            o = o * fa[i & 1] + src[(t * 38 + i) * 32] * fb[i & 1];
+          }
+        }
+      }
+      __syncthreads();  // the areas are free again
+    }
+
+    if (warp == 0) {
+      const bool whole = f0 == ub && f1 == ub + pages;
+      const int slot = 2 * blockIdx.x + (f0 == begin ? 0 : 1);
+      if (!whole && f0 == ub && lane == 0) {
+        const int last = (ub + pages - 1) / per;
+        a.desc[blockIdx.x] = make_int4(slot, last - blockIdx.x + 1, b, unit);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col = t * 8 + 2 * tig + c;
+          const int r = rt * COLS + col;
+          if (r >= a.S * a.G) continue;
+          const float inv = z.l[t][c] > 0.f || z.l[t][c] != z.l[t][c] ? 1.f / z.l[t][c] : 0.f;
+          const float om = z.om[t][c];
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)  // dim 32 (i / 4) + 4 gid + i % 4
+            v[i] = fmaf(z.o[t][i >> 2][(i >> 1) & 1][2 * (i & 1) + c], (i & 1) ? 0x1p20f : 0x1p24f, om);
+          if (whole) {
+            const int s = r / a.G;
+            uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const __nv_bfloat162 h0 = __floats2bfloat162_rn(v[4 * p] * inv, v[4 * p + 1] * inv);
+              const __nv_bfloat162 h1 = __floats2bfloat162_rn(v[4 * p + 2] * inv, v[4 * p + 3] * inv);
+              *reinterpret_cast<uint2*>(dst + 32 * p + 4 * gid) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+            }
+          } else {
+            float* po = a.part_o + ((int64_t)slot * COLS + col) * DH;
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              *reinterpret_cast<float4*>(po + 32 * p + 4 * gid) =
+                  make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+            if (gid == 0)
+              *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * COLS + col) * 2) =
+                  make_float2(z.R[t][c], z.l[t][c]);
+          }
+        }
+    }
+    f0 = f1;
+  }
+  // A warp that gave up leaves copies in flight: wait (bounded) for them.
+  if (dead)
+    for (int i = dead_at; i < issued; ++i) mbd::mbar_wait(bar + i % ST, (i / ST) & 1, nullptr, 0);
+}
+
+// Joins the partials of the units that start in main CTA blockIdx.x and end in
+// a later one: one warp a query row.
+template <int NT>
+__global__ void __launch_bounds__(NT * 8 * 32) attn_kv4_combine_kernel(const Args a) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  constexpr int COLS = NT * 8;
+  const int4 d = a.desc[blockIdx.x];
+  if (d.y == 0) return;
+  const int col = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = d.w / a.RT, r = (d.w - kvh * a.RT) * COLS + col;
+  if (r >= a.S * a.G) return;
+  const int c0 = blockIdx.x;
+  auto row = [&](int i) -> int64_t {  // the i-th partial: this CTA's last, then the next ones' first
+    return (int64_t)(i == 0 ? d.x : 2 * (c0 + i)) * COLS + col;
+  };
+  float M = -INFINITY;
+  for (int i = lane; i < d.y; i += 32) M = fmaxf(M, a.part_ml[row(i) * 2]);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < d.y; ++i) {
+    const int64_t at = row(i);
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+    const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * DH + lane * 4);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+    L = fmaf(ml.y, w, L);
+    acc.x = fmaf(o.x, w, acc.x);
+    acc.y = fmaf(o.y, w, acc.y);
+    acc.z = fmaf(o.z, w, acc.z);
+    acc.w = fmaf(o.w, w, acc.w);
+  }
+  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+  const __nv_bfloat162 h0 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+  const __nv_bfloat162 h1 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+  const int s = r / a.G;
+  uint16_t* dst = a.out + ((int64_t)d.z * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
+  *reinterpret_cast<uint2*>(dst + lane * 4) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+}
+
+constexpr int MAX_B = 4096;  // sequences a call: their page counts are planned in shared memory
+
+template <int NT>
+constexpr int smem_bytes(int B) {
+  return NW * ST * BLOB + (NW / 2) * area_floats<NT>() * 4 + NW * ST * 8 + (NW + NW * ST + B + 1) * 4;
+}
+
+// CTAs of one resident wave (with the shared memory of a batch of up to 64).
+template <int NT>
+int resident_ctas() {
+  static int per_sm[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) dev = 0;
+  if (!per_sm[dev]) {
+    int nb = 0;
+    if (mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes<NT>(MAX_B)) ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&nb, attn_kv4_kernel<NT>, NW * 32,
+                                                      smem_bytes<NT>(64)) != cudaSuccess || nb < 1)
+      nb = 1;
+    per_sm[dev] = nb;
+  }
+  return per_sm[dev] * mb::num_sms();
+}
+
+struct Plan {
+  int nt, rt, grid;
+  size_t bytes;
+};
+
+// Query rows of a kv head: S * G. Up to 8 take one column tile, more two (so
+// that a page is unpacked once for 16 rows), in row tiles of 16.
+Plan make_plan(int B, int S, int Hq, int Hkv, int max_pages) {
+  Plan p;
+  const int64_t rows = (int64_t)S * (Hq / Hkv);
+  p.nt = rows <= 8 ? 1 : 2;
+  p.rt = (int)((rows + p.nt * 8 - 1) / (p.nt * 8));
+  const int64_t most = (int64_t)B * Hkv * p.rt * max_pages;
+  const int res = p.nt == 1 ? resident_ctas<1>() : resident_ctas<2>();
+  p.grid = (int)(most < res ? (most > 0 ? most : 1) : res);
+  p.bytes = (size_t)p.grid * (16 + 2 * p.nt * 8 * (DH + 2) * sizeof(float));
+  return p;
+}
+
+template <int NT>
+int launch(const Args& a, int grid, cudaStream_t s) {
+  const int smem = smem_bytes<NT>(a.B);
+  int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes<NT>(MAX_B));
+  if (rc) return rc;
+  MB_CUDA(mb::launch_pdl(attn_kv4_kernel<NT>, dim3(grid), dim3(NW * 32), smem, s, a));
+  if (grid > 1)
+    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT>, dim3(grid), dim3(NT * 8 * 32), 0, s, a));
+  return MB_OK;
+}
+
+}  // namespace
+
+extern "C" size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages) {
+  if (B <= 0 || S <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_pages <= 0) return 0;
+  return make_plan(B, S, Hq, Hkv, max_pages).bytes;
+}
+
+extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache,
+                                     int num_pages, const int* block_table, int max_pages,
+                                     const int* kv_len, const int* start_pos, int B, int S, int Hq,
+                                     int Hkv, int Dh, float scale, uint16_t* out, int64_t ldo,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  MB_REQUIRE(Dh == DH, "attention: head_dim must be 128 (got %d)", Dh);
+  MB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention: Hq must be a multiple of Hkv");
+  MB_REQUIRE(B >= 0 && S >= 0 && num_pages > 0 && max_pages > 0, "attention kv4: bad sizes");
+  if (B == 0 || S == 0) return MB_OK;
+  MB_REQUIRE(B <= MAX_B, "attention kv4: at most %d sequences a call", MAX_B);
+  MB_REQUIRE(q && cache && block_table && kv_len && out, "attention kv4: null pointer");
+  MB_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0,
+             "attention kv4: q, out and the cache must be 16-byte aligned");
+  const Plan p = make_plan(B, S, Hq, Hkv, max_pages);
+  MB_REQUIRE((int64_t)B * Hkv * p.rt * max_pages < (1ll << 30) && (int64_t)max_pages * PAGE < (1ll << 30),
+             "attention kv4: too many pages");
+  MB_REQUIRE(workspace && workspace_bytes >= p.bytes && (uintptr_t)workspace % 16 == 0,
+             "attention kv4: workspace of %zu bytes required, 16-byte aligned", p.bytes);
+  uint32_t* status = mb::device_status_ptr();
+  MB_REQUIRE(status, "attention kv4: no status word");
+  Args a;
+  a.q = q;
+  a.cache = cache;
+  a.table = block_table;
+  a.kv_len = kv_len;
+  a.start_pos = start_pos;
+  a.out = out;
+  a.desc = static_cast<int4*>(workspace);
+  a.part_o = reinterpret_cast<float*>(a.desc + p.grid);
+  a.part_ml = a.part_o + (size_t)p.grid * 2 * p.nt * 8 * DH;
+  a.status = status;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.num_pages = num_pages;
+  a.max_pages = max_pages;
+  a.B = B;
+  a.S = S;
+  a.Hkv = Hkv;
+  a.G = Hq / Hkv;
+  a.RT = p.rt;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return p.nt == 1 ? launch<1>(a, p.grid, static_cast<cudaStream_t>(stream))
+                   : launch<2>(a, p.grid, static_cast<cudaStream_t>(stream));
+}

@@ -79,6 +79,7 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
 #define MB_DEV_TIMEOUT_TMA 0x1u
 #define MB_DEV_TIMEOUT_MMA 0x2u
 #define MB_DEV_TIMEOUT_EPI 0x4u
+#define MB_DEV_BAD_PAGE 0x8u /* a page index outside its cache was skipped */
 #define MB_DEV_TIMEOUT_SELFTEST 0x100u
 
 namespace mbd {

@@ -1,0 +1,492 @@
+// Page operations of a paged KV cache: growing sequences, forking and freeing
+// them, and compacting the pool. They work on the block table, the sequence
+// lengths and a use count per page, all in device memory, and on any number of
+// page pools (the keys and values of every layer, in 4 bits or bf16), whose
+// pages are moved as bytes. Nothing returns to the host, so a decode loop that
+// calls them can be captured in a CUDA graph.
+//
+// Rules. A sequence of `len` tokens owns the first ceil(len / 64) entries of
+// its table row; what stands behind them is left alone. A page may be shared
+// by sequences only while it is full; refs[p] counts the rows that name it, and
+// 0 means free. New pages are the lowest-numbered free ones, given out in row
+// order, so that results do not depend on timing. A call that cannot be served
+// (too few free pages, an entry or a parent out of range) changes nothing.
+//
+// The bookkeeping of a call is one launch of one 8-CTA cluster: its 128 warps
+// count (ballots over contiguous segments), meet at the cluster barrier, read
+// the 128 counts and place what they counted. The pages' bytes move in a
+// second launch over all SMs, 16 bytes a load, bound by HBM.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace {
+
+constexpr int PAGE = 64;
+constexpr int CTAS = 8, THREADS = 512;
+constexpr int WARPS = CTAS * THREADS / 32;  // 128
+constexpr int MAX_POOLS = 64;
+
+struct Pools {
+  uint8_t* base[MAX_POOLS];
+  int64_t bytes[MAX_POOLS];  // one page
+  int n;
+};
+
+// Caller's workspace, as the kernels see it.
+struct Work {
+  int* cnt;     // [4][WARPS]
+  int* head;    // [1] moves to make
+  int2* moves;  // [max moves] from, to
+  int* ids;     // free pages found / holes
+  int* ids2;    // moved pages
+  int* row;     // [B] per-row number
+  int* row2;    // [B]
+  int* stage;   // [B][max_pages] a fork's new rows
+};
+
+struct Meta {
+  int* table;
+  int* len;
+  int* refs;
+  int B, max_pages, num_pages;
+  int* status;
+  Work w;
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ int warp_id() { return (blockIdx.x * THREADS + threadIdx.x) >> 5; }
+
+// This warp's contiguous part of n things: a multiple of 32.
+__device__ __forceinline__ void segment(int n, int& from, int& to) {
+  const int size = ((n + WARPS - 1) / WARPS + 31) / 32 * 32;
+  const int64_t f = (int64_t)warp_id() * size;
+  from = (int)(f < n ? f : n);
+  to = (int)(f + size < n ? f + size : n);
+}
+
+// Sum of one row of counts over the warps before this one, and over all.
+__device__ __forceinline__ int2 before_and_all(const int* cnt) {
+  const int lane = threadIdx.x & 31, me = warp_id();
+  int b = 0, a = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS / 32; ++i) {
+    const int v = __ldcg(cnt + i * 32 + lane);
+    a += v;
+    if (i * 32 + lane < me) b += v;
+  }
+  return make_int2(__reduce_add_sync(0xffffffffu, b), __reduce_add_sync(0xffffffffu, a));
+}
+
+__device__ __forceinline__ int pages_of(int len) { return (len + PAGE - 1) / PAGE; }
+
+// How many pages of this warp's part of the pool are free / in use.
+template <bool FREE>
+__device__ int count_pages(const int* refs, int from, int to) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+#pragma unroll 4
+  for (int i = from; i < to; i += 32) {
+    const int p = i + lane;
+    n += __popc(__ballot_sync(0xffffffffu, p < to && (FREE ? refs[p] == 0 : refs[p] > 0)));
+  }
+  return n;
+}
+
+// The first `want` free pages of the pool, in order, into ids.
+__device__ void list_free(const int* refs, int from, int to, int rank, int want, int* ids) {
+  const int lane = threadIdx.x & 31;
+  for (int i = from; i < to && rank < want; i += 32) {
+    const int p = i + lane;
+    const bool is_free = p < to && refs[p] == 0;
+    const uint32_t m = __ballot_sync(0xffffffffu, is_free);
+    const int r = rank + __popc(m & ((1u << lane) - 1));
+    if (is_free && r < want) ids[r] = p;
+    rank += __popc(m);
+  }
+}
+
+// ---------------------------------------------------------------------------
+__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
+    kv_extend_kernel(const Meta m, const int* __restrict__ add, int* __restrict__ start) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int lane = threadIdx.x & 31, me = warp_id();
+  int r0, r1, p0, p1;
+  segment(m.B, r0, r1);
+  segment(m.num_pages, p0, p1);
+  const int most = m.max_pages * PAGE;
+  int need = 0, bad = 0;
+  for (int i = r0; i < r1; i += 32) {
+    const int b = i + lane;
+    if (b < r1) {
+      const int l = m.len[b], n = add[b];
+      if (l < 0 || n < 0 || l > most || n > most - l) bad = 1;
+      else need += pages_of(l + n) - pages_of(l);
+    }
+  }
+  need = __reduce_add_sync(0xffffffffu, need);
+  bad = __any_sync(0xffffffffu, bad);
+  const int nfree = count_pages<true>(m.refs, p0, p1);
+  if (lane == 0) {
+    m.w.cnt[me] = need;
+    m.w.cnt[WARPS + me] = nfree;
+    m.w.cnt[2 * WARPS + me] = bad;
+  }
+  cluster_sync();
+  const int2 nd = before_and_all(m.w.cnt), fr = before_and_all(m.w.cnt + WARPS);
+  const bool any_bad = before_and_all(m.w.cnt + 2 * WARPS).y != 0;
+  const int lack = nd.y > fr.y ? nd.y - fr.y : 0;
+  const bool go = !any_bad && !lack;
+  if (me == 0 && lane == 0) *m.status = any_bad ? -1 : lack;
+  if (go) {
+    list_free(m.refs, p0, p1, fr.x, nd.y, m.w.ids);
+    int run = nd.x;  // pages given to rows before this one
+    for (int i = r0; i < r1; i += 32) {
+      const int b = i + lane;
+      int n = 0;
+      if (b < r1) n = pages_of(m.len[b] + add[b]) - pages_of(m.len[b]);
+      int inc = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += y;
+      }
+      if (b < r1) m.w.row[b] = run + inc - n;
+      run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  cluster_sync();
+  for (int b = me; b < m.B; b += WARPS) {  // one warp a row
+    const int l = m.len[b];
+    __syncwarp();  // every lane has read the length before it changes
+    if (lane == 0) start[b] = l;
+    if (!go) continue;
+    const int n = add[b], old = pages_of(l), k = pages_of(l + n) - old;
+    const int off = __ldcg(m.w.row + b);
+    for (int i = lane; i < k; i += 32) {
+      const int p = __ldcg(m.w.ids + off + i);
+      m.table[(int64_t)b * m.max_pages + old + i] = p;
+      m.refs[p] = 1;
+    }
+    if (lane == 0) m.len[b] = l + n;
+  }
+}
+
+// ---------------------------------------------------------------------------
+__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
+    kv_fork_kernel(const Meta m, const int* __restrict__ parent) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int lane = threadIdx.x & 31, me = warp_id();
+  int r0, r1, p0, p1;
+  segment(m.B, r0, r1);
+  segment(m.num_pages, p0, p1);
+  const int most = m.max_pages * PAGE;
+  auto bad_len = [&](int l) { return l < 0 || l > most; };
+  // ---- count: tail pages to copy, free pages; stage the parents' rows ----
+  int tails = 0, bad = 0;
+  for (int i = r0; i < r1; i += 32) {
+    const int b = i + lane;
+    int tail = 0;
+    if (b < r1) {
+      const int p = parent[b];
+      if (p < -1 || p >= m.B || bad_len(m.len[b])) {
+        bad = 1;
+      } else {
+        const int l = p < 0 ? 0 : m.len[p];
+        if (bad_len(l)) bad = 1;
+        else tail = p != b && l % PAGE != 0;
+        m.w.row2[b] = l;
+      }
+    }
+    tails += __popc(__ballot_sync(0xffffffffu, tail));
+  }
+  const int nfree = count_pages<true>(m.refs, p0, p1);
+  for (int b = me; b < m.B; b += WARPS) {
+    const int p = parent[b];
+    if (p == b || p < -1 || p >= m.B) continue;
+    const int old = pages_of(m.len[b]), now = p < 0 ? 0 : pages_of(m.len[p]);
+    if (old < 0 || old > m.max_pages || now < 0 || now > m.max_pages) continue;  // bad, seen above
+    for (int c = lane; c < old; c += 32)
+      if ((unsigned)m.table[(int64_t)b * m.max_pages + c] >= (unsigned)m.num_pages) bad = 1;
+    for (int c = lane; c < now; c += 32) {
+      const int e = m.table[(int64_t)p * m.max_pages + c];
+      if ((unsigned)e >= (unsigned)m.num_pages) bad = 1;
+      m.w.stage[(int64_t)b * m.max_pages + c] = e;
+    }
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    m.w.cnt[me] = tails;
+    m.w.cnt[WARPS + me] = nfree;
+    m.w.cnt[2 * WARPS + me] = bad;
+  }
+  cluster_sync();
+  const int2 tl = before_and_all(m.w.cnt), fr = before_and_all(m.w.cnt + WARPS);
+  const bool any_bad = before_and_all(m.w.cnt + 2 * WARPS).y != 0;
+  const int lack = tl.y > fr.y ? tl.y - fr.y : 0;
+  const bool go = !any_bad && !lack;
+  if (me == 0 && lane == 0) {
+    *m.status = any_bad ? -1 : lack;
+    *m.w.head = go ? tl.y : 0;
+  }
+  if (go) {
+    list_free(m.refs, p0, p1, fr.x, tl.y, m.w.ids);
+    int rank = tl.x;
+    for (int i = r0; i < r1; i += 32) {
+      const int b = i + lane;
+      const bool tail = b < r1 && parent[b] >= 0 && parent[b] != b && m.len[parent[b]] % PAGE != 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, tail);
+      if (b < r1) m.w.row[b] = tail ? rank + __popc(mask & ((1u << lane) - 1)) : -1;
+      rank += __popc(mask);
+    }
+  }
+  cluster_sync();
+  if (!go) return;
+  // ---- place: uses, rows, lengths, and the list of pages to copy ----
+  for (int b = me; b < m.B; b += WARPS) {
+    if (parent[b] == b) continue;
+    const int l = __ldcg(m.w.row2 + b), tail = __ldcg(m.w.row + b);
+    const int old = pages_of(m.len[b]), now = pages_of(l);
+    __syncwarp();
+    int* row = m.table + (int64_t)b * m.max_pages;
+    for (int c = lane; c < max(old, now); c += 32) {
+      if (c < old) atomicSub(m.refs + row[c], 1);
+      if (c < now) {
+        int e = __ldcg(m.w.stage + (int64_t)b * m.max_pages + c);
+        if (tail >= 0 && c == now - 1) {
+          const int to = __ldcg(m.w.ids + tail);
+          m.w.moves[tail] = make_int2(e, to);
+          e = to;
+        }
+        atomicAdd(m.refs + e, 1);
+        row[c] = e;
+      }
+    }
+    if (lane == 0) m.len[b] = l;
+  }
+}
+
+// ---------------------------------------------------------------------------
+__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
+    kv_compact_kernel(const Meta m, int* __restrict__ remap) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int lane = threadIdx.x & 31, me = warp_id();
+  int p0, p1;
+  segment(m.num_pages, p0, p1);
+  const int live_here = count_pages<false>(m.refs, p0, p1);
+  int bad = 0;
+  for (int b = me; b < m.B; b += WARPS) {
+    const int l = m.len[b];
+    if (l < 0 || l > m.max_pages * PAGE) {
+      bad = 1;
+      continue;
+    }
+    for (int c = lane; c < pages_of(l); c += 32) {
+      const int e = m.table[(int64_t)b * m.max_pages + c];
+      if ((unsigned)e >= (unsigned)m.num_pages || m.refs[e] <= 0) bad = 1;
+    }
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    m.w.cnt[me] = live_here;
+    m.w.cnt[WARPS + me] = bad;
+  }
+  cluster_sync();
+  const int2 lv = before_and_all(m.w.cnt);
+  const bool go = before_and_all(m.w.cnt + WARPS).y == 0;
+  const int live = lv.y;
+  if (me == 0 && lane == 0) *m.status = go ? live : -1;
+  // free pages below `live` are holes, pages in use from `live` on are moved
+  // into them, in order; as many of the one as of the other
+  int rank = lv.x, below = 0;
+  for (int i = p0; i < p1; i += 32) {
+    const int p = i + lane;
+    const bool use = p < p1 && m.refs[p] > 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, use);
+    const int lb = rank + __popc(mask & ((1u << lane) - 1));  // pages in use before p
+    if (p < p1) {
+      if (!go) remap[p] = p;
+      else if (!use) remap[p] = -1;
+      else if (p < live) remap[p] = p;
+      if (go && !use && p < live) m.w.ids[p - lb] = p;
+      if (go && use && p >= live) m.w.ids2[live - 1 - lb] = p;  // counted from the last one
+    }
+    below += __popc(__ballot_sync(0xffffffffu, use && p < live));
+    rank += __popc(mask);
+  }
+  if (lane == 0) m.w.cnt[2 * WARPS + me] = below;
+  cluster_sync();
+  const int n = live - before_and_all(m.w.cnt + 2 * WARPS).y;
+  if (me == 0 && lane == 0) *m.w.head = go ? n : 0;
+  if (go)
+    for (int i = me * 32 + lane; i < n; i += WARPS * 32) {
+      const int from = __ldcg(m.w.ids2 + n - 1 - i), to = __ldcg(m.w.ids + i);
+      m.w.moves[i] = make_int2(from, to);
+      remap[from] = to;
+      m.refs[to] = m.refs[from];
+      m.refs[from] = 0;
+    }
+  cluster_sync();
+  if (!go) return;
+  for (int b = me; b < m.B; b += WARPS)
+    for (int c = lane; c < pages_of(m.len[b]); c += 32) {
+      int* e = m.table + (int64_t)b * m.max_pages + c;
+      *e = __ldcg(remap + *e);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The listed pages of every pool: no page is both read and written (a fork
+// writes free pages, a compaction moves pages above `live` below it).
+constexpr int COPY_THREADS = 256, COPY_VECS = 4;
+constexpr int COPY_CHUNK = COPY_THREADS * COPY_VECS * 16;  // bytes of a page a CTA moves at once
+
+__global__ void __launch_bounds__(COPY_THREADS)
+    kv_copy_kernel(const __grid_constant__ Pools pools, const int* __restrict__ head,
+                   const int2* __restrict__ moves, int chunks) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int n = *head;
+  const int64_t total = (int64_t)n * chunks * pools.n;
+  for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+    const int chunk = (int)(i % chunks);
+    const int64_t rest = i / chunks;
+    const int pool = (int)(rest % pools.n);
+    const int2 mv = moves[rest / pools.n];
+    const int64_t bytes = pools.bytes[pool], at = (int64_t)chunk * COPY_CHUNK;
+    const uint8_t* src = pools.base[pool] + mv.x * bytes + at;
+    uint8_t* dst = pools.base[pool] + mv.y * bytes + at;
+    const int64_t left = bytes - at;
+    uint4 v[COPY_VECS];
+#pragma unroll
+    for (int j = 0; j < COPY_VECS; ++j) {
+      const int64_t o = (int64_t)(j * COPY_THREADS + threadIdx.x) * 16;
+      if (o < left) v[j] = __ldcs(reinterpret_cast<const uint4*>(src + o));
+    }
+#pragma unroll
+    for (int j = 0; j < COPY_VECS; ++j) {
+      const int64_t o = (int64_t)(j * COPY_THREADS + threadIdx.x) * 16;
+      if (o < left) __stcs(reinterpret_cast<uint4*>(dst + o), v[j]);
+    }
+  }
+}
+
+size_t align16(size_t x) { return (x + 15) / 16 * 16; }
+
+// Workspace of any of the page calls: counts, move list, page lists, rows.
+size_t work_layout(int B, int max_pages, int num_pages, bool stage, Work* w, uint8_t* p) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* r = p + at;
+    at += align16(bytes);
+    return r;
+  };
+  int* cnt = reinterpret_cast<int*>(take(4 * WARPS * sizeof(int)));
+  int* head = reinterpret_cast<int*>(take(sizeof(int)));
+  int2* moves = reinterpret_cast<int2*>(take((size_t)num_pages * sizeof(int2)));
+  int* ids = reinterpret_cast<int*>(take((size_t)num_pages * sizeof(int)));
+  int* ids2 = reinterpret_cast<int*>(take((size_t)num_pages * sizeof(int)));
+  int* row = reinterpret_cast<int*>(take((size_t)B * sizeof(int)));
+  int* row2 = reinterpret_cast<int*>(take((size_t)B * sizeof(int)));
+  int* st = reinterpret_cast<int*>(take(stage ? (size_t)B * max_pages * sizeof(int) : 0));
+  if (w) *w = Work{cnt, head, moves, ids, ids2, row, row2, st};
+  return at;
+}
+
+int fill_meta(const char* what, Meta* m, int* table, int* len, int* refs, int B, int max_pages,
+              int num_pages, int* status, bool stage, void* ws, size_t ws_bytes) {
+  MB_REQUIRE(B >= 0 && max_pages > 0 && num_pages >= 0 && max_pages < (1 << 24), "%s: bad sizes", what);
+  MB_REQUIRE((table && len) || B == 0, "%s: null pointer", what);
+  MB_REQUIRE(refs && status, "%s: null pointer", what);
+  MB_REQUIRE((int64_t)B * max_pages < (1ll << 31), "%s: block table too large", what);
+  const size_t need = work_layout(B, max_pages, num_pages, stage, nullptr, nullptr);
+  MB_REQUIRE(ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0,
+             "%s: workspace of %zu bytes required, 16-byte aligned", what, need);
+  *m = Meta{table, len, refs, B, max_pages, num_pages, status, {}};
+  work_layout(B, max_pages, num_pages, stage, &m->w, static_cast<uint8_t*>(ws));
+  return MB_OK;
+}
+
+int copy_pages(const char* what, void* const* pools, const int64_t* bytes, int npools, const Work& w,
+               int64_t most_moves, cudaStream_t s) {
+  for (int at = 0; at < npools; at += MAX_POOLS) {
+    Pools p = {};
+    p.n = npools - at < MAX_POOLS ? npools - at : MAX_POOLS;
+    int64_t big = 0;
+    for (int i = 0; i < p.n; ++i) {
+      p.base[i] = static_cast<uint8_t*>(pools[at + i]);
+      p.bytes[i] = bytes[at + i];
+      big = bytes[at + i] > big ? bytes[at + i] : big;
+    }
+    const int chunks = (int)((big + COPY_CHUNK - 1) / COPY_CHUNK);
+    const int64_t all = most_moves * chunks * p.n, wave = (int64_t)mb::num_sms() * 8;
+    if (all == 0) continue;
+    MB_CUDA(mb::launch_pdl(kv_copy_kernel, dim3((unsigned)(all < wave ? all : wave)),
+                           dim3(COPY_THREADS), 0, s, p, w.head, w.moves, chunks));
+  }
+  return MB_OK;
+}
+
+int check_pools(const char* what, void* const* pools, const int64_t* bytes, int npools) {
+  MB_REQUIRE(npools >= 0 && (npools == 0 || (pools && bytes)), "%s: bad pools", what);
+  for (int i = 0; i < npools; ++i)
+    MB_REQUIRE(pools[i] && (uintptr_t)pools[i] % 16 == 0 && bytes[i] > 0 && bytes[i] % 16 == 0 &&
+                   bytes[i] < (1ll << 40),
+               "%s: pools must be 16-byte aligned and their pages a multiple of 16 bytes", what);
+  return MB_OK;
+}
+
+}  // namespace
+
+extern "C" size_t mb_kv_pages_workspace_bytes(int B, int max_pages, int num_pages) {
+  if (B < 0 || max_pages <= 0 || num_pages < 0) return 0;
+  return work_layout(B, max_pages, num_pages, true, nullptr, nullptr);
+}
+
+extern "C" int mb_kv_pages_extend(int* block_table, int* seq_len, int* page_refs, int B,
+                                  int max_pages, int num_pages, const int* new_len, int* start_pos,
+                                  int* status, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  Meta m;
+  int rc = fill_meta("kv_pages_extend", &m, block_table, seq_len, page_refs, B, max_pages, num_pages,
+                     status, false, workspace, workspace_bytes);
+  if (rc) return rc;
+  MB_REQUIRE(B == 0 || (new_len && start_pos), "kv_pages_extend: null pointer");
+  MB_CUDA(mb::launch_pdl(kv_extend_kernel, dim3(CTAS), dim3(THREADS), 0,
+                         static_cast<cudaStream_t>(stream), m, new_len, start_pos));
+  return MB_OK;
+}
+
+extern "C" int mb_kv_pages_fork(void* const* pools, const int64_t* page_bytes, int npools,
+                                int* block_table, int* seq_len, int* page_refs, int B, int max_pages,
+                                int num_pages, const int* parent, int* status, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  Meta m;
+  int rc = fill_meta("kv_pages_fork", &m, block_table, seq_len, page_refs, B, max_pages, num_pages,
+                     status, true, workspace, workspace_bytes);
+  if (!rc) rc = check_pools("kv_pages_fork", pools, page_bytes, npools);
+  if (rc) return rc;
+  MB_REQUIRE(B == 0 || parent, "kv_pages_fork: null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  MB_CUDA(mb::launch_pdl(kv_fork_kernel, dim3(CTAS), dim3(THREADS), 0, s, m, parent));
+  return copy_pages("kv_pages_fork", pools, page_bytes, npools, m.w, B < num_pages ? B : num_pages, s);
+}
+
+extern "C" int mb_kv_pages_compact(void* const* pools, const int64_t* page_bytes, int npools,
+                                   int* block_table, const int* seq_len, int* page_refs, int B,
+                                   int max_pages, int num_pages, int* remap, int* live,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  Meta m;
+  int rc = fill_meta("kv_pages_compact", &m, block_table, const_cast<int*>(seq_len), page_refs, B,
+                     max_pages, num_pages, live, false, workspace, workspace_bytes);
+  if (!rc) rc = check_pools("kv_pages_compact", pools, page_bytes, npools);
+  if (rc) return rc;
+  MB_REQUIRE(num_pages == 0 || remap, "kv_pages_compact: null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  MB_CUDA(mb::launch_pdl(kv_compact_kernel, dim3(CTAS), dim3(THREADS), 0, s, m, remap));
+  return copy_pages("kv_pages_compact", pools, page_bytes, npools, m.w, num_pages / 2, s);
+}

@@ -334,3 +334,7 @@ def transformer_block(x: torch.Tensor, w_qkv: torch.Tensor, w_o: torch.Tensor,
               w_ff1.data_ptr(), w_ff2.data_ptr(), out.data_ptr(), S, D, n_heads, FF, eps,
               ws.data_ptr(), nb, _stream())
     return out
+
+
+from .kv4 import (attention_kv4, kv4_append, kv4_cache, kv4_gather, kv_pages_compact,  # noqa: E402,F401
+                  kv_pages_extend, kv_pages_fork)

@@ -1,0 +1,550 @@
+"""The 4-bit paged cache, the attention over it and the page operations on the
+GPU against plain 64-bit implementations (_kv4ref)."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import _kv4ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from metalbench_b200 import ops as o
+    o.init(0)
+    return o
+
+
+@pytest.fixture(autouse=True)
+def clean_status(ops):
+    from metalbench_b200 import _lib
+    _lib.call("mb_clear_device_status")
+    yield
+    _lib.call("mb_clear_device_status")
+
+
+def status():
+    from metalbench_b200 import _lib
+    v = C.c_uint32(0)
+    _lib.call("mb_device_status", C.byref(v))
+    return v.value
+
+
+def i32(x):
+    return torch.as_tensor(np.asarray(x), dtype=torch.int32).cuda()
+
+
+def bf(x):
+    return torch.from_numpy(np.asarray(x, dtype=np.float32)).to(torch.bfloat16).cuda()
+
+
+def make_cache(rng, num_pages, H, strong=True):
+    """A filled cache (uint8 numpy) with codes, scales and minima as they come."""
+    c = rng.integers(0, 256, (num_pages, H, R.BLOB), dtype=np.uint8)
+    scale = np.exp(rng.normal(-1.2, 0.5 if strong else 0.0, (num_pages, H, 128)))
+    low = -7.5 * scale + rng.normal(0, 0.2, scale.shape)
+    par = np.stack([R.bf16_bits(scale), R.bf16_bits(low)], -1).astype(np.uint16)
+    c[..., 8192:] = par.reshape(num_pages, H, 256).view(np.uint8)
+    return c
+
+
+def make_table(rng, lens, extra=2, width=None):
+    counts = [R.pages_of(int(n)) for n in lens]
+    P = sum(counts) + extra
+    M = width or max(1, max(counts))
+    t = np.full((len(lens), M), -1, np.int32)
+    order = rng.permutation(P)
+    at = 0
+    for b, n in enumerate(counts):
+        t[b, :n] = order[at: at + n]
+        at += n
+    return t, P
+
+
+# ---------------------------------------------------------------------------
+# storing and reading back
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("B, S, H, starts, new", [
+    (1, 1, 1, [0], None), (3, 1, 8, [63, 64, 200], None), (2, 70, 2, [0, 33], [70, 5]),
+    (4, 5, 3, [1, 60, 127, 0], [0, 5, 1, 3]), (1, 257, 4, [129], None),
+])
+@pytest.mark.parametrize("strided", [False, True])
+def test_append_writes_exactly_the_defined_bytes(ops, B, S, H, starts, new, strided):
+    rng = np.random.default_rng(S * 10 + H)
+    ends = [s + (S if new is None else n) for s, n in zip(starts, new or [S] * B)]
+    table, P = make_table(rng, ends)
+    cache = rng.integers(0, 256, (P, H, R.BLOB), dtype=np.uint8)
+    k, v = (R.bf16_round(rng.standard_normal((B, S, H, 128)) * np.exp(rng.uniform(-3, 3, (B, S, H, 1)))) for _ in range(2))
+    want = cache.copy()
+    for b in range(B):
+        for s in range(S if new is None else new[b]):
+            pos = starts[b] + s
+            for h in range(H):
+                R.put_token(want[table[b, pos // 64], h], pos % 64, k[b, s, h], v[b, s, h])
+    c = torch.from_numpy(cache).cuda()
+    if strided:  # rows of a fused projection
+        row = torch.zeros(B, S, 3 * H, 128, dtype=torch.bfloat16, device="cuda")
+        row[:, :, :H], row[:, :, 2 * H:] = bf(k), bf(v)
+        kt, vt = row[:, :, :H], row[:, :, 2 * H:]
+    else:
+        kt, vt = bf(k), bf(v)
+    ops.kv4_append(kt, vt, c, i32(table), i32(starts), None if new is None else i32(new))
+    assert np.array_equal(c.cpu().numpy(), want)
+    kb, vb = ops.kv4_gather(c, i32(table), i32(starts), S, i32(ends))
+    for got, x in ((kb, k), (vb, v)):
+        u, s, m = R.quantise(x)
+        ref = (m[..., None] + s[..., None] * u).astype(np.float32)  # one rounding
+        for b in range(B):
+            ref[b, ends[b] - starts[b]:] = 0
+        assert np.array_equal(got.cpu().numpy(), ref)
+    assert status() == 0
+
+
+def test_append_of_odd_rows(ops):
+    """All dims alike, NaN, infinities, subnormals, the type's extremes: each
+    only ever changes its own token."""
+    big = 3.3895313892515355e38  # the largest bf16
+    rows = [np.full(128, 1.5), np.zeros(128), np.linspace(-1, 1, 128), np.full(128, np.nan), np.full(128, np.inf),
+            np.full(128, 1e-39), np.linspace(0, 9e-39, 128), np.linspace(-1e4, 1e4, 128), np.linspace(0, big, 128)]
+    x = np.stack([R.bf16_round(r) for r in rows])[None, :, None]
+    x[0, 2, 0, 5] = np.nan
+    cache = ops.kv4_cache(1, 1)
+    S = x.shape[1]
+    ops.kv4_append(bf(x), bf(x[:, ::-1].copy()), cache, i32([[0]]), i32([0]))
+    k, v = (t.cpu().numpy()[0, :, 0] for t in ops.kv4_gather(cache, i32([[0]]), i32([0]), S, i32([S])))
+    for i in range(S):
+        y = bf(x[0, i, 0]).double().cpu().numpy()
+        if not np.isfinite(y).all():
+            assert np.isnan(k[i]).all() and np.isnan(v[S - 1 - i]).all(), i
+        else:
+            u, s, m = R.quantise(y)
+            ref = (m + s * u).astype(np.float32)
+            assert np.array_equal(k[i], ref) and np.array_equal(v[S - 1 - i], ref), i
+
+
+def test_append_skips_bad_pages_and_positions(ops):
+    rng = np.random.default_rng(3)
+    cache = torch.from_numpy(rng.integers(0, 256, (3, 2, R.BLOB), dtype=np.uint8)).cuda()
+    before = cache.clone()
+    k = bf(rng.standard_normal((4, 2, 2, 128)))
+    table = i32([[-1], [3], [2], [1]])
+    ops.kv4_append(k, k, cache, table, i32([0, 5, 63, -1]))  # no page, beyond the pool, past the table, before it
+    changed = (cache != before).any(-1).cpu().numpy()
+    assert changed.tolist() == [[False, False], [True, True], [True, True]]  # slot 63 of page 2, slot 0 of page 1
+    assert status() == 8
+    kb, _ = ops.kv4_gather(cache, table, i32([0, 5, 0, 0]), 1, i32([1, 6, 64, 1]))
+    assert (kb[:2] == 0).all() and torch.isfinite(kb[3]).all()
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def check_attention(ops, rng, B, S, Hq, Hkv, lens, first=None, scale=None, amp=1.0, garbage=True):
+    table, P = make_table(rng, np.maximum(lens, 0))
+    cache = make_cache(rng, P, Hkv)
+    if garbage:  # what stands past the end of a sequence may be anything
+        for b, n in enumerate(lens):
+            if n > 0 and n % 64:
+                blob = cache[table[b, n // 64]]
+                for par in (8192, 8448):
+                    blob[:, par + 4 * (n % 64): par + 256] = rng.choice([0xFF, 0x7F, 0x80], blob[:, par + 4 * (n % 64): par + 256].shape)
+    q = R.bf16_round(rng.standard_normal((B, S, Hq, 128)) * amp)
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens),
+                            start_pos=None if first is None else i32(first), scale=scale)
+    ref, slack = R.attention(q, cache, table, lens, first, 128 ** -0.5 if scale is None else scale)
+    err = np.abs(got.double().cpu().numpy() - ref)
+    tol = slack + 2 ** -8 * (np.abs(ref) + slack)  # the output's own rounding to bf16
+    assert (err <= tol).all(), float((err - tol).max())
+    assert status() == 0
+
+
+@pytest.mark.parametrize("Hq, Hkv", [(1, 1), (8, 8), (8, 1), (16, 1), (6, 2), (24, 8), (40, 8)])
+@pytest.mark.parametrize("lens", [[1], [64, 65, 0], [63, 128, 700, 1, 0, 2000]])
+def test_decode_heads_and_lengths(ops, Hq, Hkv, lens):
+    check_attention(ops, np.random.default_rng(Hq * 100 + len(lens)), len(lens), 1, Hq, Hkv, lens)
+
+
+@pytest.mark.parametrize("S", [2, 3, 5, 16, 33])
+@pytest.mark.parametrize("Hq, Hkv", [(4, 4), (8, 2), (5, 1)])
+def test_causal_rows(ops, S, Hq, Hkv):
+    rng = np.random.default_rng(S)
+    lens = np.array([S, S + 61, 300, 0, 1])
+    check_attention(ops, rng, 5, S, Hq, Hkv, lens, first=lens - S)  # some rows stand before the first key
+
+
+@pytest.mark.parametrize("S", [1, 4])
+def test_rows_that_see_nothing_are_zero(ops, S):
+    rng = np.random.default_rng(9)
+    check_attention(ops, rng, 3, S, 8, 2, np.array([100, 100, 64]), first=np.array([-100, -2, -(2 ** 31)]))
+
+
+def test_start_far_past_the_end_sees_every_key(ops):
+    check_attention(ops, np.random.default_rng(10), 2, 3, 8, 2, np.array([100, 64]), first=np.array([2 ** 31 - 1, 64]))
+
+
+def test_whole_cta_shares_and_many_units(ops):
+    """More (sequence, head) units than CTAs, and one unit over all of them."""
+    rng = np.random.default_rng(11)
+    check_attention(ops, rng, 70, 1, 16, 16, rng.integers(0, 200, 70), garbage=False)
+    check_attention(ops, rng, 1, 1, 8, 1, np.array([70001]), garbage=False)
+
+
+def test_large_scores_and_small_values(ops):
+    rng = np.random.default_rng(12)
+    check_attention(ops, rng, 2, 1, 8, 2, np.array([500, 64]), amp=30.0)
+    check_attention(ops, rng, 2, 2, 8, 2, np.array([500, 64]), first=np.array([498, 62]), scale=1e-3)
+
+
+def test_value_scales_of_very_different_size(ops):
+    """Weights are rounded with their value scale in: a token with small values
+    and nearly all of the weight is not lost beside large ones."""
+    rng = np.random.default_rng(13)
+    table, P = make_table(rng, [300])
+    cache = make_cache(rng, P, 1)
+    par = cache[..., 8448:].copy().view(np.uint16).reshape(P, 1, 64, 2)
+    s = np.exp2(rng.integers(-40, 3, (P, 1, 64)).astype(np.float64))
+    par[..., 0], par[..., 1] = R.bf16_bits(s), R.bf16_bits(-7 * s)
+    s[0, 0, :5] = 0  # all dims alike: codes are zero
+    cache[..., 8448:] = par.reshape(P, 1, 128).view(np.uint8).reshape(P, 1, 256)
+    q = R.bf16_round(rng.standard_normal((1, 1, 8, 128)) * 4)
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32([300])).double().cpu().numpy()
+    ref, slack = R.attention(q, cache, table, [300], None)
+    assert (np.abs(got - ref) <= slack + 2 ** -8 * (np.abs(ref) + slack)).all()
+
+
+def test_constant_values_come_back(ops):
+    """All dims of every value alike (scale 0): the output is that number."""
+    cache = ops.kv4_cache(2, 1)
+    v = torch.full((1, 100, 1, 128), 0.375, dtype=torch.bfloat16, device="cuda")
+    k = torch.randn(1, 100, 1, 128, device="cuda").to(torch.bfloat16)
+    ops.kv4_append(k, v, cache, i32([[1, 0]]), i32([0]))
+    q = torch.randn(1, 1, 8, 128, device="cuda").to(torch.bfloat16)
+    got = ops.attention_kv4(q, cache, i32([[1, 0]]), i32([100]))
+    assert ((got.float() - 0.375).abs() <= 0.375 * 2 ** -8).all()
+
+
+def test_bad_pages_are_left_out(ops):
+    rng = np.random.default_rng(14)
+    cache = make_cache(rng, 4, 2)
+    table = np.array([[0, 99, 1, -5], [2, 3, 2, 3]], np.int32)
+    q = R.bf16_round(rng.standard_normal((2, 1, 4, 128)))
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32([256, 200]))
+    assert status() == 8
+    # the same sequence with the bad pages cut out
+    ref, slack = R.attention(q, cache, np.array([[0, 1, 0, 0], [2, 3, 2, 3]]), [128, 200], None)
+    err = np.abs(got.double().cpu().numpy() - ref)
+    assert (err <= slack + 2 ** -8 * (np.abs(ref) + slack)).all()
+
+
+def test_length_past_the_table_is_cut(ops):
+    rng = np.random.default_rng(15)
+    cache, table = make_cache(rng, 2, 1), np.array([[1, 0]], np.int32)
+    q = bf(rng.standard_normal((1, 1, 8, 128)))
+    a, b = (ops.attention_kv4(q, torch.from_numpy(cache).cuda(), i32(table), i32([n])) for n in (128, 10 ** 9))
+    assert torch.equal(a, b)
+
+
+def test_far_pages(ops):
+    """Byte offsets of the cache past 32 bits."""
+    P = 530000  # 4.6 GB
+    cache = torch.empty((P, 1, R.BLOB), dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(16)
+    x = R.bf16_round(rng.standard_normal((1, 150, 1, 128)))
+    far, near = i32([[P - 1, 500001, 3]]), i32([[0, 1, 2]])
+    outs = []
+    for t in (far, near):
+        ops.kv4_append(bf(x), bf(x), cache, t, i32([0]))
+        k, _ = ops.kv4_gather(cache, t, i32([0]), 150, i32([150]))
+        outs.append((ops.attention_kv4(bf(x[:, :1]), cache, t, i32([150])), k))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_views_streams_and_single_token_form(ops):
+    rng = np.random.default_rng(17)
+    lens = np.array([90, 300])
+    table, P = make_table(rng, lens)
+    cache = torch.from_numpy(make_cache(rng, P, 2)).cuda()
+    q = bf(rng.standard_normal((2, 1, 8, 128)))
+    want = ops.attention_kv4(q, cache, i32(table), i32(lens))
+    row = torch.zeros(2, 1, 12, 128, dtype=torch.bfloat16, device="cuda")
+    row[:, :, 2:10] = q
+    assert torch.equal(ops.attention_kv4(row[:, :, 2:10], cache, i32(table), i32(lens)), want)
+    assert torch.equal(ops.attention_kv4(q[:, 0], cache, i32(table), i32(lens)), want[:, 0])
+    out = torch.zeros(2, 1, 12, 128, dtype=torch.bfloat16, device="cuda")
+    ops.attention_kv4(q, cache, i32(table), i32(lens), out=out[:, :, 4:])
+    assert torch.equal(out[:, :, 4:], want) and (out[:, :, :4] == 0).all()
+    t, n = i32(table), i32(lens)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [ops.attention_kv4(q, cache, t, n) for _ in range(3)]
+    s.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_refusals(ops):
+    cache, t, n = ops.kv4_cache(4, 2), i32([[0, 1]]), i32([5])
+    q = torch.zeros(1, 1, 4, 128, dtype=torch.bfloat16, device="cuda")
+    for bad in (q.float(), q.half()):
+        with pytest.raises(TypeError):
+            ops.attention_kv4(bad, cache, t, n)
+    for bad in (q[..., :64], q[:, :, :3], q.expand(2, 1, 4, 128), q.cpu(), torch.zeros(1, 1, 128, 4, dtype=torch.bfloat16, device="cuda").transpose(2, 3)):
+        with pytest.raises(ValueError):
+            ops.attention_kv4(bad, cache, t, n)
+    with pytest.raises(TypeError):
+        ops.attention_kv4(q, cache, t.long(), n)
+    with pytest.raises(ValueError):
+        ops.attention_kv4(q, cache, t, i32([5, 5]))
+    with pytest.raises(ValueError):
+        ops.attention_kv4(q, cache[:, :, :4096], t, n)
+    k = torch.zeros(1, 3, 2, 128, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        ops.kv4_append(k, k[:, :2], cache, t, n)
+    with pytest.raises(ValueError):
+        ops.kv4_append(torch.zeros(1, 3, 2, 132, dtype=torch.bfloat16, device="cuda")[..., :128], k, cache, t, n)
+    with pytest.raises(ValueError):
+        ops.kv_pages_fork([cache, cache], t, n, i32([0, 0, 0, 0]), i32([0]))
+    with pytest.raises(ValueError):
+        ops.kv_pages_fork([cache], t, n, i32([0, 0, 0]), i32([0]))
+
+
+# ---------------------------------------------------------------------------
+# pages
+# ---------------------------------------------------------------------------
+def start_state(rng, B, M, P, pools, shapes):
+    ref = R.Pages(np.full((B, M), -7, np.int32), np.zeros(B, np.int32), np.zeros(P, np.int32))
+    data = [rng.integers(0, 256, (P,) + shapes[i % len(shapes)], dtype=np.uint8) for i in range(pools)]
+    dev = dict(table=i32(ref.table), lens=i32(ref.lens), refs=i32(ref.refs), pools=[torch.from_numpy(d).cuda() for d in data])
+    return ref, data, dev
+
+
+def same_state(ref, data, dev):
+    assert np.array_equal(dev["table"].cpu().numpy(), ref.table)
+    assert np.array_equal(dev["lens"].cpu().numpy(), ref.lens)
+    assert np.array_equal(dev["refs"].cpu().numpy(), ref.refs)
+    for a, b in zip(dev["pools"], data):
+        assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("B, M, P, pools", [(1, 1, 1, 1), (5, 4, 13, 2), (33, 9, 200, 1), (130, 70, 5000, 2), (7, 40, 300, 66)])
+def test_random_page_operations(ops, B, M, P, pools):
+    rng = np.random.default_rng(B * 1000 + P)
+    ref, data, dev = start_state(rng, B, M, P, pools, [(16,), (3, 48), (17, 1024)] if pools < 10 else [(32,)])
+    seen = set()
+    for step in range(14):
+        what = ("extend", "extend", "fork", "compact")[step % 4] if step < 8 else rng.choice(["extend", "fork", "compact"])
+        if what == "extend":
+            new = rng.integers(0, max(2, 2 * P * 64 // B // 5), B) * (rng.random(B) < 0.7)
+            new = np.minimum(new, np.maximum(0, M * 64 - ref.lens)) if rng.random() < 0.8 else new
+            was = ref.lens.copy()
+            want = ref.extend(new)
+            start, st = ops.kv_pages_extend(dev["table"], dev["lens"], dev["refs"], i32(new))
+            assert np.array_equal(start.cpu().numpy(), was)
+        elif what == "fork":
+            parent = np.arange(B)
+            m = rng.random(B) < 0.5
+            parent[m] = rng.integers(-1, B, int(m.sum()))
+            want = ref.fork(parent, data)
+            st = ops.kv_pages_fork(dev["pools"], dev["table"], dev["lens"], dev["refs"], i32(parent))
+        else:
+            want, remap = ref.compact(data)
+            got, st = ops.kv_pages_compact(dev["pools"], dev["table"], dev["lens"], dev["refs"])
+            assert np.array_equal(got.cpu().numpy(), remap)
+        assert int(st) == want, what
+        seen.add((what, want > 0))
+        same_state(ref, data, dev)
+    assert len({w for w, _ in seen}) == 3
+
+
+def test_beams_that_change_places(ops):
+    """Rows that are parents and children at once read the state before the call."""
+    rng = np.random.default_rng(5)
+    ref, data, dev = start_state(rng, 4, 5, 40, 2, [(64,)])
+    ref.extend([100, 130, 64, 7])
+    ops.kv_pages_extend(dev["table"], dev["lens"], dev["refs"], i32([100, 130, 64, 7]))
+    for parent in ([1, 0, 3, 2], [3, 3, 3, 3], [0, 0, 1, 1], [-1, -1, 0, 3], [0, 0, -1, -1], [-1, -1, -1, -1]):
+        want = ref.fork(parent, data)
+        assert int(ops.kv_pages_fork(dev["pools"], dev["table"], dev["lens"], dev["refs"], i32(parent))) == want == 0
+        same_state(ref, data, dev)
+    assert (ref.refs == 0).all()
+
+
+def test_page_calls_that_cannot_be_served_change_nothing(ops):
+    rng = np.random.default_rng(6)
+    ref, data, dev = start_state(rng, 3, 4, 5, 1, [(64,)])
+    ref.extend([100, 100, 0])
+    ops.kv_pages_extend(dev["table"], dev["lens"], dev["refs"], i32([100, 100, 0]))
+    for new, want in (([0, 0, 129], 2), ([-1, 0, 0], -1), ([0, 0, 257], -1), ([2 ** 31 - 1, 0, 0], -1)):
+        assert int(ops.kv_pages_extend(dev["table"], dev["lens"], dev["refs"], i32(new))[1]) == want == ref.extend(new)
+        same_state(ref, data, dev)
+    for parent, want in (([1, 0, 0], 2), ([3, 1, 2], -1), ([0, 1, -2], -1)):
+        assert int(ops.kv_pages_fork(dev["pools"], dev["table"], dev["lens"], dev["refs"], i32(parent))) == want == ref.fork(parent, data)
+        same_state(ref, data, dev)
+    for name, at, bad in (("table", (1, 1), 5), ("table", (0, 0), -1), ("lens", (2,), -3), ("lens", (0,), 257)):
+        good = dev[name][at].clone()
+        dev[name][at], getattr(ref, name)[at] = bad, bad
+        parent = [1, 0, 2] if name == "table" else [0, 0, 0] if bad < 0 else [1, 1, 2]
+        assert int(ops.kv_pages_fork(dev["pools"], dev["table"], dev["lens"], dev["refs"], i32(parent))) == -1
+        assert int(ops.kv_pages_compact(dev["pools"], dev["table"], dev["lens"], dev["refs"])[1]) == -1
+        if name == "lens":
+            assert int(ops.kv_pages_extend(dev["table"], dev["lens"], dev["refs"], i32([0, 0, 0]))[1]) == -1
+        same_state(ref, data, dev)
+        dev[name][at], getattr(ref, name)[at] = good, int(good)
+
+
+def test_empty_batches_and_pools(ops):
+    e = torch.empty(0, dtype=torch.int32, device="cuda")
+    t = torch.empty(0, 3, dtype=torch.int32, device="cuda")
+    start, st = ops.kv_pages_extend(t, e, i32([0, 0]), e)
+    assert start.numel() == 0 and int(st) == 0
+    assert int(ops.kv_pages_fork([], t, e, i32([0, 1]), e)) == 0
+    pool = torch.arange(32, dtype=torch.uint8, device="cuda").view(2, 16)
+    remap, live = ops.kv_pages_compact([pool], t, e, i32([0, 1]))  # a page held outside the table
+    assert remap.tolist() == [-1, 0] and int(live) == 1 and pool[0].tolist() == list(range(16, 32))
+    cache = ops.kv4_cache(1, 1)
+    assert ops.attention_kv4(torch.empty(0, 1, 4, 128, dtype=torch.bfloat16, device="cuda"), cache, t, e).shape == (0, 1, 4, 128)
+    assert ops.attention_kv4(torch.empty(2, 0, 4, 128, dtype=torch.bfloat16, device="cuda"), cache, i32([[0], [0]]), i32([1, 1])).shape == (2, 0, 4, 128)
+    assert ops.attention_kv4(torch.ones(2, 1, 4, 128, dtype=torch.bfloat16, device="cuda"), cache, i32([[0], [0]]), i32([0, 0])).abs().sum() == 0
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+def test_a_serving_run(ops):
+    """Two requests; one branches into three beams that go on with tokens of
+    their own; requests end, pages are compacted; every step's attention is
+    that over the tokens the sequence has had, and compaction changes no bit."""
+    rng = np.random.default_rng(21)
+    B, M, P, H, Hq, layers = 5, 6, 24, 2, 8, 2
+    pools = [ops.kv4_cache(P, H) for _ in range(layers)]
+    table, lens, refs = i32(np.full((B, M), -1)), i32(np.zeros(B)), i32(np.zeros(P))
+    past = [[np.zeros((0, H, 128)), np.zeros((0, H, 128))] for _ in range(B)]
+
+    def step(new):
+        S = max(new)
+        k, v = (R.bf16_round(rng.standard_normal((B, S, H, 128))) for _ in range(2))
+        start, st = ops.kv_pages_extend(table, lens, refs, i32(new))
+        for pool in pools:
+            ops.kv4_append(bf(k), bf(v), pool, table, start, i32(new))
+        for b in range(B):
+            past[b] = [np.concatenate([past[b][0], k[b, : new[b]]]), np.concatenate([past[b][1], v[b, : new[b]]])]
+        assert int(st) == 0
+
+    def attend(pool):
+        q = R.bf16_round(rng.standard_normal((B, 1, Hq, 128)))
+        got = ops.attention_kv4(bf(q), pool, table, lens, start_pos=lens - 1)
+        for b in range(B):
+            blob = np.zeros((R.pages_of(len(past[b][0])) or 1, H, R.BLOB), np.uint8)
+            for i, (k, v) in enumerate(zip(*past[b])):
+                for h in range(H):
+                    R.put_token(blob[i // 64, h], i % 64, k[h], v[h])
+            ref, slack = R.attention(q[b: b + 1], blob, np.arange(len(blob))[None], [len(past[b][0])], None)
+            assert (np.abs(got[b: b + 1].double().cpu().numpy() - ref) <= slack + 2 ** -8 * (np.abs(ref) + slack)).all()
+        return bf(q), got
+
+    def fork(parent):
+        assert int(ops.kv_pages_fork(pools, table, lens, refs, i32(parent))) == 0
+        past[:] = [[x.copy() for x in past[p]] if p >= 0 else [np.zeros((0, H, 128))] * 2 for p in parent]
+
+    step([130, 70, 0, 0, 0])
+    fork([0, 1, 0, 0, -1])
+    for _ in range(3):
+        step([1, 1, 1, 1, 0])
+    attend(pools[1])
+    fork([2, 1, 2, 0, 1])   # beams reordered, the second request branches too
+    step([1, 60, 1, 1, 2])
+    attend(pools[0])
+    fork([-1, 1, 2, -1, 4])
+    q, before = attend(pools[0])
+    remap, live = ops.kv_pages_compact(pools, table, lens, refs)
+    n = int(live)
+    assert (refs[:n] > 0).all() and (refs[n:] == 0).all()
+    assert torch.equal(ops.attention_kv4(q, pools[0], table, lens, start_pos=lens - 1), before)
+    attend(pools[1])
+    assert status() == 0
+
+
+def test_a_captured_decode_step(ops):
+    """Growing, storing and attending in one CUDA graph, replayed over a page
+    border, next to a second captured graph and eager calls."""
+    rng = np.random.default_rng(22)
+    B, M, P, H, Hq = 3, 3, 9, 2, 8
+    graphs = []
+    for _ in range(2):
+        st = dict(pool=ops.kv4_cache(P, H), table=i32(np.full((B, M), -1)), lens=i32(np.zeros(B)), refs=i32(np.zeros(P)),
+                  one=i32([1, 1, 0]), k=torch.zeros(B, 1, H, 128, dtype=torch.bfloat16, device="cuda"),
+                  q=torch.zeros(B, 1, Hq, 128, dtype=torch.bfloat16, device="cuda"))
+
+        def step(st=st):
+            start, status = ops.kv_pages_extend(st["table"], st["lens"], st["refs"], st["one"])
+            ops.kv4_append(st["k"], st["k"], st["pool"], st["table"], start, st["one"])
+            return ops.attention_kv4(st["q"], st["pool"], st["table"], st["lens"], start_pos=start), status
+
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        for n in ("lens", "refs"):
+            st[n].zero_()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            st["out"], st["status"] = step()
+        graphs.append((g, st))
+    past = [[] for _ in graphs]
+    for i in range(66):
+        for j, (g, st) in enumerate(graphs):
+            k, q = R.bf16_round(rng.standard_normal((B, 1, H, 128))), R.bf16_round(rng.standard_normal((B, 1, Hq, 128)))
+            st["k"].copy_(bf(k))
+            st["q"].copy_(bf(q))
+            g.replay()
+            past[j].append(k)
+            if i in (0, 62, 63, 64, 65):
+                assert st["lens"].tolist() == [i + 1, i + 1, 0] and int(st["status"]) == 0
+                cache = st["pool"].cpu().numpy()
+                ref, slack = R.attention(q, cache, st["table"].cpu().numpy(), [i + 1, i + 1, 0], None)
+                err = np.abs(st["out"].double().cpu().numpy() - ref)
+                assert (err <= slack + 2 ** -8 * (np.abs(ref) + slack)).all()
+    for (g, st), hist in zip(graphs, past):
+        k, _ = ops.kv4_gather(st["pool"], st["table"], i32(np.zeros(B)), 66, st["lens"])
+        u, s, m = R.quantise(np.concatenate(hist, 1))
+        assert np.array_equal(k[:2].cpu().numpy(), (m[..., None] + s[..., None] * u).astype(np.float32)[:2])
+
+
+def test_attention_agrees_with_the_bf16_cache(ops):
+    """Next to the framework's own decode attention: with keys and values that
+    4 bits hold exactly, both give the same to bf16's rounding."""
+    from metalbench_b200 import _lib
+    rng = np.random.default_rng(23)
+    B, Hq, Hkv, L = 3, 8, 2, 200
+    lo = rng.integers(-6, 0, (B, L, Hkv, 1)).astype(np.float64)
+    u = rng.integers(0, 16, (B, L, Hkv, 128)).astype(np.float64)
+    u[..., 0], u[..., 1] = 0, 15
+    kv = [(lo + u) * 2.0 ** -3, (lo + u[..., ::-1]) * 2.0 ** -2]
+    M = R.pages_of(L)
+    table = np.arange(B * M, dtype=np.int32).reshape(B, M)
+    bfc = [np.zeros((B * M, Hkv, 64, 128)) for _ in kv]
+    for c, x in zip(bfc, kv):
+        for b in range(B):
+            for p in range(L):
+                c[table[b, p // 64], :, p % 64] = x[b, p]
+    cache = ops.kv4_cache(B * M, Hkv)
+    ops.kv4_append(bf(kv[0]), bf(kv[1]), cache, i32(table), i32([0] * B))
+    q = bf(R.bf16_round(rng.standard_normal((B, 1, Hq, 128))))
+    lens = np.array([200, 64, 1])
+    got = ops.attention_kv4(q, cache, i32(table), i32(lens))
+    kc, vc = (bf(c) for c in bfc)
+    out = torch.empty(B, Hq * 128, dtype=torch.bfloat16, device="cuda")
+    t, n = i32(table), i32(lens)
+    nb = _lib.lib().mb_attention_decode_workspace_bytes(B, Hq, Hkv, L)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    _lib.call("mb_attention_decode_bf16", q.data_ptr(), Hq * 128, kc.data_ptr(), vc.data_ptr(), t.data_ptr(), M, n.data_ptr(),
+              L, B, Hq, Hkv, 128, out.data_ptr(), Hq * 128, ws.data_ptr(), nb, torch.cuda.current_stream().cuda_stream)
+    # each side: its weights rounded (bf16 2^-8, fp16 2^-11) and its output (2^-8); values up to 2.25
+    bound = (2 ** -8 + 2 ** -10) * 2.25 + 2 * 2 ** -8 * 2.25
+    assert (got.view(B, -1).float() - out.float()).abs().max() <= bound
