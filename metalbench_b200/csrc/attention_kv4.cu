@@ -26,12 +26,13 @@
 // head of the group); NT column tiles of 8 per pass over the cache.
 //
 // Schedule: the flat list of (sequence, kv head, row tile, page) is cut into
-// equal shares, one a CTA, planned on the device from kv_len, so that ragged
-// batches balance. Each warp takes every NW-th page of its CTA's share through
-// its own ring of whole-page bulk copies (8704 bytes, one mbarrier each); the
-// warps meet only when a (sequence, kv head, row tile) ends. One that lies
-// within a share is written at once, the others as partials (at most two a
-// CTA) which attn_kv4_combine_kernel joins.
+// equal shares, one a warp, planned on the device from kv_len, so that ragged
+// batches balance; every (sequence, kv head, row tile) counts UNIT_COST pages
+// more than it has, for its start and end. Warps never wait for one another:
+// each streams its share through its own ring of whole-page bulk copies (8704
+// bytes, one mbarrier each). A unit that lies within a share is written at
+// once, the others as partials (at most two a warp) which
+// attn_kv4_combine_kernel joins.
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
@@ -42,6 +43,7 @@ using namespace kv4;
 
 constexpr int NW = 4;  // warps per CTA
 constexpr int ST = 3;  // pages in a warp's ring
+constexpr int UNIT_COST = 2;  // pages that starting and ending a unit cost
 
 struct Args {
   const uint16_t* q;
@@ -50,9 +52,9 @@ struct Args {
   const int* kv_len;
   const int* start_pos;  // null: every key below kv_len is seen
   uint16_t* out;
-  float* part_o;   // [grid][2][cols][DH]
-  float* part_ml;  // [grid][2][cols][2]
-  int4* desc;      // [grid]: first slot, number of partials (0: none), b, unit
+  float* part_o;   // [warps][2][cols][DH]: unit began before this share, in it
+  float* part_ml;  // [warps][2][cols][2]
+  int* plan;       // [2 (B + 1)]: pre, vpre for the combine kernel
   uint32_t* status;
   int64_t ldq, ldo;  // elements between two positions' rows
   int num_pages, max_pages, B, S, Hkv, G, RT;
@@ -101,34 +103,54 @@ __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return max(0, min(a.kv_len[b], a.max_pages * PAGE));
 }
 
-// pre[b] = flat index of the first page of sequence b, pre[B] = their number.
-__device__ void plan(const Args& a, int* pre, int* wsum) {
+// pre[b] = flat index of the first page of sequence b, pre[B] = their number;
+// vpre the same with UNIT_COST more pages a unit.
+__device__ void plan(const Args& a, int* pre, int* vpre, int2* wsum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + NW * 32 - 1) / (NW * 32);
-  const int b0 = tid * per, b1 = min(a.B, b0 + per);
-  int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += (seq_len(a, b) + PAGE - 1) / PAGE;
-  sum *= a.Hkv * a.RT;
-  int inc = sum;
+  const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  const int units = a.Hkv * a.RT;
+  int2 sum = make_int2(0, 0);
+  for (int b = b0; b < b1; ++b) {
+    const int pages = (seq_len(a, b) + PAGE - 1) / PAGE;
+    sum.x += pages * units;
+    sum.y += pages ? (pages + UNIT_COST) * units : 0;
+  }
+  int2 inc = sum;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += y;
+    const int x = __shfl_up_sync(0xffffffffu, inc.x, off), y = __shfl_up_sync(0xffffffffu, inc.y, off);
+    if (lane >= off) inc.x += x, inc.y += y;
   }
   if (lane == 31) wsum[warp] = inc;
   __syncthreads();
-  int run = inc - sum;
-  for (int w = 0; w < warp; ++w) run += wsum[w];
+  int2 run = make_int2(inc.x - sum.x, inc.y - sum.y);
+  for (int w = 0; w < warp; ++w) run.x += wsum[w].x, run.y += wsum[w].y;
   for (int b = b0; b < b1; ++b) {
-    pre[b] = run;
-    run += (seq_len(a, b) + PAGE - 1) / PAGE * a.Hkv * a.RT;
+    pre[b] = run.x;
+    vpre[b] = run.y;
+    const int pages = (seq_len(a, b) + PAGE - 1) / PAGE;
+    run.x += pages * units;
+    run.y += pages ? (pages + UNIT_COST) * units : 0;
   }
   if (tid == NW * 32 - 1) {
-    int all = 0;
-    for (int w = 0; w < NW; ++w) all += wsum[w];
-    pre[a.B] = all;
+    pre[a.B] = run.x;  // the last thread's end is everybody's
+    vpre[a.B] = run.y;
   }
   __syncthreads();
+}
+
+// Pages whose place in the costed list lies before v.
+__device__ __forceinline__ int pages_before(const int* pre, const int* vpre, int B, int units, int v) {
+  if (v >= vpre[B]) return pre[B];
+  int lo = 0, hi = B;  // vpre[lo] <= v < vpre[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (vpre[mid] <= v) lo = mid; else hi = mid;
+  }
+  const int pages = (pre[lo + 1] - pre[lo]) / units;
+  const int rem = v - vpre[lo], unit = rem / (pages + UNIT_COST);
+  return pre[lo] + unit * pages + max(0, rem - unit * (pages + UNIT_COST) - UNIT_COST);
 }
 
 // Sequence of flat page f: pre[b] <= f < pre[b + 1].
@@ -164,10 +186,6 @@ struct State {
   }
 };
 
-// Floats of one warp's state in shared memory.
-template <int NT>
-constexpr int area_floats() { return NT * 38 * 32; }
-
 template <int NT>
 __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   mbd::pdl_trigger();
@@ -175,11 +193,11 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   constexpr int COLS = NT * 8;
   extern __shared__ __align__(128) uint8_t sm[];
   uint8_t* ring = sm + (threadIdx.x >> 5) * ST * BLOB;
-  float* area = reinterpret_cast<float*>(sm + NW * ST * BLOB);  // [NW/2][area_floats]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(area + (NW / 2) * area_floats<NT>());  // [NW][ST]
-  int* wsum = reinterpret_cast<int*>(bars + NW * ST);          // [NW]
-  int* page_ok = wsum + NW;                                    // [NW][ST]
-  int* pre = page_ok + NW * ST;                                // [B + 1]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + NW * ST * BLOB);  // [NW][ST]
+  int2* wsum = reinterpret_cast<int2*>(bars + NW * ST);               // [NW]
+  int* page_ok = reinterpret_cast<int*>(wsum + NW);                   // [NW][ST]
+  int* pre = page_ok + NW * ST;                                       // [B + 1]
+  int* vpre = pre + a.B + 1;                                          // [B + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   uint64_t* bar = bars + warp * ST;
@@ -187,7 +205,7 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   if (lane == 0)
     for (int i = 0; i < ST; ++i) mbd::mbar_init(bar + i, 1);
   mbd::fence_mbar_init();
-  plan(a, pre, wsum);
+  plan(a, pre, vpre, wsum);
 
   // sequences without keys: their rows are zeros
   const int row_elems = a.Hkv * a.G * DH;
@@ -197,20 +215,22 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
         for (int i = threadIdx.x * 8; i < row_elems; i += NW * 32 * 8)
           *reinterpret_cast<uint4*>(a.out + ((int64_t)b * a.S + s) * a.ldo + i) = make_uint4(0, 0, 0, 0);
 
-  const int total = pre[a.B];
-  const int per = (total + gridDim.x - 1) / gridDim.x;
-  const int begin = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
-  const int end = min(begin + per, total);
-  const int units = a.Hkv * a.RT;
-  if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < 2 * (a.B + 1); i += NW * 32) a.plan[i] = pre[i];
 
-  // ---- this warp's loads: pages begin + warp, + NW, ... ----
-  const int mine = end - begin > warp ? (end - begin - warp + NW - 1) / NW : 0;
+  const int units = a.Hkv * a.RT;
+  const int me = blockIdx.x * NW + warp;
+  const int per = (vpre[a.B] + gridDim.x * NW - 1) / (gridDim.x * NW);
+  const int begin = pages_before(pre, vpre, a.B, units, min((int64_t)me * per, (int64_t)vpre[a.B]));
+  const int end = pages_before(pre, vpre, a.B, units, min((int64_t)(me + 1) * per, (int64_t)vpre[a.B]));
+  const int mine = end - begin;
+
+  // ---- this warp's loads, page after page ----
   int issued = 0;
-  int win_pid = 0, win_ok = 0, win_kvh = 0;  // lane i: page (issued / 32) * 32 + i of this warp
+  int win_pid = 0, win_ok = 0, win_kvh = 0;  // lane i: page (issued / 32) * 32 + i of this share
   auto issue = [&]() {
     if ((issued & 31) == 0) {
-      const int f = begin + warp + NW * (issued + lane);
+      const int f = begin + issued + lane;
       if (f < end) {
         const int b = find_seq(pre, a.B, f);
         const int rem = f - pre[b], pages = (pre[b + 1] - pre[b]) / units;
@@ -242,7 +262,7 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   State<NT> z;
   int f0 = begin;
   while (f0 < end) {
-    // one segment: the pages of one (sequence, kv head, row tile) in this share
+    // one segment: the pages of one unit (sequence, kv head, row tile) in this share
     const int b = find_seq(pre, a.B, f0);
     const int pages = (pre[b + 1] - pre[b]) / units;
     const int unit = (f0 - pre[b]) / pages;
@@ -253,9 +273,7 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
     // row s sees the keys up to position first + s
     const int first = a.start_pos ? min(a.start_pos[b], L) : L;
     z.reset();
-
-    int f = begin + warp + NW * used;
-    if (f < f1) {
+    {
       // ---- q of this unit as B fragments ----
       uint32_t qf[NT][16];
       float cq[NT][2], qs[NT][2];
@@ -316,7 +334,7 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
       }
       const int all_seen = min(L, first + (rt * COLS) / a.G + 1);  // keys that every column sees
 
-      for (; f < f1; f += NW) {
+      for (int f = f0; f < f1; ++f) {
         const int st = used % ST;
         if (!dead) {
           dead = !mbd::mbar_wait(bar + st, (used / ST) & 1, a.status, MB_DEV_TIMEOUT_TMA);
@@ -462,7 +480,7 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
       }
     }
 
-    // ---- the warps' states of this segment, joined pairwise ----
+    // ---- the unit's rows, or its partial ----
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -472,56 +490,9 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
           z.l[t][c] += __shfl_xor_sync(0xffffffffu, z.l[t][c], off);
           z.om[t][c] += __shfl_xor_sync(0xffffffffu, z.om[t][c], off);
         }
-#pragma unroll
-    for (int half = NW / 2; half >= 1; half >>= 1) {
-      if (warp >= half && warp < 2 * half) {
-        float* dst = area + (warp - half) * area_floats<NT>() + lane;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            dst[(t * 38 + i) * 32] = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            dst[(t * 38 + 32 + c) * 32] = z.R[t][c];
-            dst[(t * 38 + 34 + c) * 32] = z.l[t][c];
-            dst[(t * 38 + 36 + c) * 32] = z.om[t][c];
-          }
-        }
-      }
-      __syncthreads();
-      if (warp < half) {
-        const float* src = area + warp * area_floats<NT>() + lane;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float fa[2], fb[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float Ro = src[(t * 38 + 32 + c) * 32];
-            const float Rn = fmaxf(z.R[t][c], Ro);
-            fa[c] = z.R[t][c] == -INFINITY ? 0.f : fast_exp2(z.R[t][c] - Rn);
-            fb[c] = Ro == -INFINITY ? 0.f : fast_exp2(Ro - Rn);
-            z.R[t][c] = Rn;
-            z.l[t][c] = z.l[t][c] * fa[c] + src[(t * 38 + 34 + c) * 32] * fb[c];
-            z.om[t][c] = z.om[t][c] * fa[c] + src[(t * 38 + 36 + c) * 32] * fb[c];
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float& o = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
-            o = o * fa[i & 1] + src[(t * 38 + i) * 32] * fb[i & 1];
-          }
-        }
-      }
-      __syncthreads();  // the areas are free again
-    }
-
-    if (warp == 0) {
+    {
       const bool whole = f0 == ub && f1 == ub + pages;
-      const int slot = 2 * blockIdx.x + (f0 == begin ? 0 : 1);
-      if (!whole && f0 == ub && lane == 0) {
-        const int last = (ub + pages - 1) / per;
-        a.desc[blockIdx.x] = make_int4(slot, last - blockIdx.x + 1, b, unit);
-      }
+      const int slot = 2 * me + (f0 == ub ? 1 : 0);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -564,30 +535,34 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
     for (int i = dead_at; i < issued; ++i) mbd::mbar_wait(bar + i % ST, (i / ST) & 1, nullptr, 0);
 }
 
-// Joins the partials of the units that start in main CTA blockIdx.x and end in
-// a later one: one warp a query row.
-template <int NT>
-__global__ void __launch_bounds__(NT * 8 * 32) attn_kv4_combine_kernel(const Args a) {
+// Joins the partials of the units that more than one warp worked on. A CTA is
+// one unit and COLS / gridDim.y of its query rows; its 8 warps take a row each
+// (many units: few partials each), or share one row's partials (few units).
+template <int NT, bool SPLIT>
+__global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a, int warps) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   constexpr int COLS = NT * 8;
-  const int4 d = a.desc[blockIdx.x];
-  if (d.y == 0) return;
-  const int col = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = d.w / a.RT, r = (d.w - kvh * a.RT) * COLS + col;
-  if (r >= a.S * a.G) return;
-  const int c0 = blockIdx.x;
-  auto row = [&](int i) -> int64_t {  // the i-th partial: this CTA's last, then the next ones' first
-    return (int64_t)(i == 0 ? d.x : 2 * (c0 + i)) * COLS + col;
-  };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = a.Hkv * a.RT;
+  const int b = blockIdx.x / units, unit = blockIdx.x - b * units;
+  const int col = SPLIT ? blockIdx.y : blockIdx.y * 8 + warp;
+  const int kvh = unit / a.RT, r = (unit - kvh * a.RT) * COLS + col;
+  const int pages = (a.plan[b + 1] - a.plan[b]) / units;
+  const int* vpre = a.plan + a.B + 1;
+  const int per = (vpre[a.B] + warps - 1) / warps;
+  const int v = vpre[b] + unit * (pages + UNIT_COST) + UNIT_COST;  // place of the first page
+  const int w0 = pages ? v / per : 0, n = pages ? (v + pages - 1) / per - w0 + 1 : 0;
+  if (n < 2 || r >= a.S * a.G) return;
+  auto row = [&](int i) -> int64_t { return (int64_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * COLS + col; };
   float M = -INFINITY;
-  for (int i = lane; i < d.y; i += 32) M = fmaxf(M, a.part_ml[row(i) * 2]);
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[row(i) * 2]);
 #pragma unroll
   for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   float L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < d.y; ++i) {
+#pragma unroll 8
+  for (int i = SPLIT ? warp : 0; i < n; i += SPLIT ? 8 : 1) {
     const int64_t at = row(i);
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
     const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * DH + lane * 4);
@@ -598,20 +573,33 @@ __global__ void __launch_bounds__(NT * 8 * 32) attn_kv4_combine_kernel(const Arg
     acc.z = fmaf(o.z, w, acc.z);
     acc.w = fmaf(o.w, w, acc.w);
   }
+  if (SPLIT) {
+    __shared__ float4 so[8][32];
+    __shared__ float sl[8];
+    so[warp][lane] = acc;
+    if (lane == 0) sl[warp] = L;
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      const float4 o = so[w][lane];
+      acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+      L += sl[w];
+    }
+  }
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
   const __nv_bfloat162 h0 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
   const __nv_bfloat162 h1 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
   const int s = r / a.G;
-  uint16_t* dst = a.out + ((int64_t)d.z * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
+  uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
   *reinterpret_cast<uint2*>(dst + lane * 4) =
       make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
 }
 
 constexpr int MAX_B = 4096;  // sequences a call: their page counts are planned in shared memory
 
-template <int NT>
 constexpr int smem_bytes(int B) {
-  return NW * ST * BLOB + (NW / 2) * area_floats<NT>() * 4 + NW * ST * 8 + (NW + NW * ST + B + 1) * 4;
+  return NW * ST * BLOB + NW * ST * 8 + NW * 8 + (NW * ST + 2 * (B + 1)) * 4;
 }
 
 // CTAs of one resident wave (with the shared memory of a batch of up to 64).
@@ -623,9 +611,9 @@ int resident_ctas() {
   if (dev < 0 || dev >= 64) dev = 0;
   if (!per_sm[dev]) {
     int nb = 0;
-    if (mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes<NT>(MAX_B)) ||
+    if (mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes(MAX_B)) ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&nb, attn_kv4_kernel<NT>, NW * 32,
-                                                      smem_bytes<NT>(64)) != cudaSuccess || nb < 1)
+                                                      smem_bytes(64)) != cudaSuccess || nb < 1)
       nb = 1;
     per_sm[dev] = nb;
   }
@@ -646,19 +634,25 @@ Plan make_plan(int B, int S, int Hq, int Hkv, int max_pages) {
   p.rt = (int)((rows + p.nt * 8 - 1) / (p.nt * 8));
   const int64_t most = (int64_t)B * Hkv * p.rt * max_pages;
   const int res = p.nt == 1 ? resident_ctas<1>() : resident_ctas<2>();
-  p.grid = (int)(most < res ? (most > 0 ? most : 1) : res);
-  p.bytes = (size_t)p.grid * (16 + 2 * p.nt * 8 * (DH + 2) * sizeof(float));
+  const int64_t ctas = (most * (1 + UNIT_COST) + NW - 1) / NW;
+  p.grid = (int)(ctas < res ? ctas : res);
+  p.bytes = ((size_t)2 * (B + 1) * sizeof(int) + 15) / 16 * 16 +
+            (size_t)p.grid * NW * 2 * p.nt * 8 * (DH + 2) * sizeof(float);
   return p;
 }
 
 template <int NT>
 int launch(const Args& a, int grid, cudaStream_t s) {
-  const int smem = smem_bytes<NT>(a.B);
-  int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes<NT>(MAX_B));
+  const int smem = smem_bytes(a.B);
+  int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes(MAX_B));
   if (rc) return rc;
   MB_CUDA(mb::launch_pdl(attn_kv4_kernel<NT>, dim3(grid), dim3(NW * 32), smem, s, a));
-  if (grid > 1)
-    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT>, dim3(grid), dim3(NT * 8 * 32), 0, s, a));
+  const int units = a.B * a.Hkv * a.RT;
+  // few units are many partials each: 8 warps to a row
+  if (units <= 2 * mb::num_sms())
+    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT, true>, dim3(units, NT * 8), dim3(256), 0, s, a, grid * NW));
+  else
+    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT, false>, dim3(units, NT), dim3(256), 0, s, a, grid * NW));
   return MB_OK;
 }
 
@@ -683,7 +677,7 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
   MB_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0,
              "attention kv4: q, out and the cache must be 16-byte aligned");
   const Plan p = make_plan(B, S, Hq, Hkv, max_pages);
-  MB_REQUIRE((int64_t)B * Hkv * p.rt * max_pages < (1ll << 30) && (int64_t)max_pages * PAGE < (1ll << 30),
+  MB_REQUIRE((int64_t)B * Hkv * p.rt * ((int64_t)max_pages + UNIT_COST) < (1ll << 30) && (int64_t)max_pages * PAGE < (1ll << 30),
              "attention kv4: too many pages");
   MB_REQUIRE(workspace && workspace_bytes >= p.bytes && (uintptr_t)workspace % 16 == 0,
              "attention kv4: workspace of %zu bytes required, 16-byte aligned", p.bytes);
@@ -696,9 +690,9 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
   a.kv_len = kv_len;
   a.start_pos = start_pos;
   a.out = out;
-  a.desc = static_cast<int4*>(workspace);
-  a.part_o = reinterpret_cast<float*>(a.desc + p.grid);
-  a.part_ml = a.part_o + (size_t)p.grid * 2 * p.nt * 8 * DH;
+  a.plan = static_cast<int*>(workspace);
+  a.part_o = reinterpret_cast<float*>(a.plan + (2 * (B + 1) + 3) / 4 * 4);
+  a.part_ml = a.part_o + (size_t)p.grid * NW * 2 * p.nt * 8 * DH;
   a.status = status;
   a.ldq = ldq;
   a.ldo = ldo;
