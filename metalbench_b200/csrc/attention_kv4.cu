@@ -12,7 +12,7 @@
 // multiplies exactly. Eight codes become four operand registers in five
 // logic operations; the powers of two are taken out of q (2^-4) and of the
 // sums. q is scaled by a power of two into fp16's range, which loses nothing
-// of a bf16 number down to 2^-22 of the row's largest.
+// of a bf16 number down to 2^-20 of the tile's largest.
 // The value scale goes into the exponent: P_j = 2^(score_j + log2(sv_j) - R)
 // with a running reference R per query row, so that P_j sv-weighted is what is
 // rounded to fp16 (11 bits, and 2^-24 absolute at a range up to 2^15), and the
@@ -42,7 +42,7 @@ namespace {
 using namespace kv4;
 
 constexpr int NW = 4;  // warps per CTA
-constexpr int ST = 3;  // pages in a warp's ring
+constexpr int ST = 2;  // pages in a warp's ring
 constexpr int UNIT_COST = 2;  // pages that starting and ending a unit cost
 
 struct Args {
@@ -98,7 +98,18 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return r;
 }
 
-// Attended pages of sequence b.
+__device__ __forceinline__ float fast_log2(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Attended keys of sequence b.
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return max(0, min(a.kv_len[b], a.max_pages * PAGE));
 }
@@ -163,11 +174,22 @@ __device__ __forceinline__ int find_seq(const int* pre, int B, int f) {
   return lo;
 }
 
-// A warp's running state over the pages of one unit: NT column tiles.
+// A key's numbers as the scores use them, worked out once a page by the lane
+// that owns the key and read by the four lanes that need it.
+struct __align__(16) KeyParams {
+  float sk, mk;  // key scale and minimum, with the softmax scale and q's power of two
+  float lg, rv;  // log2 and reciprocal of the value scale
+};
+
+// A warp's running state over the pages of one unit: NT column tiles of 8.
 template <int NT>
 struct State {
-  float o[NT][4][2][4];   // [32-dim piece][dim pair][accumulator]
+  float o[NT][4][2][4];  // [32-dim piece][dim pair][accumulator]
   float R[NT][2], l[NT][2], om[NT][2];
+  uint32_t qf[NT][16];   // q as B fragments
+  float qs[NT][2];       // sum of q's dims
+  int lim[NT][2];        // keys below lim are seen by column 2 tig + e
+
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -184,6 +206,142 @@ struct State {
       }
     }
   }
+
+  // One page (pg, in shared memory) of keys key0 .. key0 + 63. MASKED: some of
+  // them stand past the end (len) or are not seen by every column.
+  template <bool MASKED>
+  __device__ __forceinline__ void page(const uint8_t* pg, KeyParams* kp, float* vmin, int key0, int len,
+                                       float ck, float cm) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = lane + 32 * i;
+      uint32_t k = *reinterpret_cast<const uint32_t*>(pg + K_PARAMS + key * 4);
+      uint32_t v = *reinterpret_cast<const uint32_t*>(pg + V_PARAMS + key * 4);
+      if (MASKED && key0 + key >= len) k = v = 0;  // what stands past the end may be anything
+      // a value scale of 0 (all dims alike, codes 0) must not enter the logarithm
+      const float sv = lo_bf(v), s = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p90f);
+      const float r = fast_rcp(s);
+      kp[key] = KeyParams{lo_bf(k) * ck, hi_bf(k) * cm, fast_log2(s), r};
+      // a scale that is no number makes the row none (clamping would hide it)
+      vmin[key] = sv < INFINITY ? hi_bf(v) * r : NAN;
+    }
+    __syncwarp();
+
+    // ---- scores: log2 of the softmax terms times their value scales ----
+    float sc[NT][4][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[t][mt][e] = 0.f;
+      const uint4 ka = *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid) * ROW + tig * 16);
+      const uint4 kb = *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid + 8) * ROW + tig * 16);
+      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t ea[4], eb[4];
+        spread(wa[w], ea);
+        spread(wb[w], eb);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma_f16_16816(sc[t][mt], ea[0], eb[0], ea[1], eb[1], qf[t][4 * w], qf[t][4 * w + 1]);
+          mma_f16_16816(sc[t][mt], ea[2], eb[2], ea[3], eb[3], qf[t][4 * w + 2], qf[t][4 * w + 3]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int key = mt * 16 + gid + 8 * r;
+        const KeyParams p = kp[key];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = fmaf(p.mk, qs[t][c], fmaf(p.sk, sc[t][mt][2 * r + c], p.lg));
+            if (MASKED && key0 + key >= lim[t][c]) x = -INFINITY;
+            sc[t][mt][2 * r + c] = x;
+          }
+      }
+    }
+
+    // ---- reference ----
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float mx[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mx[c] = sc[t][0][c];
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) mx[c] = fmaxf(mx[c], fmaxf(sc[t][mt][c], sc[t][mt][2 + c]));
+      }
+      // a lane whose own maximum passes the reference calls for all to raise it
+      const bool raise = mx[0] > R[t][0] + 15.f || mx[1] > R[t][1] + 15.f;
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1)
+            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], off));
+          const float Rn = mx[c] > R[t][c] + 15.f ? mx[c] - 8.f : R[t][c];
+          const float f = R[t][c] == Rn ? 1.f : fast_exp2(R[t][c] - Rn);
+          R[t][c] = Rn;
+          l[t][c] *= f;
+          om[t][c] *= f;
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              o[t][p][h][c] *= f;
+              o[t][p][h][2 + c] *= f;
+            }
+        }
+      }
+    }
+
+    // ---- weights and O^T += V^T P^T, 16 keys at a time ----
+    const uint32_t pg_s = mbd::smem_u32(pg);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int key = mt * 16 + gid + 8 * r;
+        const float rv = kp[key].rv, mv = vmin[key];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float p[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            // R is -inf while a column has seen nothing
+            p[c] = fast_exp2(sc[t][mt][2 * r + c] - (MASKED && R[t][c] == -INFINITY ? 0.f : R[t][c]));
+            l[t][c] = fmaf(p[c], rv, l[t][c]);
+            om[t][c] = fmaf(p[c], mv, om[t][c]);
+          }
+          pf[t][r] = transpose8x8(pack_h2(p[0], p[1]));
+        }
+      }
+      const int key = mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+      const uint32_t rowp = pg_s + V_CODES + key * ROW;
+      const int sw = (key >> 1) & 3;
+#pragma unroll
+      for (int p = 0; p < 4; p += 2) {
+        uint32_t v[4];  // octets 0, 1 of piece p, then of piece p + 1
+        ldsm_x4_t(v, rowp + (((p + (lane >> 4)) ^ sw) << 4));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t e0[4], e1[4];
+          spread(v[2 * j], e0);
+          spread(v[2 * j + 1], e1);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            mma_f16_16816(o[t][p + j][0], e0[0], e0[1], e1[0], e1[1], pf[t][0], pf[t][1]);
+            mma_f16_16816(o[t][p + j][1], e0[2], e0[3], e1[2], e1[3], pf[t][0], pf[t][1]);
+          }
+        }
+      }
+    }
+  }
 };
 
 template <int NT>
@@ -193,7 +351,9 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   constexpr int COLS = NT * 8;
   extern __shared__ __align__(128) uint8_t sm[];
   uint8_t* ring = sm + (threadIdx.x >> 5) * ST * BLOB;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + NW * ST * BLOB);  // [NW][ST]
+  KeyParams* kp = reinterpret_cast<KeyParams*>(sm + NW * ST * BLOB) + (threadIdx.x >> 5) * PAGE;
+  float* vmin = reinterpret_cast<float*>(sm + NW * (ST * BLOB + PAGE * 16)) + (threadIdx.x >> 5) * PAGE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + NW * (ST * BLOB + PAGE * 20));  // [NW][ST]
   int2* wsum = reinterpret_cast<int2*>(bars + NW * ST);               // [NW]
   int* page_ok = reinterpret_cast<int*>(wsum + NW);                   // [NW][ST]
   int* pre = page_ok + NW * ST;                                       // [B + 1]
@@ -274,64 +434,58 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
     const int first = a.start_pos ? min(a.start_pos[b], L) : L;
     z.reset();
     {
-      // ---- q of this unit as B fragments ----
-      uint32_t qf[NT][16];
-      float cq[NT][2], qs[NT][2];
-      int lim[NT][2];  // keys below lim are seen by column 2 tig + e
+      // ---- q of this unit as B fragments, scaled by a power of two ----
+      float x[NT][32];
+      float big = 0.f;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int r = rt * COLS + t * 8 + gid;
-        const bool have = r < a.S * a.G;
         const int s = r / a.G;
-        float x[32];
-        if (have) {
+        if (r < a.S * a.G) {
           const uint4* p = reinterpret_cast<const uint4*>(
               a.q + ((int64_t)b * a.S + s) * a.ldq + (kvh * a.G + (r - s * a.G)) * DH + 32 * tig);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint4 w = p[i];
-            x[8 * i] = lo_bf(w.x), x[8 * i + 1] = hi_bf(w.x), x[8 * i + 2] = lo_bf(w.y);
-            x[8 * i + 3] = hi_bf(w.y), x[8 * i + 4] = lo_bf(w.z), x[8 * i + 5] = hi_bf(w.z);
-            x[8 * i + 6] = lo_bf(w.w), x[8 * i + 7] = hi_bf(w.w);
+            x[t][8 * i] = lo_bf(w.x), x[t][8 * i + 1] = hi_bf(w.x), x[t][8 * i + 2] = lo_bf(w.y);
+            x[t][8 * i + 3] = hi_bf(w.y), x[t][8 * i + 4] = lo_bf(w.z), x[t][8 * i + 5] = hi_bf(w.z);
+            x[t][8 * i + 6] = lo_bf(w.w), x[t][8 * i + 7] = hi_bf(w.w);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = 0.f;
+          for (int i = 0; i < 32; ++i) x[t][i] = 0.f;
         }
-        float mx = 0.f, sum = 0.f;
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          mx = fmaxf(mx, fabsf(x[i]));
-          sum += x[i];
+          big = fmaxf(big, fabsf(x[t][i]));
+          sum += x[t][i];
         }
 #pragma unroll
-        for (int off = 1; off <= 2; off <<= 1) {
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-          sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        }
-        // 2^e brings the row's largest to [2^11, 2^12)
-        int e = 11 - ((int)(__float_as_uint(mx) >> 23) - 127);
-        e = max(-100, min(100, e));
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        const float up16 = up * 0.0625f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          qf[t][4 * w] = pack_h2(x[8 * w] * up, x[8 * w + 4] * up);
-          qf[t][4 * w + 1] = pack_h2(x[8 * w + 1] * up16, x[8 * w + 5] * up16);
-          qf[t][4 * w + 2] = pack_h2(x[8 * w + 2] * up, x[8 * w + 6] * up);
-          qf[t][4 * w + 3] = pack_h2(x[8 * w + 3] * up16, x[8 * w + 7] * up16);
-        }
-        const float down = a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - max(e, -100)) << 23);
-        const float sq = a.scale_log2 * sum;
+        for (int off = 1; off <= 2; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const int mylim = min(L, first + s + 1);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int from = (2 * tig + c) * 4;  // a lane whose fragment row is column 2 tig + c
-          cq[t][c] = __shfl_sync(0xffffffffu, down, from);
-          qs[t][c] = __shfl_sync(0xffffffffu, sq, from);
-          lim[t][c] = __shfl_sync(0xffffffffu, mylim, from);
+          z.qs[t][c] = __shfl_sync(0xffffffffu, sum, from);
+          z.lim[t][c] = __shfl_sync(0xffffffffu, mylim, from);
         }
       }
+#pragma unroll
+      for (int off = 1; off <= 16; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+      // 2^e brings the tile's largest to [2^11, 2^12)
+      const int e = max(-100, min(100, 11 - ((int)(__float_as_uint(big) >> 23) - 127)));
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23), up16 = up * 0.0625f;
+      const float ck = a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          z.qf[t][4 * w] = pack_h2(x[t][8 * w] * up, x[t][8 * w + 4] * up);
+          z.qf[t][4 * w + 1] = pack_h2(x[t][8 * w + 1] * up16, x[t][8 * w + 5] * up16);
+          z.qf[t][4 * w + 2] = pack_h2(x[t][8 * w + 2] * up, x[t][8 * w + 6] * up);
+          z.qf[t][4 * w + 3] = pack_h2(x[t][8 * w + 3] * up16, x[t][8 * w + 7] * up16);
+        }
       const int all_seen = min(L, first + (rt * COLS) / a.G + 1);  // keys that every column sees
 
       for (int f = f0; f < f1; ++f) {
@@ -342,137 +496,11 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
           dead_at = used;
         }
         if (!dead && ok_flag[st]) {
-          const uint8_t* pg = ring + st * BLOB;
-          const uint32_t pg_s = mbd::smem_u32(pg);
           const int key0 = (f - ub) * PAGE;
-          const bool masked = key0 + PAGE > all_seen;
-          // ---- scores of 64 keys: t = log2 of the value-weighted softmax term ----
-          float sc[NT][4][4];
-          float rv[4][2], mv[4][2];  // 1 / sv and mv / sv of keys 16 mt + gid (+ 8)
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[t][mt][e] = 0.f;
-            const uint4 ka = *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid) * ROW + tig * 16);
-            const uint4 kb =
-                *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid + 8) * ROW + tig * 16);
-            const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t ea[4], eb[4];
-              spread(wa[w], ea);
-              spread(wb[w], eb);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                mma_f16_16816(sc[t][mt], ea[0], eb[0], ea[1], eb[1], qf[t][4 * w], qf[t][4 * w + 1]);
-                mma_f16_16816(sc[t][mt], ea[2], eb[2], ea[3], eb[3], qf[t][4 * w + 2],
-                              qf[t][4 * w + 3]);
-              }
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int t0 = mt * 16 + gid + 8 * r;
-              const uint32_t kp = *reinterpret_cast<const uint32_t*>(pg + K_PARAMS + t0 * 4);
-              uint32_t vp = *reinterpret_cast<const uint32_t*>(pg + V_PARAMS + t0 * 4);
-              if (masked && key0 + t0 >= L) vp = 0;  // what stands past the end may be anything
-              const float sv = lo_bf(vp);
-              // scale 0 (all dims alike, codes 0) must not enter the logarithm
-              const float svc = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p90f);
-              const float lg = __log2f(svc);
-              rv[mt][r] = __frcp_rn(svc);
-              mv[mt][r] = hi_bf(vp) * rv[mt][r];
-              const float sk = lo_bf(kp), mk = hi_bf(kp);
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  float x = fmaf(mk, qs[t][c], fmaf(sk, sc[t][mt][2 * r + c] * cq[t][c], lg));
-                  if (masked && key0 + t0 >= lim[t][c]) x = -INFINITY;
-                  sc[t][mt][2 * r + c] = x;
-                }
-            }
-          }
-          // ---- reference, weights ----
-          uint32_t pf[NT][4][2];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float mx[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              mx[c] = sc[t][0][c];
-#pragma unroll
-              for (int mt = 0; mt < 4; ++mt) {
-                mx[c] = fmaxf(mx[c], sc[t][mt][c]);
-                mx[c] = fmaxf(mx[c], sc[t][mt][2 + c]);
-              }
-#pragma unroll
-              for (int off = 4; off <= 16; off <<= 1)
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], off));
-            }
-            const bool raise = mx[0] > z.R[t][0] + 15.f || mx[1] > z.R[t][1] + 15.f;
-            if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float Rn = mx[c] > z.R[t][c] + 15.f ? mx[c] - 8.f : z.R[t][c];
-                const float f = z.R[t][c] == Rn ? 1.f : fast_exp2(z.R[t][c] - Rn);
-                z.R[t][c] = Rn;
-                z.l[t][c] *= f;
-                z.om[t][c] *= f;
-#pragma unroll
-                for (int p = 0; p < 4; ++p)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    z.o[t][p][h][c] *= f;
-                    z.o[t][p][h][2 + c] *= f;
-                  }
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float R = z.R[t][c] == -INFINITY ? 0.f : z.R[t][c];  // nothing seen so far
-#pragma unroll
-              for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  const float p = fast_exp2(sc[t][mt][2 * r + c] - R);
-                  sc[t][mt][2 * r + c] = p;
-                  z.l[t][c] = fmaf(p, rv[mt][r], z.l[t][c]);
-                  z.om[t][c] = fmaf(p, mv[mt][r], z.om[t][c]);
-                }
-            }
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-              pf[t][mt][0] = transpose8x8(pack_h2(sc[t][mt][0], sc[t][mt][1]));
-              pf[t][mt][1] = transpose8x8(pack_h2(sc[t][mt][2], sc[t][mt][3]));
-            }
-          }
-          // ---- O^T += V^T P^T ----
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-            const int key = mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-            const uint32_t rowp = pg_s + V_CODES + key * ROW;
-            const int sw = (key >> 1) & 3;
-#pragma unroll
-            for (int p = 0; p < 4; p += 2) {
-              uint32_t v[4];  // octets 0, 1 of piece p, then of piece p + 1
-              ldsm_x4_t(v, rowp + (((p + (lane >> 4)) ^ sw) << 4));
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                uint32_t e0[4], e1[4];
-                spread(v[2 * j], e0);
-                spread(v[2 * j + 1], e1);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                  mma_f16_16816(z.o[t][p + j][0], e0[0], e0[1], e1[0], e1[1], pf[t][mt][0],
-                                pf[t][mt][1]);
-                  mma_f16_16816(z.o[t][p + j][1], e0[2], e0[3], e1[2], e1[3], pf[t][mt][0],
-                                pf[t][mt][1]);
-                }
-              }
-            }
-          }
+          if (key0 + PAGE <= all_seen)
+            z.template page<false>(ring + st * BLOB, kp, vmin, key0, L, ck, a.scale_log2);
+          else
+            z.template page<true>(ring + st * BLOB, kp, vmin, key0, L, ck, a.scale_log2);
         }
         __syncwarp();  // all lanes are done with this page
         ++used;
@@ -599,7 +627,7 @@ __global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a, int
 constexpr int MAX_B = 4096;  // sequences a call: their page counts are planned in shared memory
 
 constexpr int smem_bytes(int B) {
-  return NW * ST * BLOB + NW * ST * 8 + NW * 8 + (NW * ST + 2 * (B + 1)) * 4;
+  return NW * (ST * BLOB + PAGE * 20) + NW * ST * 8 + NW * 8 + (NW * ST + 2 * (B + 1)) * 4;
 }
 
 // CTAs of one resident wave (with the shared memory of a batch of up to 64).
