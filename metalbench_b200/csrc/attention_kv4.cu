@@ -27,12 +27,13 @@
 //
 // Schedule: the flat list of (sequence, kv head, row tile, page) is cut into
 // equal shares, one a warp, planned on the device from kv_len, so that ragged
-// batches balance; every (sequence, kv head, row tile) counts UNIT_COST pages
-// more than it has, for its start and end. Warps never wait for one another:
-// each streams its share through its own ring of whole-page bulk copies (8704
-// bytes, one mbarrier each). A unit that lies within a share is written at
-// once, the others as partials (at most two a warp) which
-// attn_kv4_combine_kernel joins.
+// batches balance; every (sequence, kv head, row tile), a unit, counts
+// UNIT_COST pages more than it has, for its start and end. Each warp streams
+// its share through its own ring of whole-page bulk copies (8704 bytes, one
+// mbarrier each) without waiting for another. A unit that lies within a share
+// is written at once. At the end the warps of a CTA that stopped in the same
+// unit join their states in shared memory; what is then still in parts (at
+// most two a warp) goes to the workspace, and attn_kv4_combine_kernel joins it.
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
@@ -63,8 +64,7 @@ struct Args {
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                               uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -72,8 +72,7 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
 __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -231,25 +230,44 @@ struct State {
     // ---- scores: log2 of the softmax terms times their value scales ----
     float sc[NT][4][4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[t][mt][e] = 0.f;
-      const uint4 ka = *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid) * ROW + tig * 16);
-      const uint4 kb = *reinterpret_cast<const uint4*>(pg + (mt * 16 + gid + 8) * ROW + tig * 16);
-      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+    // KI key tiles side by side: their accumulators are independent, which
+    // hides the latency of the eight products that follow one another in each
+    constexpr int KI = 2;
+#pragma unroll
+    for (int m0 = 0; m0 < 4; m0 += KI) {
+      uint32_t wd[KI][2][4];
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint4 k = *reinterpret_cast<const uint4*>(pg + ((m0 + i) * 16 + gid + 8 * r) * ROW + tig * 16);
+          wd[i][r][0] = k.x, wd[i][r][1] = k.y, wd[i][r][2] = k.z, wd[i][r][3] = k.w;
+        }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        uint32_t ea[4], eb[4];
-        spread(wa[w], ea);
-        spread(wb[w], eb);
+        uint32_t ea[KI][4], eb[KI][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          mma_f16_16816(sc[t][mt], ea[0], eb[0], ea[1], eb[1], qf[t][4 * w], qf[t][4 * w + 1]);
-          mma_f16_16816(sc[t][mt], ea[2], eb[2], ea[3], eb[3], qf[t][4 * w + 2], qf[t][4 * w + 3]);
+        for (int i = 0; i < KI; ++i) {
+          spread(wd[i][0][w], ea[i]);
+          spread(wd[i][1][w], eb[i]);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < KI; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              mma_f16_16816(sc[t][m0 + i], ea[i][2 * h], eb[i][2 * h], ea[i][2 * h + 1], eb[i][2 * h + 1],
+                            qf[t][4 * w + 2 * h], qf[t][4 * w + 2 * h + 1]);
       }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = mt * 16 + gid + 8 * r;
@@ -355,7 +373,8 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   float* vmin = reinterpret_cast<float*>(sm + NW * (ST * BLOB + PAGE * 16)) + (threadIdx.x >> 5) * PAGE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + NW * (ST * BLOB + PAGE * 20));  // [NW][ST]
   int2* wsum = reinterpret_cast<int2*>(bars + NW * ST);               // [NW]
-  int* page_ok = reinterpret_cast<int*>(wsum + NW);                   // [NW][ST]
+  int4* seg = reinterpret_cast<int4*>(wsum + NW);                     // [NW]
+  int* page_ok = reinterpret_cast<int*>(seg + NW);                    // [NW][ST]
   int* pre = page_ok + NW * ST;                                       // [B + 1]
   int* vpre = pre + a.B + 1;                                          // [B + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -420,13 +439,51 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   int dead_at = 0;
 
   State<NT> z;
-  int f0 = begin;
+  // The state as finished rows (whole), or as the partial of a slot.
+  auto emit = [&](int b, int unit, int slot, bool whole) {
+    const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = t * 8 + 2 * tig + c;
+        const int r = rt * COLS + col;
+        if (r >= a.S * a.G) continue;
+        const float inv = z.l[t][c] > 0.f || z.l[t][c] != z.l[t][c] ? 1.f / z.l[t][c] : 0.f;
+        const float om = z.om[t][c];
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)  // dim 32 (i / 4) + 4 gid + i % 4
+          v[i] = fmaf(z.o[t][i >> 2][(i >> 1) & 1][2 * (i & 1) + c], (i & 1) ? 0x1p20f : 0x1p24f, om);
+        if (whole) {
+          const int s = r / a.G;
+          uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const __nv_bfloat162 h0 = __floats2bfloat162_rn(v[4 * p] * inv, v[4 * p + 1] * inv);
+            const __nv_bfloat162 h1 = __floats2bfloat162_rn(v[4 * p + 2] * inv, v[4 * p + 3] * inv);
+            *reinterpret_cast<uint2*>(dst + 32 * p + 4 * gid) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+          }
+        } else {
+          float* po = a.part_o + ((int64_t)slot * COLS + col) * DH;
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            *reinterpret_cast<float4*>(po + 32 * p + 4 * gid) =
+                make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+          if (gid == 0)
+            *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * COLS + col) * 2) =
+                make_float2(z.R[t][c], z.l[t][c]);
+        }
+      }
+  };
+  int f0 = begin, ub = -1, b = 0, unit = 0, pages = 0;
   while (f0 < end) {
     // one segment: the pages of one unit (sequence, kv head, row tile) in this share
-    const int b = find_seq(pre, a.B, f0);
-    const int pages = (pre[b + 1] - pre[b]) / units;
-    const int unit = (f0 - pre[b]) / pages;
-    const int ub = pre[b] + unit * pages;  // flat index of the unit's first page
+    b = find_seq(pre, a.B, f0);
+    pages = (pre[b + 1] - pre[b]) / units;
+    unit = (f0 - pre[b]) / pages;
+    ub = pre[b] + unit * pages;  // flat index of the unit's first page
     const int f1 = min(end, ub + pages);
     const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
     const int L = seq_len(a, b);
@@ -508,7 +565,6 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
       }
     }
 
-    // ---- the unit's rows, or its partial ----
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -518,49 +574,59 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
           z.l[t][c] += __shfl_xor_sync(0xffffffffu, z.l[t][c], off);
           z.om[t][c] += __shfl_xor_sync(0xffffffffu, z.om[t][c], off);
         }
-    {
-      const bool whole = f0 == ub && f1 == ub + pages;
-      const int slot = 2 * me + (f0 == ub ? 1 : 0);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = t * 8 + 2 * tig + c;
-          const int r = rt * COLS + col;
-          if (r >= a.S * a.G) continue;
-          const float inv = z.l[t][c] > 0.f || z.l[t][c] != z.l[t][c] ? 1.f / z.l[t][c] : 0.f;
-          const float om = z.om[t][c];
-          float v[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i)  // dim 32 (i / 4) + 4 gid + i % 4
-            v[i] = fmaf(z.o[t][i >> 2][(i >> 1) & 1][2 * (i & 1) + c], (i & 1) ? 0x1p20f : 0x1p24f, om);
-          if (whole) {
-            const int s = r / a.G;
-            uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              const __nv_bfloat162 h0 = __floats2bfloat162_rn(v[4 * p] * inv, v[4 * p + 1] * inv);
-              const __nv_bfloat162 h1 = __floats2bfloat162_rn(v[4 * p + 2] * inv, v[4 * p + 3] * inv);
-              *reinterpret_cast<uint2*>(dst + 32 * p + 4 * gid) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
-            }
-          } else {
-            float* po = a.part_o + ((int64_t)slot * COLS + col) * DH;
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-              *reinterpret_cast<float4*>(po + 32 * p + 4 * gid) =
-                  make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
-            if (gid == 0)
-              *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * COLS + col) * 2) =
-                  make_float2(z.R[t][c], z.l[t][c]);
-          }
-        }
-    }
+    if (f1 == end) break;  // the last one may go on in the next warp
+    emit(b, unit, 2 * me, f0 == ub);
     f0 = f1;
   }
   // A warp that gave up leaves copies in flight: wait (bounded) for them.
   if (dead)
     for (int i = dead_at; i < issued; ++i) mbd::mbar_wait(bar + i % ST, (i / ST) & 1, nullptr, 0);
+
+  // ---- neighbouring warps whose last unit is the same join their states ----
+  if (lane == 0) seg[warp] = make_int4(ub, f0, end, 0);
+  __syncthreads();  // every ring is free: a warp's state takes the place of its pages
+  const bool leads = ub >= 0 && (warp == 0 || seg[warp - 1].x != ub);
+  if (ub >= 0 && !leads) {
+    float* dst = reinterpret_cast<float*>(ring) + lane;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dst[(t * 38 + i) * 32] = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        dst[(t * 38 + 32 + c) * 32] = z.R[t][c];
+        dst[(t * 38 + 34 + c) * 32] = z.l[t][c];
+        dst[(t * 38 + 36 + c) * 32] = z.om[t][c];
+      }
+    }
+  }
+  __syncthreads();
+  if (!leads) return;
+  int f1 = end;
+  for (int w = warp + 1; w < NW && seg[w].x == ub; ++w) {
+    f1 = seg[w].z;
+    const float* src = reinterpret_cast<const float*>(ring + (w - warp) * ST * BLOB) + lane;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float fa[2], fb[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float Ro = src[(t * 38 + 32 + c) * 32];
+        const float Rn = fmaxf(z.R[t][c], Ro);
+        fa[c] = z.R[t][c] == -INFINITY ? 0.f : fast_exp2(z.R[t][c] - Rn);
+        fb[c] = Ro == -INFINITY ? 0.f : fast_exp2(Ro - Rn);
+        z.R[t][c] = Rn;
+        z.l[t][c] = z.l[t][c] * fa[c] + src[(t * 38 + 34 + c) * 32] * fb[c];
+        z.om[t][c] = z.om[t][c] * fa[c] + src[(t * 38 + 36 + c) * 32] * fb[c];
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float& o = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
+        o = o * fa[i & 1] + src[(t * 38 + i) * 32] * fb[i & 1];
+      }
+    }
+  }
+  emit(b, unit, 2 * me + (f0 == ub ? 1 : 0), f0 == ub && f1 == ub + pages);
 }
 
 // Joins the partials of the units that more than one warp worked on. A CTA is
@@ -580,9 +646,17 @@ __global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a, int
   const int* vpre = a.plan + a.B + 1;
   const int per = (vpre[a.B] + warps - 1) / warps;
   const int v = vpre[b] + unit * (pages + UNIT_COST) + UNIT_COST;  // place of the first page
-  const int w0 = pages ? v / per : 0, n = pages ? (v + pages - 1) / per - w0 + 1 : 0;
-  if (n < 2 || r >= a.S * a.G) return;
-  auto row = [&](int i) -> int64_t { return (int64_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * COLS + col; };
+  if (pages == 0 || r >= a.S * a.G) return;
+  const int w0 = v / per, w1 = (v + pages - 1) / per, c0 = w0 / NW, c1 = w1 / NW;
+  // w1's share ends with this unit: then it joined its CTA's other warps on it
+  const bool ends = v + pages == vpre[a.B] || v + pages + UNIT_COST >= (int64_t)(w1 + 1) * per;
+  const int joined = c1 - c0 + (ends || w1 > max(w0, c1 * NW) ? 1 : 0);
+  const int n = joined + (ends ? 0 : 1);
+  if (n < 2) return;  // written by the main kernel
+  auto row = [&](int i) -> int64_t {
+    const int w = i < joined ? max(w0, (c0 + i) * NW) : w1;
+    return (int64_t)(2 * w + (w == w0 ? 1 : 0)) * COLS + col;
+  };
   float M = -INFINITY;
   for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[row(i) * 2]);
 #pragma unroll
@@ -627,7 +701,7 @@ __global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a, int
 constexpr int MAX_B = 4096;  // sequences a call: their page counts are planned in shared memory
 
 constexpr int smem_bytes(int B) {
-  return NW * (ST * BLOB + PAGE * 20) + NW * ST * 8 + NW * 8 + (NW * ST + 2 * (B + 1)) * 4;
+  return NW * (ST * BLOB + PAGE * 20) + NW * ST * 8 + NW * 24 + (NW * ST + 2 * (B + 1)) * 4;
 }
 
 // CTAs of one resident wave (with the shared memory of a batch of up to 64).

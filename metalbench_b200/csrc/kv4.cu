@@ -135,28 +135,27 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(
 
 extern "C" size_t mb_kv4_page_bytes(int Hkv) { return Hkv > 0 ? (size_t)Hkv * kv4::BLOB : 0; }
 
-extern "C" int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, const int64_t* k_strides,
-                                  const int64_t* v_strides, uint8_t* cache, int num_pages, int Hkv,
+extern "C" int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, int64_t k_batch,
+                                  int64_t k_token, int64_t k_head, int64_t v_batch, int64_t v_token,
+                                  int64_t v_head, uint8_t* cache, int num_pages, int Hkv,
                                   const int* block_table, int max_pages, const int* start_pos,
                                   const int* new_len, int B, int S, void* stream) {
   MB_REQUIRE(B >= 0 && S >= 0 && Hkv > 0 && num_pages >= 0 && max_pages >= 0,
              "kv4 append: bad sizes");
   if (B == 0 || S == 0) return MB_OK;
-  MB_REQUIRE(k && v && k_strides && v_strides && cache && block_table && start_pos,
+  MB_REQUIRE(k && v && cache && block_table && start_pos,
              "kv4 append: null pointer");
   MB_REQUIRE(((uintptr_t)k | (uintptr_t)v | (uintptr_t)cache) % 16 == 0,
              "kv4 append: k, v and the cache must be 16-byte aligned");
-  for (int i = 0; i < 3; ++i)
-    MB_REQUIRE(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0,
-               "kv4 append: strides must be multiples of 8 elements");
+  MB_REQUIRE((k_batch | k_token | k_head | v_batch | v_token | v_head) % 8 == 0,
+             "kv4 append: strides must be multiples of 8 elements");
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "kv4 append: no status word");
   const int64_t total = (int64_t)B * S * Hkv;
   MB_REQUIRE((total + 7) / 8 <= 0x7fffffff, "kv4 append: too many tokens");
   MB_CUDA(mb::launch_pdl(kv4_append_kernel, dim3((unsigned)((total + 7) / 8)), dim3(256), 0,
-                         static_cast<cudaStream_t>(stream), k, v, k_strides[0], k_strides[1],
-                         k_strides[2], v_strides[0], v_strides[1], v_strides[2], cache, num_pages,
-                         Hkv, block_table, max_pages, start_pos, new_len, total, S, status));
+                         static_cast<cudaStream_t>(stream), k, v, k_batch, k_token, k_head,
+                         v_batch, v_token, v_head, cache, num_pages, Hkv, block_table, max_pages, start_pos, new_len, total, S, status));
   return MB_OK;
 }
 

@@ -21,57 +21,67 @@ HEAD_DIM = 128
 PAGE_HEAD_BYTES = 8704  # one page of one kv head: codes and scales of 64 keys and values
 
 
-def _i32(t: torch.Tensor, name: str, device, shape) -> int:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
-        raise TypeError(f"{name}: expected an int32 tensor")
-    if t.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor of shape {shape}, got {tuple(t.shape)}")
+_I32, _BF16 = torch.int32, torch.bfloat16
+
+
+def _refuse(t, name: str, dtype, dev: int, shape) -> None:
+    """Say what is wrong with a tensor that did not pass a call's check."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype {t.dtype} is not {dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor (no CPU fallback)")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: expected a tensor on cuda:{dev}, got one on {t.device}")
+    raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got "
+                     f"{tuple(t.shape)} with strides {t.stride()}")
+
+
+def _rows(t: torch.Tensor, name: str, dev: int, n: int) -> int:
+    """Address of a contiguous int32 [n] on device `dev`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32 or t.get_device() != dev or t.shape != (n,) \
+            or not t.is_contiguous():
+        _refuse(t, name, _I32, dev, (n,))
     return t.data_ptr()
 
 
-def _table(block_table: torch.Tensor, name: str, device) -> tuple[int, int]:
-    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
-        raise ValueError(f"{name}: block_table must be [B, max_pages]")
-    B, M = block_table.shape
-    _i32(block_table, f"{name}(block_table)", device, (B, M))
-    if M == 0:
-        raise ValueError(f"{name}: block_table has no columns")
-    return B, M
+def _table(t: torch.Tensor, name: str, dev: int):
+    """B, max_pages and address of a block table on device `dev`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32 or t.get_device() != dev or t.dim() != 2 \
+            or not t.is_contiguous() or t.shape[1] == 0:
+        _refuse(t, name, _I32, dev, ("B", "max_pages >= 1"))
+    B, M = t.shape
+    return B, M, t.data_ptr()
 
 
-def _cache(cache: torch.Tensor, name: str) -> tuple[int, int]:
-    if not isinstance(cache, torch.Tensor) or not cache.is_cuda:
-        raise ValueError(f"{name}: expected a CUDA tensor (no CPU fallback)")
-    if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[2] != PAGE_HEAD_BYTES \
-            or not cache.is_contiguous() or cache.data_ptr() % 16:
-        raise ValueError(f"{name}: the cache must be a contiguous, 16-byte aligned uint8 tensor "
-                         f"[num_pages, n_kv_heads, {PAGE_HEAD_BYTES}]")
-    if cache.shape[0] == 0 or cache.shape[1] == 0:
-        raise ValueError(f"{name}: the cache has no pages or no heads")
-    return cache.shape[0], cache.shape[1]
+def _cache(t: torch.Tensor, name: str):
+    """num_pages, heads, device and address of a 4-bit cache."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8 or not t.is_cuda or t.dim() != 3 \
+            or t.shape[2] != PAGE_HEAD_BYTES or not t.is_contiguous() or t.numel() == 0 or t.data_ptr() % 16:
+        _refuse(t, f"{name}(cache)", torch.uint8, t.get_device() if isinstance(t, torch.Tensor) else 0,
+                ("num_pages", "n_kv_heads", PAGE_HEAD_BYTES))
+    P, H, _ = t.shape
+    return P, H, t.get_device(), t.data_ptr()
 
 
-def _on_device(fn):
-    """Run on the device of the first argument (a tensor, or a list of tensors
-    and then the block table) when that is not the current one."""
-    def call(*args, **kw):
-        t = args[0] if args else None
-        if isinstance(t, (list, tuple)):
-            t = args[1] if len(args) > 1 else None
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
-                return fn(*args, **kw)
-        return fn(*args, **kw)
-    call.__name__, call.__doc__, call.__wrapped__ = fn.__name__, fn.__doc__, fn
-    return call
+def _stream(dev: int) -> int:
+    """torch's current stream on the current device `dev`; libmb200 set up there."""
+    if dev not in _ready:
+        from . import ops
+        ops.init(dev)
+        _ready.add(dev)
+    return _raw_stream(dev)
 
 
-def _start(device) -> int:
-    from . import ops
-    ops.init(device.index)
-    return torch.cuda.current_stream().cuda_stream
+_ready: set[int] = set()
+# the public accessor builds a Stream object first, which takes longer than a small launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _fn(name: str):
+    return getattr(_lib.lib(), name)
 
 
 def kv4_cache(num_pages: int, n_kv_heads: int, device=None) -> torch.Tensor:
@@ -82,17 +92,26 @@ def kv4_cache(num_pages: int, n_kv_heads: int, device=None) -> torch.Tensor:
     return torch.zeros((num_pages, n_kv_heads, PAGE_HEAD_BYTES), dtype=torch.uint8, device=device)
 
 
-def _strides(t: torch.Tensor, name: str):
-    B, S, H, D = t.shape
-    if t.stride(3) != 1 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: the head dim must be contiguous and 16-byte aligned")
-    st = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], (B, S, H))]
-    if any(s % 8 for s in st):
-        raise ValueError(f"{name}: strides must be multiples of 8 elements, got {t.stride()}")
-    return (C.c_int64 * 3)(*st)
+def _token_strides(t: torch.Tensor, name: str, dev: int, B: int, H: int):
+    """Batch, token and head strides (elements) of bf16 [B, S, H, 128]."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.get_device() != dev or t.dim() != 4:
+        _refuse(t, name, _BF16, dev, (B, "S", H, HEAD_DIM))
+    b, S, h, D = t.shape
+    if b != B or h != H or D != HEAD_DIM:
+        _refuse(t, name, _BF16, dev, (B, "S", H, HEAD_DIM))
+    sb, ss, sh, sd = t.stride()
+    if B == 1:
+        sb = 0  # a stride that is never taken may be anything
+    if S == 1:
+        ss = 0
+    if H == 1:
+        sh = 0
+    if sd != 1 or (sb | ss | sh) % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: the head dim must be contiguous and 16-byte aligned, the other strides "
+                         f"multiples of 8 elements; got strides {t.stride()}")
+    return sb, ss, sh
 
 
-@_on_device
 def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                start_pos: torch.Tensor, new_len: torch.Tensor | None = None) -> None:
     """Store the (already rotated) keys and values of S new tokens a sequence.
@@ -101,47 +120,68 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_tabl
     fused projection's rows are fine); token s < new_len[b] (default: all S)
     goes to position start_pos[b] + s of sequence b. Other slots of the cache
     stay as they are."""
-    P, H = _cache(cache, "kv4_append")
-    B, M = _table(block_table, "kv4_append", cache.device)
-    for n, t in (("k", k), ("v", v)):
-        if not t.is_cuda or t.device != cache.device:
-            raise ValueError(f"kv4_append({n}): expected a tensor on {cache.device}")
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"kv4_append({n}): dtype {t.dtype} is not bfloat16")
-        if t.dim() != 4 or t.shape[0] != B or t.shape[2] != H or t.shape[3] != HEAD_DIM:
-            raise ValueError(f"kv4_append({n}): expected [{B}, S, {H}, {HEAD_DIM}], got {tuple(t.shape)}")
+    P, H, dev, cp = _cache(cache, "kv4_append")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv4_append(k, v, cache, block_table, start_pos, new_len)
+    B, M, tp = _table(block_table, "kv4_append(block_table)", dev)
+    ks = _token_strides(k, "kv4_append(k)", dev, B, H)
+    vs = _token_strides(v, "kv4_append(v)", dev, B, H)
     if k.shape != v.shape:
         raise ValueError("kv4_append: k and v shapes differ")
-    sp = _i32(start_pos, "kv4_append(start_pos)", cache.device, (B,))
-    nl = _i32(new_len, "kv4_append(new_len)", cache.device, (B,)) if new_len is not None else None
-    if k.numel() == 0:
-        return
-    ks, vs = _strides(k, "kv4_append(k)"), _strides(v, "kv4_append(v)")
-    _lib.call("mb_kv4_append_bf16", k.data_ptr(), v.data_ptr(), ks, vs, cache.data_ptr(), P, H,
-              block_table.data_ptr(), M, sp, nl, B, k.shape[1], _start(cache.device))
+    sp = _rows(start_pos, "kv4_append(start_pos)", dev, B)
+    nl = None if new_len is None else _rows(new_len, "kv4_append(new_len)", dev, B)
+    rc = _fn("mb_kv4_append_bf16")(k.data_ptr(), v.data_ptr(), *ks, *vs, cp, P, H, tp, M, sp, nl, B,
+                                   k.shape[1], _stream(dev))
+    if rc:
+        _lib.check("mb_kv4_append_bf16", rc)
 
 
-@_on_device
 def kv4_gather(cache: torch.Tensor, block_table: torch.Tensor, start_pos: torch.Tensor, length: int,
                kv_len: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of positions start_pos[b] .. start_pos[b] + length - 1 as
     the numbers they stand for: fp32 [B, length, n_kv_heads, 128], zeros at
     positions kv_len[b] and later."""
-    P, H = _cache(cache, "kv4_gather")
-    B, M = _table(block_table, "kv4_gather", cache.device)
-    sp = _i32(start_pos, "kv4_gather(start_pos)", cache.device, (B,))
-    kl = _i32(kv_len, "kv4_gather(kv_len)", cache.device, (B,))
+    P, H, dev, cp = _cache(cache, "kv4_gather")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv4_gather(cache, block_table, start_pos, length, kv_len)
+    B, M, tp = _table(block_table, "kv4_gather(block_table)", dev)
+    sp = _rows(start_pos, "kv4_gather(start_pos)", dev, B)
+    kl = _rows(kv_len, "kv4_gather(kv_len)", dev, B)
     if length < 0:
         raise ValueError("kv4_gather: negative length")
-    k, v = (torch.empty((B, length, H, HEAD_DIM), dtype=torch.float32, device=cache.device)
-            for _ in range(2))
-    if k.numel():
-        _lib.call("mb_kv4_gather_f32", cache.data_ptr(), P, H, block_table.data_ptr(), M, sp, kl, B,
-                  length, k.data_ptr(), v.data_ptr(), _start(cache.device))
+    k = torch.empty((B, length, H, HEAD_DIM), dtype=torch.float32, device=cache.device)
+    v = torch.empty_like(k)
+    rc = _fn("mb_kv4_gather_f32")(cp, P, H, tp, M, sp, kl, B, length, k.data_ptr(), v.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check("mb_kv4_gather_f32", rc)
     return k, v
 
 
-@_on_device
+def _row_stride(t: torch.Tensor, name: str, dev: int, B: int, H: int):
+    """S, heads and elements between two positions' rows of bf16 [B, S, heads,
+    128] or [B, heads, 128] (S = 1), heads contiguous and a multiple of H."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.get_device() != dev or t.dim() not in (3, 4):
+        _refuse(t, name, _BF16, dev, (B, "S", f"heads (a multiple of {H})", HEAD_DIM))
+    shape, st = t.shape, t.stride()
+    if len(shape) == 4:
+        b, S, Hq, D = shape
+        sb, ss, sh, sd = st
+    else:
+        b, Hq, D = shape
+        sb, sh, sd = st
+        S, ss = 1, 0
+    if b != B or D != HEAD_DIM or Hq == 0 or Hq % H:
+        _refuse(t, name, _BF16, dev, (B, "S", f"heads (a multiple of {H})", HEAD_DIM))
+    ld = ss if S > 1 else sb if B > 1 else Hq * HEAD_DIM
+    if t.numel() and (sd != 1 or (Hq > 1 and sh != HEAD_DIM) or (S > 1 and B > 1 and sb != S * ss)
+                      or ld < Hq * HEAD_DIM or ld % 8 or t.data_ptr() % 16):
+        raise ValueError(f"{name}: heads must be contiguous, positions evenly spaced (a multiple of 8 "
+                         f"elements) and 16-byte aligned; got strides {st}")
+    return S, Hq, ld
+
+
 def attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                   kv_len: torch.Tensor, start_pos: torch.Tensor | None = None,
                   scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -152,85 +192,65 @@ def attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     0..kv_len[b]-1 are seen; with start_pos, row s sees those at positions <=
     start_pos[b] + s (causal). A row that sees no key becomes zeros. scale:
     1/sqrt(128) by default."""
-    P, H = _cache(cache, "attention_kv4")
-    B, M = _table(block_table, "attention_kv4", cache.device)
-    if q.dtype != torch.bfloat16:
-        raise TypeError(f"attention_kv4(q): dtype {q.dtype} is not bfloat16")
-    if q.device != cache.device:
-        raise ValueError(f"attention_kv4(q): expected a tensor on {cache.device}")
-    single = q.dim() == 3
-    x = q.unsqueeze(1) if single else q
-    if x.dim() != 4 or x.shape[0] != B or x.shape[3] != HEAD_DIM or x.shape[2] == 0 or x.shape[2] % H:
-        raise ValueError(f"attention_kv4(q): expected [{B}, S, n_heads (a multiple of {H}), "
-                         f"{HEAD_DIM}], got {tuple(q.shape)}")
-    S, Hq = x.shape[1], x.shape[2]
-    ldq = _row_stride(x, "attention_kv4(q)")
-    kl = _i32(kv_len, "attention_kv4(kv_len)", cache.device, (B,))
-    sp = _i32(start_pos, "attention_kv4(start_pos)", cache.device, (B,)) if start_pos is not None else None
+    P, H, dev, cp = _cache(cache, "attention_kv4")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return attention_kv4(q, cache, block_table, kv_len, start_pos, scale, out)
+    B, M, tp = _table(block_table, "attention_kv4(block_table)", dev)
+    S, Hq, ldq = _row_stride(q, "attention_kv4(q)", dev, B, H)
+    kl = _rows(kv_len, "attention_kv4(kv_len)", dev, B)
+    sp = None if start_pos is None else _rows(start_pos, "attention_kv4(start_pos)", dev, B)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.device != q.device or out.shape != q.shape:
-        raise ValueError("attention_kv4(out): expected a bf16 tensor of q's shape and device")
-    if x.numel() == 0:
-        return out
-    ldo = _row_stride(out.unsqueeze(1) if single else out, "attention_kv4(out)")
-    nb = _lib.lib().mb_attention_kv4_workspace_bytes(B, S, Hq, H, M)
-    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=q.device)
-    _lib.call("mb_attention_kv4_bf16", x.data_ptr(), ldq, cache.data_ptr(), P, block_table.data_ptr(),
-              M, kl, sp, B, S, Hq, H, HEAD_DIM, 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale),
-              out.data_ptr(), ldo, ws.data_ptr(), nb, _start(cache.device))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ldo = Hq * HEAD_DIM
+    else:
+        if out.shape != q.shape:
+            raise ValueError(f"attention_kv4(out): shape {tuple(out.shape)} is not q's {tuple(q.shape)}")
+        ldo = _row_stride(out, "attention_kv4(out)", dev, B, H)[2]
+    nb = _fn("mb_attention_kv4_workspace_bytes")(B, S, Hq, H, M)
+    ws = torch.empty(nb, dtype=torch.uint8, device=cache.device)
+    rc = _fn("mb_attention_kv4_bf16")(q.data_ptr(), ldq, cp, P, tp, M, kl, sp, B, S, Hq, H, HEAD_DIM,
+                                      _SCALE if scale is None else scale, out.data_ptr(), ldo,
+                                      ws.data_ptr(), nb, _stream(dev))
+    if rc:
+        _lib.check("mb_attention_kv4_bf16", rc)
     return out
 
 
-def _row_stride(x: torch.Tensor, name: str) -> int:
-    """Elements between two positions' rows of [B, S, heads, 128], heads contiguous."""
-    B, S, H, D = x.shape
-    if x.numel() == 0:
-        return H * D
-    ld = x.stride(1) if S > 1 else (x.stride(0) if B > 1 else H * D)
-    if x.stride(3) != 1 or (H > 1 and x.stride(2) != D) or (B > 1 and S > 1 and x.stride(0) != S * ld) \
-            or ld < H * D or ld % 8 or x.data_ptr() % 16:
-        raise ValueError(f"{name}: heads must be contiguous, positions evenly spaced (a multiple of 8 "
-                         f"elements) and 16-byte aligned; got strides {x.stride()}")
-    return ld
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 # ---------------------------------------------------------------------------
 # pages
 # ---------------------------------------------------------------------------
-def _meta(block_table, seq_len, page_refs, name):
+def _pages(block_table, seq_len, page_refs, name: str):
+    """Device, sizes and addresses of the three tensors of a page call."""
     if not isinstance(block_table, torch.Tensor) or not block_table.is_cuda:
         raise ValueError(f"{name}: expected CUDA tensors (no CPU fallback)")
-    dev = block_table.device
-    B, M = _table(block_table, name, dev)
+    dev = block_table.get_device()
+    B, M, tp = _table(block_table, f"{name}(block_table)", dev)
     if not isinstance(page_refs, torch.Tensor) or page_refs.dim() != 1:
         raise ValueError(f"{name}: page_refs must be [num_pages]")
     P = page_refs.shape[0]
-    return dev, B, M, P, _i32(seq_len, f"{name}(seq_len)", dev, (B,)), _i32(
-        page_refs, f"{name}(page_refs)", dev, (P,))
+    return dev, B, M, P, tp, _rows(seq_len, name, dev, B), _rows(page_refs, name, dev, P)
 
 
-def _pools(pools, name, dev, P):
+def _pools(pools, name: str, dev: int, P: int):
     n = len(pools)
-    ptrs, sizes = (C.c_void_p * max(n, 1))(), (C.c_int64 * max(n, 1))()
-    for i, t in enumerate(pools):
-        if t.device != dev or not t.is_contiguous() or t.dim() < 1 or t.shape[0] != P:
-            raise ValueError(f"{name}: pool {i} must be a contiguous tensor on {dev} with {P} pages")
-        size = t.numel() * t.element_size() // P if P else 16
+    ptrs, sizes = [], []
+    for t in pools:
+        if t.get_device() != dev or t.dim() < 1 or t.shape[0] != P or not t.is_contiguous():
+            raise ValueError(f"{name}: a pool must be a contiguous tensor on cuda:{dev} with {P} pages")
+        size = t.nbytes // P if P else 16
         if size == 0 or size % 16 or t.data_ptr() % 16:
-            raise ValueError(f"{name}: pool {i}'s pages must be a multiple of 16 bytes and 16-byte aligned")
-        ptrs[i], sizes[i] = t.data_ptr(), size
-    if len(set(ptrs[:n])) < n:
+            raise ValueError(f"{name}: a pool's pages must be a multiple of 16 bytes and 16-byte aligned")
+        ptrs.append(t.data_ptr())
+        sizes.append(size)
+    if len(set(ptrs)) < n:
         raise ValueError(f"{name}: the same pool twice")
-    return ptrs, sizes, n
+    return (C.c_void_p * n)(*ptrs), (C.c_int64 * n)(*sizes), n
 
 
-def _workspace(B, M, P, dev):
-    nb = _lib.lib().mb_kv_pages_workspace_bytes(B, M, P)
-    return torch.empty(nb, dtype=torch.uint8, device=dev), nb
-
-
-@_on_device
 def kv_pages_extend(block_table: torch.Tensor, seq_len: torch.Tensor, page_refs: torch.Tensor,
                     new_len: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Room for new_len[b] more tokens of every sequence, in place: new pages
@@ -238,18 +258,22 @@ def kv_pages_extend(block_table: torch.Tensor, seq_len: torch.Tensor, page_refs:
     grows. Returns (start_pos, status): the lengths before, and an int32 that is
     0, or the number of pages that were lacking, or -1 for a length out of range
     (then nothing was changed)."""
-    name = "kv_pages_extend"
-    dev, B, M, P, sl, pr = _meta(block_table, seq_len, page_refs, name)
-    nl = _i32(new_len, f"{name}(new_len)", dev, (B,))
-    start = torch.empty((B,), dtype=torch.int32, device=dev)
-    status = torch.empty((1,), dtype=torch.int32, device=dev)
-    ws, nb = _workspace(B, M, P, dev)
-    _lib.call("mb_kv_pages_extend", block_table.data_ptr(), sl, pr, B, M, P, nl, start.data_ptr(),
-              status.data_ptr(), ws.data_ptr(), nb, _start(dev))
+    dev, B, M, P, tp, sl, pr = _pages(block_table, seq_len, page_refs, "kv_pages_extend")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv_pages_extend(block_table, seq_len, page_refs, new_len)
+    nl = _rows(new_len, "kv_pages_extend(new_len)", dev, B)
+    start = torch.empty_like(seq_len)
+    status = torch.empty(1, dtype=_I32, device=seq_len.device)
+    nb = _fn("mb_kv_pages_workspace_bytes")(B, M, P)
+    ws = torch.empty(nb, dtype=torch.uint8, device=seq_len.device)
+    rc = _fn("mb_kv_pages_extend")(tp, sl, pr, B, M, P, nl, start.data_ptr(), status.data_ptr(),
+                                   ws.data_ptr(), nb, _stream(dev))
+    if rc:
+        _lib.check("mb_kv_pages_extend", rc)
     return start, status
 
 
-@_on_device
 def kv_pages_fork(pools, block_table: torch.Tensor, seq_len: torch.Tensor, page_refs: torch.Tensor,
                   parent: torch.Tensor) -> torch.Tensor:
     """Row b becomes a fork of row parent[b] as it was before the call, in
@@ -258,18 +282,22 @@ def kv_pages_fork(pools, block_table: torch.Tensor, seq_len: torch.Tensor, page_
     pools: the page tensors [num_pages, ...] of all layers (bf16 or 4-bit).
     Returns an int32 status: 0, or the number of pages that were lacking, or -1
     for an index or length out of range (then nothing was changed)."""
-    name = "kv_pages_fork"
-    dev, B, M, P, sl, pr = _meta(block_table, seq_len, page_refs, name)
-    pa = _i32(parent, f"{name}(parent)", dev, (B,))
-    ptrs, sizes, n = _pools(pools, name, dev, P)
-    status = torch.empty((1,), dtype=torch.int32, device=dev)
-    ws, nb = _workspace(B, M, P, dev)
-    _lib.call("mb_kv_pages_fork", ptrs, sizes, n, block_table.data_ptr(), sl, pr, B, M, P, pa,
-              status.data_ptr(), ws.data_ptr(), nb, _start(dev))
+    dev, B, M, P, tp, sl, pr = _pages(block_table, seq_len, page_refs, "kv_pages_fork")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv_pages_fork(pools, block_table, seq_len, page_refs, parent)
+    pa = _rows(parent, "kv_pages_fork(parent)", dev, B)
+    ptrs, sizes, n = _pools(pools, "kv_pages_fork", dev, P)
+    status = torch.empty(1, dtype=_I32, device=seq_len.device)
+    nb = _fn("mb_kv_pages_workspace_bytes")(B, M, P)
+    ws = torch.empty(nb, dtype=torch.uint8, device=seq_len.device)
+    rc = _fn("mb_kv_pages_fork")(ptrs, sizes, n, tp, sl, pr, B, M, P, pa, status.data_ptr(),
+                                 ws.data_ptr(), nb, _stream(dev))
+    if rc:
+        _lib.check("mb_kv_pages_fork", rc)
     return status
 
 
-@_on_device
 def kv_pages_compact(pools, block_table: torch.Tensor, seq_len: torch.Tensor,
                      page_refs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Move the pages in use into 0..live-1, in place, with the fewest moves:
@@ -277,12 +305,17 @@ def kv_pages_compact(pools, block_table: torch.Tensor, seq_len: torch.Tensor,
     (remap, live): every page's new number (-1: was free) for references held
     outside the table, and the number of pages in use (-1: a table entry was
     out of range or not in use, and nothing was changed)."""
-    name = "kv_pages_compact"
-    dev, B, M, P, sl, pr = _meta(block_table, seq_len, page_refs, name)
-    ptrs, sizes, n = _pools(pools, name, dev, P)
-    remap = torch.empty((P,), dtype=torch.int32, device=dev)
-    live = torch.empty((1,), dtype=torch.int32, device=dev)
-    ws, nb = _workspace(B, M, P, dev)
-    _lib.call("mb_kv_pages_compact", ptrs, sizes, n, block_table.data_ptr(), sl, pr, B, M, P,
-              remap.data_ptr(), live.data_ptr(), ws.data_ptr(), nb, _start(dev))
+    dev, B, M, P, tp, sl, pr = _pages(block_table, seq_len, page_refs, "kv_pages_compact")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv_pages_compact(pools, block_table, seq_len, page_refs)
+    ptrs, sizes, n = _pools(pools, "kv_pages_compact", dev, P)
+    remap = torch.empty_like(page_refs)
+    live = torch.empty(1, dtype=_I32, device=seq_len.device)
+    nb = _fn("mb_kv_pages_workspace_bytes")(B, M, P)
+    ws = torch.empty(nb, dtype=torch.uint8, device=seq_len.device)
+    rc = _fn("mb_kv_pages_compact")(ptrs, sizes, n, tp, sl, pr, B, M, P, remap.data_ptr(),
+                                    live.data_ptr(), ws.data_ptr(), nb, _stream(dev))
+    if rc:
+        _lib.check("mb_kv_pages_compact", rc)
     return remap, live

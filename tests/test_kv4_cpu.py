@@ -60,14 +60,13 @@ def test_attention_arguments(lib, change, word):
 
 
 @pytest.mark.parametrize("change, word", [
-    (dict(k=None), "null"), (dict(k=FAKE + 2), "aligned"), (dict(Hkv=0), "sizes"), (dict(ks=(1024, 129, 128)), "strides"),
+    (dict(k=None), "null"), (dict(k=FAKE + 2), "aligned"), (dict(Hkv=0), "sizes"), (dict(k1=129), "strides"), (dict(v2=-4), "strides"),
     (dict(S=-1), "sizes"),
 ])
 def test_append_arguments(lib, change, word):
-    a = dict(k=FAKE, v=FAKE, ks=(1024, 128, 128), vs=(1024, 128, 128), cache=FAKE, num_pages=4, Hkv=1, table=FAKE,
+    a = dict(k=FAKE, v=FAKE, k0=1024, k1=128, k2=128, v0=1024, v1=128, v2=128, cache=FAKE, num_pages=4, Hkv=1, table=FAKE,
              max_pages=4, start=FAKE, new=None, B=2, S=8)
     a.update(change)
-    a["ks"], a["vs"] = (C.c_int64 * 3)(*a["ks"]), (C.c_int64 * 3)(*a["vs"])
     rc = lib.mb_kv4_append_bf16(*a.values(), None)
     assert rc == -1 and word in lib.mb_last_error().decode()
 
@@ -87,8 +86,7 @@ def test_page_arguments(lib, change, word):
 
 
 def test_empty_calls_launch_nothing(lib):
-    n3 = (C.c_int64 * 3)(0, 0, 0)
-    assert lib.mb_kv4_append_bf16(None, None, n3, n3, None, 1, 1, None, 1, None, None, 0, 4, None) == 0
+    assert lib.mb_kv4_append_bf16(None, None, 0, 0, 0, 0, 0, 0, None, 1, 1, None, 1, None, None, 0, 4, None) == 0
     assert lib.mb_kv4_gather_f32(None, 1, 1, None, 1, None, None, 2, 0, None, None, None) == 0
     assert lib.mb_attention_kv4_bf16(None, 0, None, 1, None, 1, None, None, 0, 1, 8, 8, 128, 1.0, None, 0, None, 0, None) == 0
     assert lib.mb_attention_kv4_workspace_bytes(0, 1, 8, 8, 4) == 0
