@@ -260,8 +260,7 @@ int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv, const int* b
  * 0..kv_len[b]-1; with start_pos, row s sees the keys at positions <=
  * start_pos[b] + s only (causal), else all. q, out: bf16 [B][S][Hq][128] with ldq /
  * ldo elements between two positions' rows (multiples of 8), the heads
- * contiguous. A row that sees no key becomes zeros. B <= 4096; every length is
- * read on the device, so ragged batches balance and the call can be captured. */
+ * contiguous. A row that sees no key becomes zeros. Every length is read on the device, so ragged batches balance and the call can be captured. */
 size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages);
 int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache, int num_pages,
                           const int* block_table, int max_pages, const int* kv_len,

@@ -25,15 +25,16 @@
 // the operand layout by movmatrix. Query rows are the S * G pairs (position,
 // head of the group); NT column tiles of 8 per pass over the cache.
 //
-// Schedule: the flat list of (sequence, kv head, row tile, page) is cut into
-// equal shares, one a warp, planned on the device from kv_len, so that ragged
-// batches balance; every (sequence, kv head, row tile), a unit, counts
-// UNIT_COST pages more than it has, for its start and end. Each warp streams
-// its share through its own ring of whole-page bulk copies (8704 bytes, one
-// mbarrier each) without waiting for another. A unit that lies within a share
-// is written at once. At the end the warps of a CTA that stopped in the same
-// unit join their states in shared memory; what is then still in parts (at
-// most two a warp) goes to the workspace, and attn_kv4_combine_kernel joins it.
+// Schedule: one CTA an SM. The flat list of (sequence, kv head, row tile, page)
+// is cut into equal shares, one a warp, planned on the device from kv_len, so
+// that ragged batches balance; every (sequence, kv head, row tile), a unit,
+// counts UNIT_COST pages more than it has, for its start and end. Each warp
+// streams its share through its own ring of whole-page bulk copies (8704
+// bytes, one mbarrier each) without waiting for another. A unit that lies
+// within a share is written at once. At the end the warps that stopped in the
+// same unit join their states in shared memory; what is then still in parts
+// (at most two a warp) goes to the workspace, and attn_kv4_combine_kernel,
+// which plans for itself while the last warps stream, joins it.
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
@@ -42,8 +43,13 @@
 namespace {
 using namespace kv4;
 
-constexpr int NW = 4;  // warps per CTA
-constexpr int ST = 2;  // pages in a warp's ring
+// Warps of a CTA and pages in a warp's ring, for NT column tiles of 8 rows: as
+// many warps as the registers of an SM hold (168 and 255 a thread), and as many
+// pages in flight as its shared memory does.
+template <int NT> struct Shape;
+template <> struct Shape<1> { static constexpr int NW = 12, ST = 2; };
+template <> struct Shape<2> { static constexpr int NW = 8, ST = 3; };
+constexpr int MAX_B = 512;  // sequences a launch: their page counts are planned in shared memory
 constexpr int UNIT_COST = 2;  // pages that starting and ending a unit cost
 
 struct Args {
@@ -55,10 +61,11 @@ struct Args {
   uint16_t* out;
   float* part_o;   // [warps][2][cols][DH]: unit began before this share, in it
   float* part_ml;  // [warps][2][cols][2]
-  int* plan;       // [2 (B + 1)]: pre, vpre for the combine kernel
   uint32_t* status;
   int64_t ldq, ldo;  // elements between two positions' rows
   int num_pages, max_pages, B, S, Hkv, G, RT;
+  int warps;  // shares
+  int active; // warps of a CTA that have one
   float scale_log2;
 };
 
@@ -108,23 +115,32 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return r;
 }
 
-// Attended keys of sequence b.
+// Attended keys of sequence b (from L2: the combine kernel plans before it has
+// waited for the main one).
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
-  return max(0, min(a.kv_len[b], a.max_pages * PAGE));
+  return max(0, min(__ldcg(a.kv_len + b), a.max_pages * PAGE));
 }
 
-// pre[b] = flat index of the first page of sequence b, pre[B] = their number;
-// vpre the same with UNIT_COST more pages a unit.
-__device__ void plan(const Args& a, int* pre, int* vpre, int2* wsum) {
+// Flat page list of the batch, in shared memory.
+struct Plan {
+  int2 wsum[12];
+  int pre[MAX_B + 1];   // index of the first page of sequence b; [B]: how many there are
+  int vpre[MAX_B + 1];  // the same with UNIT_COST more pages a unit
+};
+
+template <int NW>
+__device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (a.B + NW * 32 - 1) / (NW * 32);
-  const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  constexpr int MOST = (MAX_B + NW * 32 - 1) / (NW * 32);
+  const int per = (a.B + NW * 32 - 1) / (NW * 32), b0 = min(a.B, tid * per);
   const int units = a.Hkv * a.RT;
+  int pages[MOST];
   int2 sum = make_int2(0, 0);
-  for (int b = b0; b < b1; ++b) {
-    const int pages = (seq_len(a, b) + PAGE - 1) / PAGE;
-    sum.x += pages * units;
-    sum.y += pages ? (pages + UNIT_COST) * units : 0;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    pages[i] = i < per && b0 + i < a.B ? (seq_len(a, b0 + i) + PAGE - 1) / PAGE : 0;
+    sum.x += pages[i] * units;
+    sum.y += pages[i] ? (pages[i] + UNIT_COST) * units : 0;
   }
   int2 inc = sum;
 #pragma unroll
@@ -132,35 +148,43 @@ __device__ void plan(const Args& a, int* pre, int* vpre, int2* wsum) {
     const int x = __shfl_up_sync(0xffffffffu, inc.x, off), y = __shfl_up_sync(0xffffffffu, inc.y, off);
     if (lane >= off) inc.x += x, inc.y += y;
   }
-  if (lane == 31) wsum[warp] = inc;
+  if (lane == 31) p.wsum[warp] = inc;
   __syncthreads();
   int2 run = make_int2(inc.x - sum.x, inc.y - sum.y);
-  for (int w = 0; w < warp; ++w) run.x += wsum[w].x, run.y += wsum[w].y;
-  for (int b = b0; b < b1; ++b) {
-    pre[b] = run.x;
-    vpre[b] = run.y;
-    const int pages = (seq_len(a, b) + PAGE - 1) / PAGE;
-    run.x += pages * units;
-    run.y += pages ? (pages + UNIT_COST) * units : 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w)
+    if (w < warp) run.x += p.wsum[w].x, run.y += p.wsum[w].y;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    if (i < per && b0 + i < a.B) {
+      p.pre[b0 + i] = run.x;
+      p.vpre[b0 + i] = run.y;
+    }
+    run.x += pages[i] * units;
+    run.y += pages[i] ? (pages[i] + UNIT_COST) * units : 0;
   }
   if (tid == NW * 32 - 1) {
-    pre[a.B] = run.x;  // the last thread's end is everybody's
-    vpre[a.B] = run.y;
+    p.pre[a.B] = run.x;  // the last thread's end is everybody's
+    p.vpre[a.B] = run.y;
   }
   __syncthreads();
 }
 
+// The last i < n with list[i] <= v (list ascends, list[0] <= v): a warp together.
+__device__ __forceinline__ int find_warp(const int* list, int n, int v) {
+  int c = 0;
+  for (int i = threadIdx.x & 31; i - (int)(threadIdx.x & 31) < n; i += 32)
+    c += __popc(__ballot_sync(0xffffffffu, i < n && list[i] <= v));
+  return c - 1;
+}
+
 // Pages whose place in the costed list lies before v.
-__device__ __forceinline__ int pages_before(const int* pre, const int* vpre, int B, int units, int v) {
-  if (v >= vpre[B]) return pre[B];
-  int lo = 0, hi = B;  // vpre[lo] <= v < vpre[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (vpre[mid] <= v) lo = mid; else hi = mid;
-  }
-  const int pages = (pre[lo + 1] - pre[lo]) / units;
-  const int rem = v - vpre[lo], unit = rem / (pages + UNIT_COST);
-  return pre[lo] + unit * pages + max(0, rem - unit * (pages + UNIT_COST) - UNIT_COST);
+__device__ __forceinline__ int pages_before(const Plan& p, int B, int units, int64_t v64) {
+  if (v64 >= p.vpre[B]) return p.pre[B];
+  const int v = (int)v64, b = find_warp(p.vpre, B, v);
+  const int pages = (p.pre[b + 1] - p.pre[b]) / units;
+  const int rem = v - p.vpre[b], unit = rem / (pages + UNIT_COST);
+  return p.pre[b] + unit * pages + max(0, rem - unit * (pages + UNIT_COST) - UNIT_COST);
 }
 
 // Sequence of flat page f: pre[b] <= f < pre[b + 1].
@@ -362,29 +386,58 @@ struct State {
   }
 };
 
+// Four dims a lane of one query row: finished (whole), or as a slot's partial.
+__device__ __forceinline__ void store_row(const Args& a, int b, int kvh, int r, int slot, int col, int cols,
+                                          bool whole, float R, float l, float4 o) {
+  const int lane = threadIdx.x & 31;
+  if (!whole) {
+    *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * cols + col) * DH + lane * 4) = o;
+    if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * cols + col) * 2) = make_float2(R, l);
+    return;
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // 0: the row has seen no key
+  const __nv_bfloat162 h0 = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+  const __nv_bfloat162 h1 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+  const int s = r / a.G;
+  uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH + lane * 4;
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+}
+
+// Floats of a warp's state of one column tile, while warps join: 4 pieces of
+// 8 x 32 accumulators, each one bank further, and R, l, om of the 8 columns.
+constexpr int STATE = 1028 + 32;
+
 template <int NT>
-__global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
-  mbd::pdl_trigger();
-  mbd::pdl_wait();
-  constexpr int COLS = NT * 8;
-  extern __shared__ __align__(128) uint8_t sm[];
-  uint8_t* ring = sm + (threadIdx.x >> 5) * ST * BLOB;
-  KeyParams* kp = reinterpret_cast<KeyParams*>(sm + NW * ST * BLOB) + (threadIdx.x >> 5) * PAGE;
-  float* vmin = reinterpret_cast<float*>(sm + NW * (ST * BLOB + PAGE * 16)) + (threadIdx.x >> 5) * PAGE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + NW * (ST * BLOB + PAGE * 20));  // [NW][ST]
-  int2* wsum = reinterpret_cast<int2*>(bars + NW * ST);               // [NW]
-  int4* seg = reinterpret_cast<int4*>(wsum + NW);                     // [NW]
-  int* page_ok = reinterpret_cast<int*>(seg + NW);                    // [NW][ST]
-  int* pre = page_ok + NW * ST;                                       // [B + 1]
-  int* vpre = pre + a.B + 1;                                          // [B + 1]
+struct Shared {
+  static constexpr int NW = Shape<NT>::NW, ST = Shape<NT>::ST;
+  static_assert(NT * STATE * 4 <= ST * BLOB && NW <= 16, "a warp's state takes the place of its pages");
+  uint8_t ring[NW][ST][BLOB];
+  KeyParams kp[NW][PAGE];
+  float vmin[NW][PAGE];
+  int4 seg[NW];       // last unit, its first and end page in this share
+  uint64_t bar[NW][ST];
+  int page_ok[NW][ST];
+  Plan plan;
+};
+
+template <int NT>
+__global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args a) {
+  constexpr int COLS = NT * 8, NW = Shape<NT>::NW, ST = Shape<NT>::ST;
+  extern __shared__ __align__(128) uint8_t sm_raw[];
+  Shared<NT>& sm = *reinterpret_cast<Shared<NT>*>(sm_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  uint64_t* bar = bars + warp * ST;
-  int* ok_flag = page_ok + warp * ST;
+  uint8_t* ring = sm.ring[warp][0];
+  uint64_t* bar = sm.bar[warp];
+  int* ok_flag = sm.page_ok[warp];
+  const int *pre = sm.plan.pre, *vpre = sm.plan.vpre;
   if (lane == 0)
     for (int i = 0; i < ST; ++i) mbd::mbar_init(bar + i, 1);
   mbd::fence_mbar_init();
-  plan(a, pre, vpre, wsum);
+  mbd::pdl_wait();
+  mbd::pdl_trigger();  // after the wait: what the combine kernel plans from is complete
+  make_plan<NW>(a, sm.plan);
 
   // sequences without keys: their rows are zeros
   const int row_elems = a.Hkv * a.G * DH;
@@ -394,14 +447,14 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
         for (int i = threadIdx.x * 8; i < row_elems; i += NW * 32 * 8)
           *reinterpret_cast<uint4*>(a.out + ((int64_t)b * a.S + s) * a.ldo + i) = make_uint4(0, 0, 0, 0);
 
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < 2 * (a.B + 1); i += NW * 32) a.plan[i] = pre[i];
-
   const int units = a.Hkv * a.RT;
-  const int me = blockIdx.x * NW + warp;
-  const int per = (vpre[a.B] + gridDim.x * NW - 1) / (gridDim.x * NW);
-  const int begin = pages_before(pre, vpre, a.B, units, min((int64_t)me * per, (int64_t)vpre[a.B]));
-  const int end = pages_before(pre, vpre, a.B, units, min((int64_t)(me + 1) * per, (int64_t)vpre[a.B]));
+  const int per = (vpre[a.B] + a.warps - 1) / a.warps;
+  const int me = blockIdx.x * a.active + warp;  // share of this warp
+  int begin = 0, end = 0;
+  if (warp < a.active) {
+    begin = pages_before(sm.plan, a.B, units, (int64_t)me * per);
+    end = pages_before(sm.plan, a.B, units, (int64_t)(me + 1) * per);
+  }
   const int mine = end - begin;
 
   // ---- this warp's loads, page after page ----
@@ -480,7 +533,7 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
   int f0 = begin, ub = -1, b = 0, unit = 0, pages = 0;
   while (f0 < end) {
     // one segment: the pages of one unit (sequence, kv head, row tile) in this share
-    b = find_seq(pre, a.B, f0);
+    b = find_warp(pre, a.B, f0);
     pages = (pre[b + 1] - pre[b]) / units;
     unit = (f0 - pre[b]) / pages;
     ub = pre[b] + unit * pages;  // flat index of the unit's first page
@@ -555,9 +608,9 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
         if (!dead && ok_flag[st]) {
           const int key0 = (f - ub) * PAGE;
           if (key0 + PAGE <= all_seen)
-            z.template page<false>(ring + st * BLOB, kp, vmin, key0, L, ck, a.scale_log2);
+            z.template page<false>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
           else
-            z.template page<true>(ring + st * BLOB, kp, vmin, key0, L, ck, a.scale_log2);
+            z.template page<true>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
         }
         __syncwarp();  // all lanes are done with this page
         ++used;
@@ -583,178 +636,209 @@ __global__ void __launch_bounds__(NW * 32) attn_kv4_kernel(const Args a) {
     for (int i = dead_at; i < issued; ++i) mbd::mbar_wait(bar + i % ST, (i / ST) & 1, nullptr, 0);
 
   // ---- neighbouring warps whose last unit is the same join their states ----
-  if (lane == 0) seg[warp] = make_int4(ub, f0, end, 0);
+  int4* seg = sm.seg;
+  if (lane == 0) seg[warp] = make_int4(ub, f0, end, b);
   __syncthreads();  // every ring is free: a warp's state takes the place of its pages
-  const bool leads = ub >= 0 && (warp == 0 || seg[warp - 1].x != ub);
-  if (ub >= 0 && !leads) {
-    float* dst = reinterpret_cast<float*>(ring) + lane;
+  const bool prev = ub >= 0 && warp > 0 && seg[warp - 1].x == ub;
+  const bool next = ub >= 0 && warp + 1 < NW && seg[warp + 1].x == ub;
+  if (ub >= 0 && !prev && !next) emit(b, unit, 2 * me + (f0 == ub ? 1 : 0), f0 == ub && end == ub + pages);
+  float* mine_z = reinterpret_cast<float*>(ring);
+  if (prev || next) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      float* to = mine_z + t * STATE + lane;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) dst[(t * 38 + i) * 32] = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
+      for (int i = 0; i < 32; ++i)  // a piece's 8 numbers a lane; pieces one bank apart for the readers
+        to[i * 32 + (i >> 3)] = z.o[t][i >> 3][(i >> 2) & 1][i & 3] * ((i & 2) ? 0x1p20f : 0x1p24f);
+      if (gid == 0) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        dst[(t * 38 + 32 + c) * 32] = z.R[t][c];
-        dst[(t * 38 + 34 + c) * 32] = z.l[t][c];
-        dst[(t * 38 + 36 + c) * 32] = z.om[t][c];
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<float4*>(mine_z + t * STATE + 1028 + (2 * tig + c) * 4) =
+              make_float4(z.R[t][c], z.l[t][c], z.om[t][c], 0.f);
       }
     }
   }
   __syncthreads();
-  if (!leads) return;
-  int f1 = end;
-  for (int w = warp + 1; w < NW && seg[w].x == ub; ++w) {
-    f1 = seg[w].z;
-    const float* src = reinterpret_cast<const float*>(ring + (w - warp) * ST * BLOB) + lane;
+  // (run of warps, query row) pairs over all warps; a lane takes four dims
+  int item = 0;
+  for (int w0 = 0; w0 < NW;) {
+    const int4 sg = seg[w0];
+    int w1 = w0 + 1, gf1 = sg.z;
+    for (; w1 < NW && seg[w1].x == sg.x; ++w1) gf1 = seg[w1].z;
+    if (sg.x >= 0 && w1 > w0 + 1) {
+      const int gpages = (pre[sg.w + 1] - pre[sg.w]) / units, gunit = (sg.x - pre[sg.w]) / gpages;
+      const bool first_here = sg.y == sg.x, whole = first_here && gf1 == sg.x + gpages;
+      const int kvh = gunit / a.RT, rt = gunit - kvh * a.RT;
+      for (int col = 0; col < COLS; ++col, ++item) {
+        const int r = rt * COLS + col;
+        if (item % NW != warp || r >= a.S * a.G) continue;
+        const float* base = reinterpret_cast<const float*>(sm.ring[w0][0]) + (col >> 3) * STATE;
+        constexpr int STEP = ST * BLOB / 4;  // floats between two warps' states
+        float4 m = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        if (lane < w1 - w0) m = *reinterpret_cast<const float4*>(base + lane * STEP + 1028 + (col & 7) * 4);
+        float R = m.x;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float fa[2], fb[2];
+        for (int off = 8; off; off >>= 1) R = fmaxf(R, __shfl_xor_sync(0xffffffffu, R, off));
+        R = __shfl_sync(0xffffffffu, R, 0);  // the runs are at most 16 warps
+        const float f = m.x == -INFINITY ? 0.f : fast_exp2(m.x - R);
+        float l = m.y * f, om = m.z * f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float Ro = src[(t * 38 + 32 + c) * 32];
-        const float Rn = fmaxf(z.R[t][c], Ro);
-        fa[c] = z.R[t][c] == -INFINITY ? 0.f : fast_exp2(z.R[t][c] - Rn);
-        fb[c] = Ro == -INFINITY ? 0.f : fast_exp2(Ro - Rn);
-        z.R[t][c] = Rn;
-        z.l[t][c] = z.l[t][c] * fa[c] + src[(t * 38 + 34 + c) * 32] * fb[c];
-        z.om[t][c] = z.om[t][c] * fa[c] + src[(t * 38 + 36 + c) * 32] * fb[c];
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float& o = z.o[t][i >> 3][(i >> 2) & 1][i & 3];
-        o = o * fa[i & 1] + src[(t * 38 + i) * 32] * fb[i & 1];
+        for (int off = 8; off; off >>= 1) {
+          l += __shfl_xor_sync(0xffffffffu, l, off);
+          om += __shfl_xor_sync(0xffffffffu, om, off);
+        }
+        om = __shfl_sync(0xffffffffu, om, 0);
+        float4 o = make_float4(om, om, om, om);
+        const float* zp = base + (lane >> 3) * (8 * 32 + 1) + (lane & 7) * 4 + ((col & 7) >> 1) + (col & 1) * 32;
+#pragma unroll 4
+        for (int w = 0; w < w1 - w0; ++w, zp += STEP) {
+          const float fw = __shfl_sync(0xffffffffu, f, w);
+          o.x = fmaf(zp[0], fw, o.x);
+          o.y = fmaf(zp[64], fw, o.y);
+          o.z = fmaf(zp[128], fw, o.z);
+          o.w = fmaf(zp[192], fw, o.w);
+        }
+        store_row(a, sg.w, kvh, r, 2 * (blockIdx.x * a.active + w0) + (first_here ? 1 : 0), col, COLS, whole, R,
+                  __shfl_sync(0xffffffffu, l, 0), o);
       }
     }
+    w0 = w1;
   }
-  emit(b, unit, 2 * me + (f0 == ub ? 1 : 0), f0 == ub && f1 == ub + pages);
 }
 
-// Joins the partials of the units that more than one warp worked on. A CTA is
-// one unit and COLS / gridDim.y of its query rows; its 8 warps take a row each
-// (many units: few partials each), or share one row's partials (few units).
+// Joins the partials of the units that more than one CTA worked on; before it
+// waits for them it plans. A CTA takes a unit; its 8 warps take a query row
+// each, or (SPLIT: few units, so many partials each) share one row's partials.
 template <int NT, bool SPLIT>
-__global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a, int warps) {
-  mbd::pdl_trigger();
-  mbd::pdl_wait();
+__global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a) {
+  __shared__ Plan plan;
   constexpr int COLS = NT * 8;
+  mbd::pdl_trigger();
+  make_plan<8>(a, plan);
+  mbd::pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = a.Hkv * a.RT;
-  const int b = blockIdx.x / units, unit = blockIdx.x - b * units;
-  const int col = SPLIT ? blockIdx.y : blockIdx.y * 8 + warp;
-  const int kvh = unit / a.RT, r = (unit - kvh * a.RT) * COLS + col;
-  const int pages = (a.plan[b + 1] - a.plan[b]) / units;
-  const int* vpre = a.plan + a.B + 1;
-  const int per = (vpre[a.B] + warps - 1) / warps;
-  const int v = vpre[b] + unit * (pages + UNIT_COST) + UNIT_COST;  // place of the first page
-  if (pages == 0 || r >= a.S * a.G) return;
-  const int w0 = v / per, w1 = (v + pages - 1) / per, c0 = w0 / NW, c1 = w1 / NW;
-  // w1's share ends with this unit: then it joined its CTA's other warps on it
-  const bool ends = v + pages == vpre[a.B] || v + pages + UNIT_COST >= (int64_t)(w1 + 1) * per;
-  const int joined = c1 - c0 + (ends || w1 > max(w0, c1 * NW) ? 1 : 0);
-  const int n = joined + (ends ? 0 : 1);
-  if (n < 2) return;  // written by the main kernel
-  auto row = [&](int i) -> int64_t {
-    const int w = i < joined ? max(w0, (c0 + i) * NW) : w1;
-    return (int64_t)(2 * w + (w == w0 ? 1 : 0)) * COLS + col;
-  };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[row(i) * 2]);
+  const int units = a.Hkv * a.RT, act = a.active;
+  const int per = (plan.vpre[a.B] + a.warps - 1) / a.warps;
+  for (int u = blockIdx.x; u < a.B * units; u += gridDim.x) {
+    const int b = u / units, unit = u - b * units;
+    const int pages = (plan.pre[b + 1] - plan.pre[b]) / units;
+    if (pages == 0) continue;
+    const int v = plan.vpre[b] + unit * (pages + UNIT_COST) + UNIT_COST;  // place of the first page
+    const int w0 = v / per, w1 = (v + pages - 1) / per, c0 = w0 / act, c1 = w1 / act;
+    // w1's share ends with this unit: then it joined its CTA's other warps on it
+    const bool ends = v + pages == plan.vpre[a.B] || v + pages + UNIT_COST >= (int64_t)(w1 + 1) * per;
+    const int joined = c1 - c0 + (ends || w1 > max(w0, c1 * act) ? 1 : 0);
+    const int n = joined + (ends ? 0 : 1);
+    if (n < 2) continue;  // written by the main kernel
+    const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
 #pragma unroll
-  for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = SPLIT ? warp : 0; i < n; i += SPLIT ? 8 : 1) {
-    const int64_t at = row(i);
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-    const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * DH + lane * 4);
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    L = fmaf(ml.y, w, L);
-    acc.x = fmaf(o.x, w, acc.x);
-    acc.y = fmaf(o.y, w, acc.y);
-    acc.z = fmaf(o.z, w, acc.z);
-    acc.w = fmaf(o.w, w, acc.w);
-  }
-  if (SPLIT) {
-    __shared__ float4 so[8][32];
-    __shared__ float sl[8];
-    so[warp][lane] = acc;
-    if (lane == 0) sl[warp] = L;
-    __syncthreads();
-    if (warp) return;
+    for (int c8 = 0; c8 < (SPLIT ? 1 : NT); ++c8) {
+      const int col = SPLIT ? blockIdx.y : c8 * 8 + warp;
+      const int r = rt * COLS + col;
+      if (r < a.S * a.G) {
+        auto row = [&](int i) -> int64_t {
+          const int w = i < joined ? max(w0, (c0 + i) * act) : w1;
+          return (int64_t)(2 * w + (w == w0 ? 1 : 0)) * COLS + col;
+        };
+        // every lane keeps the same running reference
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = SPLIT ? warp : 0; i < n; i += SPLIT ? 32 : 4) {
+          float2 ml[4];
+          float4 o[4];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) {
-      const float4 o = so[w][lane];
-      acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
-      L += sl[w];
+          for (int k = 0; k < 4; ++k) {
+            const int j = i + k * (SPLIT ? 8 : 1);
+            ml[k] = make_float2(-INFINITY, 0.f);
+            o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (j < n) {
+              ml[k] = *reinterpret_cast<const float2*>(a.part_ml + row(j) * 2);
+              o[k] = *reinterpret_cast<const float4*>(a.part_o + row(j) * DH + lane * 4);
+            }
+          }
+          const float Mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M);
+          const float f = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+          M = Mn;
+          L *= f;
+          acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float w = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - Mn);
+            L = fmaf(ml[k].y, w, L);
+            acc.x = fmaf(o[k].x, w, acc.x);
+            acc.y = fmaf(o[k].y, w, acc.y);
+            acc.z = fmaf(o[k].z, w, acc.z);
+            acc.w = fmaf(o[k].w, w, acc.w);
+          }
+        }
+        if (SPLIT) {
+          __shared__ float4 so[8][32];
+          __shared__ float2 sl[8];
+          so[warp][lane] = acc;
+          if (lane == 0) sl[warp] = make_float2(M, L);
+          __syncthreads();
+          if (warp == 0) {
+#pragma unroll
+            for (int w = 1; w < 8; ++w) M = fmaxf(M, sl[w].x);
+            L = 0.f;
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+              const float f = sl[w].x == -INFINITY ? 0.f : fast_exp2(sl[w].x - M);
+              const float4 o = so[w][lane];
+              L = fmaf(sl[w].y, f, L);
+              acc.x = fmaf(o.x, f, acc.x);
+              acc.y = fmaf(o.y, f, acc.y);
+              acc.z = fmaf(o.z, f, acc.z);
+              acc.w = fmaf(o.w, f, acc.w);
+            }
+          }
+          __syncthreads();
+          if (warp) continue;
+        }
+        store_row(a, b, kvh, r, 0, col, COLS, true, M, L, acc);
+      }
+
     }
   }
-  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-  const __nv_bfloat162 h0 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-  const __nv_bfloat162 h1 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-  const int s = r / a.G;
-  uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
-  *reinterpret_cast<uint2*>(dst + lane * 4) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
 }
 
-constexpr int MAX_B = 4096;  // sequences a call: their page counts are planned in shared memory
-
-constexpr int smem_bytes(int B) {
-  return NW * (ST * BLOB + PAGE * 20) + NW * ST * 8 + NW * 24 + (NW * ST + 2 * (B + 1)) * 4;
-}
-
-// CTAs of one resident wave (with the shared memory of a batch of up to 64).
-template <int NT>
-int resident_ctas() {
-  static int per_sm[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) dev = 0;
-  if (!per_sm[dev]) {
-    int nb = 0;
-    if (mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes(MAX_B)) ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&nb, attn_kv4_kernel<NT>, NW * 32,
-                                                      smem_bytes(64)) != cudaSuccess || nb < 1)
-      nb = 1;
-    per_sm[dev] = nb;
-  }
-  return per_sm[dev] * mb::num_sms();
-}
-
-struct Plan {
-  int nt, rt, grid;
+struct Launch {
+  int nt, rt, ctas, active;
   size_t bytes;
 };
 
 // Query rows of a kv head: S * G. Up to 8 take one column tile, more two (so
 // that a page is unpacked once for 16 rows), in row tiles of 16.
-Plan make_plan(int B, int S, int Hq, int Hkv, int max_pages) {
-  Plan p;
+Launch plan_launch(int B, int S, int Hq, int Hkv, int max_pages) {
+  Launch p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   p.nt = rows <= 8 ? 1 : 2;
   p.rt = (int)((rows + p.nt * 8 - 1) / (p.nt * 8));
-  const int64_t most = (int64_t)B * Hkv * p.rt * max_pages;
-  const int res = p.nt == 1 ? resident_ctas<1>() : resident_ctas<2>();
-  const int64_t ctas = (most * (1 + UNIT_COST) + NW - 1) / NW;
-  p.grid = (int)(ctas < res ? ctas : res);
-  p.bytes = ((size_t)2 * (B + 1) * sizeof(int) + 15) / 16 * 16 +
-            (size_t)p.grid * NW * 2 * p.nt * 8 * (DH + 2) * sizeof(float);
+  // shares of at least a page; as few warps a CTA as that leaves, over all SMs
+  const int64_t most = (int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)max_pages + UNIT_COST);
+  const int sms = mb::num_sms(), nw = p.nt == 1 ? Shape<1>::NW : Shape<2>::NW;
+  p.ctas = (int)(most < sms ? most : sms);
+  const int64_t act = (most + p.ctas - 1) / p.ctas;
+  p.active = (int)(act < nw ? act : nw);
+  p.bytes = (size_t)p.ctas * p.active * 2 * p.nt * 8 * (DH + 2) * sizeof(float);
   return p;
 }
 
 template <int NT>
-int launch(const Args& a, int grid, cudaStream_t s) {
-  const int smem = smem_bytes(a.B);
-  int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem_bytes(MAX_B));
+int launch(const Args& a, int ctas, cudaStream_t s) {
+  const int smem = (int)sizeof(Shared<NT>);
+  int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem);
   if (rc) return rc;
-  MB_CUDA(mb::launch_pdl(attn_kv4_kernel<NT>, dim3(grid), dim3(NW * 32), smem, s, a));
-  const int units = a.B * a.Hkv * a.RT;
-  // few units are many partials each: 8 warps to a row
-  if (units <= 2 * mb::num_sms())
-    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT, true>, dim3(units, NT * 8), dim3(256), 0, s, a, grid * NW));
+  MB_CUDA(mb::launch_pdl(attn_kv4_kernel<NT>, dim3(ctas), dim3(Shape<NT>::NW * 32), smem, s, a));
+  if (a.warps == 1) return MB_OK;  // one share: nothing is in parts
+  const int units = a.B * a.Hkv * a.RT, sms = mb::num_sms();
+  // few units are many parts each (about sms / units): 8 warps to a row
+  if (units * 8 <= sms)
+    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT, true>, dim3(units, NT * 8), dim3(256), 0, s, a));
   else
-    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT, false>, dim3(units, NT), dim3(256), 0, s, a, grid * NW));
+    MB_CUDA(mb::launch_pdl(attn_kv4_combine_kernel<NT, false>, dim3(units < 4 * sms ? units : 4 * sms), dim3(256),
+                           0, s, a));
   return MB_OK;
 }
 
@@ -762,7 +846,7 @@ int launch(const Args& a, int grid, cudaStream_t s) {
 
 extern "C" size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages) {
   if (B <= 0 || S <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_pages <= 0) return 0;
-  return make_plan(B, S, Hq, Hkv, max_pages).bytes;
+  return plan_launch(B, S, Hq, Hkv, max_pages).bytes;
 }
 
 extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache,
@@ -774,38 +858,44 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
   MB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention: Hq must be a multiple of Hkv");
   MB_REQUIRE(B >= 0 && S >= 0 && num_pages > 0 && max_pages > 0, "attention kv4: bad sizes");
   if (B == 0 || S == 0) return MB_OK;
-  MB_REQUIRE(B <= MAX_B, "attention kv4: at most %d sequences a call", MAX_B);
   MB_REQUIRE(q && cache && block_table && kv_len && out, "attention kv4: null pointer");
   MB_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0,
              "attention kv4: q, out and the cache must be 16-byte aligned");
-  const Plan p = make_plan(B, S, Hq, Hkv, max_pages);
-  MB_REQUIRE((int64_t)B * Hkv * p.rt * ((int64_t)max_pages + UNIT_COST) < (1ll << 30) && (int64_t)max_pages * PAGE < (1ll << 30),
+  MB_REQUIRE((int64_t)S * Hq < (1ll << 30) && (int64_t)max_pages * PAGE < (1ll << 30),
+             "attention kv4: too many rows or pages");
+  const Launch p = plan_launch(B, S, Hq, Hkv, max_pages);
+  MB_REQUIRE((int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)max_pages + UNIT_COST) < (1ll << 30),
              "attention kv4: too many pages");
   MB_REQUIRE(workspace && workspace_bytes >= p.bytes && (uintptr_t)workspace % 16 == 0,
              "attention kv4: workspace of %zu bytes required, 16-byte aligned", p.bytes);
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "attention kv4: no status word");
-  Args a;
-  a.q = q;
-  a.cache = cache;
-  a.table = block_table;
-  a.kv_len = kv_len;
-  a.start_pos = start_pos;
-  a.out = out;
-  a.plan = static_cast<int*>(workspace);
-  a.part_o = reinterpret_cast<float*>(a.plan + (2 * (B + 1) + 3) / 4 * 4);
-  a.part_ml = a.part_o + (size_t)p.grid * NW * 2 * p.nt * 8 * DH;
-  a.status = status;
-  a.ldq = ldq;
-  a.ldo = ldo;
-  a.num_pages = num_pages;
-  a.max_pages = max_pages;
-  a.B = B;
-  a.S = S;
-  a.Hkv = Hkv;
-  a.G = Hq / Hkv;
-  a.RT = p.rt;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  return p.nt == 1 ? launch<1>(a, p.grid, static_cast<cudaStream_t>(stream))
-                   : launch<2>(a, p.grid, static_cast<cudaStream_t>(stream));
+  for (int b = 0; b < B; b += MAX_B) {
+    Args a;
+    a.q = q + (int64_t)b * S * ldq;
+    a.cache = cache;
+    a.table = block_table + (int64_t)b * max_pages;
+    a.kv_len = kv_len + b;
+    a.start_pos = start_pos ? start_pos + b : nullptr;
+    a.out = out + (int64_t)b * S * ldo;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)p.ctas * p.active * 2 * p.nt * 8 * DH;
+    a.status = status;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.num_pages = num_pages;
+    a.max_pages = max_pages;
+    a.B = B - b < MAX_B ? B - b : MAX_B;
+    a.S = S;
+    a.Hkv = Hkv;
+    a.G = Hq / Hkv;
+    a.RT = p.rt;
+    a.warps = p.ctas * p.active;
+    a.active = p.active;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const int rc = p.nt == 1 ? launch<1>(a, p.ctas, static_cast<cudaStream_t>(stream))
+                             : launch<2>(a, p.ctas, static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
+  }
+  return MB_OK;
 }

@@ -46,9 +46,9 @@ FAKE = 1 << 20  # an aligned address that is refused before anything reads it
 
 
 @pytest.mark.parametrize("change, word", [
-    (dict(Dh=64), "head_dim"), (dict(Hq=3, Hkv=2), "multiple of Hkv"), (dict(B=5000), "at most 4096"),
+    (dict(Dh=64), "head_dim"), (dict(Hq=3, Hkv=2), "multiple of Hkv"), (dict(B=-1), "sizes"),
     (dict(q=None), "null"), (dict(q=FAKE + 8), "aligned"), (dict(ldq=132), "aligned"), (dict(num_pages=0), "sizes"),
-    (dict(max_pages=1 << 25), "too many pages"), (dict(ws=None), "workspace"), (dict(ws_bytes=16), "workspace"),
+    (dict(max_pages=1 << 25), "pages"), (dict(S=1 << 28), "rows"), (dict(ws=None), "workspace"), (dict(ws_bytes=16), "workspace"),
     (dict(S=-1), "sizes"),
 ])
 def test_attention_arguments(lib, change, word):
