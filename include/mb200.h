@@ -234,8 +234,9 @@ int mb_attention_prefill_bf16(const uint16_t* q, int ldq, const uint16_t* k_cach
  *
  * block_table [B][max_pages], kv_len, start_pos, new_len [B] are int32 in
  * device memory. A position outside the table, or a table entry outside
- * 0..num_pages-1, is never accessed: it is skipped (not stored; read back as
- * zeros; not attended) and recorded in the device status word (0x8). */
+ * 0..num_pages-1, is never accessed: it is not stored, is read back as zeros,
+ * leaves the attention rows of its sequence unspecified, and is recorded in the
+ * device status word (0x8). */
 
 /* Bytes of one page of all Hkv heads. */
 size_t mb_kv4_page_bytes(int Hkv);

@@ -842,11 +842,34 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
   return MB_OK;
 }
 
+// Pieces of a prompt: from TC_ROWS rows a sequence on, unpacking every page
+// once a row tile of 16 costs more than expanding the cache to bf16 pages in
+// the workspace and running the tcgen05 prefill attention over those.
+constexpr int TC_ROWS = 64;
+
+struct Expand {
+  int seqs;  // sequences expanded at a time: up to 512 MB of pages, at least one
+  size_t pages, bytes;
+};
+
+bool expand_plan(int B, int S, int Hq, int Hkv, int max_pages, Expand* e) {
+  const int64_t per_seq = (int64_t)max_pages * Hkv * PAGE * DH * 2;  // keys or values, bytes
+  if (S < TC_ROWS || Hq > 65535 || Hkv > 65535 || (int64_t)max_pages * Hkv * PAGE >= (1ll << 31)) return false;
+  int64_t n = (256ll << 20) / per_seq;
+  n = n < 1 ? 1 : n > 65535 ? 65535 : n;
+  e->seqs = (int)(n < B ? n : B);
+  e->pages = (size_t)per_seq * e->seqs;
+  e->bytes = 2 * e->pages + ((size_t)e->seqs * (max_pages + 2) * sizeof(int) + 15) / 16 * 16;
+  return true;
+}
+
 }  // namespace
 
 extern "C" size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages) {
   if (B <= 0 || S <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_pages <= 0) return 0;
-  return plan_launch(B, S, Hq, Hkv, max_pages).bytes;
+  const size_t n = plan_launch(B, S, Hq, Hkv, max_pages).bytes;
+  Expand e;
+  return expand_plan(B, S, Hq, Hkv, max_pages, &e) && e.bytes > n ? e.bytes : n;
 }
 
 extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache,
@@ -870,6 +893,27 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
              "attention kv4: workspace of %zu bytes required, 16-byte aligned", p.bytes);
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "attention kv4: no status word");
+  Expand e;
+  if (expand_plan(B, S, Hq, Hkv, max_pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
+      mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo)) {
+    MB_REQUIRE(workspace_bytes >= e.bytes, "attention kv4: workspace of %zu bytes required", e.bytes);
+    uint16_t* kx = static_cast<uint16_t*>(workspace);
+    uint16_t* vx = kx + e.pages / 2;
+    int* tx = reinterpret_cast<int*>(vx + e.pages / 2);
+    int *lx = tx + (size_t)e.seqs * max_pages, *sx = lx + e.seqs;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    for (int b = 0; b < B; b += e.seqs) {
+      const int n = B - b < e.seqs ? B - b : e.seqs;
+      int rc = mb::kv4_expand(cache, num_pages, Hkv, block_table + (int64_t)b * max_pages, max_pages, kv_len + b,
+                              start_pos ? start_pos + b : nullptr, n, kx, vx, tx, lx, sx, status, s);
+      if (!rc)
+        rc = mb::attention_prefill_tc(q + (int64_t)b * S * ldq, (int)ldq, kx, vx, tx, max_pages, sx, lx, n, S, Hq,
+                                      Hkv, start_pos != nullptr, out + (int64_t)b * S * ldo, (int)ldo, s, 1, 0,
+                                      nullptr, nullptr, scale);
+      if (rc) return rc;
+    }
+    return MB_OK;
+  }
   for (int b = 0; b < B; b += MAX_B) {
     Args a;
     a.q = q + (int64_t)b * S * ldq;

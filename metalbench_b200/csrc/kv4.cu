@@ -131,7 +131,62 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(
   dst[1] = make_float4(o[4], o[5], o[6], o[7]);
 }
 
+// Pages of B sequences as bf16 pages [B * max_pages][Hkv][64][128], with the
+// block table, lengths and first positions that go with them: one CTA a page
+// and kv head, lanes as in the storing kernel. A value is rounded to bf16 here
+// (2^-9 relative), as a bf16 cache would hold it.
+__global__ void __launch_bounds__(256) kv4_expand_kernel(
+    const uint8_t* __restrict__ cache, int num_pages, int Hkv, const int* __restrict__ table,
+    int max_pages, const int* __restrict__ kv_len, const int* __restrict__ start_pos,
+    uint16_t* __restrict__ ko, uint16_t* __restrict__ vo, int* __restrict__ table_o,
+    int* __restrict__ len_o, int* __restrict__ start_o, uint32_t* status) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int page = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int L = max(0, min(kv_len[b], max_pages * PAGE));
+  if (threadIdx.x == 0 && h == 0 && page == 0) {
+    len_o[b] = L;
+    start_o[b] = start_pos ? min(start_pos[b], L) : L;
+  }
+  if (page * PAGE >= L) return;
+  const int64_t to = (int64_t)b * max_pages + page;
+  if (threadIdx.x == 0 && h == 0) table_o[to] = (int)to;
+  const int pg = page_of(table, max_pages, num_pages, b, (int64_t)page * PAGE, status);
+  const uint8_t* blob = cache + ((int64_t)max(pg, 0) * Hkv + h) * BLOB;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  uint16_t* dst = (half ? vo : ko) + (to * Hkv + h) * (PAGE * DH) + l * 8;
+  const int par_at = half ? V_PARAMS : K_PARAMS;
+#pragma unroll
+  for (int i = 0; i < PAGE / 8; ++i) {
+    const int t = i * 8 + (threadIdx.x >> 5);
+    uint32_t w[4] = {};
+    if (pg >= 0 && page * PAGE + t < L) {  // the rest is read as zeros: what stands there may be anything
+      const uint32_t code = *reinterpret_cast<const uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4));
+      const uint32_t par = *reinterpret_cast<const uint32_t*>(blob + par_at + t * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(
+            fmaf(lo_bf(par), (float)((code >> (8 * j)) & 15u), hi_bf(par)),
+            fmaf(lo_bf(par), (float)((code >> (8 * j + 4)) & 15u), hi_bf(par)));
+        w[j] = *reinterpret_cast<const uint32_t*>(&x);
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + t * DH) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 }  // namespace
+
+namespace mb {
+int kv4_expand(const uint8_t* cache, int num_pages, int Hkv, const int* table, int max_pages,
+               const int* kv_len, const int* start_pos, int B, uint16_t* ko, uint16_t* vo,
+               int* table_o, int* len_o, int* start_o, uint32_t* status, cudaStream_t s) {
+  MB_CUDA(launch_pdl(kv4_expand_kernel, dim3(max_pages, Hkv, B), dim3(256), 0, s, cache, num_pages,
+                     Hkv, table, max_pages, kv_len, start_pos, ko, vo, table_o, len_o, start_o,
+                     status));
+  return MB_OK;
+}
+}  // namespace mb
 
 extern "C" size_t mb_kv4_page_bytes(int Hkv) { return Hkv > 0 ? (size_t)Hkv * kv4::BLOB : 0; }
 

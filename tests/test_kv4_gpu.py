@@ -176,19 +176,65 @@ def test_causal_rows(ops, S, Hq, Hkv):
     check_attention(ops, rng, 5, S, Hq, Hkv, lens, first=lens - S)  # some rows stand before the first key
 
 
-@pytest.mark.parametrize("S", [1, 4])
+@pytest.mark.parametrize("S, Hq, Hkv, lens, causal", [
+    (64, 8, 2, [200, 64, 0, 1], True), (65, 4, 4, [129, 65], False), (130, 5, 1, [130, 700], True),
+    (257, 8, 8, [300], True), (64, 16, 2, [128, 500, 63], False),
+])
+def test_pieces_of_a_prompt(ops, S, Hq, Hkv, lens, causal):
+    """Many rows a sequence: the cache is expanded to bf16 pages first."""
+    rng = np.random.default_rng(S + Hq)
+    lens = np.array(lens)
+    table, P = make_table(rng, lens)
+    cache = make_cache(rng, P, Hkv)
+    for b, n in enumerate(lens):  # what stands past the end of a sequence may be anything
+        if n % 64:
+            cache[table[b, n // 64], :, 8192 + 4 * (n % 64): 8448] = 0xFF
+            cache[table[b, n // 64], :, 8448 + 4 * (n % 64):] = 0xFF
+    q = R.bf16_round(rng.standard_normal((len(lens), S, Hq, 128)))
+    first = lens - S if causal else None  # some rows stand before the first key
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens), start_pos=None if first is None else i32(first))
+    ref, _ = R.attention(q, cache, table, lens, first)
+    slack = R.prompt_slack(q, cache, table, lens, first)
+    err = np.abs(got.double().cpu().numpy() - ref)
+    tol = slack + 2 ** -8 * (np.abs(ref) + slack)
+    assert (err <= tol).all(), float((err - tol).max())
+    if causal:  # the last rows again, few at a time: the other form
+        few = ops.attention_kv4(bf(q[:, -7:]), torch.from_numpy(cache).cuda(), i32(table), i32(lens), start_pos=i32(first + S - 7))
+        err = np.abs(got[:, -7:].double().cpu().numpy() - few.double().cpu().numpy())
+        assert (err <= tol[:, -7:] * 2).all()
+    neg = ops.attention_kv4(bf(q[:, :, :]), torch.from_numpy(cache).cuda(), i32(table), i32(lens), scale=-128 ** -0.5)
+    ref, slack = R.attention(q, cache, table, lens, None, -(128 ** -0.5))
+    assert (np.abs(neg.double().cpu().numpy() - ref) <= np.abs(slack) + 2 ** -8 * (np.abs(ref) + np.abs(slack))).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("S", [1, 4, 70])
 def test_rows_that_see_nothing_are_zero(ops, S):
     rng = np.random.default_rng(9)
-    check_attention(ops, rng, 3, S, 8, 2, np.array([100, 100, 64]), first=np.array([-100, -2, -(2 ** 31)]))
+    if S < 64:
+        check_attention(ops, rng, 3, S, 8, 2, np.array([100, 100, 64]), first=np.array([-100, -2, -(2 ** 31)]))
+    cache, table = torch.from_numpy(make_cache(rng, 6, 2)).cuda(), i32([[0, 1], [2, 3], [4, 5]])
+    q = bf(rng.standard_normal((3, S, 8, 128)))
+    got = ops.attention_kv4(q, cache, table, i32([100, 0, 64]), start_pos=i32([-S, 5, -(2 ** 31)]))
+    assert (got == 0).all()
 
 
 def test_start_far_past_the_end_sees_every_key(ops):
     check_attention(ops, np.random.default_rng(10), 2, 3, 8, 2, np.array([100, 64]), first=np.array([2 ** 31 - 1, 64]))
+    rng = np.random.default_rng(10)
+    cache, table = torch.from_numpy(make_cache(rng, 3, 2)).cuda(), i32([[0, 1], [2, 2]])
+    q = bf(rng.standard_normal((2, 80, 8, 128)))
+    far, every = (ops.attention_kv4(q, cache, table, i32([100, 64]), start_pos=p) for p in (i32([2 ** 31 - 1, 64]), None))
+    assert torch.equal(far, every)
 
 
 def test_whole_cta_shares_and_many_units(ops):
-    """More (sequence, head) units than CTAs, and one unit over all of them."""
+    """More (sequence, head) units than shares, more sequences than one launch
+    plans (512), and one unit over all shares."""
     rng = np.random.default_rng(11)
+    lens = rng.integers(0, 80, 700)
+    check_attention(ops, rng, 700, 1, 2, 2, lens, garbage=False)
+    check_attention(ops, rng, 513, 3, 6, 1, np.minimum(lens[:513], 70), first=np.minimum(lens[:513], 70) - 3)
     check_attention(ops, rng, 70, 1, 16, 16, rng.integers(0, 200, 70), garbage=False)
     check_attention(ops, rng, 1, 1, 8, 1, np.array([70001]), garbage=False)
 
