@@ -37,6 +37,8 @@
 // which plans for itself while the last warps stream, joins it.
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "kv4.cuh"
 #include "kernels.h"
 
@@ -842,9 +844,16 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
   return MB_OK;
 }
 
-// Pieces of a prompt: from TC_ROWS rows a sequence on, unpacking every page
-// once a row tile of 16 costs more than expanding the cache to bf16 pages in
-// the workspace and running the tcgen05 prefill attention over those.
+// Pieces of a prompt (64 rows a sequence or more): instead of unpacking every
+// page once a row tile of 16, expand the cache once to bf16 pages in the
+// workspace and run the tcgen05 prefill attention over those, where the times
+// (us) that expand_plan expects say so: 0.29 a page and row tile on one SM, or
+// 1.37 a 128-key tile and wave of CTAs and the expanded bytes at 5.5 TB/s. Measured in us, expanded / unpacked:
+//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 111 / 81,
+//     128 rows 113 / 144, 512 rows 202 / 513 (the prefill kernel takes 1.37 us
+//     a 128-key tile one after another, so few CTAs leave SMs idle);
+//   16 of 2048, 8, 4:  64 rows 143 / 149, 128 rows 149 / 276;
+//   1 of 1024, 8, 1:  128 rows 21 / 17;  8 of 512, 8, 4:  64 rows 27 / 46.
 constexpr int TC_ROWS = 64;
 
 struct Expand {
@@ -860,7 +869,12 @@ bool expand_plan(int B, int S, int Hq, int Hkv, int max_pages, Expand* e) {
   e->seqs = (int)(n < B ? n : B);
   e->pages = (size_t)per_seq * e->seqs;
   e->bytes = 2 * e->pages + ((size_t)e->seqs * (max_pages + 2) * sizeof(int) + 15) / 16 * 16;
-  return true;
+  const double sms = mb::num_sms(), pages = (double)B * Hkv * max_pages;
+  const double unpack = 14 + pages * plan_launch(B, S, Hq, Hkv, max_pages).rt * 0.29 / sms;
+  const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128);
+  const double expand = 3 + calls * (6 + std::ceil(ctas / sms) * ((max_pages + 1) / 2) * 1.37) +
+                        pages * (BLOB + 2 * PAGE * DH * 2) / 5.5e6;
+  return expand < unpack;
 }
 
 }  // namespace
