@@ -5,7 +5,8 @@
 Every ``csrc/*.cu`` is compiled with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` into ``_build/`` and
 linked (static cudart, NCCL from the torch-bundled wheel or the system) into
-``metalbench_b200/libmb200.so``. Objects are rebuilt only when a source or
+``metalbench_b200/libmb200.so``; ``host/kv4_ext.cpp`` becomes the extension
+module ``metalbench_b200/_kv4.so`` (torch's headers, libmb200.so). Objects are rebuilt only when a source or
 header is newer. No GPU is needed.
 """
 from __future__ import annotations
@@ -24,6 +25,7 @@ CSRC = PKG / "csrc"
 BUILD = REPO / "_build"
 LIB = PKG / "libmb200.so"
 HOST = PKG / "mb200_host"
+EXT = PKG / "_kv4.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -107,7 +109,31 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         p = subprocess.run(cmd, capture_output=True, text=True)
         if p.returncode != 0:
             raise RuntimeError(f"mb200_host build failed:\n{p.stdout}\n{p.stderr}")
+    ext_src = PKG / "host" / "kv4_ext.cpp"
+    if force or _stale(EXT, [ext_src] + list((REPO / "include").glob("*.h"))):
+        build_ext(ext_src)
     return LIB
+
+
+def build_ext(src: Path) -> None:
+    """The CPython extension on torch's tensors (its symbols are resolved from
+    the libraries that `import torch` has loaded)."""
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent / "include"
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda,
+           Path(sysconfig.get_paths()["include"])]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for i in inc:
+        cmd += ["-isystem", str(i)]
+    cmd += [str(src), "-o", str(EXT), "-L", str(PKG), "-l:libmb200.so", "-L", str(root / "lib"),
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"_kv4 build failed:\n{p.stdout}\n{p.stderr}")
 
 
 def main(argv=None):
