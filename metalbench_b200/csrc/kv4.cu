@@ -6,13 +6,13 @@
 //   m = min x,  s = bf16((max x - m) / 15),  u = clamp(rint((x - m) / s), 0, 15)
 // with u = 0 where s = 0; the stored value is m + s u. m is exact (x is bf16);
 // s is rounded to bf16 (2^-9 relative: at most 3 % of one code step at u = 15)
-// because its 2 bytes a token are read by every later step. The arithmetic is
-// IEEE fp32 with one rounding per operation.
+// because its 2 bytes a token are read by every later step.
 #include "kv4.cuh"
 #include "kernels.h"
 
 namespace {
 using namespace kv4;
+static_assert(PAGE == 64, "positions are split by shifts");
 
 __device__ __forceinline__ float min_nan(float a, float b) {  // a NaN stays one
   float r;
@@ -35,30 +35,13 @@ __device__ __forceinline__ int page_of(const int* __restrict__ table, int max_pa
   return -1;
 }
 
-// One warp stores one (token, kv head): lanes 0-15 the key, lanes 16-31 the
-// value, eight dims a lane, so that minimum and maximum take four shuffles and
-// every lane packs one 32-bit word of codes.
-__global__ void __launch_bounds__(256) kv4_append_kernel(
-    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t stride_b,
-    int64_t stride_s, int64_t stride_h, int64_t vstride_b, int64_t vstride_s, int64_t vstride_h,
-    uint8_t* __restrict__ cache, int num_pages, int Hkv, const int* __restrict__ table,
-    int max_pages, const int* __restrict__ start_pos, const int* __restrict__ new_len, int64_t total,
-    int S, uint32_t* status) {
-  mbd::pdl_trigger();
-  mbd::pdl_wait();
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= total) return;
-  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
-  const int64_t tok = item / Hkv;
-  const int h = (int)(item - tok * Hkv);
-  const int b = (int)(tok / S), s = (int)(tok - (int64_t)b * S);
-  if (new_len && s >= new_len[b]) return;
-  const int64_t pos = (int64_t)start_pos[b] + s;
-  const uint16_t* src = half ? v + b * vstride_b + s * vstride_s + h * vstride_h
-                             : k + b * stride_b + s * stride_s + h * stride_h;
-  const uint4 raw = *reinterpret_cast<const uint4*>(src + l * 8);
-  const int pg = page_of(table, max_pages, num_pages, b, pos, status);
-  if (pg < 0) return;
+// One half-warp's 8 dims a lane of a row of 128: codes of one 32-bit word, and
+// the row's scale and minimum (the same in every lane of the half). A call, not
+// inlined: eight copies in a loop over rows miss the instruction cache.
+struct Row {
+  uint32_t code, par;
+};
+__device__ __noinline__ Row quantise(uint4 raw) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   float x[8];
 #pragma unroll
@@ -66,69 +49,218 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(
     x[2 * i] = lo_bf(w[i]);
     x[2 * i + 1] = hi_bf(w[i]);
   }
-  float lo = x[0], hi = x[0];
+  float lo = x[0], hi = x[0], tiny = fabsf(x[0]);
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
     lo = min_nan(lo, x[i]);
     hi = max_nan(hi, x[i]);
+    tiny = fminf(tiny, fabsf(x[i]));
   }
 #pragma unroll
   for (int off = 8; off; off >>= 1) {
     lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
     hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
   }
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f));
+  // Quotients: y (1 / c) corrected once by its exact remainder is within half a
+  // last place of y / c, and what is exactly halfway comes out exactly.
+  const float range = hi - lo;
+  const float q15 = range * (1.f / 15.f);
+  const bool plain = range >= 0x1p-100f && range < INFINITY;  // no subnormals on the way
+  const __nv_bfloat16 sb = __float2bfloat16_rn(plain ? fmaf(fmaf(-15.f, q15, range), 1.f / 15.f, q15)
+                                                     : __fdiv_rn(range, 15.f));
   const float sc = __bfloat162float(sb);
-  uint32_t code = 0;
-  if (sc > 0.f) {
+  Row r;
+  r.par = (uint32_t)__bfloat16_as_ushort(sb) | (__float_as_uint(lo) & 0xFFFF0000u);
+  // x - m is exact in fp32 unless x is smaller than 2^-15 of the range (or
+  // zero, which the test does not tell apart): those rows go the long way.
+  // A remainder d - s q is exact too (s has 8 bits), so with q' next to d / s
+  // adding 1.5 * 2^23 rounds to the nearest whole number, ties to the even one:
+  // a d that is no tie is off one by more than half a last place of q'.
+  if (plain && tiny >= range * 0x1p-15f) {
+    const float inv = __frcp_rn(sc);
+    uint32_t sum = 0;  // of (bits of 1.5 * 2^23 + u) * 16^i: u <= 15, as s is within 2^-9 of range / 15
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = fminf(fmaxf(rintf(__fdiv_rn(x[i] - lo, sc)), 0.f), 15.f);
-      code |= (uint32_t)u << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+      const float d = x[i] - lo, q = d * inv;
+      sum = sum * 16u + __float_as_uint(fmaf(fmaf(-sc, q, d), inv, q) + 12582912.f);
+    }
+    r.code = sum - 0x4B400000u * 0x11111111u;
+  } else {
+    r.code = 0;
+    if (sc > 0.f) {
+      const float half = 0.5f * sc;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = x[i] - lo, b = d - x[i];
+        const float lost = (x[i] - (d - b)) + (-lo - b);  // x - m = d + lost, exactly
+        float u = fminf(fmaxf(rintf(__fdiv_rn(d, sc)), 0.f), 15.f);
+        const float e = fmaf(-sc, u, d);
+        const bool odd = (int)u & 1;
+        if (e > half || (e == half && (lost > 0.f || (lost == 0.f && odd)))) u += 1.f;
+        else if (e < -half || (e == -half && (lost < 0.f || (lost == 0.f && odd)))) u -= 1.f;
+        r.code |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
+      }
     }
   }
-  uint8_t* blob = cache + ((int64_t)pg * Hkv + h) * BLOB;
-  const int t = (int)(pos & (PAGE - 1));
-  *reinterpret_cast<uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4)) = code;
-  if (l == 0) {
-    const uint32_t par = (uint32_t)__bfloat16_as_ushort(sb) | (__float_as_uint(lo) & 0xFFFF0000u);
-    *reinterpret_cast<uint32_t*>(blob + (half ? V_PARAMS : K_PARAMS) + t * 4) = par;
-  }
+  return r;
 }
 
-// Positions start_pos[b] .. start_pos[b] + S - 1 back as fp32 [B][S][Hkv][128]
-// (zeros at and past kv_len[b]); lanes as in the storing kernel.
-__global__ void __launch_bounds__(256) kv4_gather_kernel(
-    const uint8_t* __restrict__ cache, int num_pages, int Hkv, const int* __restrict__ table,
-    int max_pages, const int* __restrict__ start_pos, const int* __restrict__ kv_len, int64_t total,
-    int S, float* __restrict__ ko, float* __restrict__ vo, uint32_t* status) {
+// Few tokens a sequence (decode): one warp stores one (token, kv head), lanes
+// 0-15 the key, lanes 16-31 the value, eight dims a lane, so that minimum and
+// maximum take four shuffles and every lane packs one 32-bit word of codes.
+// What bounds it is the chain of loads, length -> page -> store.
+struct AppendArgs {
+  const uint16_t *k, *v;
+  int64_t kb, ks, kh, vb, vs, vh;  // element strides: batch, token, head
+  uint8_t* cache;
+  const int *table, *start_pos, *new_len;
+  int num_pages, max_pages, Hkv, S;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ const uint16_t* row_at(const AppendArgs& a, int half, int b, int s, int h) {
+  return half ? a.v + b * a.vb + s * a.vs + h * a.vh : a.k + b * a.kb + s * a.ks + h * a.kh;
+}
+__device__ __forceinline__ void put(uint8_t* blob, int half, int l, int t, Row r) {
+  *reinterpret_cast<uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4)) = r.code;
+  if (l == 0) *reinterpret_cast<uint32_t*>(blob + (half ? V_PARAMS : K_PARAMS) + t * 4) = r.par;
+}
+
+__global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a, int64_t total) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (item >= total) return;
   const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
-  const int64_t tok = item / Hkv;
-  const int h = (int)(item - tok * Hkv);
-  const int b = (int)(tok / S), s = (int)(tok - (int64_t)b * S);
-  const int64_t pos = (int64_t)start_pos[b] + s;
-  float o[8] = {};
-  if (pos < kv_len[b]) {
-    const int pg = page_of(table, max_pages, num_pages, b, pos, status);
-    if (pg >= 0) {
-      const uint8_t* blob = cache + ((int64_t)pg * Hkv + h) * BLOB;
-      const int t = (int)(pos & (PAGE - 1));
-      const uint32_t code =
-          *reinterpret_cast<const uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4));
-      const uint32_t par =
-          *reinterpret_cast<const uint32_t*>(blob + (half ? V_PARAMS : K_PARAMS) + t * 4);
+  const int64_t tok = item / a.Hkv;
+  const int h = (int)(item - tok * a.Hkv), b = (int)(tok / a.S), s = (int)(tok - (int64_t)b * a.S);
+  const uint4 raw = *reinterpret_cast<const uint4*>(row_at(a, half, b, s, h) + l * 8);
+  if (a.new_len && s >= a.new_len[b]) return;
+  const int64_t pos = (int64_t)a.start_pos[b] + s;
+  const int pg = page_of(a.table, a.max_pages, a.num_pages, b, pos, a.status);
+  if (pg < 0) return;
+  put(a.cache + ((int64_t)pg * a.Hkv + h) * BLOB, half, l, (int)(pos & (PAGE - 1)), quantise(raw));
+}
+
+// Many tokens a sequence (prompts): a CTA stores all heads of 2^lt tokens that
+// lie in one page, 64 rows (token, head) at a time, heads first, so that it
+// reads whole rows of a projection's output, looks one page up, and has eight
+// rows a half-warp in flight. (A CTA a page and head, 256-byte pieces 6 KB
+// apart, took 37 us for 4 x 2048 tokens of 8 heads where this takes 9.)
+__global__ void __launch_bounds__(256) kv4_append_tokens_kernel(const AppendArgs a, int lt) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int b = blockIdx.y;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int64_t start = a.start_pos[b];
+  const int n = a.new_len ? min(a.new_len[b], a.S) : a.S;
+  const int64_t p0 = ((start >> lt) + blockIdx.x) << lt;  // first position of this CTA
+  const int64_t from = max(p0, start), to = min(p0 + (1 << lt), start + n);
+  if (from >= to) return;
+  const int rows = (int)(to - from) * a.Hkv;
+  int pg = -1;
+  for (int base = 0; base < rows; base += 64) {
+    uint4 raw[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)  // one rounding: scale * code is exact (8 + 4 bits)
-        o[i] = fmaf(lo_bf(par), (float)((code >> (4 * i)) & 15u), hi_bf(par));
+    for (int i = 0; i < 8; ++i) {
+      const int r = base + i * 8 + (threadIdx.x >> 5), s = r / a.Hkv;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows)
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(row_at(a, half, b, (int)(from - start) + s, r - s * a.Hkv) + l * 8));
+    }
+    if (base == 0) pg = page_of(a.table, a.max_pages, a.num_pages, b, p0, a.status);
+    if (pg < 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = base + i * 8 + (threadIdx.x >> 5), s = r / a.Hkv;
+      if (r >= rows) continue;  // the same for the whole warp
+      put(a.cache + ((int64_t)pg * a.Hkv + (r - s * a.Hkv)) * BLOB, half, l, (int)((from + s) & (PAGE - 1)),
+          quantise(raw[i]));
     }
   }
-  float4* dst = reinterpret_cast<float4*>((half ? vo : ko) + item * DH + l * 8);
-  dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+}
+
+// Positions start_pos[b] .. start_pos[b] + S - 1 back as fp32 [B][S][Hkv][128]
+// (zeros at and past kv_len[b]); rows, lanes and the two forms as for storing.
+struct GatherArgs {
+  const uint8_t* cache;
+  const int *table, *start_pos, *kv_len;
+  float *ko, *vo;
+  int num_pages, max_pages, Hkv, S;
+  uint32_t* status;
+};
+
+// Lane l of a half-warp: dims 4 l .. 4 l + 3 (low half of x) and 64 more, so
+// that both 16-byte stores of a row are contiguous over the lanes.
+__device__ __forceinline__ uint2 get(const uint8_t* blob, int half, int l, int t) {
+  const uint8_t* p = half ? blob + v_word(t, l >> 1) : blob + t * ROW + (l >> 1) * 4;
+  const uint8_t* p2 = half ? blob + v_word(t, 8 + (l >> 1)) : p + 32;
+  const uint32_t c = *reinterpret_cast<const uint16_t*>(p + (l & 1) * 2), c2 = *reinterpret_cast<const uint16_t*>(p2 + (l & 1) * 2);
+  return make_uint2(c | (c2 << 16), *reinterpret_cast<const uint32_t*>(blob + (half ? V_PARAMS : K_PARAMS) + t * 4));
+}
+__device__ __forceinline__ void write_row(float* row, int l, uint2 x) {
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)  // one rounding: scale * code is exact (8 + 4 bits)
+    o[j] = fmaf(lo_bf(x.y), (float)((x.x >> (4 * j)) & 15u), hi_bf(x.y));
+  __stcs(reinterpret_cast<float4*>(row) + l, make_float4(o[0], o[1], o[2], o[3]));
+  __stcs(reinterpret_cast<float4*>(row) + 16 + l, make_float4(o[4], o[5], o[6], o[7]));
+}
+
+__global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherArgs a, int64_t total) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (item >= total) return;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int64_t tok = item / a.Hkv;
+  const int h = (int)(item - tok * a.Hkv), b = (int)(tok / a.S), s = (int)(tok - (int64_t)b * a.S);
+  const int64_t pos = (int64_t)a.start_pos[b] + s;
+  uint2 x = make_uint2(0, 0);  // reads as zeros
+  if (pos < a.kv_len[b]) {
+    const int pg = page_of(a.table, a.max_pages, a.num_pages, b, pos, a.status);
+    if (pg >= 0) x = get(a.cache + ((int64_t)pg * a.Hkv + h) * BLOB, half, l, (int)(pos & (PAGE - 1)));
+  }
+  write_row((half ? a.vo : a.ko) + item * DH, l, x);
+}
+
+__global__ void __launch_bounds__(256) kv4_gather_tokens_kernel(const GatherArgs a, int lt) {
+  mbd::pdl_trigger();
+  mbd::pdl_wait();
+  const int b = blockIdx.y;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int64_t start = a.start_pos[b], end = a.kv_len[b];
+  const int64_t p0 = ((start >> lt) + blockIdx.x) << lt;
+  const int64_t from = max(p0, start), to = min(p0 + (1 << lt), start + a.S);
+  if (from >= to) return;
+  int pg = -1;
+  if (from < end) pg = page_of(a.table, a.max_pages, a.num_pages, b, p0, a.status);
+  const int rows = (int)(to - from) * a.Hkv;
+  const int there = pg < 0 ? 0 : (int)(min(to, end) - from) * a.Hkv;  // the rest reads as zeros
+  const int64_t out = (((int64_t)b * a.S + (from - start)) * a.Hkv) * DH;
+  for (int base = 0; base < rows; base += 64) {
+    uint2 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = base + i * 8 + (threadIdx.x >> 5), s = r / a.Hkv;
+      x[i] = make_uint2(0, 0);
+      if (r < there)
+        x[i] = get(a.cache + ((int64_t)pg * a.Hkv + (r - s * a.Hkv)) * BLOB, half, l, (int)((from + s) & (PAGE - 1)));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = base + i * 8 + (threadIdx.x >> 5);
+      if (r < rows) write_row((half ? a.vo : a.ko) + out + (int64_t)r * DH, l, x[i]);
+    }
+  }
+}
+
+// Tokens a CTA takes in the form for many: 64 rows, a power of two within a
+// page; -1: few tokens a sequence, a warp each.
+int log_tokens(int S, int Hkv) {
+  int lt = 6;
+  while (lt > 0 && (Hkv << lt) > 64) --lt;
+  return S >= 32 && S >= (1 << lt) ? lt : -1;
 }
 
 // Pages of B sequences as bf16 pages [B * max_pages][Hkv][64][128], with the
@@ -206,11 +338,17 @@ extern "C" int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, int64_t 
              "kv4 append: strides must be multiples of 8 elements");
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "kv4 append: no status word");
+  const AppendArgs a = {k,     v,           k_batch,   k_token, k_head,    v_batch,   v_token, v_head, cache,
+                        block_table, start_pos, new_len, num_pages, max_pages, Hkv,     S,      status};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int lt = log_tokens(S, Hkv);
+  if (lt >= 0 && B <= 65535) {
+    MB_CUDA(mb::launch_pdl(kv4_append_tokens_kernel, dim3((S >> lt) + 2, B), dim3(256), 0, s, a, lt));
+    return MB_OK;
+  }
   const int64_t total = (int64_t)B * S * Hkv;
   MB_REQUIRE((total + 7) / 8 <= 0x7fffffff, "kv4 append: too many tokens");
-  MB_CUDA(mb::launch_pdl(kv4_append_kernel, dim3((unsigned)((total + 7) / 8)), dim3(256), 0,
-                         static_cast<cudaStream_t>(stream), k, v, k_batch, k_token, k_head,
-                         v_batch, v_token, v_head, cache, num_pages, Hkv, block_table, max_pages, start_pos, new_len, total, S, status));
+  MB_CUDA(mb::launch_pdl(kv4_append_kernel, dim3((unsigned)((total + 7) / 8)), dim3(256), 0, s, a, total));
   return MB_OK;
 }
 
@@ -227,10 +365,15 @@ extern "C" int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv,
              "kv4 gather: the outputs and the cache must be 16-byte aligned");
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "kv4 gather: no status word");
+  const GatherArgs a = {cache, block_table, start_pos, kv_len, k_out, v_out, num_pages, max_pages, Hkv, S, status};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int lt = log_tokens(S, Hkv);
+  if (lt >= 0 && B <= 65535) {
+    MB_CUDA(mb::launch_pdl(kv4_gather_tokens_kernel, dim3((S >> lt) + 2, B), dim3(256), 0, s, a, lt));
+    return MB_OK;
+  }
   const int64_t total = (int64_t)B * S * Hkv;
   MB_REQUIRE((total + 7) / 8 <= 0x7fffffff, "kv4 gather: too many tokens");
-  MB_CUDA(mb::launch_pdl(kv4_gather_kernel, dim3((unsigned)((total + 7) / 8)), dim3(256), 0,
-                         static_cast<cudaStream_t>(stream), cache, num_pages, Hkv, block_table,
-                         max_pages, start_pos, kv_len, total, S, k_out, v_out, status));
+  MB_CUDA(mb::launch_pdl(kv4_gather_kernel, dim3((unsigned)((total + 7) / 8)), dim3(256), 0, s, a, total));
   return MB_OK;
 }

@@ -108,10 +108,12 @@ def test_append_of_odd_rows(ops):
     """All dims alike, NaN, infinities, subnormals, the type's extremes: each
     only ever changes its own token."""
     big = 3.3895313892515355e38  # the largest bf16
-    rows = [np.full(128, 1.5), np.zeros(128), np.linspace(-1, 1, 128), np.full(128, np.nan), np.full(128, np.inf),
+    edge = np.linspace(-19, 11, 128)  # scale 2: a number next to nothing lies next to the border 9.5
+    edge[3:6] = -3.67e-7, 3.67e-7, 0
+    rows = [edge, np.arange(128) / 8 - 4, np.full(128, 1.5), np.zeros(128), np.linspace(-1, 1, 128), np.full(128, np.nan), np.full(128, np.inf),
             np.full(128, 1e-39), np.linspace(0, 9e-39, 128), np.linspace(-1e4, 1e4, 128), np.linspace(0, big, 128)]
     x = np.stack([R.bf16_round(r) for r in rows])[None, :, None]
-    x[0, 2, 0, 5] = np.nan
+    x[0, 4, 0, 5] = np.nan
     cache = ops.kv4_cache(1, 1)
     S = x.shape[1]
     ops.kv4_append(bf(x), bf(x[:, ::-1].copy()), cache, i32([[0]]), i32([0]))
