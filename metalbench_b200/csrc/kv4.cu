@@ -14,14 +14,15 @@ namespace {
 using namespace kv4;
 static_assert(PAGE == 64, "positions are split by shifts");
 
-__device__ __forceinline__ float min_nan(float a, float b) {  // a NaN stays one
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// bf16 pairs; a NaN stays one.
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -35,31 +36,34 @@ __device__ __forceinline__ int page_of(const int* __restrict__ table, int max_pa
   return -1;
 }
 
-// One half-warp's 8 dims a lane of a row of 128: codes of one 32-bit word, and
-// the row's scale and minimum (the same in every lane of the half). A call, not
-// inlined: eight copies in a loop over rows miss the instruction cache.
+// W words (2 W dims) a lane of a row of 128, 64 / W lanes a row: W / 4 words of
+// codes, and the row's scale and minimum (the same in all its lanes). A call,
+// not inlined: copies in a loop over rows miss the instruction cache.
+template <int W>
 struct Row {
-  uint32_t code, par;
+  uint32_t code[W / 4], par;
 };
-__device__ __noinline__ Row quantise(uint4 raw) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
+template <int W>
+__device__ __noinline__ Row<W> quantise(uint4 ra, uint4 rb) {
+  const uint32_t w[8] = {ra.x, ra.y, ra.z, ra.w, rb.x, rb.y, rb.z, rb.w};
+  // minimum and maximum in packed bf16, then both at once as (min, -max)
+  uint32_t mn = w[0], mx = w[0], tn = w[0] & 0x7FFF7FFFu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 1; i < W; ++i) {
+    mn = min2(mn, w[i]);
+    mx = max2(mx, w[i]);
+    tn = min2(tn, w[i] & 0x7FFF7FFFu);
+  }
+  uint32_t both = min2(__byte_perm(mn, mx ^ 0x80008000u, 0x5410), __byte_perm(mn, mx ^ 0x80008000u, 0x7632));
+#pragma unroll
+  for (int off = 32 / W; off; off >>= 1) both = min2(both, __shfl_xor_sync(0xffffffffu, both, off));
+  const float lo = lo_bf(both), hi = -hi_bf(both);
+  const float tiny = fminf(lo_bf(tn), hi_bf(tn));
+  float x[2 * W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
     x[2 * i] = lo_bf(w[i]);
     x[2 * i + 1] = hi_bf(w[i]);
-  }
-  float lo = x[0], hi = x[0], tiny = fabsf(x[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
-    tiny = fminf(tiny, fabsf(x[i]));
-  }
-#pragma unroll
-  for (int off = 8; off; off >>= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
   }
   // Quotients: y (1 / c) corrected once by its exact remainder is within half a
   // last place of y / c, and what is exactly halfway comes out exactly.
@@ -69,7 +73,7 @@ __device__ __noinline__ Row quantise(uint4 raw) {
   const __nv_bfloat16 sb = __float2bfloat16_rn(plain ? fmaf(fmaf(-15.f, q15, range), 1.f / 15.f, q15)
                                                      : __fdiv_rn(range, 15.f));
   const float sc = __bfloat162float(sb);
-  Row r;
+  Row<W> r;
   r.par = (uint32_t)__bfloat16_as_ushort(sb) | (__float_as_uint(lo) & 0xFFFF0000u);
   // x - m is exact in fp32 unless x is smaller than 2^-15 of the range (or
   // zero, which the test does not tell apart): those rows go the long way.
@@ -78,19 +82,23 @@ __device__ __noinline__ Row quantise(uint4 raw) {
   // a d that is no tie is off one by more than half a last place of q'.
   if (plain && tiny >= range * 0x1p-15f) {
     const float inv = __frcp_rn(sc);
-    uint32_t sum = 0;  // of (bits of 1.5 * 2^23 + u) * 16^i: u <= 15, as s is within 2^-9 of range / 15
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-      const float d = x[i] - lo, q = d * inv;
-      sum = sum * 16u + __float_as_uint(fmaf(fmaf(-sc, q, d), inv, q) + 12582912.f);
+    for (int k = 0; k < W / 4; ++k) {
+      uint32_t sum = 0;  // of (bits of 1.5 * 2^23 + u) * 16^i: u <= 15, as s is within 2^-9 of range / 15
+#pragma unroll
+      for (int i = 7; i >= 0; --i) {
+        const float d = x[8 * k + i] - lo, q = d * inv;
+        sum = sum * 16u + __float_as_uint(fmaf(fmaf(-sc, q, d), inv, q) + 12582912.f);
+      }
+      r.code[k] = sum - 0x4B400000u * 0x11111111u;
     }
-    r.code = sum - 0x4B400000u * 0x11111111u;
   } else {
-    r.code = 0;
-    if (sc > 0.f) {
-      const float half = 0.5f * sc;
+    const float half = 0.5f * sc;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+    for (int k = 0; k < W / 4; ++k) r.code[k] = 0;
+    if (sc > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) {
         const float d = x[i] - lo, b = d - x[i];
         const float lost = (x[i] - (d - b)) + (-lo - b);  // x - m = d + lost, exactly
         float u = fminf(fmaxf(rintf(__fdiv_rn(d, sc)), 0.f), 15.f);
@@ -98,17 +106,13 @@ __device__ __noinline__ Row quantise(uint4 raw) {
         const bool odd = (int)u & 1;
         if (e > half || (e == half && (lost > 0.f || (lost == 0.f && odd)))) u += 1.f;
         else if (e < -half || (e == -half && (lost < 0.f || (lost == 0.f && odd)))) u -= 1.f;
-        r.code |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
+        r.code[i >> 3] |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * (i & 7));
       }
     }
   }
   return r;
 }
 
-// Few tokens a sequence (decode): one warp stores one (token, kv head), lanes
-// 0-15 the key, lanes 16-31 the value, eight dims a lane, so that minimum and
-// maximum take four shuffles and every lane packs one 32-bit word of codes.
-// What bounds it is the chain of loads, length -> page -> store.
 struct AppendArgs {
   const uint16_t *k, *v;
   int64_t kb, ks, kh, vb, vs, vh;  // element strides: batch, token, head
@@ -118,64 +122,84 @@ struct AppendArgs {
   uint32_t* status;
 };
 
-__device__ __forceinline__ const uint16_t* row_at(const AppendArgs& a, int half, int b, int s, int h) {
-  return half ? a.v + b * a.vb + s * a.vs + h * a.vh : a.k + b * a.kb + s * a.ks + h * a.kh;
+__device__ __forceinline__ const uint16_t* row_at(const AppendArgs& a, int val, int b, int s, int h) {
+  return val ? a.v + b * a.vb + s * a.vs + h * a.vh : a.k + b * a.kb + s * a.ks + h * a.kh;
 }
-__device__ __forceinline__ void put(uint8_t* blob, int half, int l, int t, Row r) {
-  *reinterpret_cast<uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4)) = r.code;
-  if (l == 0) *reinterpret_cast<uint32_t*>(blob + (half ? V_PARAMS : K_PARAMS) + t * 4) = r.par;
+template <int W>
+__device__ __forceinline__ void put(uint8_t* blob, int val, int l, int t, const Row<W>& r) {
+  uint8_t* at = blob + (val ? v_word(t, W / 4 * l) : t * ROW + l * W);
+  if (W == 4) *reinterpret_cast<uint32_t*>(at) = r.code[0];
+  else *reinterpret_cast<uint2*>(at) = make_uint2(r.code[0], r.code[W / 4 - 1]);
+  if (l == 0) *reinterpret_cast<uint32_t*>(blob + (val ? V_PARAMS : K_PARAMS) + t * 4) = r.par;
 }
 
+// Few tokens a sequence (decode): a warp stores one (token, kv head), lanes
+// 0-15 the key, lanes 16-31 the value. What bounds it is the chain of loads,
+// length -> page -> store (64 tokens of 8 heads: 3.8 us, and 4.9 us with eight
+// lanes a row, which stores prompts faster).
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a, int64_t total) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (item >= total) return;
-  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int lane = threadIdx.x & 31, val = lane >> 4, l = lane & 15;
   const int64_t tok = item / a.Hkv;
   const int h = (int)(item - tok * a.Hkv), b = (int)(tok / a.S), s = (int)(tok - (int64_t)b * a.S);
-  const uint4 raw = *reinterpret_cast<const uint4*>(row_at(a, half, b, s, h) + l * 8);
+  const uint4 x = __ldg(reinterpret_cast<const uint4*>(row_at(a, val, b, s, h)) + l);
   if (a.new_len && s >= a.new_len[b]) return;
   const int64_t pos = (int64_t)a.start_pos[b] + s;
   const int pg = page_of(a.table, a.max_pages, a.num_pages, b, pos, a.status);
   if (pg < 0) return;
-  put(a.cache + ((int64_t)pg * a.Hkv + h) * BLOB, half, l, (int)(pos & (PAGE - 1)), quantise(raw));
+  put(a.cache + ((int64_t)pg * a.Hkv + h) * BLOB, val, l, (int)(pos & (PAGE - 1)), quantise<4>(x, x));
 }
 
 // Many tokens a sequence (prompts): a CTA stores all heads of 2^lt tokens that
 // lie in one page, 64 rows (token, head) at a time, heads first, so that it
-// reads whole rows of a projection's output, looks one page up, and has eight
-// rows a half-warp in flight. (A CTA a page and head, 256-byte pieces 6 KB
-// apart, took 37 us for 4 x 2048 tokens of 8 heads where this takes 9.)
+// reads whole rows of a projection's output, looks one page up, and has four
+// rows a quarter-warp in flight. (A CTA a page and head, 256-byte pieces 6 KB
+// apart, took twice as long for 4 x 2048 tokens of 8 heads.)
 __global__ void __launch_bounds__(256) kv4_append_tokens_kernel(const AppendArgs a, int lt) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int b = blockIdx.y;
-  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int lane = threadIdx.x & 31, val = (lane >> 3) & 1, l = lane & 7;
   const int64_t start = a.start_pos[b];
   const int n = a.new_len ? min(a.new_len[b], a.S) : a.S;
   const int64_t p0 = ((start >> lt) + blockIdx.x) << lt;  // first position of this CTA
   const int64_t from = max(p0, start), to = min(p0 + (1 << lt), start + n);
   if (from >= to) return;
   const int rows = (int)(to - from) * a.Hkv;
-  int pg = -1;
+  // a lane's rows are 16 apart: token and head step along without dividing
+  const int first = (threadIdx.x >> 5) * 2 + (lane >> 4), ds = 16 / a.Hkv, dh = 16 - ds * a.Hkv;
+  const int64_t ss = val ? a.vs : a.ks, sh = val ? a.vh : a.kh;
+  const uint16_t* src = row_at(a, val, b, (int)(from - start), 0) + l * 16;
+  int s0 = first / a.Hkv, h0 = first - s0 * a.Hkv, pg = -1;
+  uint8_t* page = a.cache;
   for (int base = 0; base < rows; base += 64) {
-    uint4 raw[8];
+    uint4 x[4], y[4];
+    int s = s0, h = h0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = base + i * 8 + (threadIdx.x >> 5), s = r / a.Hkv;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows)
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(row_at(a, half, b, (int)(from - start) + s, r - s * a.Hkv) + l * 8));
+    for (int i = 0; i < 4; ++i) {
+      x[i] = y[i] = make_uint4(0, 0, 0, 0);
+      if (base + i * 16 + first < rows) {
+        const uint4* p = reinterpret_cast<const uint4*>(src + s * ss + h * sh);
+        x[i] = __ldg(p), y[i] = __ldg(p + 1);
+      }
+      s += ds, h += dh;
+      if (h >= a.Hkv) h -= a.Hkv, ++s;
     }
-    if (base == 0) pg = page_of(a.table, a.max_pages, a.num_pages, b, p0, a.status);
-    if (pg < 0) return;
+    if (base == 0) {
+      pg = page_of(a.table, a.max_pages, a.num_pages, b, p0, a.status);
+      if (pg < 0) return;
+      page += (int64_t)pg * a.Hkv * BLOB;
+    }
+    const int t0 = (int)(from & (PAGE - 1));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = base + i * 8 + (threadIdx.x >> 5), s = r / a.Hkv;
-      if (r >= rows) continue;  // the same for the whole warp
-      put(a.cache + ((int64_t)pg * a.Hkv + (r - s * a.Hkv)) * BLOB, half, l, (int)((from + s) & (PAGE - 1)),
-          quantise(raw[i]));
+    for (int i = 0; i < 4; ++i) {
+      const Row<8> r = quantise<8>(x[i], y[i]);  // all lanes: they shuffle
+      if (base + i * 16 + first < rows) put(page + (int64_t)h0 * BLOB, val, l, t0 + s0, r);
+      s0 += ds, h0 += dh;
+      if (h0 >= a.Hkv) h0 -= a.Hkv, ++s0;
     }
   }
 }
