@@ -106,6 +106,9 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return r;
 }
 
+// unit / RT and row / G; one row tile and one position are the decode step's
+__device__ __forceinline__ int head_of(const Args& a, int unit) { return a.RT == 1 ? unit : unit / a.RT; }
+__device__ __forceinline__ int pos_of(const Args& a, int r) { return a.S == 1 ? 0 : r / a.G; }
 __device__ __forceinline__ float fast_log2(float x) {
   float r;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -206,6 +209,10 @@ struct __align__(16) KeyParams {
   float lg, rv;  // log2 and reciprocal of the value scale
 };
 
+// Floats of a warp's state of one column tile, while warps join: 4 pieces of
+// 8 x 32 accumulators, each one bank further, and R, l, om of the 8 columns.
+constexpr int STATE = 1028 + 32;
+
 // A warp's running state over the pages of one unit: NT column tiles of 8.
 template <int NT>
 struct State {
@@ -228,6 +235,96 @@ struct State {
       for (int e = 0; e < 2; ++e) {
         R[t][e] = -INFINITY;
         l[t][e] = om[t][e] = 0.f;
+      }
+    }
+  }
+
+  // q of row tile rt as B fragments, scaled by a power of two; the factor that
+  // key scales take for it and the softmax scale. L keys in all, row s sees
+  // those at positions <= first + s.
+  __device__ __forceinline__ float load_q(const Args& a, int b, int kvh, int rt, int L, int first) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    // ---- q of this unit as B fragments, scaled by a power of two ----
+    float x[NT][32];
+    float big = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = rt * (NT * 8) + t * 8 + gid;
+      const int s = pos_of(a, r);
+      if (r < a.S * a.G) {
+        const uint4* p = reinterpret_cast<const uint4*>(
+            a.q + ((int64_t)b * a.S + s) * a.ldq + (kvh * a.G + (r - s * a.G)) * DH + 32 * tig);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 w = p[i];
+          x[t][8 * i] = lo_bf(w.x), x[t][8 * i + 1] = hi_bf(w.x), x[t][8 * i + 2] = lo_bf(w.y);
+          x[t][8 * i + 3] = hi_bf(w.y), x[t][8 * i + 4] = lo_bf(w.z), x[t][8 * i + 5] = hi_bf(w.z);
+          x[t][8 * i + 6] = lo_bf(w.w), x[t][8 * i + 7] = hi_bf(w.w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[t][i] = 0.f;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        big = fmaxf(big, fabsf(x[t][i]));
+        sum += x[t][i];
+      }
+#pragma unroll
+      for (int off = 1; off <= 2; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      const int mylim = min(L, first + s + 1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int from = (2 * tig + c) * 4;  // a lane whose fragment row is column 2 tig + c
+        qs[t][c] = __shfl_sync(0xffffffffu, sum, from);
+        lim[t][c] = __shfl_sync(0xffffffffu, mylim, from);
+      }
+    }
+#pragma unroll
+    for (int off = 1; off <= 16; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+    // 2^e brings the tile's largest to [2^11, 2^12)
+    const int e = max(-100, min(100, 11 - ((int)(__float_as_uint(big) >> 23) - 127)));
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23), up16 = up * 0.0625f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        qf[t][4 * w] = pack_h2(x[t][8 * w] * up, x[t][8 * w + 4] * up);
+        qf[t][4 * w + 1] = pack_h2(x[t][8 * w + 1] * up16, x[t][8 * w + 5] * up16);
+        qf[t][4 * w + 2] = pack_h2(x[t][8 * w + 2] * up, x[t][8 * w + 6] * up);
+        qf[t][4 * w + 3] = pack_h2(x[t][8 * w + 3] * up16, x[t][8 * w + 7] * up16);
+      }
+    return a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
+  }
+
+  // l and om are sums over a lane's keys until here.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) {
+          l[t][c] += __shfl_xor_sync(0xffffffffu, l[t][c], off);
+          om[t][c] += __shfl_xor_sync(0xffffffffu, om[t][c], off);
+        }
+  }
+
+  // The state in shared memory (STATE floats a column tile), for warps to join.
+  __device__ __forceinline__ void deposit(float* at) const {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float* to = at + t * STATE + lane;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)  // a piece's 8 numbers a lane; pieces one bank apart for the readers
+        to[i * 32 + (i >> 3)] = o[t][i >> 3][(i >> 2) & 1][i & 3] * ((i & 2) ? 0x1p20f : 0x1p24f);
+      if (gid == 0) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<float4*>(at + t * STATE + 1028 + (2 * tig + c) * 4) =
+              make_float4(R[t][c], l[t][c], om[t][c], 0.f);
       }
     }
   }
@@ -388,27 +485,81 @@ struct State {
   }
 };
 
-// Four dims a lane of one query row: finished (whole), or as a slot's partial.
-__device__ __forceinline__ void store_row(const Args& a, int b, int kvh, int r, int slot, int col, int cols,
-                                          bool whole, float R, float l, float4 o) {
+// One column (query row) of the states that warps deposited STEP floats apart,
+// `who` of them: reference, denominator, and four dims a lane. Every lane reads
+// every state's numbers: that is shorter than reducing over lanes.
+struct Joined {
+  float R, l;
+  float4 o;
+};
+template <int STEP, int MOST>
+__device__ __forceinline__ Joined join_row(const float* states, int col, uint32_t who) {
   const int lane = threadIdx.x & 31;
-  if (!whole) {
-    *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * cols + col) * DH + lane * 4) = o;
-    if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * cols + col) * 2) = make_float2(R, l);
-    return;
+  const float* ml = states + (col >> 3) * STATE + 1028 + (col & 7) * 4;
+  const float* zp = states + (col >> 3) * STATE + (lane >> 3) * (8 * 32 + 1) + (lane & 7) * 4 + ((col & 7) >> 1) + (col & 1) * 32;
+  // without branches, so that the loads of all states are in flight at once;
+  // what stands in the place of a state that is not there is read and dropped
+  float4 m[MOST];
+  Joined j;
+  j.R = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < MOST; ++w) {
+    m[w] = *reinterpret_cast<const float4*>(ml + w * STEP);
+    if (!((who >> w) & 1)) m[w].x = -INFINITY;
+    j.R = fmaxf(j.R, m[w].x);
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // 0: the row has seen no key
-  const __nv_bfloat162 h0 = __floats2bfloat162_rn(o.x * inv, o.y * inv);
-  const __nv_bfloat162 h1 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-  const int s = r / a.G;
-  uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH + lane * 4;
-  *reinterpret_cast<uint2*>(dst) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  j.l = 0.f;
+  j.o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < MOST; ++w) {
+    const float* z = zp + w * STEP;
+    float4 v = make_float4(z[0] + m[w].z, z[64] + m[w].z, z[128] + m[w].z, z[192] + m[w].z);
+    const bool in = (who >> w) & 1;
+    const float f = m[w].x == -INFINITY ? 0.f : fast_exp2(m[w].x - j.R);
+    j.l = in ? fmaf(m[w].y, f, j.l) : j.l;
+    j.o.x = in ? fmaf(v.x, f, j.o.x) : j.o.x;
+    j.o.y = in ? fmaf(v.y, f, j.o.y) : j.o.y;
+    j.o.z = in ? fmaf(v.z, f, j.o.z) : j.o.z;
+    j.o.w = in ? fmaf(v.w, f, j.o.w) : j.o.w;
+  }
+  return j;
 }
 
-// Floats of a warp's state of one column tile, while warps join: 4 pieces of
-// 8 x 32 accumulators, each one bank further, and R, l, om of the 8 columns.
-constexpr int STATE = 1028 + 32;
+// Where a row goes: finished to dst, or as a partial to o and ml, or (all null)
+// nowhere.
+struct To {
+  uint16_t* dst;
+  float *o, *ml;
+};
+__device__ __forceinline__ To row_to(const Args& a, int b, int kvh, int r, int slot, int col, int cols, bool whole) {
+  To t = {nullptr, nullptr, nullptr};
+  const int s = pos_of(a, r);
+  if (whole) t.dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
+  else t.o = a.part_o + ((int64_t)slot * cols + col) * DH, t.ml = a.part_ml + ((int64_t)slot * cols + col) * 2;
+  return t;
+}
+__device__ __forceinline__ void store_row(To t, float R, float l, float4 o) {
+  const int lane = threadIdx.x & 31;
+  if (t.o) {
+    *reinterpret_cast<float4*>(t.o + lane * 4) = o;
+    if (lane == 0) *reinterpret_cast<float2*>(t.ml) = make_float2(R, l);
+  }
+  if (t.dst) {
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // 0: the row has seen no key
+    const __nv_bfloat162 h0 = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+    const __nv_bfloat162 h1 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(t.dst + lane * 4) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  }
+}
+// Not inlined: it runs once, at the end of a CTA's life, when every instruction
+// of it would have to be fetched; a call without rows at the start, while the
+// first pages are on their way, has it in the instruction cache by then.
+template <int STEP, int MOST>
+__device__ __noinline__ void join_store(const float* states, int col, uint32_t who, To t) {
+  const Joined j = join_row<STEP, MOST>(states, col, who);
+  store_row(t, j.R, j.l, j.o);
+}
 
 template <int NT>
 struct Shared {
@@ -417,7 +568,7 @@ struct Shared {
   uint8_t ring[NW][ST][BLOB];
   KeyParams kp[NW][PAGE];
   float vmin[NW][PAGE];
-  int4 seg[NW];       // last unit, its first and end page in this share
+  int4 seg[NW];       // last unit's first page, sequence, number, and whether it starts and ends here
   uint64_t bar[NW][ST];
   int page_ok[NW][ST];
   Plan plan;
@@ -469,7 +620,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
         const int b = find_seq(pre, a.B, f);
         const int rem = f - pre[b], pages = (pre[b + 1] - pre[b]) / units;
         const int unit = rem / pages;
-        win_kvh = unit / a.RT;
+        win_kvh = head_of(a, unit);
         const int pid = a.table[(int64_t)b * a.max_pages + (rem - unit * pages)];
         win_ok = pid >= 0 && pid < a.num_pages;
         win_pid = win_ok ? pid : 0;
@@ -489,6 +640,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
     ++issued;
   };
   for (int i = 0; i < ST && i < mine; ++i) issue();
+  if (warp == 0) join_store<ST * BLOB / 4, NW>(reinterpret_cast<const float*>(sm.ring), 0, 0, To{nullptr, nullptr, nullptr});
   int used = 0;       // pages consumed
   bool dead = false;  // a copy never arrived: consume and load nothing more
   int dead_at = 0;
@@ -496,7 +648,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
   State<NT> z;
   // The state as finished rows (whole), or as the partial of a slot.
   auto emit = [&](int b, int unit, int slot, bool whole) {
-    const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
+    const int kvh = head_of(a, unit), rt = unit - kvh * a.RT;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -511,7 +663,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
         for (int i = 0; i < 16; ++i)  // dim 32 (i / 4) + 4 gid + i % 4
           v[i] = fmaf(z.o[t][i >> 2][(i >> 1) & 1][2 * (i & 1) + c], (i & 1) ? 0x1p20f : 0x1p24f, om);
         if (whole) {
-          const int s = r / a.G;
+          const int s = pos_of(a, r);
           uint16_t* dst = a.out + ((int64_t)b * a.S + s) * a.ldo + (kvh * a.G + (r - s * a.G)) * DH;
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
@@ -540,64 +692,13 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
     unit = (f0 - pre[b]) / pages;
     ub = pre[b] + unit * pages;  // flat index of the unit's first page
     const int f1 = min(end, ub + pages);
-    const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
+    const int kvh = head_of(a, unit), rt = unit - kvh * a.RT;
     const int L = seq_len(a, b);
     // row s sees the keys up to position first + s
     const int first = a.start_pos ? min(a.start_pos[b], L) : L;
     z.reset();
     {
-      // ---- q of this unit as B fragments, scaled by a power of two ----
-      float x[NT][32];
-      float big = 0.f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int r = rt * COLS + t * 8 + gid;
-        const int s = r / a.G;
-        if (r < a.S * a.G) {
-          const uint4* p = reinterpret_cast<const uint4*>(
-              a.q + ((int64_t)b * a.S + s) * a.ldq + (kvh * a.G + (r - s * a.G)) * DH + 32 * tig);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 w = p[i];
-            x[t][8 * i] = lo_bf(w.x), x[t][8 * i + 1] = hi_bf(w.x), x[t][8 * i + 2] = lo_bf(w.y);
-            x[t][8 * i + 3] = hi_bf(w.y), x[t][8 * i + 4] = lo_bf(w.z), x[t][8 * i + 5] = hi_bf(w.z);
-            x[t][8 * i + 6] = lo_bf(w.w), x[t][8 * i + 7] = hi_bf(w.w);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[t][i] = 0.f;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          big = fmaxf(big, fabsf(x[t][i]));
-          sum += x[t][i];
-        }
-#pragma unroll
-        for (int off = 1; off <= 2; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        const int mylim = min(L, first + s + 1);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int from = (2 * tig + c) * 4;  // a lane whose fragment row is column 2 tig + c
-          z.qs[t][c] = __shfl_sync(0xffffffffu, sum, from);
-          z.lim[t][c] = __shfl_sync(0xffffffffu, mylim, from);
-        }
-      }
-#pragma unroll
-      for (int off = 1; off <= 16; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-      // 2^e brings the tile's largest to [2^11, 2^12)
-      const int e = max(-100, min(100, 11 - ((int)(__float_as_uint(big) >> 23) - 127)));
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23), up16 = up * 0.0625f;
-      const float ck = a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          z.qf[t][4 * w] = pack_h2(x[t][8 * w] * up, x[t][8 * w + 4] * up);
-          z.qf[t][4 * w + 1] = pack_h2(x[t][8 * w + 1] * up16, x[t][8 * w + 5] * up16);
-          z.qf[t][4 * w + 2] = pack_h2(x[t][8 * w + 2] * up, x[t][8 * w + 6] * up);
-          z.qf[t][4 * w + 3] = pack_h2(x[t][8 * w + 3] * up16, x[t][8 * w + 7] * up16);
-        }
+      const float ck = z.load_q(a, b, kvh, rt, L, first);
       const int all_seen = min(L, first + (rt * COLS) / a.G + 1);  // keys that every column sees
 
       for (int f = f0; f < f1; ++f) {
@@ -620,15 +721,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
       }
     }
 
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int off = 4; off <= 16; off <<= 1) {
-          z.l[t][c] += __shfl_xor_sync(0xffffffffu, z.l[t][c], off);
-          z.om[t][c] += __shfl_xor_sync(0xffffffffu, z.om[t][c], off);
-        }
+    z.finish();
     if (f1 == end) break;  // the last one may go on in the next warp
     emit(b, unit, 2 * me, f0 == ub);
     f0 = f1;
@@ -638,74 +731,177 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
     for (int i = dead_at; i < issued; ++i) mbd::mbar_wait(bar + i % ST, (i / ST) & 1, nullptr, 0);
 
   // ---- neighbouring warps whose last unit is the same join their states ----
-  int4* seg = sm.seg;
-  if (lane == 0) seg[warp] = make_int4(ub, f0, end, b);
+  if (lane == 0) {
+    sm.seg[warp] = make_int4(ub, b, unit, (f0 == ub ? 1 : 0) | (end == ub + pages ? 2 : 0));
+  }
   __syncthreads();  // every ring is free: a warp's state takes the place of its pages
-  const bool prev = ub >= 0 && warp > 0 && seg[warp - 1].x == ub;
-  const bool next = ub >= 0 && warp + 1 < NW && seg[warp + 1].x == ub;
-  if (ub >= 0 && !prev && !next) emit(b, unit, 2 * me + (f0 == ub ? 1 : 0), f0 == ub && end == ub + pages);
-  float* mine_z = reinterpret_cast<float*>(ring);
-  if (prev || next) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float* to = mine_z + t * STATE + lane;
-#pragma unroll
-      for (int i = 0; i < 32; ++i)  // a piece's 8 numbers a lane; pieces one bank apart for the readers
-        to[i * 32 + (i >> 3)] = z.o[t][i >> 3][(i >> 2) & 1][i & 3] * ((i & 2) ? 0x1p20f : 0x1p24f);
-      if (gid == 0) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          *reinterpret_cast<float4*>(mine_z + t * STATE + 1028 + (2 * tig + c) * 4) =
-              make_float4(z.R[t][c], z.l[t][c], z.om[t][c], 0.f);
-      }
-    }
-  }
+  if (ub >= 0) z.deposit(reinterpret_cast<float*>(ring));
   __syncthreads();
-  // (run of warps, query row) pairs over all warps; a lane takes four dims
-  int item = 0;
-  for (int w0 = 0; w0 < NW;) {
-    const int4 sg = seg[w0];
-    int w1 = w0 + 1, gf1 = sg.z;
-    for (; w1 < NW && seg[w1].x == sg.x; ++w1) gf1 = seg[w1].z;
-    if (sg.x >= 0 && w1 > w0 + 1) {
-      const int gpages = (pre[sg.w + 1] - pre[sg.w]) / units, gunit = (sg.x - pre[sg.w]) / gpages;
-      const bool first_here = sg.y == sg.x, whole = first_here && gf1 == sg.x + gpages;
-      const int kvh = gunit / a.RT, rt = gunit - kvh * a.RT;
-      for (int col = 0; col < COLS; ++col, ++item) {
-        const int r = rt * COLS + col;
-        if (item % NW != warp || r >= a.S * a.G) continue;
-        const float* base = reinterpret_cast<const float*>(sm.ring[w0][0]) + (col >> 3) * STATE;
-        constexpr int STEP = ST * BLOB / 4;  // floats between two warps' states
-        float4 m = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-        if (lane < w1 - w0) m = *reinterpret_cast<const float4*>(base + lane * STEP + 1028 + (col & 7) * 4);
-        float R = m.x;
-#pragma unroll
-        for (int off = 8; off; off >>= 1) R = fmaxf(R, __shfl_xor_sync(0xffffffffu, R, off));
-        R = __shfl_sync(0xffffffffu, R, 0);  // the runs are at most 16 warps
-        const float f = m.x == -INFINITY ? 0.f : fast_exp2(m.x - R);
-        float l = m.y * f, om = m.z * f;
-#pragma unroll
-        for (int off = 8; off; off >>= 1) {
-          l += __shfl_xor_sync(0xffffffffu, l, off);
-          om += __shfl_xor_sync(0xffffffffu, om, off);
-        }
-        om = __shfl_sync(0xffffffffu, om, 0);
-        float4 o = make_float4(om, om, om, om);
-        const float* zp = base + (lane >> 3) * (8 * 32 + 1) + (lane & 7) * 4 + ((col & 7) >> 1) + (col & 1) * 32;
-#pragma unroll 4
-        for (int w = 0; w < w1 - w0; ++w, zp += STEP) {
-          const float fw = __shfl_sync(0xffffffffu, f, w);
-          o.x = fmaf(zp[0], fw, o.x);
-          o.y = fmaf(zp[64], fw, o.y);
-          o.z = fmaf(zp[128], fw, o.z);
-          o.w = fmaf(zp[192], fw, o.w);
-        }
-        store_row(a, sg.w, kvh, r, 2 * (blockIdx.x * a.active + w0) + (first_here ? 1 : 0), col, COLS, whole, R,
-                  __shfl_sync(0xffffffffu, l, 0), o);
-      }
-    }
-    w0 = w1;
+  // lane w knows warp w's last unit; runs of warps with the same one, each a
+  // row after the other, go round the warps
+  const int4 sg = lane < NW ? sm.seg[lane] : make_int4(-1, 0, 0, 0);
+  const int left = __shfl_up_sync(0xffffffffu, sg.x, 1);
+  const bool leads = sg.x >= 0 && (lane == 0 || left != sg.x);
+  const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+  const int nth = __popc(leaders & ((1u << lane) - 1)), items = __popc(leaders) * COLS;
+  for (int i = warp; i < items; i += NW) {
+    const int w0 = __ffs(__ballot_sync(0xffffffffu, leads && nth == i / COLS)) - 1, col = i % COLS;
+    const int gub = __shfl_sync(0xffffffffu, sg.x, w0), gb = __shfl_sync(0xffffffffu, sg.y, w0);
+    const int gunit = __shfl_sync(0xffffffffu, sg.z, w0), starts = __shfl_sync(0xffffffffu, sg.w, w0) & 1;
+    const uint32_t who = __ballot_sync(0xffffffffu, sg.x == gub);
+    const int ends = __shfl_sync(0xffffffffu, sg.w, 31 - __clz(who)) & 2;
+    const int gkvh = head_of(a, gunit), r = (gunit - gkvh * a.RT) * COLS + col;
+    if (r < a.S * a.G)
+      join_store<ST * BLOB / 4, NW>(reinterpret_cast<const float*>(sm.ring), col, who,
+                                    row_to(a, gb, gkvh, r, 2 * (blockIdx.x * a.active + w0) + starts, col, COLS,
+                                           starts && ends));
   }
+}
+
+// One sequence (B = 1): every length is the same, so a cluster of CTAs takes a
+// unit, its pages split evenly over the warps, and joins it over distributed
+// shared memory: nothing to plan, no partials in memory and no second kernel.
+// (8 kv heads: 517 keys 8.7 -> 7.5 us, 16000 keys 16.6 -> 11.3 us.)
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Address of the same shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(mbd::smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_one_kernel(const Args a) {
+  constexpr int COLS = NT * 8, NW = Shape<NT>::NW, ST = Shape<NT>::ST;
+  extern __shared__ __align__(128) uint8_t sm_raw[];
+  Shared<NT>& sm = *reinterpret_cast<Shared<NT>*>(sm_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = cluster_rank(), C = cluster_size();
+  const int unit = blockIdx.x / C, kvh = head_of(a, unit), rt = unit - kvh * a.RT;
+  uint8_t* ring = sm.ring[warp][0];
+  uint64_t* bar = sm.bar[warp];
+  int* ok_flag = sm.page_ok[warp];
+  if (lane == 0)
+    for (int i = 0; i < ST; ++i) mbd::mbar_init(bar + i, 1);
+  mbd::fence_mbar_init();
+  mbd::pdl_wait();
+  mbd::pdl_trigger();
+  const int L = seq_len(a, 0), pages = (L + PAGE - 1) / PAGE;
+  // warps of different CTAs side by side: a short sequence is spread over them
+  const int64_t share = warp * C + rank, shares = C * NW;
+  const int begin = (int)(pages * share / shares), end = (int)(pages * (share + 1) / shares), mine = end - begin;
+  int issued = 0, win_pid = 0, win_ok = 0;
+  auto issue = [&]() {
+    if ((issued & 31) == 0 && begin + issued + lane < end) {
+      const int pid = a.table[begin + issued + lane];
+      win_ok = pid >= 0 && pid < a.num_pages;
+      win_pid = win_ok ? pid : 0;
+      if (!win_ok) atomicOr(a.status, MB_DEV_BAD_PAGE);
+    }
+    const int pid = __shfl_sync(0xffffffffu, win_pid, issued & 31);
+    const int good = __shfl_sync(0xffffffffu, win_ok, issued & 31);
+    const int st = issued % ST;
+    if (lane == 0) {
+      ok_flag[st] = good;
+      mbd::mbar_expect_tx(bar + st, BLOB);
+      mbd::bulk_load(ring + st * BLOB, a.cache + ((int64_t)pid * a.Hkv + kvh) * BLOB, BLOB, bar + st);
+    }
+    ++issued;
+  };
+  for (int i = 0; i < ST && i < mine; ++i) issue();
+  bool dead = false;  // a copy never arrived: consume and load nothing more
+  int dead_at = 0;
+  State<NT> z;
+  z.reset();
+  if (mine > 0) {
+    const int first = a.start_pos ? min(a.start_pos[0], L) : L;
+    const float ck = z.load_q(a, 0, kvh, rt, L, first);
+    const int all_seen = min(L, first + (rt * COLS) / a.G + 1);
+    for (int used = 0; used < mine; ++used) {
+      const int st = used % ST;
+      if (!dead) {
+        dead = !mbd::mbar_wait(bar + st, (used / ST) & 1, a.status, MB_DEV_TIMEOUT_TMA);
+        dead = __any_sync(0xffffffffu, dead);
+        dead_at = used;
+      }
+      if (!dead && ok_flag[st]) {
+        const int key0 = (begin + used) * PAGE;
+        if (key0 + PAGE <= all_seen)
+          z.template page<false>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
+        else
+          z.template page<true>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
+      }
+      __syncwarp();
+      if (issued < mine && !dead) issue();
+    }
+    if (dead)
+      for (int i = dead_at; i < issued; ++i) mbd::mbar_wait(bar + i % ST, (i / ST) & 1, nullptr, 0);
+    z.finish();
+    z.deposit(reinterpret_cast<float*>(ring));
+  }
+  if (lane == 0) sm.seg[warp].x = mine;
+  __syncthreads();
+  // this CTA's part of every row, in place of the key numbers
+  float* part = reinterpret_cast<float*>(sm.kp);  // [COLS][DH], then [COLS] (reference, denominator)
+  static_assert(COLS * (DH + 2) * 4 <= NW * PAGE * 20, "a CTA's rows take the place of its key numbers");
+  const uint32_t who = __ballot_sync(0xffffffffu, lane < NW && sm.seg[lane < NW ? lane : 0].x > 0);
+  for (int col = warp; col < COLS; col += NW) {
+    const Joined j = join_row<ST * BLOB / 4, NW>(reinterpret_cast<const float*>(sm.ring), col, who);
+    *reinterpret_cast<float4*>(part + col * DH + lane * 4) = j.o;
+    if (lane == 0) *reinterpret_cast<float2*>(part + COLS * DH + col * 2) = make_float2(j.R, j.l);
+  }
+  cluster_sync();
+  for (int col = rank + warp * C; col < COLS; col += NW * C) {
+    const int r = rt * COLS + col;
+    if (r >= a.S * a.G) continue;
+    float2 m = make_float2(-INFINITY, 0.f);
+    if (lane < C) m = ld_cluster2(in_cta(part + COLS * DH + col * 2, lane));
+    float R = m.x;
+#pragma unroll
+    for (int off = 8; off; off >>= 1) R = fmaxf(R, __shfl_xor_sync(0xffffffffu, R, off));
+    R = __shfl_sync(0xffffffffu, R, 0);
+    const float f = m.x == -INFINITY ? 0.f : fast_exp2(m.x - R);
+    float l = m.y * f;
+#pragma unroll
+    for (int off = 8; off; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < C; ++c) {
+      const float fc = __shfl_sync(0xffffffffu, f, c);
+      const float4 v = ld_cluster4(in_cta(part + col * DH + lane * 4, c));
+      o.x = fmaf(v.x, fc, o.x);
+      o.y = fmaf(v.y, fc, o.y);
+      o.z = fmaf(v.z, fc, o.z);
+      o.w = fmaf(v.w, fc, o.w);
+    }
+    store_row(row_to(a, 0, kvh, r, 0, col, COLS, true), R, __shfl_sync(0xffffffffu, l, 0), o);
+  }
+  cluster_sync();  // nobody leaves while its rows are read
 }
 
 // Joins the partials of the units that more than one CTA worked on; before it
@@ -732,7 +928,7 @@ __global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a) {
     const int joined = c1 - c0 + (ends || w1 > max(w0, c1 * act) ? 1 : 0);
     const int n = joined + (ends ? 0 : 1);
     if (n < 2) continue;  // written by the main kernel
-    const int kvh = unit / a.RT, rt = unit - kvh * a.RT;
+    const int kvh = head_of(a, unit), rt = unit - kvh * a.RT;
 #pragma unroll
     for (int c8 = 0; c8 < (SPLIT ? 1 : NT); ++c8) {
       const int col = SPLIT ? blockIdx.y : c8 * 8 + warp;
@@ -798,7 +994,7 @@ __global__ void __launch_bounds__(256) attn_kv4_combine_kernel(const Args a) {
           __syncthreads();
           if (warp) continue;
         }
-        store_row(a, b, kvh, r, 0, col, COLS, true, M, L, acc);
+        store_row(row_to(a, b, kvh, r, 0, col, COLS, true), M, L, acc);
       }
 
     }
@@ -827,8 +1023,81 @@ Launch plan_launch(int B, int S, int Hq, int Hkv, int max_pages) {
   return p;
 }
 
+// Clusters of `size` CTAs of the one-sequence kernel that run at a time.
+template <int NT>
+int resident_clusters(int size) {
+  static int known[64][5] = {};
+  int dev = 0, slot = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return 0;
+  while ((1 << slot) < size) ++slot;
+  if (!known[dev][slot]) {
+    const void* fn = reinterpret_cast<const void*>(attn_kv4_one_kernel<NT>);
+    int n = 0;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(size * 8);
+    cfg.blockDim = dim3(Shape<NT>::NW * 32);
+    cfg.dynamicSmemBytes = sizeof(Shared<NT>);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    if (mb::ensure_smem_attr(fn, (int)sizeof(Shared<NT>)) ||
+        cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, attn_kv4_one_kernel<NT>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    known[dev][slot] = n + 1;
+  }
+  return known[dev][slot] - 1;
+}
+
+// Cluster size for one sequence, 0: the kernel for many. Expected times in us
+// (measured with 1, 2 and 8 kv heads and 60 to 64000 keys): 5.3 and 0.7 for
+// every doubling of the cluster up to four, 0.2 a page and warp rounds of
+// pages of its unit, against 13 and 0.18 a page on every SM. (8 heads: 517 keys
+// 7.5 and 8.7, 4000 keys 8.0 and 12.1, 16000 keys 12.2 and 16.6, 64000 keys 30
+// and 26.)
+template <int NT>
+int one_cluster(int units, int max_pages) {
+  const double flat = 13 + 0.18 * (double)units * max_pages / mb::num_sms();
+  double best = flat;
+  int at = 0;
+  for (int c = 1; c <= 16; c <<= 1) {
+    const double t = 5.3 + (c == 1 ? 0 : c == 2 ? 0.3 : 0.6) + 0.2 * max_pages / c;
+    if (t < best && units <= resident_clusters<NT>(c)) best = t, at = c;
+  }
+  return at;
+}
+
+template <int NT>
+int launch_one(const Args& a, int c, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(a.Hkv * a.RT * c);
+  cfg.blockDim = dim3(Shape<NT>::NW * 32);
+  cfg.dynamicSmemBytes = sizeof(Shared<NT>);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = mb::pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = c;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  MB_CUDA(cudaLaunchKernelEx(&cfg, attn_kv4_one_kernel<NT>, a));
+  return MB_OK;
+}
+
 template <int NT>
 int launch(const Args& a, int ctas, cudaStream_t s) {
+  if (a.B == 1) {
+    const int c = one_cluster<NT>(a.Hkv * a.RT, a.max_pages);
+    if (c) return launch_one<NT>(a, c, s);
+  }
   const int smem = (int)sizeof(Shared<NT>);
   int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_kv4_kernel<NT>), smem);
   if (rc) return rc;

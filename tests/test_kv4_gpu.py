@@ -241,6 +241,23 @@ def test_whole_cta_shares_and_many_units(ops):
     check_attention(ops, rng, 1, 1, 8, 1, np.array([70001]), garbage=False)
 
 
+@pytest.mark.parametrize("Hq, Hkv, S, L, width", [
+    (32, 8, 1, 517, 9), (8, 1, 1, 1, 1), (64, 8, 1, 20000, 400), (40, 8, 3, 777, 2000), (16, 16, 1, 4097, 65),
+    (4, 2, 5, 130, 3), (8, 8, 1, 0, 4), (48, 24, 2, 3000, 47), (128, 64, 1, 130, 300), (16, 2, 40, 900, 15),
+])
+def test_one_sequence(ops, Hq, Hkv, S, L, width):
+    """A single sequence: clusters of CTAs to a unit, of every size."""
+    rng = np.random.default_rng(L)
+    table, P = make_table(rng, [L], width=width)
+    cache = make_cache(rng, P, Hkv)
+    q = R.bf16_round(rng.standard_normal((1, S, Hq, 128)))
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32([L]), start_pos=i32([L - S]))
+    ref, slack = R.attention(q, cache, table, [L], [L - S])
+    err = np.abs(got.double().cpu().numpy() - ref)
+    assert (err <= slack + 2 ** -8 * (np.abs(ref) + slack)).all()
+    assert status() == 0
+
+
 def test_large_scores_and_small_values(ops):
     rng = np.random.default_rng(12)
     check_attention(ops, rng, 2, 1, 8, 2, np.array([500, 64]), amp=30.0)
