@@ -179,6 +179,7 @@ def test_causal_rows(ops, S, Hq, Hkv):
 
 
 @pytest.mark.parametrize("S, Hq, Hkv, lens, causal", [
+    (200, 3, 1, [190, 450, 0], True), (128, 2, 2, [128], True), (129, 4, 1, [129, 1000], False),
     (64, 8, 2, [200, 64, 0, 1], True), (65, 4, 4, [129, 65], False), (130, 5, 1, [130, 700], True),
     (257, 8, 8, [300], True), (64, 16, 2, [128, 500, 63], False),
 ])
