@@ -15,7 +15,7 @@
 // The bookkeeping of a call is one launch of one 8-CTA cluster: its 128 warps
 // count (ballots over contiguous segments), meet at the cluster barrier, read
 // the 128 counts and place what they counted. The pages' bytes move in a
-// second launch over all SMs, 16 bytes a load, bound by HBM.
+// second launch over all SMs, bound by HBM.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -29,6 +29,7 @@ constexpr int MAX_POOLS = 64;
 struct Pools {
   uint8_t* base[MAX_POOLS];
   int64_t bytes[MAX_POOLS];  // one page
+  int32_t piece[MAX_POOLS];  // bytes moved at once: a page in equal parts
   int n;
 };
 
@@ -341,38 +342,75 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
 
 // ---------------------------------------------------------------------------
 // The listed pages of every pool: no page is both read and written (a fork
-// writes free pages, a compaction moves pages above `live` below it).
-constexpr int COPY_THREADS = 256, COPY_VECS = 4;
-constexpr int COPY_CHUNK = COPY_THREADS * COPY_VECS * 16;  // bytes of a page a CTA moves at once
+// writes free pages, a compaction moves pages above `live` below it). A CTA is
+// one warp, whose first lane moves pieces of up to 16 KB through a ring in
+// shared memory with bulk copies in both directions: no registers and no
+// instructions a byte, and pieces on their way in while others go out. (1843
+// pages of 4 pools of 68 KB, 1.0 GB read and written: 193 us with 16-byte loads
+// and stores by 256 threads and 8 CTAs an SM, 177 us here, 6.4 TB/s.)
+constexpr int PIECE = 16384;
+constexpr int RING = 6, LAG = 2;  // pieces; a piece's place is filled again LAG pieces after it went out
+constexpr int COPY_SMEM = RING * PIECE + RING * 8;
 
-__global__ void __launch_bounds__(COPY_THREADS)
+__global__ void __launch_bounds__(32)
     kv_copy_kernel(const __grid_constant__ Pools pools, const int* __restrict__ head,
-                   const int2* __restrict__ moves, int chunks) {
+                   const int2* __restrict__ moves, int chunks, uint32_t* status) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + RING * PIECE);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) mbd::mbar_init(full + i, 1);
+    mbd::fence_mbar_init();
+  }
   mbd::pdl_trigger();
   mbd::pdl_wait();
-  const int n = *head;
-  const int64_t total = (int64_t)n * chunks * pools.n;
-  for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
-    const int chunk = (int)(i % chunks);
-    const int64_t rest = i / chunks;
-    const int pool = (int)(rest % pools.n);
-    const int2 mv = moves[rest / pools.n];
-    const int64_t bytes = pools.bytes[pool], at = (int64_t)chunk * COPY_CHUNK;
-    const uint8_t* src = pools.base[pool] + mv.x * bytes + at;
-    uint8_t* dst = pools.base[pool] + mv.y * bytes + at;
-    const int64_t left = bytes - at;
-    uint4 v[COPY_VECS];
-#pragma unroll
-    for (int j = 0; j < COPY_VECS; ++j) {
-      const int64_t o = (int64_t)(j * COPY_THREADS + threadIdx.x) * 16;
-      if (o < left) v[j] = __ldcs(reinterpret_cast<const uint4*>(src + o));
+  if (threadIdx.x) return;
+  const int64_t total = (int64_t)*head * chunks * pools.n;
+  const int64_t mine = total > blockIdx.x ? (total - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+  uint8_t* to[RING];
+  uint32_t size[RING];
+  auto load = [&](int64_t k, int st) {  // the k-th piece of this CTA
+    const int64_t i = blockIdx.x + k * gridDim.x;
+    int64_t rest, move;  // (piece within rest, then pool within move); short divisions where they do
+    if (total <= 0xFFFFFFFFll) rest = (uint32_t)i / (uint32_t)chunks, move = (uint32_t)rest / (uint32_t)pools.n;
+    else rest = i / chunks, move = rest / pools.n;
+    const int pool = (int)(rest - move * pools.n);
+    const int64_t bytes = pools.bytes[pool], piece = pools.piece[pool], at = (i - rest * chunks) * piece;
+    const int2 mv = moves[move];
+    size[st] = at < bytes ? (uint32_t)(bytes - at < piece ? bytes - at : piece) : 0;
+    to[st] = pools.base[pool] + mv.y * bytes + at;
+    if (size[st]) {
+      mbd::mbar_expect_tx(full + st, size[st]);
+      mbd::bulk_load(ring + st * PIECE, pools.base[pool] + mv.x * bytes + at, size[st], full + st);
+    } else {
+      mbd::mbar_arrive(full + st);
     }
+  };
 #pragma unroll
-    for (int j = 0; j < COPY_VECS; ++j) {
-      const int64_t o = (int64_t)(j * COPY_THREADS + threadIdx.x) * 16;
-      if (o < left) __stcs(reinterpret_cast<uint4*>(dst + o), v[j]);
+  for (int st = 0; st < RING; ++st)
+    if (st < mine) load(st, st);
+  bool ok = true;
+  int64_t k = 0;
+  for (uint32_t phase = 0; k < mine && ok; phase ^= 1) {
+#pragma unroll
+    for (int st = 0; st < RING; ++st, ++k) {
+      if (k >= mine || !ok) break;
+      ok = mbd::mbar_wait(full + st, phase, status, MB_DEV_TIMEOUT_TMA);
+      if (!ok) break;
+      if (size[st])
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to[st]),
+                     "r"(mbd::smem_u32(ring + st * PIECE)), "r"(size[st])
+                     : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      // the piece that went out LAG ago has been read: its place is free
+      if (k >= LAG && k - LAG + RING < mine) {
+        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LAG) : "memory");
+        load(k - LAG + RING, (st + RING - LAG) % RING);
+      }
     }
   }
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (!ok)  // a copy never came: wait (bounded) for the others before the memory goes
+    for (int st = 0; st < RING; ++st) mbd::mbar_wait(full + st, 0, nullptr, 0, nullptr, 1000000);
 }
 
 size_t align16(size_t x) { return (x + 15) / 16 * 16; }
@@ -422,11 +460,16 @@ int copy_pages(const char* what, void* const* pools, const int64_t* bytes, int n
       p.bytes[i] = bytes[at + i];
       big = bytes[at + i] > big ? bytes[at + i] : big;
     }
-    const int chunks = (int)((big + COPY_CHUNK - 1) / COPY_CHUNK);
-    const int64_t all = most_moves * chunks * p.n, wave = (int64_t)mb::num_sms() * 8;
+    const int chunks = (int)((big + PIECE - 1) / PIECE);
+    for (int i = 0; i < p.n; ++i) p.piece[i] = (int32_t)(((p.bytes[i] + chunks - 1) / chunks + 15) / 16 * 16);
+    const int64_t all = most_moves * chunks * p.n, wave = (int64_t)mb::num_sms() * 2;
     if (all == 0) continue;
-    MB_CUDA(mb::launch_pdl(kv_copy_kernel, dim3((unsigned)(all < wave ? all : wave)),
-                           dim3(COPY_THREADS), 0, s, p, w.head, w.moves, chunks));
+    uint32_t* status = mb::device_status_ptr();
+    MB_REQUIRE(status, "%s: no status word", what);
+    const int rc = mb::ensure_smem_attr(reinterpret_cast<const void*>(kv_copy_kernel), COPY_SMEM);
+    if (rc) return rc;
+    MB_CUDA(mb::launch_pdl(kv_copy_kernel, dim3((unsigned)(all < wave ? all : wave)), dim3(32), COPY_SMEM, s,
+                           p, w.head, w.moves, chunks, status));
   }
   return MB_OK;
 }
