@@ -374,6 +374,19 @@ int mb_decoder_layer_forward_chain(const void* layer, const uint16_t* x, const f
                                    int causal, void* workspace, size_t workspace_bytes,
                                    void* stream);
 
+/* mb_decoder_layer_forward_chain over a 4-bit cache (mb_kv4_append_bf16's
+ * layout, this rank's kv heads): the new tokens' rotated keys and values are
+ * stored in 4 bits and attention reads them there. new_len (null: S) gives the
+ * tokens of each sequence that are stored; kv_len[b] = start_pos[b] + new_len[b];
+ * the rows of y behind them are unspecified. Every length is read on the device. */
+size_t mb_decoder_layer_workspace_bytes_kv4(const void* layer, int B, int S, int max_pages);
+int mb_decoder_layer_forward_kv4(const void* layer, const uint16_t* x, const float* x_res32,
+                                 const float* rstd_in, uint16_t* y, float* y_res32, float* rstd_out,
+                                 int B, int S, const int* start_pos, const int* kv_len,
+                                 const int* new_len, uint8_t* cache, int num_pages,
+                                 const int* block_table, int max_pages, int causal, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 /* fp32 decoder layer for the reference's own llama_decoder_layer_f32 entry
  * (mlx/kernels/full/llama_decoder_layer.py:24-64; registry
  * mlx/kernels/full/registry.py:87-104: S 64, D 128, H 4 / H_kv 2, head_dim 32,

@@ -419,13 +419,14 @@ struct Plan {
   int64_t T;
   int ks_qkv, ks_o, ks_gu, ks_down;
   size_t off_rstd1, off_rstd2, off_q, off_attn, off_x1, off_x1f, off_p32, off_act, off_part,
-      off_attn_ws, total;
+      off_attn_ws, off_kv, total;
   size_t attn_ws;
 };
 
 size_t a256(size_t x) { return (x + 255) & ~size_t(255); }
 
-Plan make_plan(const Layer& L, int B, int S, int max_kv_len) {
+// kv4_pages > 0: over a 4-bit cache with that many pages a sequence.
+Plan make_plan(const Layer& L, int B, int S, int max_kv_len, int kv4_pages = 0) {
   Plan p;
   const int D = L.cfg.d_model;
   p.T = (int64_t)B * S;
@@ -452,7 +453,9 @@ Plan make_plan(const Layer& L, int B, int S, int max_kv_len) {
   upd(p.ks_o, D);
   upd(p.ks_gu, 2 * L.FF);
   upd(p.ks_down, D);
-  p.attn_ws = S == 1 ? mb_attention_decode_workspace_bytes(B, L.Hq, L.Hkv, max_kv_len) : 0;
+  p.attn_ws = kv4_pages ? mb_attention_kv4_workspace_bytes(B, S, L.Hq, L.Hkv, kv4_pages)
+              : S == 1  ? mb_attention_decode_workspace_bytes(B, L.Hq, L.Hkv, max_kv_len)
+                        : 0;
   size_t o = 0;
   p.off_rstd1 = o; o += a256(T * 4);
   p.off_rstd2 = o; o += a256(T * 4);
@@ -464,6 +467,7 @@ Plan make_plan(const Layer& L, int B, int S, int max_kv_len) {
   p.off_act = o; o += a256(T * L.FF * 2);
   p.off_part = o; o += a256(part);
   p.off_attn_ws = o; o += a256(p.attn_ws);
+  p.off_kv = o; o += kv4_pages ? 2 * a256(T * L.Dkv * 2) : 0;  // the new keys and values in bf16
   p.total = o;
   return p;
 }
@@ -585,22 +589,32 @@ extern "C" size_t mb_decoder_layer_workspace_bytes(const void* layer, int B, int
 }
 
 namespace {
+// A 4-bit cache in the place of the bf16 one.
+struct Kv4 {
+  uint8_t* cache;
+  int num_pages;
+  const int* new_len;
+};
+
 int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, uint16_t* y,
                     float* y_res32, const float* rstd_in, float* rstd_out, int B, int S,
                     const int* start_pos, const int* kv_len, int max_kv_len, uint16_t* k_cache,
                     uint16_t* v_cache, const int* block_table, int max_pages, int causal,
-                    void* workspace, size_t workspace_bytes, void* stream) {
-  MB_REQUIRE(layer && x && y && start_pos && kv_len && k_cache && v_cache && block_table,
+                    void* workspace, size_t workspace_bytes, void* stream,
+                    const Kv4* kv4 = nullptr) {
+  MB_REQUIRE(layer && x && y && start_pos && kv_len && block_table &&
+                 (kv4 ? kv4->cache != nullptr : k_cache && v_cache),
              "decoder forward: null argument");
   MB_REQUIRE(!rstd_out || y_res32, "decoder forward: rstd_out needs the fp32 output y_res32");
   MB_REQUIRE(B >= 0 && S >= 0, "decoder forward: negative size");
   if (B == 0 || S == 0) return MB_OK;
   const Layer& L = *static_cast<const Layer*>(layer);
-  MB_REQUIRE(max_kv_len >= S && max_kv_len <= max_pages * 64,
+  MB_REQUIRE(kv4 || (max_kv_len >= S && max_kv_len <= max_pages * 64),
              "decoder forward: max_kv_len must be in [S, max_pages*64]");
+  MB_REQUIRE(max_pages > 0, "decoder forward: the block table has no columns");
   MB_REQUIRE((reinterpret_cast<uintptr_t>(x_res32) | reinterpret_cast<uintptr_t>(y_res32)) % 16 == 0,
              "decoder forward: fp32 residual buffers must be 16-byte aligned");
-  const Plan p = make_plan(L, B, S, max_kv_len);
+  const Plan p = make_plan(L, B, S, max_kv_len, kv4 ? max_pages : 0);
   MB_REQUIRE(workspace && workspace_bytes >= p.total &&
                  reinterpret_cast<uintptr_t>(workspace) % 256 == 0,
              "decoder forward: workspace of %zu bytes (256-byte aligned) required", p.total);
@@ -647,7 +661,10 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
   qp.rstd = rstd1;
   qp.start_pos = start_pos;
   qp.q_out = q;
-  qp.kv = dec::KvCache{k_cache, v_cache, block_table, max_pages, 64};
+  uint16_t* k_new = reinterpret_cast<uint16_t*>(w + p.off_kv);
+  uint16_t* v_new = k_new + a256(T * L.Dkv * 2) / 2;
+  qp.kv = kv4 ? dec::KvCache{k_new, v_new, nullptr, 0, 64}
+              : dec::KvCache{k_cache, v_cache, block_table, max_pages, 64};
   if (p.ks_qkv > 1 || use_streamk(T, Nqkv)) {
     PartSum ps;
     rc = gemm_partial(x, L.wqkv, part, T, Nqkv, D, p.ks_qkv, s, &ps);
@@ -665,7 +682,15 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
   MB_CUDA(cudaGetLastError());
 
   // 3. attention
-  if (S == 1)
+  if (kv4) {
+    const int64_t tok = L.Dkv, seq = (int64_t)S * L.Dkv;
+    rc = mb_kv4_append_bf16(k_new, v_new, seq, tok, Dh, seq, tok, Dh, kv4->cache, kv4->num_pages, L.Hkv,
+                            block_table, max_pages, start_pos, kv4->new_len, B, S, s);
+    if (!rc)
+      rc = mb_attention_kv4_bf16(q, L.Dq, kv4->cache, kv4->num_pages, block_table, max_pages, kv_len,
+                                 causal ? start_pos : nullptr, B, S, L.Hq, L.Hkv, Dh,
+                                 1.f / sqrtf((float)Dh), attn, L.Dq, w + p.off_attn_ws, p.attn_ws, s);
+  } else if (S == 1)
     rc = mb_attention_decode_bf16(q, L.Dq, k_cache, v_cache, block_table, max_pages, kv_len,
                                   max_kv_len, B, L.Hq, L.Hkv, Dh, attn, L.Dq, w + p.off_attn_ws,
                                   p.attn_ws, s);
@@ -803,6 +828,26 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
   return MB_OK;
 }
 }  // namespace
+
+extern "C" size_t mb_decoder_layer_workspace_bytes_kv4(const void* layer, int B, int S,
+                                                       int max_pages) {
+  if (!layer || B <= 0 || S <= 0 || max_pages <= 0) return 0;
+  return make_plan(*static_cast<const Layer*>(layer), B, S, 0, max_pages).total;
+}
+
+extern "C" int mb_decoder_layer_forward_kv4(const void* layer, const uint16_t* x,
+                                            const float* x_res32, const float* rstd_in, uint16_t* y,
+                                            float* y_res32, float* rstd_out, int B, int S,
+                                            const int* start_pos, const int* kv_len,
+                                            const int* new_len, uint8_t* cache, int num_pages,
+                                            const int* block_table, int max_pages, int causal,
+                                            void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+  const Kv4 kv4{cache, num_pages, new_len};
+  return decoder_forward(layer, x, x_res32, y, y_res32, rstd_in, rstd_out, B, S, start_pos, kv_len,
+                         0, nullptr, nullptr, block_table, max_pages, causal, workspace,
+                         workspace_bytes, stream, &kv4);
+}
 
 extern "C" int mb_decoder_layer_forward_ex(const void* layer, const uint16_t* x,
                                            const float* x_res32, uint16_t* y, float* y_res32,

@@ -21,7 +21,7 @@ namespace dec {
 struct KvCache {
   uint16_t* k;
   uint16_t* v;
-  const int* block_table;
+  const int* block_table;  // null: k and v are [rows][Hkv][Dh], one row a token
   int max_pages;
   int page;
 };
@@ -70,8 +70,13 @@ struct QkvParams {
     const int c = is_k ? col - Dq : col - Dq - Dk;
     const int head = c / Dh, d = c % Dh;
     if (is_k) rope<W>(v, pos, d);
-    const int pg = kv.block_table[b * kv.max_pages + pos / kv.page];
-    const int64_t off = (((int64_t)pg * Hkv + head) * kv.page + pos % kv.page) * Dh + d;
+    int64_t off;
+    if (kv.block_table) {
+      const int pg = kv.block_table[b * kv.max_pages + pos / kv.page];
+      off = (((int64_t)pg * Hkv + head) * kv.page + pos % kv.page) * Dh + d;
+    } else {
+      off = ((int64_t)row * Hkv + head) * Dh + d;
+    }
     gemm::storeW_bf16<W>((is_k ? kv.k : kv.v) + off, v);
   }
 };

@@ -5,7 +5,8 @@ Mirrors the reference hook ``mlx/kernels/full/llama_decoder_layer.py``:
 weights in the reference (in, out) layout. ``DecoderLayer`` packs them once
 (K-major, this rank's tensor-parallel shard) and runs the fused kernels;
 ``PagedKVCache`` holds the rotated keys and values of every sequence in
-64-token pages.
+64-token pages; ``PagedKV4Cache`` holds them in 4 bits, for the layers of a
+model together, with the pages' bookkeeping on the device.
 """
 from __future__ import annotations
 
@@ -64,6 +65,68 @@ class PagedKVCache:
             self.v[pg, :, p % PAGE] = v[:, p - start]
 
 
+class PagedKV4Cache:
+    """The keys and values of ``n_layers`` layers in 4 bits (layout and rounding
+    in include/mb200.h): one page pool a layer, uint8 [num_pages, Hkv, 8704],
+    under one block table [batch, max_pages], sequence lengths and page use
+    counts, all int32 on the device. Pages are given out as sequences grow,
+    shared by forks and returned when the last sequence that holds them ends.
+
+    A step is ``start = cache.extend(new_len)``, then for every layer either
+    ``layer(x, cache.layer(i), start, ...)`` or ``append`` and ``attend``. Nothing is
+    read back by the host, so steps can be captured in a CUDA graph;
+    ``cache.status`` tells, when the program next looks, whether the last page
+    operation was served (0), or how many pages were lacking (then it changed
+    nothing)."""
+
+    def __init__(self, batch: int, max_len: int, n_kv_heads: int, n_layers: int = 1,
+                 num_pages: int | None = None, device=None):
+        device = device or torch.device("cuda", torch.cuda.current_device())
+        if batch < 1 or max_len < 1 or n_layers < 1:
+            raise ValueError("PagedKV4Cache: batch, max_len and n_layers must be at least 1")
+        self.batch, self.n_layers = batch, n_layers
+        self.max_pages = (max_len + PAGE - 1) // PAGE
+        num_pages = batch * self.max_pages if num_pages is None else num_pages
+        self.pools = [ops.kv4_cache(num_pages, n_kv_heads, device) for _ in range(n_layers)]
+        self.block_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.seq_len = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.page_refs = torch.zeros(num_pages, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def extend(self, new_len: torch.Tensor) -> torch.Tensor:
+        """Room for new_len[b] more tokens a sequence; the positions of the first of them."""
+        start, self.status = ops.kv_pages_extend(self.block_table, self.seq_len, self.page_refs, new_len)
+        return start
+
+    def fork(self, parent: torch.Tensor) -> None:
+        """Row b becomes a fork of row parent[b] (its own number: stays; -1: is freed)."""
+        self.status = ops.kv_pages_fork(self.pools, self.block_table, self.seq_len, self.page_refs, parent)
+
+    def compact(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Move the pages in use to the front of every pool: (new numbers, pages in use)."""
+        return ops.kv_pages_compact(self.pools, self.block_table, self.seq_len, self.page_refs)
+
+    def append(self, i: int, k: torch.Tensor, v: torch.Tensor, start_pos: torch.Tensor,
+               new_len: torch.Tensor | None = None) -> None:
+        """Store layer i's keys and values [B, S, Hkv, 128] of the new tokens."""
+        ops.kv4_append(k, v, self.pools[i], self.block_table, start_pos, new_len)
+
+    def attend(self, i: int, q: torch.Tensor, start_pos: torch.Tensor | None = None,
+               scale: float | None = None) -> torch.Tensor:
+        """Layer i's attention of q [B, S, H, 128] over each sequence's tokens."""
+        return ops.attention_kv4(q, self.pools[i], self.block_table, self.seq_len, start_pos, scale)
+
+    def layer(self, i: int) -> "KV4Layer":
+        return KV4Layer(self, i)
+
+
+@dataclass
+class KV4Layer:
+    """One layer's part of a PagedKV4Cache, as a DecoderLayer takes it."""
+    owner: PagedKV4Cache
+    index: int
+
+
 class DecoderLayer:
     def __init__(self, cfg: DecoderConfig, W_qkv: torch.Tensor, W_o: torch.Tensor,
                  W_gu: torch.Tensor, W_down: torch.Tensor, tp_rank: int = 0, tp_world: int = 1):
@@ -100,13 +163,14 @@ class DecoderLayer:
     def workspace_bytes(self, B: int, S: int, max_kv_len: int) -> int:
         return _lib.lib().mb_decoder_layer_workspace_bytes(self._h, B, S, max_kv_len)
 
-    def forward(self, x: torch.Tensor, cache: PagedKVCache, start_pos: torch.Tensor,
+    def forward(self, x: torch.Tensor, cache: "PagedKVCache | KV4Layer", start_pos: torch.Tensor,
                 causal: bool = True, out: torch.Tensor | None = None,
                 max_kv_len: int | None = None, kv_len: torch.Tensor | None = None,
                 x_res32: torch.Tensor | None = None,
                 y_res32: torch.Tensor | None = None,
                 rstd_in: torch.Tensor | None = None,
-                rstd_out: torch.Tensor | None = None) -> torch.Tensor:
+                rstd_out: torch.Tensor | None = None,
+                new_len: torch.Tensor | None = None) -> torch.Tensor:
         """x: [B, S, D] bf16 (or [S, D] for B = 1); start_pos: int32 [B] on the device.
 
         The new tokens' keys/values are appended at start_pos[b].. and attention
@@ -117,21 +181,43 @@ class DecoderLayer:
         y_res32 receives the fp32 output. rstd_in / rstd_out (fp32, one entry
         per token) chain the input RMSNorm factor between layers: rstd_out
         receives rsqrt(mean(y_res32^2) + eps) for the next layer, which takes
-        it as rstd_in instead of computing it (rstd_out needs y_res32)."""
+        it as rstd_in instead of computing it (rstd_out needs y_res32).
+
+        cache may be a layer of a PagedKV4Cache (``cache.layer(i)``), whose
+        pages were extended for this step: keys and values are then held in 4
+        bits, kv_len is the cache's seq_len, and new_len (int32 [B]) may say how
+        many of the S tokens each sequence has (the rows of y behind them are
+        unspecified)."""
         squeeze = x.dim() == 2
         X = x.unsqueeze(0) if squeeze else x
         ops._cuda(X, "DecoderLayer.forward(x)", (torch.bfloat16,))
         B, S, D = X.shape
         if start_pos.dtype != torch.int32 or not start_pos.is_cuda or start_pos.numel() != B:
             raise ValueError("start_pos must be an int32 CUDA tensor with one entry per sequence")
-        if kv_len is None:
-            kv_len = (start_pos + S).contiguous()
-        if max_kv_len is None:
-            max_kv_len = int(kv_len.max().item())
+        kv4 = isinstance(cache, KV4Layer)
+        if kv4:
+            own, pool = cache.owner, cache.owner.pools[cache.index]
+            if own.batch != B or pool.shape[1] != self.h_kv_local or pool.device != X.device:
+                raise ValueError("the 4-bit cache has another batch, number of kv heads or device")
+            if kv_len is None:
+                kv_len = own.seq_len
+            if new_len is not None and (new_len.dtype != torch.int32 or new_len.device != X.device
+                                        or tuple(new_len.shape) != (B,) or not new_len.is_contiguous()):
+                raise ValueError("new_len must be an int32 tensor with one entry per sequence")
+            ws_bytes = _lib.lib().mb_decoder_layer_workspace_bytes_kv4(self._h, B, S, own.max_pages)
+            # a workspace of the call: captured graphs and other streams keep theirs
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
+        else:
+            if new_len is not None:
+                raise ValueError("new_len needs a 4-bit cache")
+            if kv_len is None:
+                kv_len = (start_pos + S).contiguous()
+            if max_kv_len is None:
+                max_kv_len = int(kv_len.max().item())
+            ws_bytes = self.workspace_bytes(B, S, max_kv_len)
+            ws = ops._workspace(ws_bytes, X.device)
         if out is None:
             out = torch.empty_like(X)
-        ws_bytes = self.workspace_bytes(B, S, max_kv_len)
-        ws = ops._workspace(ws_bytes, X.device)
         self._kv_len = kv_len  # keep alive until the stream has consumed it
         for nm, t in (("x_res32", x_res32), ("y_res32", y_res32)):
             if t is not None:
@@ -145,6 +231,14 @@ class DecoderLayer:
                     raise ValueError(f"{nm} must hold one float per token")
         if rstd_out is not None and y_res32 is None:
             raise ValueError("rstd_out needs y_res32")
+        if kv4:
+            ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+            _lib.call("mb_decoder_layer_forward_kv4", self._h, X.data_ptr(), ptr(x_res32), ptr(rstd_in),
+                      out.data_ptr(), ptr(y_res32), ptr(rstd_out), B, S, start_pos.data_ptr(),
+                      kv_len.data_ptr(), ptr(new_len), pool.data_ptr(), pool.shape[0],
+                      own.block_table.data_ptr(), own.max_pages, 1 if causal else 0, ws.data_ptr(),
+                      ws_bytes, ops._stream())
+            return out[0] if squeeze else out
         _lib.call("mb_decoder_layer_forward_chain", self._h, X.data_ptr(),
                   0 if x_res32 is None else x_res32.data_ptr(),
                   0 if rstd_in is None else rstd_in.data_ptr(), out.data_ptr(),

@@ -16,7 +16,7 @@ import uuid
 import torch
 
 from . import _lib, ops
-from .decoder import DecoderConfig, DecoderLayer, PagedKVCache
+from .decoder import DecoderConfig, DecoderLayer, PagedKV4Cache, PagedKVCache
 
 _tp_ready = False
 
@@ -44,11 +44,16 @@ def init_tensor_parallel(rank: int, world: int, local_rank: int, timeout_ms: int
 
 class DecoderStack:
     """``n_layers`` decoder layers with random N(0, std) weights (seeded per
-    layer, identical on every rank) and one paged KV cache per layer."""
+    layer, identical on every rank) and one paged KV cache per layer; with
+    kv_bits=4 one PagedKV4Cache for all of them (``kv4``), whose pages are given
+    out by the steps (``num_pages`` of them, by default enough for every
+    sequence's max_len)."""
 
     def __init__(self, cfg: DecoderConfig, n_layers: int, batch: int, max_len: int,
                  tp_rank: int = 0, tp_world: int = 1, seed: int = 4, std: float = 0.02,
-                 weights=None):
+                 weights=None, kv_bits: int = 16, num_pages: int | None = None):
+        if kv_bits not in (4, 16):
+            raise ValueError("DecoderStack: kv_bits must be 4 or 16")
         self.cfg, self.n_layers, self.batch = cfg, n_layers, batch
         self.tp_rank, self.tp_world = tp_rank, tp_world
         self.layers: list[DecoderLayer] = []
@@ -64,13 +69,32 @@ class DecoderStack:
                      for s in [(D, D + 2 * Hkv * Dh), (D, D), (D, 2 * FF), (FF, D)]]
             self.layers.append(DecoderLayer(cfg, *W, tp_rank=tp_rank, tp_world=tp_world))
             del W
-            self.caches.append(PagedKVCache(batch, max_len, Hkv // tp_world, Dh, device=dev))
+            if kv_bits == 16:
+                self.caches.append(PagedKVCache(batch, max_len, Hkv // tp_world, Dh, device=dev))
+        self.kv4 = None
+        if kv_bits == 4:
+            self.kv4 = PagedKV4Cache(batch, max_len, Hkv // tp_world, n_layers, num_pages, dev)
+            self.caches = [self.kv4.layer(i) for i in range(n_layers)]
         torch.cuda.empty_cache()
         self._graph = None
 
     def fill_cache_random(self, length: int, seed: int = 4) -> None:
         """Fill positions 0..length-1 of every cache with N(0,1) keys/values
         (stand-in for an already-processed prompt)."""
+        if self.kv4 is not None:
+            dev = self.kv4.block_table.device
+            g = torch.Generator(device=dev).manual_seed(seed + 7919 * self.tp_rank)
+            start = self.kv4.extend(torch.full((self.batch,), length, dtype=torch.int32, device=dev) -
+                                    self.kv4.seq_len)
+            zero = torch.zeros_like(start)
+            Hkv = self.kv4.pools[0].shape[1]
+            for i in range(self.n_layers):
+                for p in range(0, length, 512):
+                    n = min(512, length - p)
+                    k, v = (torch.randn((self.batch, n, Hkv, self.cfg.head_dim), generator=g, device=dev).to(torch.bfloat16)
+                            for _ in range(2))
+                    self.kv4.append(i, k, v, zero + p)
+            return
         g = torch.Generator(device=self.caches[0].k.device).manual_seed(seed + 7919 * self.tp_rank)
         for c in self.caches:
             c.k.normal_(generator=g)
@@ -80,7 +104,7 @@ class DecoderStack:
                 kv_len_max: int | None = None) -> torch.Tensor:
         # one kv_len for all layers: no extra kernel between two layers' launches
         S = x.shape[-2] if x.dim() == 3 else x.shape[0]
-        self._kv_len = (start_pos + S).contiguous()
+        self._kv_len = (start_pos + S).contiguous() if self.kv4 is None else self.kv4.seq_len
         # the residual stream stays fp32 from layer to layer (two ping-pong
         # buffers); each layer also emits the bf16 copy the next one's GEMMs read
         key = tuple(x.shape)
