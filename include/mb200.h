@@ -236,7 +236,7 @@ int mb_attention_prefill_bf16(const uint16_t* q, int ldq, const uint16_t* k_cach
  * device memory. A position outside the table, or a table entry outside
  * 0..num_pages-1, is never accessed: it is not stored, is read back as zeros,
  * leaves the attention rows of its sequence unspecified, and is recorded in the
- * device status word (0x8). */
+ * device status word (0x8, until mb_clear_device_status). */
 
 /* Bytes of one page of all Hkv heads. */
 size_t mb_kv4_page_bytes(int Hkv);
@@ -259,13 +259,16 @@ int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv, const int* b
 
 /* out = softmax(scale * q k^T) v for S query rows a sequence over keys
  * 0..kv_len[b]-1; with start_pos, row s sees the keys at positions <=
- * start_pos[b] + s only (causal), else all. q, out: bf16 [B][S][Hq][128] with ldq /
+ * start_pos[b] + s only (causal), else all. max_kv_len (1 .. 64 max_pages): no
+ * kv_len is larger (one that is is cut to it); it sizes the workspace and chooses
+ * the form, so a bound near the longest length serves wide block tables best. q, out: bf16 [B][S][Hq][128] with ldq /
  * ldo elements between two positions' rows (multiples of 8), the heads
  * contiguous. A row that sees no key becomes zeros. Every length is read on the device, so ragged batches balance and the call can be captured. */
-size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages);
+size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_kv_len);
 int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache, int num_pages,
                           const int* block_table, int max_pages, const int* kv_len,
-                          const int* start_pos, int B, int S, int Hq, int Hkv, int Dh, float scale,
+                          int max_kv_len, const int* start_pos, int B, int S, int Hq, int Hkv,
+                          int Dh, float scale,
                           uint16_t* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                           void* stream);
 
@@ -378,12 +381,13 @@ int mb_decoder_layer_forward_chain(const void* layer, const uint16_t* x, const f
  * layout, this rank's kv heads): the new tokens' rotated keys and values are
  * stored in 4 bits and attention reads them there. new_len (null: S) gives the
  * tokens of each sequence that are stored; kv_len[b] = start_pos[b] + new_len[b];
- * the rows of y behind them are unspecified. Every length is read on the device. */
-size_t mb_decoder_layer_workspace_bytes_kv4(const void* layer, int B, int S, int max_pages);
+ * the rows of y behind them are unspecified. Every length is read on the device;
+ * max_kv_len as for mb_attention_kv4_bf16. */
+size_t mb_decoder_layer_workspace_bytes_kv4(const void* layer, int B, int S, int max_kv_len);
 int mb_decoder_layer_forward_kv4(const void* layer, const uint16_t* x, const float* x_res32,
                                  const float* rstd_in, uint16_t* y, float* y_res32, float* rstd_out,
                                  int B, int S, const int* start_pos, const int* kv_len,
-                                 const int* new_len, uint8_t* cache, int num_pages,
+                                 int max_kv_len, const int* new_len, uint8_t* cache, int num_pages,
                                  const int* block_table, int max_pages, int causal, void* workspace,
                                  size_t workspace_bytes, void* stream);
 

@@ -100,7 +100,7 @@ SIGNATURES = {
     "mb_kv4_append_bf16": (C.c_int, [_P, _P] + [_I64] * 6 + [_P, _I, _I, _P, _I, _P, _P, _I, _I, _P]),
     "mb_kv4_gather_f32": (C.c_int, [_P, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P]),
     "mb_attention_kv4_workspace_bytes": (C.c_size_t, [_I] * 5),
-    "mb_attention_kv4_bf16": (C.c_int, [_P, _I64, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I,
+    "mb_attention_kv4_bf16": (C.c_int, [_P, _I64, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I,
                                         C.c_float, _P, _I64, _P, C.c_size_t, _P]),
     "mb_kv_pages_workspace_bytes": (C.c_size_t, [_I] * 3),
     "mb_kv_pages_extend": (C.c_int, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, C.c_size_t, _P]),
@@ -119,8 +119,8 @@ SIGNATURES = {
     "mb_decoder_layer_forward_chain": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _I,
                                                  _P, _P, _P, _I, _I, _P, C.c_size_t, _P]),
     "mb_decoder_layer_workspace_bytes_kv4": (C.c_size_t, [_P, _I, _I, _I]),
-    "mb_decoder_layer_forward_kv4": (C.c_int, [_P] * 7 + [_I, _I] + [_P] * 4 + [_I, _P, _I, _I, _P,
-                                                                            C.c_size_t, _P]),
+    "mb_decoder_layer_forward_kv4": (C.c_int, [_P] * 7 + [_I, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I,
+                                                          _P, C.c_size_t, _P]),
     "mb_tp_allreduce_bf16": (C.c_int, [_P, C.c_size_t, _P]),
     "mb_rms_norm_linear_workspace_bytes": (C.c_size_t, [_I64]),
     "mb_rms_norm_linear_bf16": (C.c_int, [_P, _P, _P, _I64, _I64, _I64, C.c_float, _P,

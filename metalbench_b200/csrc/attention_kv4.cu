@@ -65,7 +65,7 @@ struct Args {
   float* part_ml;  // [warps][2][cols][2]
   uint32_t* status;
   int64_t ldq, ldo;  // elements between two positions' rows
-  int num_pages, max_pages, B, S, Hkv, G, RT;
+  int num_pages, max_pages, max_len, B, S, Hkv, G, RT;
   int warps;  // shares
   int active; // warps of a CTA that have one
   float scale_log2;
@@ -123,7 +123,7 @@ __device__ __forceinline__ float fast_rcp(float x) {
 // Attended keys of sequence b (from L2: the combine kernel plans before it has
 // waited for the main one).
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
-  return max(0, min(__ldcg(a.kv_len + b), a.max_pages * PAGE));
+  return max(0, min(__ldcg(a.kv_len + b), a.max_len));
 }
 
 // Flat page list of the batch, in shared memory.
@@ -1008,13 +1008,13 @@ struct Launch {
 
 // Query rows of a kv head: S * G. Up to 8 take one column tile, more two (so
 // that a page is unpacked once for 16 rows), in row tiles of 16.
-Launch plan_launch(int B, int S, int Hq, int Hkv, int max_pages) {
+Launch plan_launch(int B, int S, int Hq, int Hkv, int pages) {
   Launch p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   p.nt = rows <= 8 ? 1 : 2;
   p.rt = (int)((rows + p.nt * 8 - 1) / (p.nt * 8));
   // shares of at least a page; as few warps a CTA as that leaves, over all SMs
-  const int64_t most = (int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)max_pages + UNIT_COST);
+  const int64_t most = (int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)pages + UNIT_COST);
   const int sms = mb::num_sms(), nw = p.nt == 1 ? Shape<1>::NW : Shape<2>::NW;
   p.ctas = (int)(most < sms ? most : sms);
   const int64_t act = (most + p.ctas - 1) / p.ctas;
@@ -1062,12 +1062,12 @@ int resident_clusters(int size) {
 // 7.5 and 8.7, 4000 keys 8.0 and 12.1, 16000 keys 12.2 and 16.6, 64000 keys 30
 // and 26.)
 template <int NT>
-int one_cluster(int units, int max_pages) {
-  const double flat = 13 + 0.18 * (double)units * max_pages / mb::num_sms();
+int one_cluster(int units, int pages) {
+  const double flat = 13 + 0.18 * (double)units * pages / mb::num_sms();
   double best = flat;
   int at = 0;
   for (int c = 1; c <= 16; c <<= 1) {
-    const double t = 5.3 + (c == 1 ? 0 : c == 2 ? 0.3 : 0.6) + 0.2 * max_pages / c;
+    const double t = 5.3 + (c == 1 ? 0 : c == 2 ? 0.3 : 0.6) + 0.2 * pages / c;
     if (t < best && units <= resident_clusters<NT>(c)) best = t, at = c;
   }
   return at;
@@ -1095,7 +1095,7 @@ int launch_one(const Args& a, int c, cudaStream_t s) {
 template <int NT>
 int launch(const Args& a, int ctas, cudaStream_t s) {
   if (a.B == 1) {
-    const int c = one_cluster<NT>(a.Hkv * a.RT, a.max_pages);
+    const int c = one_cluster<NT>(a.Hkv * a.RT, (a.max_len + PAGE - 1) / PAGE);
     if (c) return launch_one<NT>(a, c, s);
   }
   const int smem = (int)sizeof(Shared<NT>);
@@ -1130,35 +1130,36 @@ struct Expand {
   size_t pages, bytes;
 };
 
-bool expand_plan(int B, int S, int Hq, int Hkv, int max_pages, Expand* e) {
-  const int64_t per_seq = (int64_t)max_pages * Hkv * PAGE * DH * 2;  // keys or values, bytes
-  if (S < TC_ROWS || Hq > 65535 || Hkv > 65535 || (int64_t)max_pages * Hkv * PAGE >= (1ll << 31)) return false;
+bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
+  const int64_t per_seq = (int64_t)n_pages * Hkv * PAGE * DH * 2;  // keys or values, bytes
+  if (S < TC_ROWS || Hq > 65535 || Hkv > 65535 || (int64_t)n_pages * Hkv * PAGE >= (1ll << 31)) return false;
   int64_t n = (256ll << 20) / per_seq;
   n = n < 1 ? 1 : n > 65535 ? 65535 : n;
   e->seqs = (int)(n < B ? n : B);
   e->pages = (size_t)per_seq * e->seqs;
-  e->bytes = 2 * e->pages + ((size_t)e->seqs * (max_pages + 2) * sizeof(int) + 15) / 16 * 16;
-  const double sms = mb::num_sms(), pages = (double)B * Hkv * max_pages;
-  const double unpack = 14 + pages * plan_launch(B, S, Hq, Hkv, max_pages).rt * 0.29 / sms;
+  e->bytes = 2 * e->pages + ((size_t)e->seqs * (n_pages + 2) * sizeof(int) + 15) / 16 * 16;
+  const double sms = mb::num_sms(), pages = (double)B * Hkv * n_pages;
+  const double unpack = 14 + pages * plan_launch(B, S, Hq, Hkv, n_pages).rt * 0.29 / sms;
   const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128);
-  const double expand = 3 + calls * (6 + std::ceil(ctas / sms) * ((max_pages + 1) / 2) * 1.37) +
+  const double expand = 3 + calls * (6 + std::ceil(ctas / sms) * ((n_pages + 1) / 2) * 1.37) +
                         pages * (BLOB + 2 * PAGE * DH * 2) / 5.5e6;
   return expand < unpack;
 }
 
 }  // namespace
 
-extern "C" size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_pages) {
-  if (B <= 0 || S <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_pages <= 0) return 0;
-  const size_t n = plan_launch(B, S, Hq, Hkv, max_pages).bytes;
+extern "C" size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_kv_len) {
+  if (B <= 0 || S <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_kv_len <= 0) return 0;
+  const int pages = (int)(((int64_t)max_kv_len + PAGE - 1) / PAGE);
+  const size_t n = plan_launch(B, S, Hq, Hkv, pages).bytes;
   Expand e;
-  return expand_plan(B, S, Hq, Hkv, max_pages, &e) && e.bytes > n ? e.bytes : n;
+  return expand_plan(B, S, Hq, Hkv, pages, &e) && e.bytes > n ? e.bytes : n;
 }
 
 extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache,
                                      int num_pages, const int* block_table, int max_pages,
-                                     const int* kv_len, const int* start_pos, int B, int S, int Hq,
-                                     int Hkv, int Dh, float scale, uint16_t* out, int64_t ldo,
+                                     const int* kv_len, int max_kv_len, const int* start_pos, int B, int S,
+                                     int Hq, int Hkv, int Dh, float scale, uint16_t* out, int64_t ldo,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   MB_REQUIRE(Dh == DH, "attention: head_dim must be 128 (got %d)", Dh);
   MB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention: Hq must be a multiple of Hkv");
@@ -1169,28 +1170,30 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
              "attention kv4: q, out and the cache must be 16-byte aligned");
   MB_REQUIRE((int64_t)S * Hq < (1ll << 30) && (int64_t)max_pages * PAGE < (1ll << 30),
              "attention kv4: too many rows or pages");
-  const Launch p = plan_launch(B, S, Hq, Hkv, max_pages);
-  MB_REQUIRE((int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)max_pages + UNIT_COST) < (1ll << 30),
+  MB_REQUIRE(max_kv_len > 0 && max_kv_len <= max_pages * PAGE, "attention kv4: max_kv_len must be in [1, max_pages*64]");
+  const int pages = (max_kv_len + PAGE - 1) / PAGE;
+  const Launch p = plan_launch(B, S, Hq, Hkv, pages);
+  MB_REQUIRE((int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)pages + UNIT_COST) < (1ll << 30),
              "attention kv4: too many pages");
   MB_REQUIRE(workspace && workspace_bytes >= p.bytes && (uintptr_t)workspace % 16 == 0,
              "attention kv4: workspace of %zu bytes required, 16-byte aligned", p.bytes);
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "attention kv4: no status word");
   Expand e;
-  if (expand_plan(B, S, Hq, Hkv, max_pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
+  if (expand_plan(B, S, Hq, Hkv, pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
       mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo)) {
     MB_REQUIRE(workspace_bytes >= e.bytes, "attention kv4: workspace of %zu bytes required", e.bytes);
     uint16_t* kx = static_cast<uint16_t*>(workspace);
     uint16_t* vx = kx + e.pages / 2;
     int* tx = reinterpret_cast<int*>(vx + e.pages / 2);
-    int *lx = tx + (size_t)e.seqs * max_pages, *sx = lx + e.seqs;
+    int *lx = tx + (size_t)e.seqs * pages, *sx = lx + e.seqs;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int b = 0; b < B; b += e.seqs) {
       const int n = B - b < e.seqs ? B - b : e.seqs;
-      int rc = mb::kv4_expand(cache, num_pages, Hkv, block_table + (int64_t)b * max_pages, max_pages, kv_len + b,
+      int rc = mb::kv4_expand(cache, num_pages, Hkv, block_table + (int64_t)b * max_pages, max_pages, max_kv_len, kv_len + b,
                               start_pos ? start_pos + b : nullptr, n, kx, vx, tx, lx, sx, status, s);
       if (!rc)
-        rc = mb::attention_prefill_tc(q + (int64_t)b * S * ldq, (int)ldq, kx, vx, tx, max_pages, sx, lx, n, S, Hq,
+        rc = mb::attention_prefill_tc(q + (int64_t)b * S * ldq, (int)ldq, kx, vx, tx, pages, sx, lx, n, S, Hq,
                                       Hkv, start_pos != nullptr, out + (int64_t)b * S * ldo, (int)ldo, s, 1, 0,
                                       nullptr, nullptr, scale);
       if (rc) return rc;
@@ -1212,6 +1215,7 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
     a.ldo = ldo;
     a.num_pages = num_pages;
     a.max_pages = max_pages;
+    a.max_len = max_kv_len;
     a.B = B - b < MAX_B ? B - b : MAX_B;
     a.S = S;
     a.Hkv = Hkv;

@@ -425,8 +425,7 @@ struct Plan {
 
 size_t a256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// kv4_pages > 0: over a 4-bit cache with that many pages a sequence.
-Plan make_plan(const Layer& L, int B, int S, int max_kv_len, int kv4_pages = 0) {
+Plan make_plan(const Layer& L, int B, int S, int max_kv_len, bool kv4 = false) {
   Plan p;
   const int D = L.cfg.d_model;
   p.T = (int64_t)B * S;
@@ -453,9 +452,9 @@ Plan make_plan(const Layer& L, int B, int S, int max_kv_len, int kv4_pages = 0) 
   upd(p.ks_o, D);
   upd(p.ks_gu, 2 * L.FF);
   upd(p.ks_down, D);
-  p.attn_ws = kv4_pages ? mb_attention_kv4_workspace_bytes(B, S, L.Hq, L.Hkv, kv4_pages)
-              : S == 1  ? mb_attention_decode_workspace_bytes(B, L.Hq, L.Hkv, max_kv_len)
-                        : 0;
+  p.attn_ws = kv4      ? mb_attention_kv4_workspace_bytes(B, S, L.Hq, L.Hkv, max_kv_len)
+              : S == 1 ? mb_attention_decode_workspace_bytes(B, L.Hq, L.Hkv, max_kv_len)
+                       : 0;
   size_t o = 0;
   p.off_rstd1 = o; o += a256(T * 4);
   p.off_rstd2 = o; o += a256(T * 4);
@@ -467,7 +466,7 @@ Plan make_plan(const Layer& L, int B, int S, int max_kv_len, int kv4_pages = 0) 
   p.off_act = o; o += a256(T * L.FF * 2);
   p.off_part = o; o += a256(part);
   p.off_attn_ws = o; o += a256(p.attn_ws);
-  p.off_kv = o; o += kv4_pages ? 2 * a256(T * L.Dkv * 2) : 0;  // the new keys and values in bf16
+  p.off_kv = o; o += kv4 ? 2 * a256(T * L.Dkv * 2) : 0;  // the new keys and values in bf16
   p.total = o;
   return p;
 }
@@ -609,12 +608,11 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
   MB_REQUIRE(B >= 0 && S >= 0, "decoder forward: negative size");
   if (B == 0 || S == 0) return MB_OK;
   const Layer& L = *static_cast<const Layer*>(layer);
-  MB_REQUIRE(kv4 || (max_kv_len >= S && max_kv_len <= max_pages * 64),
+  MB_REQUIRE(max_kv_len >= (kv4 ? 1 : S) && max_kv_len <= max_pages * 64,
              "decoder forward: max_kv_len must be in [S, max_pages*64]");
-  MB_REQUIRE(max_pages > 0, "decoder forward: the block table has no columns");
   MB_REQUIRE((reinterpret_cast<uintptr_t>(x_res32) | reinterpret_cast<uintptr_t>(y_res32)) % 16 == 0,
              "decoder forward: fp32 residual buffers must be 16-byte aligned");
-  const Plan p = make_plan(L, B, S, max_kv_len, kv4 ? max_pages : 0);
+  const Plan p = make_plan(L, B, S, max_kv_len, kv4 != nullptr);
   MB_REQUIRE(workspace && workspace_bytes >= p.total &&
                  reinterpret_cast<uintptr_t>(workspace) % 256 == 0,
              "decoder forward: workspace of %zu bytes (256-byte aligned) required", p.total);
@@ -688,7 +686,7 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
                             block_table, max_pages, start_pos, kv4->new_len, B, S, s);
     if (!rc)
       rc = mb_attention_kv4_bf16(q, L.Dq, kv4->cache, kv4->num_pages, block_table, max_pages, kv_len,
-                                 causal ? start_pos : nullptr, B, S, L.Hq, L.Hkv, Dh,
+                                 max_kv_len, causal ? start_pos : nullptr, B, S, L.Hq, L.Hkv, Dh,
                                  1.f / sqrtf((float)Dh), attn, L.Dq, w + p.off_attn_ws, p.attn_ws, s);
   } else if (S == 1)
     rc = mb_attention_decode_bf16(q, L.Dq, k_cache, v_cache, block_table, max_pages, kv_len,
@@ -830,22 +828,22 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
 }  // namespace
 
 extern "C" size_t mb_decoder_layer_workspace_bytes_kv4(const void* layer, int B, int S,
-                                                       int max_pages) {
-  if (!layer || B <= 0 || S <= 0 || max_pages <= 0) return 0;
-  return make_plan(*static_cast<const Layer*>(layer), B, S, 0, max_pages).total;
+                                                       int max_kv_len) {
+  if (!layer || B <= 0 || S <= 0 || max_kv_len <= 0) return 0;
+  return make_plan(*static_cast<const Layer*>(layer), B, S, max_kv_len, true).total;
 }
 
 extern "C" int mb_decoder_layer_forward_kv4(const void* layer, const uint16_t* x,
                                             const float* x_res32, const float* rstd_in, uint16_t* y,
                                             float* y_res32, float* rstd_out, int B, int S,
                                             const int* start_pos, const int* kv_len,
-                                            const int* new_len, uint8_t* cache, int num_pages,
+                                            int max_kv_len, const int* new_len, uint8_t* cache, int num_pages,
                                             const int* block_table, int max_pages, int causal,
                                             void* workspace, size_t workspace_bytes,
                                             void* stream) {
   const Kv4 kv4{cache, num_pages, new_len};
   return decoder_forward(layer, x, x_res32, y, y_res32, rstd_in, rstd_out, B, S, start_pos, kv_len,
-                         0, nullptr, nullptr, block_table, max_pages, causal, workspace,
+                         max_kv_len, nullptr, nullptr, block_table, max_pages, causal, workspace,
                          workspace_bytes, stream, &kv4);
 }
 

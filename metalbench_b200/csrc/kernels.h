@@ -102,11 +102,11 @@ int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
                          int max_kv_len = 0, float* part_o = nullptr, float* part_ml = nullptr,
                          float scale = 0.08838834764831845f /* 1 / sqrt(128); > 0 */);
 int attention_split_plan(int64_t B, int64_t S, int64_t Hq, int64_t kv_len);
-// kv4.cu: the pages of B sequences of a 4-bit cache as bf16 pages
-// [B * max_pages][Hkv][64][128] (zeros past a length or for a bad page), with
-// their block table, clamped lengths and first positions.
+// kv4.cu: the pages of B sequences of at most max_len tokens of a 4-bit cache as
+// bf16 pages [B * ceil(max_len / 64)][Hkv][64][128] (zeros past a length or for
+// a bad page), with their block table, clamped lengths and first positions.
 int kv4_expand(const uint8_t* cache, int num_pages, int Hkv, const int* table, int max_pages,
-               const int* kv_len, const int* start_pos, int B, uint16_t* ko, uint16_t* vo,
+               int max_len, const int* kv_len, const int* start_pos, int B, uint16_t* ko, uint16_t* vo,
                int* table_o, int* len_o, int* start_o, uint32_t* status, cudaStream_t s);
 // decoder.cu helpers shared with fused_ops.cu
 int rownorm(const uint16_t* x, int M, int D, float eps, float* rstd, cudaStream_t s);

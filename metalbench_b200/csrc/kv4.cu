@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a, int
   const int lane = threadIdx.x & 31, val = lane >> 4, l = lane & 15;
   const int64_t tok = item / a.Hkv;
   const int h = (int)(item - tok * a.Hkv), b = (int)(tok / a.S), s = (int)(tok - (int64_t)b * a.S);
-  const uint4 x = __ldg(reinterpret_cast<const uint4*>(row_at(a, val, b, s, h)) + l);
+  const uint4 x = reinterpret_cast<const uint4*>(row_at(a, val, b, s, h))[l];
   if (a.new_len && s >= a.new_len[b]) return;
   const int64_t pos = (int64_t)a.start_pos[b] + s;
   const int pg = page_of(a.table, a.max_pages, a.num_pages, b, pos, a.status);
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(256) kv4_append_tokens_kernel(const AppendArgs
       x[i] = y[i] = make_uint4(0, 0, 0, 0);
       if (base + i * 16 + first < rows) {
         const uint4* p = reinterpret_cast<const uint4*>(src + s * ss + h * sh);
-        x[i] = __ldg(p), y[i] = __ldg(p + 1);
+        x[i] = p[0], y[i] = p[1];
       }
       s += ds, h += dh;
       if (h >= a.Hkv) h -= a.Hkv, ++s;
@@ -287,25 +287,25 @@ int log_tokens(int S, int Hkv) {
   return S >= 32 && S >= (1 << lt) ? lt : -1;
 }
 
-// Pages of B sequences as bf16 pages [B * max_pages][Hkv][64][128], with the
+// Pages of B sequences as bf16 pages [B * pages][Hkv][64][128], with the
 // block table, lengths and first positions that go with them: one CTA a page
 // and kv head, lanes as in the storing kernel. A value is rounded to bf16 here
 // (2^-9 relative), as a bf16 cache would hold it.
 __global__ void __launch_bounds__(256) kv4_expand_kernel(
     const uint8_t* __restrict__ cache, int num_pages, int Hkv, const int* __restrict__ table,
-    int max_pages, const int* __restrict__ kv_len, const int* __restrict__ start_pos,
+    int max_pages, int max_len, const int* __restrict__ kv_len, const int* __restrict__ start_pos,
     uint16_t* __restrict__ ko, uint16_t* __restrict__ vo, int* __restrict__ table_o,
     int* __restrict__ len_o, int* __restrict__ start_o, uint32_t* status) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int page = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int L = max(0, min(kv_len[b], max_pages * PAGE));
+  const int L = max(0, min(kv_len[b], max_len)), pages = gridDim.x;
   if (threadIdx.x == 0 && h == 0 && page == 0) {
     len_o[b] = L;
     start_o[b] = start_pos ? min(start_pos[b], L) : L;
   }
   if (page * PAGE >= L) return;
-  const int64_t to = (int64_t)b * max_pages + page;
+  const int64_t to = (int64_t)b * pages + page;
   if (threadIdx.x == 0 && h == 0) table_o[to] = (int)to;
   const int pg = page_of(table, max_pages, num_pages, b, (int64_t)page * PAGE, status);
   const uint8_t* blob = cache + ((int64_t)max(pg, 0) * Hkv + h) * BLOB;
@@ -335,10 +335,10 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
 
 namespace mb {
 int kv4_expand(const uint8_t* cache, int num_pages, int Hkv, const int* table, int max_pages,
-               const int* kv_len, const int* start_pos, int B, uint16_t* ko, uint16_t* vo,
+               int max_len, const int* kv_len, const int* start_pos, int B, uint16_t* ko, uint16_t* vo,
                int* table_o, int* len_o, int* start_o, uint32_t* status, cudaStream_t s) {
-  MB_CUDA(launch_pdl(kv4_expand_kernel, dim3(max_pages, Hkv, B), dim3(256), 0, s, cache, num_pages,
-                     Hkv, table, max_pages, kv_len, start_pos, ko, vo, table_o, len_o, start_o,
+  MB_CUDA(launch_pdl(kv4_expand_kernel, dim3((max_len + kv4::PAGE - 1) / kv4::PAGE, Hkv, B), dim3(256), 0, s,
+                     cache, num_pages, Hkv, table, max_pages, max_len, kv_len, start_pos, ko, vo, table_o, len_o, start_o,
                      status));
   return MB_OK;
 }

@@ -112,9 +112,10 @@ class PagedKV4Cache:
         ops.kv4_append(k, v, self.pools[i], self.block_table, start_pos, new_len)
 
     def attend(self, i: int, q: torch.Tensor, start_pos: torch.Tensor | None = None,
-               scale: float | None = None) -> torch.Tensor:
+               scale: float | None = None, max_kv_len: int | None = None) -> torch.Tensor:
         """Layer i's attention of q [B, S, H, 128] over each sequence's tokens."""
-        return ops.attention_kv4(q, self.pools[i], self.block_table, self.seq_len, start_pos, scale)
+        return ops.attention_kv4(q, self.pools[i], self.block_table, self.seq_len, start_pos, scale,
+                                 max_kv_len=max_kv_len)
 
     def layer(self, i: int) -> "KV4Layer":
         return KV4Layer(self, i)
@@ -204,7 +205,9 @@ class DecoderLayer:
             if new_len is not None and (new_len.dtype != torch.int32 or new_len.device != X.device
                                         or tuple(new_len.shape) != (B,) or not new_len.is_contiguous()):
                 raise ValueError("new_len must be an int32 tensor with one entry per sequence")
-            ws_bytes = _lib.lib().mb_decoder_layer_workspace_bytes_kv4(self._h, B, S, own.max_pages)
+            if max_kv_len is None:
+                max_kv_len = own.max_pages * PAGE  # the lengths are on the device
+            ws_bytes = _lib.lib().mb_decoder_layer_workspace_bytes_kv4(self._h, B, S, max_kv_len)
             # a workspace of the call: captured graphs and other streams keep theirs
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
         else:
@@ -235,7 +238,7 @@ class DecoderLayer:
             ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
             _lib.call("mb_decoder_layer_forward_kv4", self._h, X.data_ptr(), ptr(x_res32), ptr(rstd_in),
                       out.data_ptr(), ptr(y_res32), ptr(rstd_out), B, S, start_pos.data_ptr(),
-                      kv_len.data_ptr(), ptr(new_len), pool.data_ptr(), pool.shape[0],
+                      kv_len.data_ptr(), max_kv_len, ptr(new_len), pool.data_ptr(), pool.shape[0],
                       own.block_table.data_ptr(), own.max_pages, 1 if causal else 0, ws.data_ptr(),
                       ws_bytes, ops._stream())
             return out[0] if squeeze else out

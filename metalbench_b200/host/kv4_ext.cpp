@@ -214,7 +214,7 @@ Rows query(const at::Tensor& t, const char* name, int64_t B, int64_t H) {
 }
 
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  ENTER(7)
+  ENTER(8)
   const Cache c = cache(a[1], "attention_kv4(cache)");
   const Table t = table(a[2], "attention_kv4(block_table)", c.dev);
   const at::Tensor& q = tensor(a[0], "attention_kv4(q)", at::kBFloat16, "bfloat16", c.dev);
@@ -223,6 +223,14 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int* start = a[4] == Py_None ? nullptr : rows(a[4], "attention_kv4(start_pos)", c.dev, t.B);
   double scale = 1.0 / std::sqrt((double)DH);
   if (a[5] != Py_None && (scale = PyFloat_AsDouble(a[5])) == -1.0 && PyErr_Occurred()) return nullptr;
+  int64_t most = t.M * 64;
+  if (a[7] != Py_None) {
+    const int64_t m = PyLong_AsLongLong(a[7]);
+    if (m == -1 && PyErr_Occurred()) return nullptr;
+    if (m < 1 || m > most) refuse(PyExc_ValueError, "attention_kv4", "max_kv_len must be in [1, 64 block table columns]");
+    most = m;
+  }
+  if (most > (1ll << 30)) refuse(PyExc_ValueError, "attention_kv4", "the block table is too wide");
   On on(c.dev);
   at::Tensor out;
   int64_t ldo = r.H * DH;
@@ -233,11 +241,11 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (out.sizes() != q.sizes()) bad_shape("attention_kv4(out)", "q's shape", out);
     ldo = query(out, "attention_kv4(out)", t.B, c.H).ld;
   }
-  const size_t nb = mb_attention_kv4_workspace_bytes((int)t.B, (int)r.S, (int)r.H, (int)c.H, (int)t.M);
+  const size_t nb = mb_attention_kv4_workspace_bytes((int)t.B, (int)r.S, (int)r.H, (int)c.H, (int)most);
   at::Tensor ws = empty({(int64_t)nb}, at::kByte, c.dev);
   void* s = on.stream();
   const int rc = without_gil([&] {
-    return mb_attention_kv4_bf16(b16(q), r.ld, c.p, (int)c.P, t.p, (int)t.M, len, start, (int)t.B, (int)r.S, (int)r.H,
+    return mb_attention_kv4_bf16(b16(q), r.ld, c.p, (int)c.P, t.p, (int)t.M, len, (int)most, start, (int)t.B, (int)r.S, (int)r.H,
                                  (int)c.H, (int)DH, (float)scale, static_cast<uint16_t*>(out.data_ptr()), ldo,
                                  ws.data_ptr(), nb, s);
   });

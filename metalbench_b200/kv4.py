@@ -69,15 +69,18 @@ def kv4_gather(cache: torch.Tensor, block_table: torch.Tensor, start_pos: torch.
 
 def attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
                   kv_len: torch.Tensor, start_pos: torch.Tensor | None = None,
-                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                  scale: float | None = None, out: torch.Tensor | None = None,
+                  max_kv_len: int | None = None) -> torch.Tensor:
     """softmax(scale * q k^T) v over the 4-bit cache (GQA, head dim 128).
 
     q: bf16 [B, S, n_heads, 128], or [B, n_heads, 128] for one token a sequence;
     heads contiguous, positions any multiple of 8 elements apart. Keys
     0..kv_len[b]-1 are seen; with start_pos, row s sees those at positions <=
     start_pos[b] + s (causal). A row that sees no key becomes zeros. scale:
-    1/sqrt(128) by default."""
-    r = (_ext or _kv4()).attention(q, cache, block_table, kv_len, start_pos, scale, out)
+    1/sqrt(128) by default. max_kv_len: no kv_len is larger (longer ones are
+    cut; by default the block table's width); give a bound near the longest
+    length when the table is much wider."""
+    r = (_ext or _kv4()).attention(q, cache, block_table, kv_len, start_pos, scale, out, max_kv_len)
     if type(r) is int:
         _lib.check("mb_attention_kv4_bf16", r)
     return r

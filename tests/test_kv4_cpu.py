@@ -48,11 +48,11 @@ FAKE = 1 << 20  # an aligned address that is refused before anything reads it
 @pytest.mark.parametrize("change, word", [
     (dict(Dh=64), "head_dim"), (dict(Hq=3, Hkv=2), "multiple of Hkv"), (dict(B=-1), "sizes"),
     (dict(q=None), "null"), (dict(q=FAKE + 8), "aligned"), (dict(ldq=132), "aligned"), (dict(num_pages=0), "sizes"),
-    (dict(max_pages=1 << 25), "pages"), (dict(S=1 << 28), "rows"), (dict(ws=None), "workspace"), (dict(ws_bytes=16), "workspace"),
+    (dict(max_pages=1 << 25), "pages"), (dict(S=1 << 28), "rows"), (dict(most=257), "max_kv_len"), (dict(most=0), "max_kv_len"), (dict(ws=None), "workspace"), (dict(ws_bytes=16), "workspace"),
     (dict(S=-1), "sizes"),
 ])
 def test_attention_arguments(lib, change, word):
-    a = dict(q=FAKE, ldq=1024, cache=FAKE, num_pages=4, table=FAKE, max_pages=4, kv_len=FAKE, start=None, B=2, S=1,
+    a = dict(q=FAKE, ldq=1024, cache=FAKE, num_pages=4, table=FAKE, max_pages=4, kv_len=FAKE, most=256, start=None, B=2, S=1,
              Hq=8, Hkv=8, Dh=128, scale=0.1, out=FAKE, ldo=1024, ws=FAKE, ws_bytes=1 << 30)
     a.update(change)
     rc = lib.mb_attention_kv4_bf16(*a.values(), None)
@@ -88,7 +88,7 @@ def test_page_arguments(lib, change, word):
 def test_empty_calls_launch_nothing(lib):
     assert lib.mb_kv4_append_bf16(None, None, 0, 0, 0, 0, 0, 0, None, 1, 1, None, 1, None, None, 0, 4, None) == 0
     assert lib.mb_kv4_gather_f32(None, 1, 1, None, 1, None, None, 2, 0, None, None, None) == 0
-    assert lib.mb_attention_kv4_bf16(None, 0, None, 1, None, 1, None, None, 0, 1, 8, 8, 128, 1.0, None, 0, None, 0, None) == 0
+    assert lib.mb_attention_kv4_bf16(None, 0, None, 1, None, 1, None, 64, None, 0, 1, 8, 8, 128, 1.0, None, 0, None, 0, None) == 0
     assert lib.mb_attention_kv4_workspace_bytes(0, 1, 8, 8, 4) == 0
     assert lib.mb_kv4_page_bytes(8) == 8 * R.BLOB
 

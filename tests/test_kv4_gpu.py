@@ -314,6 +314,23 @@ def test_length_past_the_table_is_cut(ops):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("S", [1, 3, 80])
+def test_a_bound_on_the_lengths(ops, S):
+    """max_kv_len: any bound that holds gives the same rows (the forms may sum in
+    another order); a length beyond it is cut."""
+    rng = np.random.default_rng(18)
+    table = np.arange(300, dtype=np.int32).reshape(2, 150)
+    cache = torch.from_numpy(make_cache(rng, 300, 2)).cuda()
+    q, n = bf(rng.standard_normal((2, S, 8, 128))), i32([130, 100])
+    wide, close, cut = (ops.attention_kv4(q, cache, i32(table), k, max_kv_len=m) for m, k in ((None, n), (130, n), (100, n)))
+    # two forms: weights and outputs rounded to bf16 at most, of values up to 8 times a scale of about 0.3
+    assert (wide.float() - close.float()).abs().max() <= 8 * 2 ** -7
+    assert torch.equal(cut, ops.attention_kv4(q, cache, i32(table[:, :2]), i32([100, 100]), max_kv_len=100))
+    for bad in (0, 9601, -1):
+        with pytest.raises(ValueError):
+            ops.attention_kv4(q, cache, i32(table), n, max_kv_len=bad)
+
+
 def test_far_pages(ops):
     """Byte offsets of the cache past 32 bits."""
     P = 530000  # 4.6 GB
