@@ -342,7 +342,8 @@ struct State {
       uint32_t v = *reinterpret_cast<const uint32_t*>(pg + V_PARAMS + key * 4);
       if (MASKED && key0 + key >= len) k = v = 0;  // what stands past the end may be anything
       // a value scale of 0 (all dims alike, codes 0) must not enter the logarithm
-      const float sv = lo_bf(v), s = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p90f);
+      // (scales below 2^-90 count as that: sums of 2^15 / s over 2^22 keys stay finite)
+      const float sv = lo_bf(v), s = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p126f);
       const float r = fast_rcp(s);
       kp[key] = KeyParams{lo_bf(k) * ck, hi_bf(k) * cm, fast_log2(s), r};
       // a scale that is no number makes the row none (clamping would hide it)
@@ -1114,7 +1115,7 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
 }
 
 // Pieces of a prompt (64 rows a sequence or more): instead of unpacking every
-// page once a row tile of 16, expand the cache once to bf16 pages in the
+// page once a row tile of 16, expand the cache once to fp16 pages in the
 // workspace and run the tcgen05 prefill attention over those, where the times
 // (us) that expand_plan expects say so: 0.29 a page and row tile on one SM, or
 // 1.37 a 128-key tile and wave of CTAs and the expanded bytes at 5.5 TB/s. Measured in us, expanded / unpacked:
@@ -1127,7 +1128,19 @@ constexpr int TC_ROWS = 64;
 
 struct Expand {
   int seqs;  // sequences expanded at a time: up to 512 MB of pages, at least one
-  size_t pages, bytes;
+  size_t pages, rows, exps, bytes;
+  mb::Kv4Expanded at(void* workspace, int n_pages) const {
+    mb::Kv4Expanded o;
+    o.k = static_cast<uint16_t*>(workspace);
+    o.v = o.k + pages / 2;
+    o.q = o.v + pages / 2;
+    o.page_exp = reinterpret_cast<int2*>(o.q + rows * DH);
+    o.row_exp = reinterpret_cast<int*>(o.page_exp + exps);
+    o.table = o.row_exp + rows;
+    o.len = o.table + (size_t)seqs * n_pages;
+    o.start = o.len + seqs;
+    return o;
+  }
 };
 
 bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
@@ -1137,12 +1150,15 @@ bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
   n = n < 1 ? 1 : n > 65535 ? 65535 : n;
   e->seqs = (int)(n < B ? n : B);
   e->pages = (size_t)per_seq * e->seqs;
-  e->bytes = 2 * e->pages + ((size_t)e->seqs * (n_pages + 2) * sizeof(int) + 15) / 16 * 16;
+  e->rows = (size_t)e->seqs * S * Hq;
+  e->exps = (size_t)e->seqs * n_pages * Hkv;
+  e->bytes = 2 * e->pages + e->rows * (DH * 2 + 4) + e->exps * 8 +
+             ((size_t)e->seqs * (n_pages + 2) * sizeof(int) + 15) / 16 * 16;
   const double sms = mb::num_sms(), pages = (double)B * Hkv * n_pages;
   const double unpack = 14 + pages * plan_launch(B, S, Hq, Hkv, n_pages).rt * 0.29 / sms;
   const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128);
   const double expand = 3 + calls * (6 + std::ceil(ctas / sms) * ((n_pages + 1) / 2) * 1.37) +
-                        pages * (BLOB + 2 * PAGE * DH * 2) / 5.5e6;
+                        (pages * (BLOB + 2 * PAGE * DH * 2) + (double)B * S * Hq * DH * 4) / 5.5e6;
   return expand < unpack;
 }
 
@@ -1183,19 +1199,17 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
   if (expand_plan(B, S, Hq, Hkv, pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
       mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo)) {
     MB_REQUIRE(workspace_bytes >= e.bytes, "attention kv4: workspace of %zu bytes required", e.bytes);
-    uint16_t* kx = static_cast<uint16_t*>(workspace);
-    uint16_t* vx = kx + e.pages / 2;
-    int* tx = reinterpret_cast<int*>(vx + e.pages / 2);
-    int *lx = tx + (size_t)e.seqs * pages, *sx = lx + e.seqs;
+    const mb::Kv4Expanded o = e.at(workspace, pages);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int b = 0; b < B; b += e.seqs) {
       const int n = B - b < e.seqs ? B - b : e.seqs;
       int rc = mb::kv4_expand(cache, num_pages, Hkv, block_table + (int64_t)b * max_pages, max_pages, max_kv_len, kv_len + b,
-                              start_pos ? start_pos + b : nullptr, n, kx, vx, tx, lx, sx, status, s);
+                              start_pos ? start_pos + b : nullptr, n, q + (int64_t)b * S * ldq, ldq, S, Hq, o,
+                              status, s);
       if (!rc)
-        rc = mb::attention_prefill_tc(q + (int64_t)b * S * ldq, (int)ldq, kx, vx, tx, pages, sx, lx, n, S, Hq,
-                                      Hkv, start_pos != nullptr, out + (int64_t)b * S * ldo, (int)ldo, s, 1, 0,
-                                      nullptr, nullptr, scale);
+        rc = mb::attention_prefill_tc_f16(o.q, o.row_exp, o.k, o.v, o.page_exp, o.table, pages, o.start, o.len, n,
+                                          S, Hq, Hkv, start_pos != nullptr, out + (int64_t)b * S * ldo, (int)ldo,
+                                          s, scale);
       if (rc) return rc;
     }
     return MB_OK;

@@ -287,45 +287,97 @@ int log_tokens(int S, int Hkv) {
   return S >= 32 && S >= (1 << lt) ? lt : -1;
 }
 
-// Pages of B sequences as bf16 pages [B * pages][Hkv][64][128], with the
-// block table, lengths and first positions that go with them: one CTA a page
-// and kv head, lanes as in the storing kernel. A value is rounded to bf16 here
-// (2^-9 relative), as a bf16 cache would hold it.
+// The exponent that takes a largest magnitude to [2^14, 2^15), within
+// [-112, 113] (all of bf16 but its subnormals; 0 for a maximum of 0): x 2^-e is
+// then an fp16 number to 2^-11 of itself down to 2^-29 of the largest, and to
+// 2^-40 of the largest below.
+__device__ __forceinline__ int fp16_exp(float most) {
+  return most > 0.f ? max(-112, min(113, (__float_as_int(most) >> 23) - 127 - 14)) : 0;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ float max_of_16(float x) {  // over the 16 lanes of a half warp
+#pragma unroll
+  for (int d = 8; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+  return x;
+}
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Pages and query rows of B sequences for the tcgen05 prefill: one CTA a page
+// and kv head, lanes as in the storing kernel, and an equal part of the
+// sequence's query rows. fp16 and not bf16: rounded to bf16, keys alone cost
+// twice the error of the whole result (0.0038 of it against 0.0017 for the
+// output's own rounding, measured with 8192 keys whose channels differ 5-fold).
 __global__ void __launch_bounds__(256) kv4_expand_kernel(
     const uint8_t* __restrict__ cache, int num_pages, int Hkv, const int* __restrict__ table,
     int max_pages, int max_len, const int* __restrict__ kv_len, const int* __restrict__ start_pos,
-    uint16_t* __restrict__ ko, uint16_t* __restrict__ vo, int* __restrict__ table_o,
-    int* __restrict__ len_o, int* __restrict__ start_o, uint32_t* status) {
+    const uint16_t* __restrict__ q, int64_t ldq, int S, int Hq, mb::Kv4Expanded o, uint32_t* status) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int page = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int L = max(0, min(kv_len[b], max_len)), pages = gridDim.x;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0 && h == 0 && page == 0) {
-    len_o[b] = L;
-    start_o[b] = start_pos ? min(start_pos[b], L) : L;
+    o.len[b] = L;
+    o.start[b] = start_pos ? min(start_pos[b], L) : L;
+  }
+  const int rows = S * Hq, step = (int)(gridDim.x * gridDim.y) * 16;
+  for (int base = (page * Hkv + h) * 16; base < rows; base += step) {
+    const int r = base + warp * 2 + half, s = r / Hq;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < rows)
+      x = *reinterpret_cast<const uint4*>(q + ((int64_t)b * S + s) * ldq + (int64_t)(r - s * Hq) * DH + l * 8);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaxf(fabsf(lo_bf(w[j])), fabsf(hi_bf(w[j]))));
+    const int e = fp16_exp(max_of_16(most));
+    const float f = pow2i(-e);
+    if (r < rows) {
+      const int64_t to = (int64_t)b * rows + r;
+      if (l == 0) o.row_exp[to] = e;
+      *reinterpret_cast<uint4*>(o.q + to * DH + l * 8) =
+          make_uint4(half2_of(lo_bf(w[0]) * f, hi_bf(w[0]) * f), half2_of(lo_bf(w[1]) * f, hi_bf(w[1]) * f),
+                     half2_of(lo_bf(w[2]) * f, hi_bf(w[2]) * f), half2_of(lo_bf(w[3]) * f, hi_bf(w[3]) * f));
+    }
   }
   if (page * PAGE >= L) return;
   const int64_t to = (int64_t)b * pages + page;
-  if (threadIdx.x == 0 && h == 0) table_o[to] = (int)to;
+  if (threadIdx.x == 0 && h == 0) o.table[to] = (int)to;
   const int pg = page_of(table, max_pages, num_pages, b, (int64_t)page * PAGE, status);
   const uint8_t* blob = cache + ((int64_t)max(pg, 0) * Hkv + h) * BLOB;
-  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
-  uint16_t* dst = (half ? vo : ko) + (to * Hkv + h) * (PAGE * DH) + l * 8;
+  uint16_t* dst = (half ? o.v : o.k) + (to * Hkv + h) * (PAGE * DH) + l * 8;
   const int par_at = half ? V_PARAMS : K_PARAMS;
+  const int there = pg >= 0 ? min(PAGE, L - page * PAGE) : 0;  // the rest may be anything: it is taken as zeros
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < PAGE / 16; ++i) {
+    const int t = i * 16 + l;
+    if (t < there) {
+      const uint32_t par = *reinterpret_cast<const uint32_t*>(blob + par_at + t * 4);
+      most = fmaxf(most, fmaxf(fabsf(hi_bf(par)), fabsf(fmaf(lo_bf(par), 15.f, hi_bf(par)))));
+    }
+  }
+  const int e = fp16_exp(max_of_16(most));
+  const float f = pow2i(-e);
+  if (warp == 0 && l == 0) {
+    int2* to_e = o.page_exp + to * Hkv + h;
+    (half ? to_e->y : to_e->x) = e;
+  }
 #pragma unroll
   for (int i = 0; i < PAGE / 8; ++i) {
-    const int t = i * 8 + (threadIdx.x >> 5);
+    const int t = i * 8 + warp;
     uint32_t w[4] = {};
-    if (pg >= 0 && page * PAGE + t < L) {  // the rest is read as zeros: what stands there may be anything
+    if (t < there) {
       const uint32_t code = *reinterpret_cast<const uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4));
       const uint32_t par = *reinterpret_cast<const uint32_t*>(blob + par_at + t * 4);
+      const float scale = lo_bf(par) * f, least = hi_bf(par) * f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(
-            fmaf(lo_bf(par), (float)((code >> (8 * j)) & 15u), hi_bf(par)),
-            fmaf(lo_bf(par), (float)((code >> (8 * j + 4)) & 15u), hi_bf(par)));
-        w[j] = *reinterpret_cast<const uint32_t*>(&x);
-      }
+      for (int j = 0; j < 4; ++j)
+        w[j] = half2_of(fmaf(scale, (float)((code >> (8 * j)) & 15u), least),
+                        fmaf(scale, (float)((code >> (8 * j + 4)) & 15u), least));
     }
     *reinterpret_cast<uint4*>(dst + t * DH) = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -335,11 +387,10 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
 
 namespace mb {
 int kv4_expand(const uint8_t* cache, int num_pages, int Hkv, const int* table, int max_pages,
-               int max_len, const int* kv_len, const int* start_pos, int B, uint16_t* ko, uint16_t* vo,
-               int* table_o, int* len_o, int* start_o, uint32_t* status, cudaStream_t s) {
+               int max_len, const int* kv_len, const int* start_pos, int B, const uint16_t* q,
+               int64_t ldq, int S, int Hq, const Kv4Expanded& o, uint32_t* status, cudaStream_t s) {
   MB_CUDA(launch_pdl(kv4_expand_kernel, dim3((max_len + kv4::PAGE - 1) / kv4::PAGE, Hkv, B), dim3(256), 0, s,
-                     cache, num_pages, Hkv, table, max_pages, max_len, kv_len, start_pos, ko, vo, table_o, len_o, start_o,
-                     status));
+                     cache, num_pages, Hkv, table, max_pages, max_len, kv_len, start_pos, q, ldq, S, Hq, o, status));
   return MB_OK;
 }
 }  // namespace mb

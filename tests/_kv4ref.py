@@ -184,9 +184,9 @@ class Pages:
 
 
 def prompt_slack(q, cache, table, lens, first, scale=DIM ** -0.5):
-    """Beside each output of attention(), how far the bf16 form for many rows
-    may be off: keys and values rounded to bf16 (2^-8 of each, half of eps),
-    weights to bf16, fp32 sums."""
+    """Beside each output of attention(), how far the fp16 form for many rows
+    may be off: keys, values and weights rounded to fp16 (2^-11 of each, half
+    of eps; weights under 2^-30 of the largest may be lost), fp32 sums."""
     B, S, Hq, _ = q.shape
     H = cache.shape[1]
     G = Hq // H
@@ -201,9 +201,8 @@ def prompt_slack(q, cache, table, lens, first, scale=DIM ** -0.5):
             k, v = ((m[..., None] + s[..., None] * u).reshape(-1, DIM)[:n] for u, s, m in (got["k"], got["v"]))
             x = q[b, :, h * G: (h + 1) * G].astype(np.float64)
             sc = scale * np.einsum("sgd,nd->sgn", x, k)
-            # a sum of 128 independent roundings, each within 2^-9 |q k|: its root sum of squares, six times over
-            # (uniform errors have a standard deviation of 1/sqrt(3) of their bound: over ten sigma)
-            off = 6 * scale * 2 ** -9 * np.sqrt(np.einsum("sgd,nd->sgn", x ** 2, k ** 2)) + 2 ** -16 * scale * np.einsum("sgd,nd->sgn", np.abs(x), np.abs(k))
+            # a key's rounding, and 128 products summed in fp32 (2^-16 with truncating adders)
+            off = scale * (2 ** -11 + 2 ** -16) * np.einsum("sgd,nd->sgn", np.abs(x), np.abs(k))
             if first is not None:
                 hide = np.arange(n)[None, :] > int(first[b]) + np.arange(S)[:, None]
                 sc[np.broadcast_to(hide[:, None], sc.shape)] = -np.inf
@@ -211,6 +210,7 @@ def prompt_slack(q, cache, table, lens, first, scale=DIM ** -0.5):
             p = np.exp(sc - np.where(np.isfinite(top), top, 0.0))
             tot = p.sum(-1, keepdims=True)
             p = p / np.where(tot > 0, tot, 1.0)
-            size = np.einsum("sgn,nd->sgd", p * (2 * off + 2 ** -9 + 2 ** -9 + 2 ** -14), np.abs(v))
+            # a score off by `off` moves its weight and the sum of all by that factor each
+            size = np.einsum("sgn,nd->sgd", p * (2 * off + 2 ** -11 + 2 ** -11 + 2 ** -14), np.abs(v)) + n * 2 ** -30 * np.abs(v).max()
             slack[b, :, h * G: (h + 1) * G] = size
     return slack

@@ -184,7 +184,7 @@ def test_causal_rows(ops, S, Hq, Hkv):
     (257, 8, 8, [300], True), (64, 16, 2, [128, 500, 63], False),
 ])
 def test_pieces_of_a_prompt(ops, S, Hq, Hkv, lens, causal):
-    """Many rows a sequence: the cache is expanded to bf16 pages first."""
+    """Many rows a sequence: the cache is expanded to fp16 pages first."""
     rng = np.random.default_rng(S + Hq)
     lens = np.array(lens)
     table, P = make_table(rng, lens)
@@ -208,6 +208,41 @@ def test_pieces_of_a_prompt(ops, S, Hq, Hkv, lens, causal):
     neg = ops.attention_kv4(bf(q[:, :, :]), torch.from_numpy(cache).cuda(), i32(table), i32(lens), scale=-128 ** -0.5)
     ref, slack = R.attention(q, cache, table, lens, None, -(128 ** -0.5))
     assert (np.abs(neg.double().cpu().numpy() - ref) <= np.abs(slack) + 2 ** -8 * (np.abs(ref) + np.abs(slack))).all()
+    assert status() == 0
+
+
+def scaled_params(cache, at, exps):
+    """`cache` with the bf16 parameters at `at` times 2^exps[page, head]."""
+    out = cache.copy()
+    par = out[:, :, at: at + 256].copy().view(np.uint16)
+    par = np.where(par & 0x7F80, (par.astype(np.int64) + (exps[:, :, None] << 7)).astype(np.uint16), 0)
+    out[:, :, at: at + 256] = par.astype(np.uint16).view(np.uint8)
+    return out
+
+
+@pytest.mark.parametrize("q_exp, k_exp, v_lo, v_hi", [
+    (100, -100, 0, 1), (-100, 100, 0, 1), (0, 0, 100, 101), (0, 0, -100, -99), (0, 0, -12, 13), (30, -30, -40, 41),
+])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("S, Hq", [(129, 4), (512, 8)])
+def test_pieces_of_a_prompt_over_the_range_of_bf16(ops, S, Hq, q_exp, k_exp, v_lo, v_hi, causal):
+    """Keys, values and rows far outside fp16's own range, values of one page far from another's."""
+    rng = np.random.default_rng(7)
+    Hkv, lens = 2, np.array([129, 400, 700])
+    table, P = make_table(rng, lens)
+    cache = make_cache(rng, P, Hkv)
+    cache = scaled_params(cache, 8192, k_exp + rng.integers(-1, 2, (P, Hkv)))
+    cache = scaled_params(cache, 8448, rng.integers(v_lo, v_hi, (P, Hkv)))
+    q = R.bf16_round(rng.standard_normal((3, S, Hq, 128))) * 2.0 ** (q_exp + rng.integers(-1, 2, (3, S, Hq, 1)))
+    first = lens - S if causal else None
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens), start_pos=None if first is None else i32(first))
+    # the form without expanded pages rounds weights of codes, so it errs by scale * code and minimum apart, not by
+    # their sum alone; and it takes value scales below 2^-90 for that: 15 codes of it
+    ref, slack = R.attention(q, cache, table, lens, first)
+    slack = R.prompt_slack(q, cache, table, lens, first) if S >= 512 else slack + 15 * 2.0 ** -90
+    err = np.abs(got.double().cpu().numpy() - ref)
+    tol = slack + 2 ** -8 * (np.abs(ref) + slack)
+    assert (err <= tol).all(), float((err - tol).max())
     assert status() == 0
 
 
