@@ -345,9 +345,11 @@ struct State {
       // (scales below 2^-90 count as that: sums of 2^15 / s over 2^22 keys stay finite)
       const float sv = lo_bf(v), s = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p126f);
       const float r = fast_rcp(s);
-      kp[key] = KeyParams{lo_bf(k) * ck, hi_bf(k) * cm, fast_log2(s), r};
-      // a scale that is no number makes the row none (clamping would hide it)
-      vmin[key] = sv < INFINITY ? hi_bf(v) * r : NAN;
+      // a key or value stored of what was no number or infinite has such a scale: it makes
+      // the rows that see it NaN, by its score (a term of 0 * NaN would spread to all rows)
+      const bool good = lo_bf(k) < INFINITY && sv < INFINITY;
+      kp[key] = KeyParams{lo_bf(k) * ck, hi_bf(k) * cm, good ? fast_log2(s) : NAN, r};
+      vmin[key] = good ? hi_bf(v) * r : 0.f;
     }
     __syncwarp();
 
@@ -1116,19 +1118,22 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
 
 // Pieces of a prompt (64 rows a sequence or more): instead of unpacking every
 // page once a row tile of 16, expand the cache once to fp16 pages in the
-// workspace and run the tcgen05 prefill attention over those, where the times
-// (us) that expand_plan expects say so: 0.29 a page and row tile on one SM, or
-// 1.37 a 128-key tile and wave of CTAs and the expanded bytes at 5.5 TB/s. Measured in us, expanded / unpacked:
-//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 111 / 81,
-//     128 rows 113 / 144, 512 rows 202 / 513 (the prefill kernel takes 1.37 us
-//     a 128-key tile one after another, so few CTAs leave SMs idle);
-//   16 of 2048, 8, 4:  64 rows 143 / 149, 128 rows 149 / 276;
-//   1 of 1024, 8, 1:  128 rows 21 / 17;  8 of 512, 8, 4:  64 rows 27 / 46.
+// workspace and run the tcgen05 prefill attention over those (the keys cut in
+// parts when the row tiles are too few for the SMs), where the times (us) that
+// expand_plan expects say so: 0.29 a page and row tile on one SM; or 1.5 a
+// 128-key tile and 4 a wave of CTAs, and the bytes at 5.5 TB/s. Measured in us,
+// expanded / unpacked:
+//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 87 / 81,
+//     96 rows 89 / 114, 128 rows 88 / 146, 512 rows 218 / 534;
+//   1 of 32768, 8, 4:  64 rows 145 / 141, 128 rows 150 / 267;
+//   16 of 2048, 8, 4:  64 rows 167 / 162, 128 rows 164 / 298;
+//   1 of 1024, 8, 1:  256 rows 20 / 13;  8 of 512, 8, 4:  64 rows 31 / 57.
 constexpr int TC_ROWS = 64;
 
 struct Expand {
   int seqs;  // sequences expanded at a time: up to 512 MB of pages, at least one
-  size_t pages, rows, exps, bytes;
+  int splits;  // parts that a row tile's keys are cut into, to fill the SMs
+  size_t pages, rows, exps, part_at, bytes;
   mb::Kv4Expanded at(void* workspace, int n_pages) const {
     mb::Kv4Expanded o;
     o.k = static_cast<uint16_t*>(workspace);
@@ -1152,12 +1157,16 @@ bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
   e->pages = (size_t)per_seq * e->seqs;
   e->rows = (size_t)e->seqs * S * Hq;
   e->exps = (size_t)e->seqs * n_pages * Hkv;
-  e->bytes = 2 * e->pages + e->rows * (DH * 2 + 4) + e->exps * 8 +
-             ((size_t)e->seqs * (n_pages + 2) * sizeof(int) + 15) / 16 * 16;
+  e->splits = mb::attention_split_plan(e->seqs, S, Hq, (int64_t)n_pages * PAGE);
+  e->part_at = (2 * e->pages + e->rows * (DH * 2 + 4) + e->exps * 8 + (size_t)e->seqs * (n_pages + 2) * sizeof(int) +
+                15) / 16 * 16;
+  e->bytes = e->part_at + (e->splits > 1 ? e->rows * e->splits * (DH + 2) * sizeof(float) : 0);
   const double sms = mb::num_sms(), pages = (double)B * Hkv * n_pages;
-  const double unpack = 14 + pages * plan_launch(B, S, Hq, Hkv, n_pages).rt * 0.29 / sms;
-  const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128);
-  const double expand = 3 + calls * (6 + std::ceil(ctas / sms) * ((n_pages + 1) / 2) * 1.37) +
+  const int rt = plan_launch(B, S, Hq, Hkv, n_pages).rt, sp = e->splits;
+  const double unpack = 9 + (pages + 8.0 * B * Hkv) * rt * 0.29 / sms;  // a unit's start and end: 8 pages
+  const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128) * sp;
+  const double tiles = ((n_pages + 1) / 2 + sp - 1) / sp;
+  const double expand = 3 + calls * (4 + std::ceil(ctas / sms) * (4 + tiles * 1.5) + (sp > 1 ? 7 : 0)) +
                         (pages * (BLOB + 2 * PAGE * DH * 2) + (double)B * S * Hq * DH * 4) / 5.5e6;
   return expand < unpack;
 }
@@ -1200,6 +1209,7 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
       mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo)) {
     MB_REQUIRE(workspace_bytes >= e.bytes, "attention kv4: workspace of %zu bytes required", e.bytes);
     const mb::Kv4Expanded o = e.at(workspace, pages);
+    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + e.part_at);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int b = 0; b < B; b += e.seqs) {
       const int n = B - b < e.seqs ? B - b : e.seqs;
@@ -1209,7 +1219,7 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
       if (!rc)
         rc = mb::attention_prefill_tc_f16(o.q, o.row_exp, o.k, o.v, o.page_exp, o.table, pages, o.start, o.len, n,
                                           S, Hq, Hkv, start_pos != nullptr, out + (int64_t)b * S * ldo, (int)ldo,
-                                          s, scale);
+                                          s, scale, e.splits, pages * PAGE, part, part + e.rows * e.splits * DH);
       if (rc) return rc;
     }
     return MB_OK;

@@ -69,7 +69,7 @@ struct AttnTcParams {
   float scale_log2;
   uint16_t* out;
   int ldo;
-  // split-KV (non-causal only): CTA split sp handles key tiles
+  // split-KV (bf16: non-causal only): CTA split sp handles key tiles
   // [sp*tiles_per_split, +tiles_per_split) and writes its unnormalised O,
   // running max and row sum per row to part_o / part_ml instead of out
   int splits, tiles_per_split, Hq;
@@ -498,13 +498,14 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
                                          __uint_as_float(o[4 * e + 3]));
       }
       if (row < p.S && half == 0) {
-        p.part_ml[prow * 2] = m;
+        p.part_ml[prow * 2] = F16 && lt != lt ? 0.f : m;
         p.part_ml[prow * 2 + 1] = lt;
       }
     } else if (fin) {
       mbd::tc_fence_after();
-      const float inv = lt > 0.f ? 1.f / lt : 0.f;
-      const uint32_t keep = lt > 0.f ? 0xFFFFFFFFu : 0u;  // no visible key: O was never written
+      const bool any = F16 ? lt != 0.f : lt > 0.f;  // F16: a NaN that a row sees stays one
+      const float inv = any ? 1.f / lt : 0.f;
+      const uint32_t keep = any ? 0xFFFFFFFFu : 0u;  // no visible key: O was never written
       uint4* dst =
           reinterpret_cast<uint4*>(p.out + ((int64_t)b * p.S + row) * p.ldo + h * DHT + c0);
 #pragma unroll 1
@@ -539,6 +540,7 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
 
 // out row = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M = max_s m_s;
 // one 128-thread block per (sequence, head, query row), thread = dim
+template <bool F16>
 __global__ void __launch_bounds__(128) attn_split_combine_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_ml, int S, int Hq,
     int splits, uint16_t* __restrict__ out, int ldo) {
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(128) attn_split_combine_kernel(
     lsum += w * ml[2 * s + 1];
     acc += w * part_o[(rid * splits + s) * DHT + threadIdx.x];
   }
-  const float v = lsum > 0.f ? acc / lsum : 0.f;
+  const float v = (F16 ? lsum != 0.f : lsum > 0.f) ? acc / lsum : 0.f;
   __nv_bfloat16 hv = __float2bfloat16_rn(v);
   out[(b * S + row) * (int64_t)ldo + h * DHT + threadIdx.x] = *reinterpret_cast<uint16_t*>(&hv);
 }
@@ -588,7 +590,7 @@ int launch_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache, const
                       const int* kv_len, int B, int S, int Hq, int Hkv, int causal, uint16_t* out,
                       int ldo, cudaStream_t stream, int splits, int max_kv_len, float* part_o,
                       float* part_ml, float scale, const int* row_exp, const int2* page_exp) {
-  MB_REQUIRE(splits == 1 || (!causal && part_o && part_ml && max_kv_len > 0),
+  MB_REQUIRE(splits == 1 || ((F16 || !causal) && part_o && part_ml && max_kv_len > 0),
              "attention: split-KV needs a non-causal call, max_kv_len and partial buffers");
   AttnTcParams p;
   const auto bf = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -630,7 +632,7 @@ int launch_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache, const
   attn_prefill_tc_kernel<F16><<<grid, 64 + NSOFT, SMEM_BYTES, stream>>>(p, device_status_ptr());
   MB_CUDA(cudaGetLastError());
   if (splits > 1) {
-    attn_split_combine_kernel<<<(unsigned)((int64_t)B * Hq * S), 128, 0, stream>>>(
+    attn_split_combine_kernel<F16><<<(unsigned)((int64_t)B * Hq * S), 128, 0, stream>>>(
         part_o, part_ml, S, Hq, splits, out, ldo);
     MB_CUDA(cudaGetLastError());
   }
@@ -652,9 +654,10 @@ int attention_prefill_tc_f16(const uint16_t* q, const int* row_exp, const uint16
                              const uint16_t* v_cache, const int2* page_exp, const int* block_table,
                              int max_pages, const int* start_pos, const int* kv_len, int B, int S,
                              int Hq, int Hkv, int causal, uint16_t* out, int ldo,
-                             cudaStream_t stream, float scale) {
+                             cudaStream_t stream, float scale, int splits, int max_kv_len,
+                             float* part_o, float* part_ml) {
   return launch_prefill_tc<true>(q, Hq * DHT, k_cache, v_cache, block_table, max_pages, start_pos, kv_len, B,
-                                 S, Hq, Hkv, causal, out, ldo, stream, 1, 0, nullptr, nullptr, scale,
+                                 S, Hq, Hkv, causal, out, ldo, stream, splits, max_kv_len, part_o, part_ml, scale,
                                  row_exp, page_exp);
 }
 

@@ -103,12 +103,13 @@ int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
                          float scale = 0.08838834764831845f /* 1 / sqrt(128); > 0 */);
 // The same over fp16 operands with power-of-two factors: q [B * S][Hq * 128]
 // holds q 2^-row_exp ([B][S][Hq]), the pages hold k 2^-x and v 2^-y of page_exp
-// ([B][max_pages][Hkv]); exponents within [-112, 113].
+// ([B][max_pages][Hkv]); exponents within [-112, 113]. splits as above, causal or not.
 int attention_prefill_tc_f16(const uint16_t* q, const int* row_exp, const uint16_t* k_cache,
                              const uint16_t* v_cache, const int2* page_exp, const int* block_table,
                              int max_pages, const int* start_pos, const int* kv_len, int B, int S,
                              int Hq, int Hkv, int causal, uint16_t* out, int ldo,
-                             cudaStream_t stream, float scale);
+                             cudaStream_t stream, float scale, int splits, int max_kv_len,
+                             float* part_o, float* part_ml);
 int attention_split_plan(int64_t B, int64_t S, int64_t Hq, int64_t kv_len);
 // kv4.cu: what attention_prefill_tc_f16 reads, made from B sequences of at most
 // max_len tokens of a 4-bit cache (pages [B * ceil(max_len / 64)][Hkv][64][128],

@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
     const int t = i * 16 + l;
     if (t < there) {
       const uint32_t par = *reinterpret_cast<const uint32_t*>(blob + par_at + t * 4);
-      most = fmaxf(most, fmaxf(fabsf(hi_bf(par)), fabsf(fmaf(lo_bf(par), 15.f, hi_bf(par)))));
+      if (lo_bf(par) < INFINITY) most = fmaxf(most, fmaxf(fabsf(hi_bf(par)), fabsf(fmaf(lo_bf(par), 15.f, hi_bf(par)))));
     }
   }
   const int e = fp16_exp(max_of_16(most));
@@ -372,8 +372,13 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
     uint32_t w[4] = {};
     if (t < there) {
       const uint32_t code = *reinterpret_cast<const uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4));
-      const uint32_t par = *reinterpret_cast<const uint32_t*>(blob + par_at + t * 4);
-      const float scale = lo_bf(par) * f, least = hi_bf(par) * f;
+      const uint32_t kpar = *reinterpret_cast<const uint32_t*>(blob + K_PARAMS + t * 4);
+      const uint32_t vpar = *reinterpret_cast<const uint32_t*>(blob + V_PARAMS + t * 4);
+      const uint32_t par = half ? vpar : kpar;
+      // stored of what was no number or infinite: the key's scores make the rows that see it
+      // NaN, and its value is 0, since a weight of 0 times NaN would spread to all rows
+      const bool good = lo_bf(kpar) < INFINITY && lo_bf(vpar) < INFINITY;
+      const float scale = good ? lo_bf(par) * f : 0.f, least = good ? hi_bf(par) * f : half ? 0.f : NAN;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         w[j] = half2_of(fmaf(scale, (float)((code >> (8 * j)) & 15u), least),

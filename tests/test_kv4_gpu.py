@@ -196,8 +196,10 @@ def test_pieces_of_a_prompt(ops, S, Hq, Hkv, lens, causal):
     q = R.bf16_round(rng.standard_normal((len(lens), S, Hq, 128)))
     first = lens - S if causal else None  # some rows stand before the first key
     got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens), start_pos=None if first is None else i32(first))
-    ref, _ = R.attention(q, cache, table, lens, first)
-    slack = R.prompt_slack(q, cache, table, lens, first)
+    # either form may be taken: unpacked pages round weights of codes (2^-11 of scale * code and of the minimum
+    # apart, which may cancel in the sum), expanded ones the values themselves
+    ref, slack = R.attention(q, cache, table, lens, first)
+    slack = np.maximum(slack, R.prompt_slack(q, cache, table, lens, first))
     err = np.abs(got.double().cpu().numpy() - ref)
     tol = slack + 2 ** -8 * (np.abs(ref) + slack)
     assert (err <= tol).all(), float((err - tol).max())
@@ -243,6 +245,48 @@ def test_pieces_of_a_prompt_over_the_range_of_bf16(ops, S, Hq, q_exp, k_exp, v_l
     err = np.abs(got.double().cpu().numpy() - ref)
     tol = slack + 2 ** -8 * (np.abs(ref) + slack)
     assert (err <= tol).all(), float((err - tol).max())
+    assert status() == 0
+
+
+@pytest.mark.parametrize("S, Hq, B, L", [(128, 4, 1, 3000), (100, 3, 2, 1500), (300, 8, 1, 2049)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_few_row_tiles_over_many_keys(ops, S, Hq, B, L, causal):
+    """The keys of a row tile are cut among several CTAs and joined."""
+    rng = np.random.default_rng(S)
+    lens = np.array([L, L // 2 + 3][:B])
+    table, P = make_table(rng, lens)
+    cache = make_cache(rng, P, 1)
+    q = R.bf16_round(rng.standard_normal((B, S, Hq, 128)))
+    first = np.array([L - S, -S // 2][:B]) if causal else None  # the second one: rows that see nothing, few keys seen
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens), start_pos=None if first is None else i32(first))
+    ref, slack = R.attention(q, cache, table, lens, first)
+    slack = np.maximum(slack, R.prompt_slack(q, cache, table, lens, first))
+    err = np.abs(got.double().cpu().numpy() - ref)
+    tol = slack + 2 ** -8 * (np.abs(ref) + slack)
+    assert (err <= tol).all(), float((err - tol).max())
+    assert status() == 0
+
+
+@pytest.mark.parametrize("at", ["k", "v"])
+@pytest.mark.parametrize("S, Hq, Hkv, L", [(4, 8, 1, 300), (33, 4, 2, 400), (512, 8, 2, 700), (128, 4, 1, 3000)])
+def test_only_rows_that_see_a_nan_become_one(ops, S, Hq, Hkv, L, at):
+    """A key or value that is no number, behind some rows' positions."""
+    rng = np.random.default_rng(L)
+    lens, first = np.array([L, L]), np.array([L - S, L - S])
+    table, P = make_table(rng, lens)
+    cache = make_cache(rng, P, Hkv)
+    q = R.bf16_round(rng.standard_normal((2, S, Hq, 128)))
+    ref, slack = R.attention(q, cache, table, lens, first)
+    slack = np.maximum(slack, R.prompt_slack(q, cache, table, lens, first))
+    hide = S // 2  # rows from here see the position
+    pos = L - S + hide
+    bad = cache.copy()
+    bad[table[0, pos // 64], 0, (8192 if at == "k" else 8448) + 4 * (pos % 64):][:4] = 0xFF  # scale and minimum: NaN
+    got = ops.attention_kv4(bf(q), torch.from_numpy(bad).cuda(), i32(table), i32(lens), start_pos=i32(first)).double().cpu().numpy()
+    G = Hq // Hkv
+    assert np.isnan(got[0, hide:, :G]).all()
+    got[0, hide:, :G] = ref[0, hide:, :G]
+    assert (np.abs(got - ref) <= slack + 2 ** -8 * (np.abs(ref) + slack)).all()
     assert status() == 0
 
 
