@@ -261,9 +261,14 @@ int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv, const int* b
  * 0..kv_len[b]-1; with start_pos, row s sees the keys at positions <=
  * start_pos[b] + s only (causal), else all. max_kv_len (1 .. 64 max_pages): no
  * kv_len is larger (one that is is cut to it); it sizes the workspace and chooses
- * the form, so a bound near the longest length serves wide block tables best. q, out: bf16 [B][S][Hq][128] with ldq /
- * ldo elements between two positions' rows (multiples of 8), the heads
- * contiguous. A row that sees no key becomes zeros. Every length is read on the device, so ragged batches balance and the call can be captured. */
+ * the form, so a bound near the longest length serves wide block tables best.
+ * q, out: bf16 [B][S][Hq][128] with ldq / ldo elements between two positions'
+ * rows (multiples of 8), the heads contiguous; out may be q. A row that sees no
+ * key becomes zeros, one that sees a token read back as NaN becomes NaN. Good for
+ * |q| below 2^111 and for a sequence's value scales within 2^90 of each other;
+ * values stored with a scale below 2^-90 may count as up to 2^-86 more. Every
+ * length is read on the device, so ragged batches balance and the call can be
+ * captured. */
 size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_kv_len);
 int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8_t* cache, int num_pages,
                           const int* block_table, int max_pages, const int* kv_len,

@@ -11,8 +11,9 @@
 // u * 2^-24 (u * 2^-20 for the odd code of a byte), a subnormal that mma.sync
 // multiplies exactly. Eight codes become four operand registers in five
 // logic operations; the powers of two are taken out of q (2^-4) and of the
-// sums. q is scaled by a power of two into fp16's range, which loses nothing
-// of a bf16 number down to 2^-20 of the tile's largest.
+// sums. Each row of q is scaled by its own power of two into fp16's range, which
+// loses nothing of a bf16 number down to 2^-20 of the row's largest (one power
+// for a tile would let a padding row that holds anything take the others' bits).
 // The value scale goes into the exponent: P_j = 2^(score_j + log2(sv_j) - R)
 // with a running reference R per query row, so that P_j sv-weighted is what is
 // rounded to fp16 (11 bits, and 2^-24 absolute at a range up to 2^15), and the
@@ -205,7 +206,7 @@ __device__ __forceinline__ int find_seq(const int* pre, int B, int f) {
 // A key's numbers as the scores use them, worked out once a page by the lane
 // that owns the key and read by the four lanes that need it.
 struct __align__(16) KeyParams {
-  float sk, mk;  // key scale and minimum, with the softmax scale and q's power of two
+  float sk, mk;  // key scale and minimum
   float lg, rv;  // log2 and reciprocal of the value scale
 };
 
@@ -219,7 +220,8 @@ struct State {
   float o[NT][4][2][4];  // [32-dim piece][dim pair][accumulator]
   float R[NT][2], l[NT][2], om[NT][2];
   uint32_t qf[NT][16];   // q as B fragments
-  float qs[NT][2];       // sum of q's dims
+  float qs[NT][2];       // sum of q's dims, scaled as the products are
+  float qc[NT][2];       // what takes these to scores in log2 units
   int lim[NT][2];        // keys below lim are seen by column 2 tig + e
 
   __device__ __forceinline__ void reset() {
@@ -239,14 +241,11 @@ struct State {
     }
   }
 
-  // q of row tile rt as B fragments, scaled by a power of two; the factor that
-  // key scales take for it and the softmax scale. L keys in all, row s sees
-  // those at positions <= first + s.
-  __device__ __forceinline__ float load_q(const Args& a, int b, int kvh, int rt, int L, int first) {
+  // q of row tile rt as B fragments, each row scaled by a power of two. L keys in
+  // all, row s sees those at positions <= first + s.
+  __device__ __forceinline__ void load_q(const Args& a, int b, int kvh, int rt, int L, int first) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-    // ---- q of this unit as B fragments, scaled by a power of two ----
     float x[NT][32];
-    float big = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = rt * (NT * 8) + t * 8 + gid;
@@ -265,29 +264,30 @@ struct State {
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[t][i] = 0.f;
       }
-      float sum = 0.f;
+      float sum = 0.f, big = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         big = fmaxf(big, fabsf(x[t][i]));
         sum += x[t][i];
       }
 #pragma unroll
-      for (int off = 1; off <= 2; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      for (int off = 1; off <= 2; off <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+      }
+      // 2^e brings the row's largest to [2^11, 2^12)
+      const int e = max(-100, min(100, 11 - ((int)(__float_as_uint(big) >> 23) - 127)));
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23), up16 = up * 0.0625f;
+      const float back = a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
+      sum *= up * 0x1p-24f;
       const int mylim = min(L, first + s + 1);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int from = (2 * tig + c) * 4;  // a lane whose fragment row is column 2 tig + c
         qs[t][c] = __shfl_sync(0xffffffffu, sum, from);
+        qc[t][c] = __shfl_sync(0xffffffffu, back, from);
         lim[t][c] = __shfl_sync(0xffffffffu, mylim, from);
       }
-    }
-#pragma unroll
-    for (int off = 1; off <= 16; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-    // 2^e brings the tile's largest to [2^11, 2^12)
-    const int e = max(-100, min(100, 11 - ((int)(__float_as_uint(big) >> 23) - 127)));
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23), up16 = up * 0.0625f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         qf[t][4 * w] = pack_h2(x[t][8 * w] * up, x[t][8 * w + 4] * up);
@@ -295,7 +295,7 @@ struct State {
         qf[t][4 * w + 2] = pack_h2(x[t][8 * w + 2] * up, x[t][8 * w + 6] * up);
         qf[t][4 * w + 3] = pack_h2(x[t][8 * w + 3] * up16, x[t][8 * w + 7] * up16);
       }
-    return a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
+    }
   }
 
   // l and om are sums over a lane's keys until here.
@@ -332,8 +332,7 @@ struct State {
   // One page (pg, in shared memory) of keys key0 .. key0 + 63. MASKED: some of
   // them stand past the end (len) or are not seen by every column.
   template <bool MASKED>
-  __device__ __forceinline__ void page(const uint8_t* pg, KeyParams* kp, float* vmin, int key0, int len,
-                                       float ck, float cm) {
+  __device__ __forceinline__ void page(const uint8_t* pg, KeyParams* kp, float* vmin, int key0, int len) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -348,7 +347,7 @@ struct State {
       // a key or value stored of what was no number or infinite has such a scale: it makes
       // the rows that see it NaN, by its score (a term of 0 * NaN would spread to all rows)
       const bool good = lo_bf(k) < INFINITY && sv < INFINITY;
-      kp[key] = KeyParams{lo_bf(k) * ck, hi_bf(k) * cm, good ? fast_log2(s) : NAN, r};
+      kp[key] = KeyParams{lo_bf(k), hi_bf(k), good ? fast_log2(s) : NAN, r};
       vmin[key] = good ? hi_bf(v) * r : 0.f;
     }
     __syncwarp();
@@ -402,7 +401,7 @@ struct State {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaf(p.mk, qs[t][c], fmaf(p.sk, sc[t][mt][2 * r + c], p.lg));
+            float x = fmaf(qc[t][c], fmaf(p.mk, qs[t][c], p.sk * sc[t][mt][2 * r + c]), p.lg);
             if (MASKED && key0 + key >= lim[t][c]) x = -INFINITY;
             sc[t][mt][2 * r + c] = x;
           }
@@ -701,7 +700,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
     const int first = a.start_pos ? min(a.start_pos[b], L) : L;
     z.reset();
     {
-      const float ck = z.load_q(a, b, kvh, rt, L, first);
+      z.load_q(a, b, kvh, rt, L, first);
       const int all_seen = min(L, first + (rt * COLS) / a.G + 1);  // keys that every column sees
 
       for (int f = f0; f < f1; ++f) {
@@ -714,9 +713,9 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
         if (!dead && ok_flag[st]) {
           const int key0 = (f - ub) * PAGE;
           if (key0 + PAGE <= all_seen)
-            z.template page<false>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
+            z.template page<false>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L);
           else
-            z.template page<true>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
+            z.template page<true>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L);
         }
         __syncwarp();  // all lanes are done with this page
         ++used;
@@ -843,7 +842,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_one_kernel(const 
   z.reset();
   if (mine > 0) {
     const int first = a.start_pos ? min(a.start_pos[0], L) : L;
-    const float ck = z.load_q(a, 0, kvh, rt, L, first);
+    z.load_q(a, 0, kvh, rt, L, first);
     const int all_seen = min(L, first + (rt * COLS) / a.G + 1);
     for (int used = 0; used < mine; ++used) {
       const int st = used % ST;
@@ -855,9 +854,9 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_one_kernel(const 
       if (!dead && ok_flag[st]) {
         const int key0 = (begin + used) * PAGE;
         if (key0 + PAGE <= all_seen)
-          z.template page<false>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
+          z.template page<false>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L);
         else
-          z.template page<true>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L, ck, a.scale_log2);
+          z.template page<true>(ring + st * BLOB, sm.kp[warp], sm.vmin[warp], key0, L);
       }
       __syncwarp();
       if (issued < mine && !dead) issue();

@@ -5,7 +5,7 @@
 // For the 128 dims x of one token and kv head (keys and values alike):
 //   m = min x,  s = bf16((max x - m) / 15),  u = clamp(rint((x - m) / s), 0, 15)
 // with u = 0 where s = 0; the stored value is m + s u. m is exact (x is bf16);
-// s is rounded to bf16 (2^-9 relative: at most 3 % of one code step at u = 15)
+// s is rounded to bf16 (2^-8 relative: at most 6 % of one code step at u = 15)
 // because its 2 bytes a token are read by every later step.
 #include "kv4.cuh"
 #include "kernels.h"
@@ -84,7 +84,7 @@ __device__ __noinline__ Row<W> quantise(uint4 ra, uint4 rb) {
     const float inv = __frcp_rn(sc);
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
-      uint32_t sum = 0;  // of (bits of 1.5 * 2^23 + u) * 16^i: u <= 15, as s is within 2^-9 of range / 15
+      uint32_t sum = 0;  // of (bits of 1.5 * 2^23 + u) * 16^i: u <= 15, as s is within 2^-8 of range / 15
 #pragma unroll
       for (int i = 7; i >= 0; --i) {
         const float d = x[8 * k + i] - lo, q = d * inv;

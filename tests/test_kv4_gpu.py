@@ -290,6 +290,40 @@ def test_only_rows_that_see_a_nan_become_one(ops, S, Hq, Hkv, L, at):
     assert status() == 0
 
 
+@pytest.mark.parametrize("B, S, Hq, Hkv", [(1, 4, 8, 2), (3, 4, 8, 2), (2, 2, 16, 1), (2, 70, 4, 4), (2, 400, 8, 2)])
+@pytest.mark.parametrize("what", [float("inf"), float("nan"), 3e38, 1e20])
+def test_padding_rows_may_hold_anything(ops, B, S, Hq, Hkv, what):
+    """Rows behind a sequence's new tokens share tiles with its own."""
+    rng = np.random.default_rng(S)
+    lens = np.array([S + 70, S + 200, S][:B])
+    table, P = make_table(rng, lens)
+    cache = make_cache(rng, P, Hkv)
+    first = lens - S
+    q = R.bf16_round(rng.standard_normal((B, S, Hq, 128)))
+    ref, slack = R.attention(q, cache, table, lens, first)
+    slack = np.maximum(slack, R.prompt_slack(q, cache, table, lens, first))
+    keep = S // 2
+    q[:, keep:] = what
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens), start_pos=i32(first))
+    err = np.abs(got.double().cpu().numpy() - ref)[:, :keep]
+    assert (err <= (slack + 2 ** -8 * (np.abs(ref) + slack))[:, :keep]).all(), float(err.max())
+    assert status() == 0
+
+
+@pytest.mark.parametrize("B, S, Hq, Hkv, L", [(1, 1, 8, 2, 700), (3, 1, 32, 8, 3000), (2, 5, 8, 2, 500), (2, 300, 8, 2, 600)])
+def test_the_output_may_take_the_place_of_the_queries(ops, B, S, Hq, Hkv, L):
+    rng = np.random.default_rng(L)
+    lens = np.array([L, L // 2, 0][:B])
+    table, P = make_table(rng, lens)
+    cache = torch.from_numpy(make_cache(rng, P, Hkv)).cuda()
+    q = bf(R.bf16_round(rng.standard_normal((B, S, Hq, 128))))
+    want = ops.attention_kv4(q, cache, i32(table), i32(lens))
+    for _ in range(3):
+        both = q.clone()
+        ops.attention_kv4(both, cache, i32(table), i32(lens), out=both)
+        assert torch.equal(both, want)
+
+
 @pytest.mark.parametrize("S", [1, 4, 70])
 def test_rows_that_see_nothing_are_zero(ops, S):
     rng = np.random.default_rng(9)
