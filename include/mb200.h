@@ -242,14 +242,16 @@ int mb_attention_prefill_bf16(const uint16_t* q, int ldq, const uint16_t* k_cach
 size_t mb_kv4_page_bytes(int Hkv);
 
 /* Store the keys and values of S tokens a sequence: token s < new_len[b] (null:
- * S) goes to position start_pos[b] + s. k, v: bf16 [B][S][Hkv][128] with the
+ * S) goes to position start_pos[b] + s, unless that is kv_len[b] or past it (null:
+ * no limit): with the lengths of mb_kv_pages_extend there, tokens that it found no
+ * pages for are not stored over what stale table entries name. k, v: bf16 [B][S][Hkv][128] with the
  * element strides given (multiples of 8; the 128 dims contiguous), 16-byte
  * aligned. Nothing else of the cache is written. */
 int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, int64_t k_batch, int64_t k_token,
                        int64_t k_head, int64_t v_batch, int64_t v_token, int64_t v_head,
                        uint8_t* cache, int num_pages, int Hkv, const int* block_table,
-                       int max_pages, const int* start_pos, const int* new_len, int B, int S,
-                       void* stream);
+                       int max_pages, const int* start_pos, const int* new_len,
+                       const int* kv_len, int B, int S, void* stream);
 
 /* Read positions start_pos[b] .. start_pos[b] + S - 1 back as fp32
  * [B][S][Hkv][128]; zeros at positions >= kv_len[b]. */

@@ -97,7 +97,7 @@ SIGNATURES = {
     "mb_attention_prefill_bf16": (C.c_int, [_P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I,
                                             _P, _I, _P]),
     "mb_kv4_page_bytes": (C.c_size_t, [_I]),
-    "mb_kv4_append_bf16": (C.c_int, [_P, _P] + [_I64] * 6 + [_P, _I, _I, _P, _I, _P, _P, _I, _I, _P]),
+    "mb_kv4_append_bf16": (C.c_int, [_P, _P] + [_I64] * 6 + [_P, _I, _I, _P, _I, _P, _P, _P, _I, _I, _P]),
     "mb_kv4_gather_f32": (C.c_int, [_P, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P]),
     "mb_attention_kv4_workspace_bytes": (C.c_size_t, [_I] * 5),
     "mb_attention_kv4_bf16": (C.c_int, [_P, _I64, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I,

@@ -1128,6 +1128,7 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
 //   16 of 2048, 8, 4:  64 rows 167 / 162, 128 rows 164 / 298;
 //   1 of 1024, 8, 1:  256 rows 20 / 13;  8 of 512, 8, 4:  64 rows 31 / 57.
 constexpr int TC_ROWS = 64;
+constexpr size_t MOST_EXPANDED = size_t(6) << 30;  // workspace: a sequence of 1.3 million tokens of 8 heads
 
 struct Expand {
   int seqs;  // sequences expanded at a time: up to 512 MB of pages, at least one
@@ -1160,6 +1161,7 @@ bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
   e->part_at = (2 * e->pages + e->rows * (DH * 2 + 4) + e->exps * 8 + (size_t)e->seqs * (n_pages + 2) * sizeof(int) +
                 15) / 16 * 16;
   e->bytes = e->part_at + (e->splits > 1 ? e->rows * e->splits * (DH + 2) * sizeof(float) : 0);
+  if (e->bytes > MOST_EXPANDED) return false;
   const double sms = mb::num_sms(), pages = (double)B * Hkv * n_pages;
   const int rt = plan_launch(B, S, Hq, Hkv, n_pages).rt, sp = e->splits;
   const double unpack = 9 + (pages + 8.0 * B * Hkv) * rt * 0.29 / sms;  // a unit's start and end: 8 pages

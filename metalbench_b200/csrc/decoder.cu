@@ -683,7 +683,7 @@ int decoder_forward(const void* layer, const uint16_t* x, const float* x_res32, 
   if (kv4) {
     const int64_t tok = L.Dkv, seq = (int64_t)S * L.Dkv;
     rc = mb_kv4_append_bf16(k_new, v_new, seq, tok, Dh, seq, tok, Dh, kv4->cache, kv4->num_pages, L.Hkv,
-                            block_table, max_pages, start_pos, kv4->new_len, B, S, s);
+                            block_table, max_pages, start_pos, kv4->new_len, kv_len, B, S, s);
     if (!rc)
       rc = mb_attention_kv4_bf16(q, L.Dq, kv4->cache, kv4->num_pages, block_table, max_pages, kv_len,
                                  max_kv_len, causal ? start_pos : nullptr, B, S, L.Hq, L.Hkv, Dh,

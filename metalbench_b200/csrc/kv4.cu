@@ -117,7 +117,7 @@ struct AppendArgs {
   const uint16_t *k, *v;
   int64_t kb, ks, kh, vb, vs, vh;  // element strides: batch, token, head
   uint8_t* cache;
-  const int *table, *start_pos, *new_len;
+  const int *table, *start_pos, *new_len, *kv_len;
   int num_pages, max_pages, Hkv, S;
   uint32_t* status;
 };
@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a, int
   const uint4 x = reinterpret_cast<const uint4*>(row_at(a, val, b, s, h))[l];
   if (a.new_len && s >= a.new_len[b]) return;
   const int64_t pos = (int64_t)a.start_pos[b] + s;
+  if (a.kv_len && pos >= a.kv_len[b]) return;
   const int pg = page_of(a.table, a.max_pages, a.num_pages, b, pos, a.status);
   if (pg < 0) return;
   put(a.cache + ((int64_t)pg * a.Hkv + h) * BLOB, val, l, (int)(pos & (PAGE - 1)), quantise<4>(x, x));
@@ -166,7 +167,8 @@ __global__ void __launch_bounds__(256) kv4_append_tokens_kernel(const AppendArgs
   const int64_t start = a.start_pos[b];
   const int n = a.new_len ? min(a.new_len[b], a.S) : a.S;
   const int64_t p0 = ((start >> lt) + blockIdx.x) << lt;  // first position of this CTA
-  const int64_t from = max(p0, start), to = min(p0 + (1 << lt), start + n);
+  const int64_t from = max(p0, start), end = a.kv_len ? min(start + n, (int64_t)a.kv_len[b]) : start + n;
+  const int64_t to = min(p0 + (1 << lt), end);
   if (from >= to) return;
   const int rows = (int)(to - from) * a.Hkv;
   // a lane's rows are 16 apart: token and head step along without dividing
@@ -406,7 +408,7 @@ extern "C" int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, int64_t 
                                   int64_t k_token, int64_t k_head, int64_t v_batch, int64_t v_token,
                                   int64_t v_head, uint8_t* cache, int num_pages, int Hkv,
                                   const int* block_table, int max_pages, const int* start_pos,
-                                  const int* new_len, int B, int S, void* stream) {
+                                  const int* new_len, const int* kv_len, int B, int S, void* stream) {
   MB_REQUIRE(B >= 0 && S >= 0 && Hkv > 0 && num_pages >= 0 && max_pages >= 0,
              "kv4 append: bad sizes");
   if (B == 0 || S == 0) return MB_OK;
@@ -419,7 +421,7 @@ extern "C" int mb_kv4_append_bf16(const uint16_t* k, const uint16_t* v, int64_t 
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "kv4 append: no status word");
   const AppendArgs a = {k,     v,           k_batch,   k_token, k_head,    v_batch,   v_token, v_head, cache,
-                        block_table, start_pos, new_len, num_pages, max_pages, Hkv,     S,      status};
+                        block_table, start_pos, new_len, kv_len, num_pages, max_pages, Hkv,     S,      status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int lt = log_tokens(S, Hkv);
   if (lt >= 0 && B <= 65535) {

@@ -110,7 +110,7 @@ __device__ void list_free(const int* refs, int from, int to, int rank, int want,
 
 // ---------------------------------------------------------------------------
 __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
-    kv_extend_kernel(const Meta m, const int* __restrict__ add, int* __restrict__ start) {
+    kv_extend_kernel(const Meta m, const int* add, int* __restrict__ start) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int lane = threadIdx.x & 31, me = warp_id();
@@ -160,11 +160,11 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
   }
   cluster_sync();
   for (int b = me; b < m.B; b += WARPS) {  // one warp a row
-    const int l = m.len[b];
-    __syncwarp();  // every lane has read the length before it changes
+    const int l = m.len[b], n = add[b];
+    __syncwarp();  // every lane has read the lengths before they change (add may be len)
     if (lane == 0) start[b] = l;
     if (!go) continue;
-    const int n = add[b], old = pages_of(l), k = pages_of(l + n) - old;
+    const int old = pages_of(l), k = pages_of(l + n) - old;
     const int off = __ldcg(m.w.row + b);
     for (int i = lane; i < k; i += 32) {
       const int p = __ldcg(m.w.ids + off + i);

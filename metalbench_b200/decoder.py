@@ -77,7 +77,7 @@ class PagedKV4Cache:
     read back by the host, so steps can be captured in a CUDA graph;
     ``cache.status`` tells, when the program next looks, whether the last page
     operation was served (0), or how many pages were lacking (then it changed
-    nothing)."""
+    nothing, and the tokens that had no room are not stored)."""
 
     def __init__(self, batch: int, max_len: int, n_kv_heads: int, n_layers: int = 1,
                  num_pages: int | None = None, device=None):
@@ -109,7 +109,7 @@ class PagedKV4Cache:
     def append(self, i: int, k: torch.Tensor, v: torch.Tensor, start_pos: torch.Tensor,
                new_len: torch.Tensor | None = None) -> None:
         """Store layer i's keys and values [B, S, Hkv, 128] of the new tokens."""
-        ops.kv4_append(k, v, self.pools[i], self.block_table, start_pos, new_len)
+        ops.kv4_append(k, v, self.pools[i], self.block_table, start_pos, new_len, self.seq_len)
 
     def attend(self, i: int, q: torch.Tensor, start_pos: torch.Tensor | None = None,
                scale: float | None = None, max_kv_len: int | None = None) -> torch.Tensor:

@@ -159,18 +159,19 @@ Tokens tokens(PyObject* o, const char* name, int dev, int64_t B, int64_t H) {
 }
 
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  ENTER(6)
+  ENTER(7)
   const Cache c = cache(a[2], "kv4_append(cache)");
   const Table t = table(a[3], "kv4_append(block_table)", c.dev);
   const Tokens k = tokens(a[0], "kv4_append(k)", c.dev, t.B, c.H), v = tokens(a[1], "kv4_append(v)", c.dev, t.B, c.H);
   if (k.S != v.S) refuse(PyExc_ValueError, "kv4_append", "k and v shapes differ");
   const int* start = rows(a[4], "kv4_append(start_pos)", c.dev, t.B);
   const int* len = a[5] == Py_None ? nullptr : rows(a[5], "kv4_append(new_len)", c.dev, t.B);
+  const int* most = a[6] == Py_None ? nullptr : rows(a[6], "kv4_append(kv_len)", c.dev, t.B);
   On on(c.dev);
   void* s = on.stream();
   return PyLong_FromLong(without_gil([&] {
     return mb_kv4_append_bf16(k.p, v.p, k.sb, k.ss, k.sh, v.sb, v.ss, v.sh, c.p, (int)c.P, (int)c.H, t.p, (int)t.M,
-                              start, len, (int)t.B, (int)k.S, s);
+                              start, len, most, (int)t.B, (int)k.S, s);
   }));
   LEAVE
 }
@@ -279,6 +280,7 @@ struct Pools {
 };
 Pools pools(PyObject* o, const char* name, const Pages& p) {
   Pools r;
+  if (THPVariable_Check(o)) refuse(PyExc_TypeError, name, "pools: expected a list of page tensors, got a tensor");
   PyObject* seq = PySequence_Fast(o, "pools: expected a list of page tensors");
   if (!seq) throw Refused();
   struct Drop {

@@ -44,14 +44,17 @@ def kv4_cache(num_pages: int, n_kv_heads: int, device=None) -> torch.Tensor:
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
-               start_pos: torch.Tensor, new_len: torch.Tensor | None = None) -> None:
+               start_pos: torch.Tensor, new_len: torch.Tensor | None = None,
+               kv_len: torch.Tensor | None = None) -> None:
     """Store the (already rotated) keys and values of S new tokens a sequence.
 
     k, v: bf16 [B, S, n_kv_heads, 128], the last axis contiguous (views into a
     fused projection's rows are fine); token s < new_len[b] (default: all S)
-    goes to position start_pos[b] + s of sequence b. Other slots of the cache
-    stay as they are."""
-    rc = (_ext or _kv4()).append(k, v, cache, block_table, start_pos, new_len)
+    goes to position start_pos[b] + s of sequence b, unless that is kv_len[b] or
+    past it: with the lengths that kv_pages_extend keeps there, nothing is stored
+    for tokens that it found no pages for. Other slots of the cache stay as they
+    are."""
+    rc = (_ext or _kv4()).append(k, v, cache, block_table, start_pos, new_len, kv_len)
     if rc:
         _lib.check("mb_kv4_append_bf16", rc)
 

@@ -65,7 +65,7 @@ def test_attention_arguments(lib, change, word):
 ])
 def test_append_arguments(lib, change, word):
     a = dict(k=FAKE, v=FAKE, k0=1024, k1=128, k2=128, v0=1024, v1=128, v2=128, cache=FAKE, num_pages=4, Hkv=1, table=FAKE,
-             max_pages=4, start=FAKE, new=None, B=2, S=8)
+             max_pages=4, start=FAKE, new=None, most=None, B=2, S=8)
     a.update(change)
     rc = lib.mb_kv4_append_bf16(*a.values(), None)
     assert rc == -1 and word in lib.mb_last_error().decode()
@@ -86,11 +86,16 @@ def test_page_arguments(lib, change, word):
 
 
 def test_empty_calls_launch_nothing(lib):
-    assert lib.mb_kv4_append_bf16(None, None, 0, 0, 0, 0, 0, 0, None, 1, 1, None, 1, None, None, 0, 4, None) == 0
+    assert lib.mb_kv4_append_bf16(None, None, 0, 0, 0, 0, 0, 0, None, 1, 1, None, 1, None, None, None, 0, 4, None) == 0
     assert lib.mb_kv4_gather_f32(None, 1, 1, None, 1, None, None, 2, 0, None, None, None) == 0
     assert lib.mb_attention_kv4_bf16(None, 0, None, 1, None, 1, None, 64, None, 0, 1, 8, 8, 128, 1.0, None, 0, None, 0, None) == 0
     assert lib.mb_attention_kv4_workspace_bytes(0, 1, 8, 8, 4) == 0
     assert lib.mb_kv4_page_bytes(8) == 8 * R.BLOB
+
+
+def test_a_wide_table_does_not_ask_for_the_memory_of_expanded_pages(lib):
+    most = max(lib.mb_attention_kv4_workspace_bytes(1, 512, 64, 8, n) for n in (1 << 17, 1 << 20, 1 << 24, 1 << 29))
+    assert 0 < most <= 6 << 30
 
 
 def test_plain_quantiser_is_within_half_a_step():

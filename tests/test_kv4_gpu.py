@@ -592,6 +592,48 @@ def test_page_calls_that_cannot_be_served_change_nothing(ops):
         dev[name][at], getattr(ref, name)[at] = good, int(good)
 
 
+@pytest.mark.parametrize("S", [1, 7, 64, 130])
+def test_tokens_without_room_are_not_stored(ops, S):
+    """Row 1 was long once; its table still names pages that are row 0's now."""
+    H, old = 2, 192
+    table, lens, refs = i32([[-1] * 8] * 2), i32([0, 0]), i32([0] * 6)
+    cache = ops.kv4_cache(6, H)
+    ops.kv_pages_extend(table, lens, refs, i32([0, old]))
+    ops.kv_pages_fork([cache], table, lens, refs, i32([0, -1]))
+    ops.kv_pages_extend(table, lens, refs, i32([6 * 64, 0]))
+    assert table[0, :6].tolist() == [0, 1, 2, 3, 4, 5] and table[1, :3].tolist() == [0, 1, 2]
+    k = torch.randn(2, S, H, 128, device="cuda").to(torch.bfloat16)
+    start, lack = ops.kv_pages_extend(table, lens, refs, i32([0, S]))
+    assert int(lack) == -(-S // 64) and start.tolist() == [384, 0] and lens.tolist() == [384, 0]
+    ops.kv4_append(k, k, cache, table, start, new_len=i32([0, S]), kv_len=lens)
+    assert not cache.any() and status() == 0
+    # and up to the length, not past it
+    ops.kv4_append(k, k, cache, table, i32([0, 0]), new_len=i32([S, 0]), kv_len=i32([S // 2, 0]))
+    want = ops.kv4_cache(6, H)
+    ops.kv4_append(k, k, want, table, i32([0, 0]), new_len=i32([S // 2, 0]))
+    assert torch.equal(cache, want) and status() == 0
+
+
+def test_lengths_that_double(ops):
+    """The lengths themselves as the number of new tokens."""
+    table, lens, refs = i32([[-1] * 40] * 40), i32([5 * i for i in range(40)]), i32([0] * 400)
+    for b in range(40):
+        for c in range(-(-5 * b // 64)):
+            p = int((refs > 0).sum())
+            table[b, c], refs[p] = p, 1
+    start, lack = ops.kv_pages_extend(table, lens, refs, lens)
+    assert int(lack) == 0 and start.tolist() == [5 * i for i in range(40)] and lens.tolist() == [10 * i for i in range(40)]
+    assert int((refs == 1).sum()) == sum(-(-10 * i // 64) for i in range(40))
+
+
+def test_a_tensor_is_no_list_of_pools(ops):
+    pool = torch.zeros(4, 4, 8704, dtype=torch.uint8, device="cuda")
+    with pytest.raises(TypeError):
+        ops.kv_pages_fork(pool, i32([[0] * 4]), i32([0]), i32([0] * 4), i32([0]))
+    with pytest.raises(TypeError):
+        ops.kv_pages_compact(pool, i32([[0] * 4]), i32([0]), i32([0] * 4))
+
+
 def test_empty_batches_and_pools(ops):
     e = torch.empty(0, dtype=torch.int32, device="cuda")
     t = torch.empty(0, 3, dtype=torch.int32, device="cuda")
