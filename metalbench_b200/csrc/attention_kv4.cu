@@ -1119,56 +1119,43 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
 // page once a row tile of 16, expand the cache once to fp16 pages in the
 // workspace and run the tcgen05 prefill attention over those (the keys cut in
 // parts when the row tiles are too few for the SMs), where the times (us) that
-// expand_plan expects say so: 0.29 a page and row tile on one SM; or 1.5 a
+// expand_plan expects say so: 0.29 a page and row tile on one SM; or 1.2 a
 // 128-key tile and 4 a wave of CTAs, and the bytes at 5.5 TB/s. Measured in us,
 // expanded / unpacked:
-//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 87 / 81,
-//     96 rows 89 / 114, 128 rows 88 / 146, 512 rows 218 / 534;
-//   1 of 32768, 8, 4:  64 rows 145 / 141, 128 rows 150 / 267;
-//   16 of 2048, 8, 4:  64 rows 167 / 162, 128 rows 164 / 298;
-//   1 of 1024, 8, 1:  256 rows 20 / 13;  8 of 512, 8, 4:  64 rows 31 / 57.
+//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 69 / 84,
+//     128 rows 74 / 151, 512 rows 172 / 551;
+//   1 of 32768, 8, 4:  64 rows 134 / 146, 128 rows 128 / 277;
+//   16 of 2048, 8, 4:  64 rows 135 / 167, 128 rows 145 / 310;
+//   1 of 1024, 8, 1:  256 rows 20 / 13;  8 of 512, 8, 4:  64 rows 27 / 58;
+//   1 of 8192, 1, 8:  64 rows 27 / 17.
 constexpr int TC_ROWS = 64;
 constexpr size_t MOST_EXPANDED = size_t(6) << 30;  // workspace: a sequence of 1.3 million tokens of 8 heads
 
 struct Expand {
   int seqs;  // sequences expanded at a time: up to 512 MB of pages, at least one
   int splits;  // parts that a row tile's keys are cut into, to fill the SMs
-  size_t pages, rows, exps, part_at, bytes;
-  mb::Kv4Expanded at(void* workspace, int n_pages) const {
-    mb::Kv4Expanded o;
-    o.k = static_cast<uint16_t*>(workspace);
-    o.v = o.k + pages / 2;
-    o.q = o.v + pages / 2;
-    o.page_exp = reinterpret_cast<int2*>(o.q + rows * DH);
-    o.row_exp = reinterpret_cast<int*>(o.page_exp + exps);
-    o.table = o.row_exp + rows;
-    o.len = o.table + (size_t)seqs * n_pages;
-    o.start = o.len + seqs;
-    return o;
-  }
+  size_t half, part_at, bytes;  // keys or values; where the partials start; all
 };
 
 bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
-  const int64_t per_seq = (int64_t)n_pages * Hkv * PAGE * DH * 2;  // keys or values, bytes
-  if (S < TC_ROWS || Hq > 65535 || Hkv > 65535 || (int64_t)n_pages * Hkv * PAGE >= (1ll << 31)) return false;
+  if (S < TC_ROWS || Hq > 65535 || Hkv > 65535 || (int64_t)(n_pages + 1) * Hkv * PAGE >= (1ll << 31)) return false;
+  const int even = (n_pages + 1) / 2 * 2;
+  const int64_t per_seq = (int64_t)even * Hkv * PAGE * DH * 2;
   int64_t n = (256ll << 20) / per_seq;
   n = n < 1 ? 1 : n > 65535 ? 65535 : n;
   e->seqs = (int)(n < B ? n : B);
-  e->pages = (size_t)per_seq * e->seqs;
-  e->rows = (size_t)e->seqs * S * Hq;
-  e->exps = (size_t)e->seqs * n_pages * Hkv;
+  e->half = (size_t)per_seq * e->seqs;
   e->splits = mb::attention_split_plan(e->seqs, S, Hq, (int64_t)n_pages * PAGE);
-  e->part_at = (2 * e->pages + e->rows * (DH * 2 + 4) + e->exps * 8 + (size_t)e->seqs * (n_pages + 2) * sizeof(int) +
-                15) / 16 * 16;
-  e->bytes = e->part_at + (e->splits > 1 ? e->rows * e->splits * (DH + 2) * sizeof(float) : 0);
+  e->part_at = 2 * e->half + ((size_t)e->seqs * even * Hkv * sizeof(int2) + 15) / 16 * 16;
+  e->bytes = e->part_at + (e->splits > 1 ? (size_t)e->seqs * S * Hq * e->splits * (DH + 2) * sizeof(float) : 0);
   if (e->bytes > MOST_EXPANDED) return false;
   const double sms = mb::num_sms(), pages = (double)B * Hkv * n_pages;
   const int rt = plan_launch(B, S, Hq, Hkv, n_pages).rt, sp = e->splits;
   const double unpack = 9 + (pages + 8.0 * B * Hkv) * rt * 0.29 / sms;  // a unit's start and end: 8 pages
   const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128) * sp;
   const double tiles = ((n_pages + 1) / 2 + sp - 1) / sp;
-  const double expand = 3 + calls * (4 + std::ceil(ctas / sms) * (4 + tiles * 1.5) + (sp > 1 ? 7 : 0)) +
-                        (pages * (BLOB + 2 * PAGE * DH * 2) + (double)B * S * Hq * DH * 4) / 5.5e6;
+  const double expand = 3 + calls * (4 + std::ceil(ctas / sms) * (4 + tiles * 1.2) + (sp > 1 ? 7 : 0)) +
+                        pages * (BLOB + 2 * PAGE * DH * 2) / 5.5e6;
   return expand < unpack;
 }
 
@@ -1209,18 +1196,31 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
   if (expand_plan(B, S, Hq, Hkv, pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
       mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo)) {
     MB_REQUIRE(workspace_bytes >= e.bytes, "attention kv4: workspace of %zu bytes required", e.bytes);
-    const mb::Kv4Expanded o = e.at(workspace, pages);
-    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + e.part_at);
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    mb::Kv4Rows r;
+    r.x.k = reinterpret_cast<uint16_t*>(w);
+    r.x.v = reinterpret_cast<uint16_t*>(w + e.half);
+    r.x.page_exp = reinterpret_cast<int2*>(w + 2 * e.half);
+    r.x.pages = (pages + 1) / 2 * 2;
+    r.part = e.splits > 1 ? reinterpret_cast<float*>(w + e.part_at) : nullptr;
+    r.splits = e.splits;
+    r.ldq = ldq;
+    r.ldo = ldo;
+    r.max_len = max_kv_len;
+    r.S = S;
+    r.Hq = Hq;
+    r.Hkv = Hkv;
+    r.scale = scale;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int b = 0; b < B; b += e.seqs) {
-      const int n = B - b < e.seqs ? B - b : e.seqs;
-      int rc = mb::kv4_expand(cache, num_pages, Hkv, block_table + (int64_t)b * max_pages, max_pages, max_kv_len, kv_len + b,
-                              start_pos ? start_pos + b : nullptr, n, q + (int64_t)b * S * ldq, ldq, S, Hq, o,
-                              status, s);
-      if (!rc)
-        rc = mb::attention_prefill_tc_f16(o.q, o.row_exp, o.k, o.v, o.page_exp, o.table, pages, o.start, o.len, n,
-                                          S, Hq, Hkv, start_pos != nullptr, out + (int64_t)b * S * ldo, (int)ldo,
-                                          s, scale, e.splits, pages * PAGE, part, part + e.rows * e.splits * DH);
+      r.B = B - b < e.seqs ? B - b : e.seqs;
+      r.q = q + (int64_t)b * S * ldq;
+      r.out = out + (int64_t)b * S * ldo;
+      r.kv_len = kv_len + b;
+      r.start_pos = start_pos ? start_pos + b : nullptr;
+      int rc = mb::kv4_expand(cache, num_pages, Hkv, block_table + (int64_t)b * max_pages, max_pages, max_kv_len,
+                              r.kv_len, r.B, r.x, status, s);
+      if (!rc) rc = mb::attention_rows_kv4(r, s);
       if (rc) return rc;
     }
     return MB_OK;

@@ -30,9 +30,6 @@
 //              (16 per clock per SM) equals the tensor work of S and P V at
 //              M = N = 128; two threads per row hide the per-thread latency.
 // TMEM: S0 (128 cols) | S1 (128) | O (128) of a 512-column allocation.
-// A second form (F16) reads fp16 operands that come with power-of-two
-// factors: it serves the 4-bit cache, whose expanded values fp16 holds to
-// 2^-11 and bf16 only to 2^-8 (attention_prefill_tc_f16 below).
 // Every mbarrier wait is bounded (common.cuh) and reports through the device
 // status word; the teardown drains the MMA pipe and in-flight copies.
 #include <algorithm>
@@ -69,16 +66,12 @@ struct AttnTcParams {
   float scale_log2;
   uint16_t* out;
   int ldo;
-  // split-KV (bf16: non-causal only): CTA split sp handles key tiles
+  // split-KV (non-causal only): CTA split sp handles key tiles
   // [sp*tiles_per_split, +tiles_per_split) and writes its unnormalised O,
   // running max and row sum per row to part_o / part_ml instead of out
   int splits, tiles_per_split, Hq;
   float* part_o;   // [B][Hq][S][splits][128]
   float* part_ml;  // [B][Hq][S][splits][2]
-  // F16: q rows are stored as q * 2^-row_exp, the pages' keys and values as
-  // k * 2^-x and v * 2^-y of page_exp
-  const int* row_exp;    // [B][S][Hq]
-  const int2* page_exp;  // [B][max_pages][Hkv]
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -107,19 +100,6 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-template <bool F16>
-__device__ __forceinline__ uint32_t pack_p(float a, float b) {
-  if constexpr (F16) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  return pack_bf16x2(a, b);
-}
-
-__device__ __forceinline__ float pow2i(int e) {  // 2^e, |e| <= 126
-  return __int_as_float((127 + e) << 23);
-}
-
 // K-major, 128B-swizzled operand of 128 rows x 128 elements stored as two
 // 64-element chunks CHUNK bytes apart; k-step kk covers elements 16kk..16kk+15.
 __device__ __forceinline__ uint64_t kmajor_desc(uint32_t base, int kk) {
@@ -130,11 +110,6 @@ __device__ __forceinline__ void pair_sync(int quad) {  // the two warps of a TME
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
 }
 
-// The F16 form: with scores in log2 units, a page's values v' = v 2^-y and the
-// reference R >= score + y (raised as above), p' = 2^(score + y - R + 6) is at
-// most 2^14 and o = sum p' v', l = sum p' 2^-y give the same quotient. The 6
-// keeps terms down to 2^-30 of the largest out of fp16's underflow.
-template <bool F16>
 __global__ void __launch_bounds__(64 + NSOFT, 1)
     attn_prefill_tc_kernel(const __grid_constant__ AttnTcParams p, uint32_t* status) {
   extern __shared__ uint8_t smem_raw[];
@@ -280,8 +255,8 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    constexpr uint32_t idesc_s = mbd::make_idesc(F16 ? 0u : 1u, TQ, TK, 0, 0);
-    constexpr uint32_t idesc_pv = mbd::make_idesc(F16 ? 0u : 1u, TQ, DHT, 0, 1);
+    constexpr uint32_t idesc_s = mbd::make_idesc(1u, TQ, TK, 0, 0);
+    constexpr uint32_t idesc_pv = mbd::make_idesc(1u, TQ, DHT, 0, 1);
     const uint32_t sq = mbd::smem_u32(base);
     bool ok = __all_sync(0xffffffffu,
                          mbd::mbar_wait(q_full, 0, status, MB_DEV_TIMEOUT_MMA, abort_flag));
@@ -344,31 +319,12 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
     const int c0 = half * 64;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    // F16: this thread's 64 keys of tile j are page 2 (jbase + j) + half
-    float row_scale = p.scale_log2;
-    int2 pe_next = make_int2(0, 0);
-    auto page_exp = [&](int j) {
-      const int pg = 2 * (jbase + j) + half;
-      return pg < valid_pages ? p.page_exp[((int64_t)b * p.max_pages + pg) * p.Hkv + kvh] : make_int2(0, 0);
-    };
-    if constexpr (F16) {
-      if (row < p.S) row_scale *= pow2i(p.row_exp[((int64_t)b * p.S + row) * p.Hq + h]);
-      pe_next = page_exp(0);
-    }
     // Every iteration runs both pair barriers, also after a failed (timed
     // out) wait, so the two warps of a quadrant never wait for each other in
     // vain: a failure only skips the work.
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1;
       const uint32_t ph = (j >> 1) & 1;
-      float scl = p.scale_log2, vexp = 0.f, vinv = 1.f;
-      if constexpr (F16) {
-        // clamped: 0 * inf and -inf * 0 must not meet
-        scl = fminf(fmaxf(row_scale * pow2i(pe_next.x), 1e-37f), 3e38f);
-        vexp = (float)pe_next.y;
-        vinv = pow2i(-pe_next.y);
-        if (j + 1 < n_tiles) pe_next = page_exp(j + 1);
-      }
       if (ok)
         ok = __all_sync(0xffffffffu,
                         mbd::mbar_wait(&sfull[st], ph, status, MB_DEV_TIMEOUT_EPI, abort_flag));
@@ -409,11 +365,10 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
             mx[e & 7] = fmaxf(mx[e & 7], __uint_as_float(s[c][e]));
           }
       }
-      const float mh = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                             fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-      red[half * TQ + r] = F16 ? fmaf(mh, scl, vexp) : mh;
+      red[half * TQ + r] = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                 fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
       pair_sync(quad);
-      const float mt = fmaxf(red[r], red[TQ + r]) * (F16 ? 1.f : p.scale_log2);
+      const float mt = fmaxf(red[r], red[TQ + r]) * p.scale_log2;
       pair_sync(quad);  // both read before either writes the next tile's
       float alpha = 1.f;
       bool rescale = false;
@@ -424,8 +379,7 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
         }
         m = mt;
       }
-      float mu = m == -INFINITY ? 0.f : m;
-      if constexpr (F16) mu -= vexp + 6.f;
+      const float mu = m == -INFINITY ? 0.f : m;
       // O columns that must follow the raised maximum: after P_{j-1} V_{j-1}
       if (ok && __any_sync(0xffffffffu, rescale)) {
         const int pj = j - 1;
@@ -451,6 +405,7 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
                                                     MB_DEV_TIMEOUT_EPI, abort_flag));
       if (!ok) continue;
       uint8_t* prow = base + OFF_P + st * TILE + half * CHUNK + r * 128;
+      const float scl = p.scale_log2;
       float sm[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) sm[e] = 0.f;
@@ -462,12 +417,11 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
           e8[e] = ex2(fmaf(__uint_as_float(s[u >> 1][(u & 1) * 8 + e]), scl, -mu));
           sm[e] += e8[e];
         }
-        const uint4 w = make_uint4(pack_p<F16>(e8[0], e8[1]), pack_p<F16>(e8[2], e8[3]),
-                                   pack_p<F16>(e8[4], e8[5]), pack_p<F16>(e8[6], e8[7]));
+        const uint4 w = make_uint4(pack_bf16x2(e8[0], e8[1]), pack_bf16x2(e8[2], e8[3]),
+                                   pack_bf16x2(e8[4], e8[5]), pack_bf16x2(e8[6], e8[7]));
         *reinterpret_cast<uint4*>(prow + ((u ^ (r & 7)) << 4)) = w;
       }
-      const float st_sum = ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
-      l = F16 ? fmaf(st_sum, vinv, l * alpha) : l * alpha + st_sum;
+      l = l * alpha + (((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7])));
       mbd::fence_proxy_async();
       mbd::tc_fence_before();
       mbd::mbar_arrive(&pfull[st]);
@@ -498,14 +452,13 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
                                          __uint_as_float(o[4 * e + 3]));
       }
       if (row < p.S && half == 0) {
-        p.part_ml[prow * 2] = F16 && lt != lt ? 0.f : m;
+        p.part_ml[prow * 2] = m;
         p.part_ml[prow * 2 + 1] = lt;
       }
     } else if (fin) {
       mbd::tc_fence_after();
-      const bool any = F16 ? lt != 0.f : lt > 0.f;  // F16: a NaN that a row sees stays one
-      const float inv = any ? 1.f / lt : 0.f;
-      const uint32_t keep = any ? 0xFFFFFFFFu : 0u;  // no visible key: O was never written
+      const float inv = lt > 0.f ? 1.f / lt : 0.f;
+      const uint32_t keep = lt > 0.f ? 0xFFFFFFFFu : 0u;  // no visible key: O was never written
       uint4* dst =
           reinterpret_cast<uint4*>(p.out + ((int64_t)b * p.S + row) * p.ldo + h * DHT + c0);
 #pragma unroll 1
@@ -540,7 +493,6 @@ __global__ void __launch_bounds__(64 + NSOFT, 1)
 
 // out row = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M = max_s m_s;
 // one 128-thread block per (sequence, head, query row), thread = dim
-template <bool F16>
 __global__ void __launch_bounds__(128) attn_split_combine_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_ml, int S, int Hq,
     int splits, uint16_t* __restrict__ out, int ldo) {
@@ -558,7 +510,7 @@ __global__ void __launch_bounds__(128) attn_split_combine_kernel(
     lsum += w * ml[2 * s + 1];
     acc += w * part_o[(rid * splits + s) * DHT + threadIdx.x];
   }
-  const float v = (F16 ? lsum != 0.f : lsum > 0.f) ? acc / lsum : 0.f;
+  const float v = lsum > 0.f ? acc / lsum : 0.f;
   __nv_bfloat16 hv = __float2bfloat16_rn(v);
   out[(b * S + row) * (int64_t)ldo + h * DHT + threadIdx.x] = *reinterpret_cast<uint16_t*>(&hv);
 }
@@ -583,17 +535,15 @@ bool attention_prefill_tc_ok(const uint16_t* q, int ldq, const uint16_t* k_cache
          getenv("MB_ATTN_NO_TC") == nullptr;
 }
 
-namespace {
-template <bool F16>
-int launch_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache, const uint16_t* v_cache,
-                      const int* block_table, int max_pages, const int* start_pos,
-                      const int* kv_len, int B, int S, int Hq, int Hkv, int causal, uint16_t* out,
-                      int ldo, cudaStream_t stream, int splits, int max_kv_len, float* part_o,
-                      float* part_ml, float scale, const int* row_exp, const int2* page_exp) {
-  MB_REQUIRE(splits == 1 || ((F16 || !causal) && part_o && part_ml && max_kv_len > 0),
+int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
+                         const uint16_t* v_cache, const int* block_table, int max_pages,
+                         const int* start_pos, const int* kv_len, int B, int S, int Hq, int Hkv,
+                         int causal, uint16_t* out, int ldo, cudaStream_t stream, int splits,
+                         int max_kv_len, float* part_o, float* part_ml, float scale) {
+  MB_REQUIRE(splits == 1 || (!causal && part_o && part_ml && max_kv_len > 0),
              "attention: split-KV needs a non-causal call, max_kv_len and partial buffers");
   AttnTcParams p;
-  const auto bf = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const auto bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
   int rc = make_tmap_2d(&p.qmap, q, bf, 2, (uint64_t)ldq, (uint64_t)B * S, (uint64_t)ldq * 2, 64,
                         TQ, sw);
@@ -619,46 +569,22 @@ int launch_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache, const
   p.Hq = Hq;
   p.part_o = part_o;
   p.part_ml = part_ml;
-  p.row_exp = row_exp;
-  p.page_exp = page_exp;
   p.tiles_per_split = splits == 1 ? (1 << 30)
                                   : ((max_kv_len + TK - 1) / TK + splits - 1) / splits;
   {
     const int arc =
-        mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_prefill_tc_kernel<F16>), SMEM_BYTES);
+        mb::ensure_smem_attr(reinterpret_cast<const void*>(attn_prefill_tc_kernel), SMEM_BYTES);
     if (arc) return arc;
   }
   dim3 grid((unsigned)(p.n_qt * splits), (unsigned)Hq, (unsigned)B);
-  attn_prefill_tc_kernel<F16><<<grid, 64 + NSOFT, SMEM_BYTES, stream>>>(p, device_status_ptr());
+  attn_prefill_tc_kernel<<<grid, 64 + NSOFT, SMEM_BYTES, stream>>>(p, device_status_ptr());
   MB_CUDA(cudaGetLastError());
   if (splits > 1) {
-    attn_split_combine_kernel<F16><<<(unsigned)((int64_t)B * Hq * S), 128, 0, stream>>>(
+    attn_split_combine_kernel<<<(unsigned)((int64_t)B * Hq * S), 128, 0, stream>>>(
         part_o, part_ml, S, Hq, splits, out, ldo);
     MB_CUDA(cudaGetLastError());
   }
   return MB_OK;
-}
-}  // namespace
-
-int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
-                         const uint16_t* v_cache, const int* block_table, int max_pages,
-                         const int* start_pos, const int* kv_len, int B, int S, int Hq, int Hkv,
-                         int causal, uint16_t* out, int ldo, cudaStream_t stream, int splits,
-                         int max_kv_len, float* part_o, float* part_ml, float scale) {
-  return launch_prefill_tc<false>(q, ldq, k_cache, v_cache, block_table, max_pages, start_pos, kv_len, B, S,
-                                  Hq, Hkv, causal, out, ldo, stream, splits, max_kv_len, part_o, part_ml,
-                                  scale, nullptr, nullptr);
-}
-
-int attention_prefill_tc_f16(const uint16_t* q, const int* row_exp, const uint16_t* k_cache,
-                             const uint16_t* v_cache, const int2* page_exp, const int* block_table,
-                             int max_pages, const int* start_pos, const int* kv_len, int B, int S,
-                             int Hq, int Hkv, int causal, uint16_t* out, int ldo,
-                             cudaStream_t stream, float scale, int splits, int max_kv_len,
-                             float* part_o, float* part_ml) {
-  return launch_prefill_tc<true>(q, Hq * DHT, k_cache, v_cache, block_table, max_pages, start_pos, kv_len, B,
-                                 S, Hq, Hkv, causal, out, ldo, stream, splits, max_kv_len, part_o, part_ml, scale,
-                                 row_exp, page_exp);
 }
 
 }  // namespace mb

@@ -101,29 +101,32 @@ int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
                          int causal, uint16_t* out, int ldo, cudaStream_t stream, int splits = 1,
                          int max_kv_len = 0, float* part_o = nullptr, float* part_ml = nullptr,
                          float scale = 0.08838834764831845f /* 1 / sqrt(128); > 0 */);
-// The same over fp16 operands with power-of-two factors: q [B * S][Hq * 128]
-// holds q 2^-row_exp ([B][S][Hq]), the pages hold k 2^-x and v 2^-y of page_exp
-// ([B][max_pages][Hkv]); exponents within [-112, 113]. splits as above, causal or not.
-int attention_prefill_tc_f16(const uint16_t* q, const int* row_exp, const uint16_t* k_cache,
-                             const uint16_t* v_cache, const int2* page_exp, const int* block_table,
-                             int max_pages, const int* start_pos, const int* kv_len, int B, int S,
-                             int Hq, int Hkv, int causal, uint16_t* out, int ldo,
-                             cudaStream_t stream, float scale, int splits, int max_kv_len,
-                             float* part_o, float* part_ml);
 int attention_split_plan(int64_t B, int64_t S, int64_t Hq, int64_t kv_len);
-// kv4.cu: what attention_prefill_tc_f16 reads, made from B sequences of at most
-// max_len tokens of a 4-bit cache (pages [B * ceil(max_len / 64)][Hkv][64][128],
-// zeros past a length or for a bad page, with block table, clamped lengths and
-// first positions) and their bf16 query rows.
+// kv4.cu: the pages of B sequences of at most max_len tokens of a 4-bit cache in
+// fp16: k 2^-x and v 2^-y [B][Hkv][pages][64][128] with a page's (x, y) in
+// page_exp, for an even number of pages; zeros past a length or for a bad page.
 struct Kv4Expanded {
-  uint16_t *q, *k, *v;
-  int* row_exp;
+  uint16_t *k, *v;
   int2* page_exp;
-  int *table, *len, *start;
+  int pages;
 };
 int kv4_expand(const uint8_t* cache, int num_pages, int Hkv, const int* table, int max_pages,
-               int max_len, const int* kv_len, const int* start_pos, int B, const uint16_t* q,
-               int64_t ldq, int S, int Hq, const Kv4Expanded& o, uint32_t* status, cudaStream_t s);
+               int max_len, const int* kv_len, int B, const Kv4Expanded& o, uint32_t* status, cudaStream_t s);
+// attention_kv4_tc.cu: attention of many rows over them; splits > 1: the keys of
+// a row tile in parts, with `part` of B * S * Hq * splits * 130 floats.
+struct Kv4Rows {
+  const uint16_t* q;
+  int64_t ldq;
+  Kv4Expanded x;
+  const int *kv_len, *start_pos;  // start_pos null: not causal
+  int max_len, B, S, Hq, Hkv;
+  uint16_t* out;
+  int64_t ldo;
+  float scale;  // > 0
+  int splits;
+  float* part;
+};
+int attention_rows_kv4(const Kv4Rows& a, cudaStream_t stream);
 // decoder.cu helpers shared with fused_ops.cu
 int rownorm(const uint16_t* x, int M, int D, float eps, float* rstd, cudaStream_t s);
 int pack_tiled_weight(const uint16_t* in, int64_t ld_in, int K, const int* col_idx_dev, int Nout,

@@ -289,14 +289,6 @@ int log_tokens(int S, int Hkv) {
   return S >= 32 && S >= (1 << lt) ? lt : -1;
 }
 
-// The exponent that takes a largest magnitude to [2^14, 2^15), within
-// [-112, 113] (all of bf16 but its subnormals; 0 for a maximum of 0): x 2^-e is
-// then an fp16 number to 2^-11 of itself down to 2^-29 of the largest, and to
-// 2^-40 of the largest below.
-__device__ __forceinline__ int fp16_exp(float most) {
-  return most > 0.f ? max(-112, min(113, (__float_as_int(most) >> 23) - 127 - 14)) : 0;
-}
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float max_of_16(float x) {  // over the 16 lanes of a half warp
 #pragma unroll
   for (int d = 8; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
@@ -307,50 +299,22 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Pages and query rows of B sequences for the tcgen05 prefill: one CTA a page
-// and kv head, lanes as in the storing kernel, and an equal part of the
-// sequence's query rows. fp16 and not bf16: rounded to bf16, keys alone cost
-// twice the error of the whole result (0.0038 of it against 0.0017 for the
-// output's own rounding, measured with 8192 keys whose channels differ 5-fold).
+// The pages of B sequences in fp16 for the tcgen05 kernel (attention_kv4_tc.cu):
+// one CTA a page and kv head, lanes as in the storing kernel. Tiles are two
+// pages: what a sequence's last tile lacks is written as zeros.
 __global__ void __launch_bounds__(256) kv4_expand_kernel(
     const uint8_t* __restrict__ cache, int num_pages, int Hkv, const int* __restrict__ table,
-    int max_pages, int max_len, const int* __restrict__ kv_len, const int* __restrict__ start_pos,
-    const uint16_t* __restrict__ q, int64_t ldq, int S, int Hq, mb::Kv4Expanded o, uint32_t* status) {
+    int max_pages, int max_len, const int* __restrict__ kv_len, mb::Kv4Expanded o, uint32_t* status) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
   const int page = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int L = max(0, min(kv_len[b], max_len)), pages = gridDim.x;
+  const int L = max(0, min(kv_len[b], max_len));
+  if (page / 2 * 2 * PAGE >= L) return;
   const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0 && h == 0 && page == 0) {
-    o.len[b] = L;
-    o.start[b] = start_pos ? min(start_pos[b], L) : L;
-  }
-  const int rows = S * Hq, step = (int)(gridDim.x * gridDim.y) * 16;
-  for (int base = (page * Hkv + h) * 16; base < rows; base += step) {
-    const int r = base + warp * 2 + half, s = r / Hq;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < rows)
-      x = *reinterpret_cast<const uint4*>(q + ((int64_t)b * S + s) * ldq + (int64_t)(r - s * Hq) * DH + l * 8);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    float most = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaxf(fabsf(lo_bf(w[j])), fabsf(hi_bf(w[j]))));
-    const int e = fp16_exp(max_of_16(most));
-    const float f = pow2i(-e);
-    if (r < rows) {
-      const int64_t to = (int64_t)b * rows + r;
-      if (l == 0) o.row_exp[to] = e;
-      *reinterpret_cast<uint4*>(o.q + to * DH + l * 8) =
-          make_uint4(half2_of(lo_bf(w[0]) * f, hi_bf(w[0]) * f), half2_of(lo_bf(w[1]) * f, hi_bf(w[1]) * f),
-                     half2_of(lo_bf(w[2]) * f, hi_bf(w[2]) * f), half2_of(lo_bf(w[3]) * f, hi_bf(w[3]) * f));
-    }
-  }
-  if (page * PAGE >= L) return;
-  const int64_t to = (int64_t)b * pages + page;
-  if (threadIdx.x == 0 && h == 0) o.table[to] = (int)to;
-  const int pg = page_of(table, max_pages, num_pages, b, (int64_t)page * PAGE, status);
+  const int64_t to = ((int64_t)b * Hkv + h) * o.pages + page;
+  const int pg = page * PAGE < L ? page_of(table, max_pages, num_pages, b, (int64_t)page * PAGE, status) : -1;
   const uint8_t* blob = cache + ((int64_t)max(pg, 0) * Hkv + h) * BLOB;
-  uint16_t* dst = (half ? o.v : o.k) + (to * Hkv + h) * (PAGE * DH) + l * 8;
+  uint16_t* dst = (half ? o.v : o.k) + to * (PAGE * DH) + l * 8;
   const int par_at = half ? V_PARAMS : K_PARAMS;
   const int there = pg >= 0 ? min(PAGE, L - page * PAGE) : 0;  // the rest may be anything: it is taken as zeros
   float most = 0.f;
@@ -365,7 +329,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
   const int e = fp16_exp(max_of_16(most));
   const float f = pow2i(-e);
   if (warp == 0 && l == 0) {
-    int2* to_e = o.page_exp + to * Hkv + h;
+    int2* to_e = o.page_exp + to;
     (half ? to_e->y : to_e->x) = e;
   }
 #pragma unroll
@@ -394,10 +358,9 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
 
 namespace mb {
 int kv4_expand(const uint8_t* cache, int num_pages, int Hkv, const int* table, int max_pages,
-               int max_len, const int* kv_len, const int* start_pos, int B, const uint16_t* q,
-               int64_t ldq, int S, int Hq, const Kv4Expanded& o, uint32_t* status, cudaStream_t s) {
-  MB_CUDA(launch_pdl(kv4_expand_kernel, dim3((max_len + kv4::PAGE - 1) / kv4::PAGE, Hkv, B), dim3(256), 0, s,
-                     cache, num_pages, Hkv, table, max_pages, max_len, kv_len, start_pos, q, ldq, S, Hq, o, status));
+               int max_len, const int* kv_len, int B, const Kv4Expanded& o, uint32_t* status, cudaStream_t s) {
+  MB_CUDA(launch_pdl(kv4_expand_kernel, dim3(o.pages, Hkv, B), dim3(256), 0, s, cache, num_pages, Hkv, table,
+                     max_pages, max_len, kv_len, o, status));
   return MB_OK;
 }
 }  // namespace mb

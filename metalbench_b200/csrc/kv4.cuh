@@ -32,4 +32,13 @@ __host__ __device__ constexpr int v_word(int t, int w) {
 }
 __device__ __forceinline__ float lo_bf(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// The exponent that takes a largest magnitude to [2^14, 2^15), within
+// [-112, 113] (all of bf16 but its subnormals; 0 for a maximum of 0): x 2^-e is
+// then an fp16 number to 2^-11 of itself down to 2^-29 of the largest, and to
+// 2^-40 of the largest below.
+__device__ __forceinline__ int fp16_exp(float most) {
+  return most > 0.f ? max(-112, min(113, (__float_as_int(most) >> 23) - 127 - 14)) : 0;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }  // |e| <= 126
 }  // namespace kv4

@@ -267,6 +267,21 @@ def test_few_row_tiles_over_many_keys(ops, S, Hq, B, L, causal):
     assert status() == 0
 
 
+@pytest.mark.parametrize("S, Hq, Hkv, lens, causal", [
+    (512, 8, 2, [129, 400, 700], True), (512, 8, 2, [129, 400, 700], False), (128, 8, 2, [5000], True), (1, 32, 8, [3000, 7, 900], True),
+])
+def test_the_same_call_gives_the_same_bits(ops, S, Hq, Hkv, lens, causal):
+    rng = np.random.default_rng(S)
+    lens = np.array(lens)
+    table, P = make_table(rng, lens)
+    cache = torch.from_numpy(make_cache(rng, P, Hkv)).cuda()
+    q = bf(rng.standard_normal((len(lens), S, Hq, 128)))
+    start = i32(lens - S) if causal else None
+    want = ops.attention_kv4(q, cache, i32(table), i32(lens), start_pos=start)
+    for _ in range(40):
+        assert torch.equal(ops.attention_kv4(q, cache, i32(table), i32(lens), start_pos=start), want)
+
+
 @pytest.mark.parametrize("at", ["k", "v"])
 @pytest.mark.parametrize("S, Hq, Hkv, L", [(4, 8, 1, 300), (33, 4, 2, 400), (512, 8, 2, 700), (128, 4, 1, 3000)])
 def test_only_rows_that_see_a_nan_become_one(ops, S, Hq, Hkv, L, at):
