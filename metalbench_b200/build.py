@@ -130,7 +130,7 @@ def build_ext(src: Path) -> None:
     for i in inc:
         cmd += ["-isystem", str(i)]
     cmd += [str(src), "-o", str(EXT), "-L", str(PKG), "-l:libmb200.so", "-L", str(root / "lib"),
-            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"_kv4 build failed:\n{p.stdout}\n{p.stderr}")

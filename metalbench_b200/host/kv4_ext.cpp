@@ -11,6 +11,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -113,9 +115,14 @@ struct On {
   void* stream() const { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 };
 
+// A tensor for results; what `empty` does behind its dispatcher (1 us a call).
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, int dev) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, (c10::DeviceIndex)dev)));
+  return at::Tensor(at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)dev), std::nullopt));
 }
+// Scratch memory of a call on the current stream, given back when the call has
+// been launched: the allocator hands it out again in stream order (in a capture:
+// it stays the graph's).
+c10::DataPtr scratch(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 template <typename F>
 int without_gil(F f) {
@@ -243,12 +250,12 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     ldo = query(out, "attention_kv4(out)", t.B, c.H).ld;
   }
   const size_t nb = mb_attention_kv4_workspace_bytes((int)t.B, (int)r.S, (int)r.H, (int)c.H, (int)most);
-  at::Tensor ws = empty({(int64_t)nb}, at::kByte, c.dev);
+  const c10::DataPtr ws = scratch(nb);
   void* s = on.stream();
   const int rc = without_gil([&] {
     return mb_attention_kv4_bf16(b16(q), r.ld, c.p, (int)c.P, t.p, (int)t.M, len, (int)most, start, (int)t.B, (int)r.S, (int)r.H,
                                  (int)c.H, (int)DH, (float)scale, static_cast<uint16_t*>(out.data_ptr()), ldo,
-                                 ws.data_ptr(), nb, s);
+                                 ws.get(), nb, s);
   });
   if (rc) return PyLong_FromLong(rc);
   return THPVariable_Wrap(out);
@@ -305,9 +312,9 @@ Pools pools(PyObject* o, const char* name, const Pages& p) {
   return r;
 }
 
-at::Tensor workspace(const Pages& p, size_t* nb) {
+c10::DataPtr workspace(const Pages& p, size_t* nb) {
   *nb = mb_kv_pages_workspace_bytes((int)p.t.B, (int)p.t.M, (int)p.P);
-  return empty({(int64_t)*nb}, at::kByte, p.dev);
+  return scratch(*nb);
 }
 
 PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -317,11 +324,11 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   On on(p.dev);
   at::Tensor start = empty({p.t.B}, at::kInt, p.dev), status = empty({1}, at::kInt, p.dev);
   size_t nb;
-  at::Tensor ws = workspace(p, &nb);
+  const c10::DataPtr ws = workspace(p, &nb);
   void* s = on.stream();
   const int rc = without_gil([&] {
     return mb_kv_pages_extend(p.t.p, p.len, p.refs, (int)p.t.B, (int)p.t.M, (int)p.P, add, start.data_ptr<int>(),
-                              status.data_ptr<int>(), ws.data_ptr(), nb, s);
+                              status.data_ptr<int>(), ws.get(), nb, s);
   });
   if (rc) return PyLong_FromLong(rc);
   return Py_BuildValue("(NN)", THPVariable_Wrap(start), THPVariable_Wrap(status));
@@ -336,11 +343,11 @@ PyObject* fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   On on(p.dev);
   at::Tensor status = empty({1}, at::kInt, p.dev);
   size_t nb;
-  at::Tensor ws = workspace(p, &nb);
+  const c10::DataPtr ws = workspace(p, &nb);
   void* s = on.stream();
   const int rc = without_gil([&] {
     return mb_kv_pages_fork(pl.ptr.data(), pl.bytes.data(), (int)pl.ptr.size(), p.t.p, p.len, p.refs, (int)p.t.B,
-                            (int)p.t.M, (int)p.P, parent, status.data_ptr<int>(), ws.data_ptr(), nb, s);
+                            (int)p.t.M, (int)p.P, parent, status.data_ptr<int>(), ws.get(), nb, s);
   });
   if (rc) return PyLong_FromLong(rc);
   return THPVariable_Wrap(status);
@@ -354,11 +361,11 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
   On on(p.dev);
   at::Tensor remap = empty({p.P}, at::kInt, p.dev), live = empty({1}, at::kInt, p.dev);
   size_t nb;
-  at::Tensor ws = workspace(p, &nb);
+  const c10::DataPtr ws = workspace(p, &nb);
   void* s = on.stream();
   const int rc = without_gil([&] {
     return mb_kv_pages_compact(pl.ptr.data(), pl.bytes.data(), (int)pl.ptr.size(), p.t.p, p.len, p.refs, (int)p.t.B,
-                               (int)p.t.M, (int)p.P, remap.data_ptr<int>(), live.data_ptr<int>(), ws.data_ptr(), nb, s);
+                               (int)p.t.M, (int)p.P, remap.data_ptr<int>(), live.data_ptr<int>(), ws.get(), nb, s);
   });
   if (rc) return PyLong_FromLong(rc);
   return Py_BuildValue("(NN)", THPVariable_Wrap(remap), THPVariable_Wrap(live));
