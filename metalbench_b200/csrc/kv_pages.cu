@@ -12,18 +12,22 @@
 // order, so that results do not depend on timing. A call that cannot be served
 // (too few free pages, an entry or a parent out of range) changes nothing.
 //
-// The bookkeeping of a call is one launch of one 8-CTA cluster: its 128 warps
-// count (ballots over contiguous segments), meet at the cluster barrier, read
-// the 128 counts and place what they counted. The pages' bytes move in a
+// The bookkeeping of a call is one launch of one CTA or, for larger tables, one
+// 8-CTA cluster: its 32 or 128 warps count (ballots over contiguous segments),
+// meet at a barrier, read all counts and place what they counted. The pages' bytes move in a
 // second launch over all SMs, bound by HBM.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace {
 
 constexpr int PAGE = 64;
-constexpr int CTAS = 8, THREADS = 512;
-constexpr int WARPS = CTAS * THREADS / 32;  // 128
+// CTAs of the bookkeeping's cluster and threads of each
+template <int CTAS> constexpr int THREADS = CTAS == 1 ? 1024 : 512;
+template <int CTAS> constexpr int WARPS = CTAS * THREADS<CTAS> / 32;
+constexpr int MOST_WARPS = WARPS<8>;  // 128
 constexpr int MAX_POOLS = 64;
 
 struct Pools {
@@ -35,7 +39,7 @@ struct Pools {
 
 // Caller's workspace, as the kernels see it.
 struct Work {
-  int* cnt;     // [4][WARPS]
+  int* cnt;     // [4][warps]
   int* head;    // [1] moves to make
   int2* moves;  // [max moves] from, to
   int* ids;     // free pages found / holes
@@ -54,25 +58,30 @@ struct Meta {
   Work w;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+template <int CTAS>
+__device__ __forceinline__ void sync_all() {
+  if (CTAS == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ int warp_id() { return (blockIdx.x * THREADS + threadIdx.x) >> 5; }
+template <int CTAS>
+__device__ __forceinline__ int warp_id() { return (blockIdx.x * THREADS<CTAS> + threadIdx.x) >> 5; }
 
 // This warp's contiguous part of n things: a multiple of 32.
+template <int CTAS>
 __device__ __forceinline__ void segment(int n, int& from, int& to) {
-  const int size = ((n + WARPS - 1) / WARPS + 31) / 32 * 32;
-  const int64_t f = (int64_t)warp_id() * size;
+  const int size = ((n + WARPS<CTAS> - 1) / WARPS<CTAS> + 31) / 32 * 32;
+  const int64_t f = (int64_t)warp_id<CTAS>() * size;
   from = (int)(f < n ? f : n);
   to = (int)(f + size < n ? f + size : n);
 }
 
 // Sum of one row of counts over the warps before this one, and over all.
+template <int CTAS>
 __device__ __forceinline__ int2 before_and_all(const int* cnt) {
-  const int lane = threadIdx.x & 31, me = warp_id();
+  const int lane = threadIdx.x & 31, me = warp_id<CTAS>();
   int b = 0, a = 0;
 #pragma unroll
-  for (int i = 0; i < WARPS / 32; ++i) {
+  for (int i = 0; i < WARPS<CTAS> / 32; ++i) {
     const int v = __ldcg(cnt + i * 32 + lane);
     a += v;
     if (i * 32 + lane < me) b += v;
@@ -109,14 +118,15 @@ __device__ void list_free(const int* refs, int from, int to, int rank, int want,
 }
 
 // ---------------------------------------------------------------------------
-__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
+template <int CTAS>
+__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS<CTAS>)
     kv_extend_kernel(const Meta m, const int* add, int* __restrict__ start) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
-  const int lane = threadIdx.x & 31, me = warp_id();
+  const int lane = threadIdx.x & 31, me = warp_id<CTAS>();
   int r0, r1, p0, p1;
-  segment(m.B, r0, r1);
-  segment(m.num_pages, p0, p1);
+  segment<CTAS>(m.B, r0, r1);
+  segment<CTAS>(m.num_pages, p0, p1);
   const int most = m.max_pages * PAGE;
   int need = 0, bad = 0;
   for (int i = r0; i < r1; i += 32) {
@@ -132,12 +142,12 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
   const int nfree = count_pages<true>(m.refs, p0, p1);
   if (lane == 0) {
     m.w.cnt[me] = need;
-    m.w.cnt[WARPS + me] = nfree;
-    m.w.cnt[2 * WARPS + me] = bad;
+    m.w.cnt[WARPS<CTAS> + me] = nfree;
+    m.w.cnt[2 * WARPS<CTAS> + me] = bad;
   }
-  cluster_sync();
-  const int2 nd = before_and_all(m.w.cnt), fr = before_and_all(m.w.cnt + WARPS);
-  const bool any_bad = before_and_all(m.w.cnt + 2 * WARPS).y != 0;
+  sync_all<CTAS>();
+  const int2 nd = before_and_all<CTAS>(m.w.cnt), fr = before_and_all<CTAS>(m.w.cnt + WARPS<CTAS>);
+  const bool any_bad = before_and_all<CTAS>(m.w.cnt + 2 * WARPS<CTAS>).y != 0;
   const int lack = nd.y > fr.y ? nd.y - fr.y : 0;
   const bool go = !any_bad && !lack;
   if (me == 0 && lane == 0) *m.status = any_bad ? -1 : lack;
@@ -158,8 +168,8 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
       run += __shfl_sync(0xffffffffu, inc, 31);
     }
   }
-  cluster_sync();
-  for (int b = me; b < m.B; b += WARPS) {  // one warp a row
+  sync_all<CTAS>();
+  for (int b = me; b < m.B; b += WARPS<CTAS>) {  // one warp a row
     const int l = m.len[b], n = add[b];
     __syncwarp();  // every lane has read the lengths before they change (add may be len)
     if (lane == 0) start[b] = l;
@@ -176,14 +186,15 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
 }
 
 // ---------------------------------------------------------------------------
-__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
+template <int CTAS>
+__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS<CTAS>)
     kv_fork_kernel(const Meta m, const int* __restrict__ parent) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
-  const int lane = threadIdx.x & 31, me = warp_id();
+  const int lane = threadIdx.x & 31, me = warp_id<CTAS>();
   int r0, r1, p0, p1;
-  segment(m.B, r0, r1);
-  segment(m.num_pages, p0, p1);
+  segment<CTAS>(m.B, r0, r1);
+  segment<CTAS>(m.num_pages, p0, p1);
   const int most = m.max_pages * PAGE;
   auto bad_len = [&](int l) { return l < 0 || l > most; };
   // ---- count: tail pages to copy, free pages; stage the parents' rows ----
@@ -205,7 +216,7 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
     tails += __popc(__ballot_sync(0xffffffffu, tail));
   }
   const int nfree = count_pages<true>(m.refs, p0, p1);
-  for (int b = me; b < m.B; b += WARPS) {
+  for (int b = me; b < m.B; b += WARPS<CTAS>) {
     const int p = parent[b];
     if (p == b || p < -1 || p >= m.B) continue;
     const int old = pages_of(m.len[b]), now = p < 0 ? 0 : pages_of(m.len[p]);
@@ -221,12 +232,12 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
     m.w.cnt[me] = tails;
-    m.w.cnt[WARPS + me] = nfree;
-    m.w.cnt[2 * WARPS + me] = bad;
+    m.w.cnt[WARPS<CTAS> + me] = nfree;
+    m.w.cnt[2 * WARPS<CTAS> + me] = bad;
   }
-  cluster_sync();
-  const int2 tl = before_and_all(m.w.cnt), fr = before_and_all(m.w.cnt + WARPS);
-  const bool any_bad = before_and_all(m.w.cnt + 2 * WARPS).y != 0;
+  sync_all<CTAS>();
+  const int2 tl = before_and_all<CTAS>(m.w.cnt), fr = before_and_all<CTAS>(m.w.cnt + WARPS<CTAS>);
+  const bool any_bad = before_and_all<CTAS>(m.w.cnt + 2 * WARPS<CTAS>).y != 0;
   const int lack = tl.y > fr.y ? tl.y - fr.y : 0;
   const bool go = !any_bad && !lack;
   if (me == 0 && lane == 0) {
@@ -244,10 +255,10 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
       rank += __popc(mask);
     }
   }
-  cluster_sync();
+  sync_all<CTAS>();
   if (!go) return;
   // ---- place: uses, rows, lengths, and the list of pages to copy ----
-  for (int b = me; b < m.B; b += WARPS) {
+  for (int b = me; b < m.B; b += WARPS<CTAS>) {
     if (parent[b] == b) continue;
     const int l = __ldcg(m.w.row2 + b), tail = __ldcg(m.w.row + b);
     const int old = pages_of(m.len[b]), now = pages_of(l);
@@ -271,16 +282,17 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
 }
 
 // ---------------------------------------------------------------------------
-__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
+template <int CTAS>
+__global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS<CTAS>)
     kv_compact_kernel(const Meta m, int* __restrict__ remap) {
   mbd::pdl_trigger();
   mbd::pdl_wait();
-  const int lane = threadIdx.x & 31, me = warp_id();
+  const int lane = threadIdx.x & 31, me = warp_id<CTAS>();
   int p0, p1;
-  segment(m.num_pages, p0, p1);
+  segment<CTAS>(m.num_pages, p0, p1);
   const int live_here = count_pages<false>(m.refs, p0, p1);
   int bad = 0;
-  for (int b = me; b < m.B; b += WARPS) {
+  for (int b = me; b < m.B; b += WARPS<CTAS>) {
     const int l = m.len[b];
     if (l < 0 || l > m.max_pages * PAGE) {
       bad = 1;
@@ -294,11 +306,11 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
     m.w.cnt[me] = live_here;
-    m.w.cnt[WARPS + me] = bad;
+    m.w.cnt[WARPS<CTAS> + me] = bad;
   }
-  cluster_sync();
-  const int2 lv = before_and_all(m.w.cnt);
-  const bool go = before_and_all(m.w.cnt + WARPS).y == 0;
+  sync_all<CTAS>();
+  const int2 lv = before_and_all<CTAS>(m.w.cnt);
+  const bool go = before_and_all<CTAS>(m.w.cnt + WARPS<CTAS>).y == 0;
   const int live = lv.y;
   if (me == 0 && lane == 0) *m.status = go ? live : -1;
   // free pages below `live` are holes, pages in use from `live` on are moved
@@ -319,21 +331,21 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS)
     below += __popc(__ballot_sync(0xffffffffu, use && p < live));
     rank += __popc(mask);
   }
-  if (lane == 0) m.w.cnt[2 * WARPS + me] = below;
-  cluster_sync();
-  const int n = live - before_and_all(m.w.cnt + 2 * WARPS).y;
+  if (lane == 0) m.w.cnt[2 * WARPS<CTAS> + me] = below;
+  sync_all<CTAS>();
+  const int n = live - before_and_all<CTAS>(m.w.cnt + 2 * WARPS<CTAS>).y;
   if (me == 0 && lane == 0) *m.w.head = go ? n : 0;
   if (go)
-    for (int i = me * 32 + lane; i < n; i += WARPS * 32) {
+    for (int i = me * 32 + lane; i < n; i += WARPS<CTAS> * 32) {
       const int from = __ldcg(m.w.ids2 + n - 1 - i), to = __ldcg(m.w.ids + i);
       m.w.moves[i] = make_int2(from, to);
       remap[from] = to;
       m.refs[to] = m.refs[from];
       m.refs[from] = 0;
     }
-  cluster_sync();
+  sync_all<CTAS>();
   if (!go) return;
-  for (int b = me; b < m.B; b += WARPS)
+  for (int b = me; b < m.B; b += WARPS<CTAS>)
     for (int c = lane; c < pages_of(m.len[b]); c += 32) {
       int* e = m.table + (int64_t)b * m.max_pages + c;
       *e = __ldcg(remap + *e);
@@ -423,7 +435,7 @@ size_t work_layout(int B, int max_pages, int num_pages, bool stage, Work* w, uin
     at += align16(bytes);
     return r;
   };
-  int* cnt = reinterpret_cast<int*>(take(4 * WARPS * sizeof(int)));
+  int* cnt = reinterpret_cast<int*>(take(4 * MOST_WARPS * sizeof(int)));
   int* head = reinterpret_cast<int*>(take(sizeof(int)));
   int2* moves = reinterpret_cast<int2*>(take((size_t)num_pages * sizeof(int2)));
   int* ids = reinterpret_cast<int*>(take((size_t)num_pages * sizeof(int)));
@@ -485,6 +497,20 @@ int check_pools(const char* what, void* const* pools, const int64_t* bytes, int 
 
 }  // namespace
 
+namespace {
+// One CTA does the bookkeeping of a small table and pool sooner: a block's
+// barrier is cheaper than a cluster's. Measured in us, 1 / 8 CTAs, at pages,
+// rows x columns: extend 2.4 / 3.8 (256, 8 x 32), 3.9 / 4.1 (8192, 128 x 64), 5.7 /
+// 4.6 (32768, 64 x 512); fork 3.8 / 5.2, 8.7 / 7.1, 17.1 / 16.3, and 7.1 / 8.1 (8192,
+// 64 x 128); compact 3.1 / 4.9, 12.2 / 7.0, 36 / 15, and 6.3 / 6.9 (4096, 32 x 128),
+// 7.3 / 6.5 (4096, 64 x 64). A row costs about as much as 64 entries.
+template <typename F>
+int launch_book(const Meta& m, int most_pages, int64_t most_work, F launch) {
+  const bool small = m.num_pages <= most_pages && (int64_t)m.B * (m.max_pages + 64) <= most_work;
+  return small ? launch(std::integral_constant<int, 1>()) : launch(std::integral_constant<int, 8>());
+}
+}  // namespace
+
 extern "C" size_t mb_kv_pages_workspace_bytes(int B, int max_pages, int num_pages) {
   if (B < 0 || max_pages <= 0 || num_pages < 0) return 0;
   return work_layout(B, max_pages, num_pages, true, nullptr, nullptr);
@@ -499,9 +525,11 @@ extern "C" int mb_kv_pages_extend(int* block_table, int* seq_len, int* page_refs
                      status, false, workspace, workspace_bytes);
   if (rc) return rc;
   MB_REQUIRE(B == 0 || (new_len && start_pos), "kv_pages_extend: null pointer");
-  MB_CUDA(mb::launch_pdl(kv_extend_kernel, dim3(CTAS), dim3(THREADS), 0,
-                         static_cast<cudaStream_t>(stream), m, new_len, start_pos));
-  return MB_OK;
+  return launch_book(m, 8192, 16384, [&](auto c) {
+    MB_CUDA(mb::launch_pdl(kv_extend_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, static_cast<cudaStream_t>(stream), m,
+                           new_len, start_pos));
+    return MB_OK;
+  });
 }
 
 extern "C" int mb_kv_pages_fork(void* const* pools, const int64_t* page_bytes, int npools,
@@ -515,7 +543,11 @@ extern "C" int mb_kv_pages_fork(void* const* pools, const int64_t* page_bytes, i
   if (rc) return rc;
   MB_REQUIRE(B == 0 || parent, "kv_pages_fork: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  MB_CUDA(mb::launch_pdl(kv_fork_kernel, dim3(CTAS), dim3(THREADS), 0, s, m, parent));
+  rc = launch_book(m, 8192, 12288, [&](auto c) {
+    MB_CUDA(mb::launch_pdl(kv_fork_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, s, m, parent));
+    return MB_OK;
+  });
+  if (rc) return rc;
   return copy_pages("kv_pages_fork", pools, page_bytes, npools, m.w, B < num_pages ? B : num_pages, s);
 }
 
@@ -530,6 +562,10 @@ extern "C" int mb_kv_pages_compact(void* const* pools, const int64_t* page_bytes
   if (rc) return rc;
   MB_REQUIRE(num_pages == 0 || remap, "kv_pages_compact: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  MB_CUDA(mb::launch_pdl(kv_compact_kernel, dim3(CTAS), dim3(THREADS), 0, s, m, remap));
+  rc = launch_book(m, 4096, 6144, [&](auto c) {
+    MB_CUDA(mb::launch_pdl(kv_compact_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, s, m, remap));
+    return MB_OK;
+  });
+  if (rc) return rc;
   return copy_pages("kv_pages_compact", pools, page_bytes, npools, m.w, num_pages / 2, s);
 }
