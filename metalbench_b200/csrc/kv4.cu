@@ -75,13 +75,24 @@ __device__ __noinline__ Row<W> quantise(uint4 ra, uint4 rb) {
   const float sc = __bfloat162float(sb);
   Row<W> r;
   r.par = (uint32_t)__bfloat16_as_ushort(sb) | (__float_as_uint(lo) & 0xFFFF0000u);
-  // x - m is exact in fp32 unless x is smaller than 2^-15 of the range (or
-  // zero, which the test does not tell apart): those rows go the long way.
-  // A remainder d - s q is exact too (s has 8 bits), so with q' next to d / s
-  // adding 1.5 * 2^23 rounds to the nearest whole number, ties to the even one:
-  // a d that is no tie is off one by more than half a last place of q'.
-  if (plain && tiny >= range * 0x1p-15f) {
+  // A remainder d - s q is exact (s has 8 bits), so with q' next to d / s adding
+  // 1.5 * 2^23 rounds to the nearest whole number, ties to the even one: a d that
+  // is no tie is off one by more than half a last place of q'. d = x - m is exact
+  // too unless x is smaller than 2^-15 of the range (1 row in 60 of normal
+  // numbers): there a quotient, off by 15 * 2^-24 at most, may round the wrong
+  // way next to a tie, and only then the row goes the long way.
+  bool slow = !plain;
+  if (plain) {
     const float inv = __frcp_rn(sc);
+    if (tiny < range * 0x1p-15f) {
+      float far = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) {
+        const float d = x[i] - lo, q = d * inv, y = fmaf(fmaf(-sc, q, d), inv, q);
+        far = fmaxf(far, fabsf(y - rintf(y)));
+      }
+      slow = far > 0.5f - 0x1p-16f;
+    }
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
       uint32_t sum = 0;  // of (bits of 1.5 * 2^23 + u) * 16^i: u <= 15, as s is within 2^-8 of range / 15
@@ -92,7 +103,8 @@ __device__ __noinline__ Row<W> quantise(uint4 ra, uint4 rb) {
       }
       r.code[k] = sum - 0x4B400000u * 0x11111111u;
     }
-  } else {
+  }
+  if (slow) {
     const float half = 0.5f * sc;
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) r.code[k] = 0;

@@ -128,6 +128,27 @@ def test_append_of_odd_rows(ops):
             assert np.array_equal(k[i], ref) and np.array_equal(v[S - 1 - i], ref), i
 
 
+@pytest.mark.parametrize("S", [5, 64, 200])
+def test_append_next_to_a_border(ops, S):
+    """Quotients next to halves, from numbers far smaller than the range: the
+    difference to the minimum is not a number of 32 bits. Both storing forms."""
+    rng = np.random.default_rng(S)
+    x = np.empty((1, S, 2, 128))
+    for i in range(S):
+        for h in range(2):
+            j = rng.integers(-14, 0)  # scale 2, the minimum an odd number: 0 is a border
+            x[0, i, h] = rng.uniform(2 * j + 1, 2 * j + 31, 128)
+            x[0, i, h, :2] = 2 * j + 1, 2 * j + 31
+            x[0, i, h, 2:40] = rng.choice([-1, 0, 1], 38) * 2.0 ** rng.integers(-36, -14, 38)
+            x[0, i, h] = rng.permutation(x[0, i, h]) * 2.0 ** rng.integers(-60, 60)
+    x = R.bf16_round(x)
+    cache = ops.kv4_cache(4, 2)
+    ops.kv4_append(bf(x), bf(-x), cache, i32([[3, 1, 0, 2]]), i32([9]))
+    for got, want in zip(ops.kv4_gather(cache, i32([[3, 1, 0, 2]]), i32([9]), S, i32([S + 9])), (x, -x)):
+        u, s, m = R.quantise(want)
+        assert np.array_equal(got.cpu().numpy(), (m[..., None] + s[..., None] * u).astype(np.float32))
+
+
 def test_append_skips_bad_pages_and_positions(ops):
     rng = np.random.default_rng(3)
     cache = torch.from_numpy(rng.integers(0, 256, (3, 2, R.BLOB), dtype=np.uint8)).cuda()
