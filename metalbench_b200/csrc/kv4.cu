@@ -327,16 +327,25 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
   const int pg = page * PAGE < L ? page_of(table, max_pages, num_pages, b, (int64_t)page * PAGE, status) : -1;
   const uint8_t* blob = cache + ((int64_t)max(pg, 0) * Hkv + h) * BLOB;
   uint16_t* dst = (half ? o.v : o.k) + to * (PAGE * DH) + l * 8;
-  const int par_at = half ? V_PARAMS : K_PARAMS;
   const int there = pg >= 0 ? min(PAGE, L - page * PAGE) : 0;  // the rest may be anything: it is taken as zeros
+  __shared__ uint32_t pars[2][PAGE];  // keys', values'
+  uint32_t code[PAGE / 8];            // (all loads on their way before the first is used)
+#pragma unroll
+  for (int i = 0; i < PAGE / 8; ++i) {
+    const int t = i * 8 + warp;
+    code[i] = t < there ? *reinterpret_cast<const uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4)) : 0;
+  }
+  if (threadIdx.x < 2 * PAGE) {
+    const int t = threadIdx.x % PAGE;
+    pars[threadIdx.x / PAGE][t] = t < there ? *reinterpret_cast<const uint32_t*>(blob + K_PARAMS + threadIdx.x * 4) : 0;
+  }
+  static_assert(V_PARAMS == K_PARAMS + PAGE * 4, "the values' parameters follow the keys'");
+  __syncthreads();
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < PAGE / 16; ++i) {
-    const int t = i * 16 + l;
-    if (t < there) {
-      const uint32_t par = *reinterpret_cast<const uint32_t*>(blob + par_at + t * 4);
-      if (lo_bf(par) < INFINITY) most = fmaxf(most, fmaxf(fabsf(hi_bf(par)), fabsf(fmaf(lo_bf(par), 15.f, hi_bf(par)))));
-    }
+    const uint32_t par = pars[half][i * 16 + l];
+    if (lo_bf(par) < INFINITY) most = fmaxf(most, fmaxf(fabsf(hi_bf(par)), fabsf(fmaf(lo_bf(par), 15.f, hi_bf(par)))));
   }
   const int e = fp16_exp(max_of_16(most));
   const float f = pow2i(-e);
@@ -347,20 +356,23 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
 #pragma unroll
   for (int i = 0; i < PAGE / 8; ++i) {
     const int t = i * 8 + warp;
-    uint32_t w[4] = {};
-    if (t < there) {
-      const uint32_t code = *reinterpret_cast<const uint32_t*>(blob + (half ? v_word(t, l) : t * ROW + l * 4));
-      const uint32_t kpar = *reinterpret_cast<const uint32_t*>(blob + K_PARAMS + t * 4);
-      const uint32_t vpar = *reinterpret_cast<const uint32_t*>(blob + V_PARAMS + t * 4);
-      const uint32_t par = half ? vpar : kpar;
-      // stored of what was no number or infinite: the key's scores make the rows that see it
-      // NaN, and its value is 0, since a weight of 0 times NaN would spread to all rows
-      const bool good = lo_bf(kpar) < INFINITY && lo_bf(vpar) < INFINITY;
-      const float scale = good ? lo_bf(par) * f : 0.f, least = good ? hi_bf(par) * f : half ? 0.f : NAN;
+    const uint32_t kpar = pars[0][t], vpar = pars[1][t], par = half ? vpar : kpar;
+    // stored of what was no number or infinite: the key's scores make the rows that see it
+    // NaN, and its value is 0, since a weight of 0 times NaN would spread to all rows
+    const bool good = lo_bf(kpar) < INFINITY && lo_bf(vpar) < INFINITY;
+    const float scale = good ? lo_bf(par) * f : 0.f, least = good ? hi_bf(par) * f : half ? 0.f : NAN;
+    // code n of a half word stands at bit 4 n: 2^23 + u 16^n - 2^23 is u 16^n (a conversion
+    // of every code to a float would be bound by its unit)
+    uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = half2_of(fmaf(scale, (float)((code >> (8 * j)) & 15u), least),
-                        fmaf(scale, (float)((code >> (8 * j + 4)) & 15u), least));
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t c = code[i] >> (16 * j);
+      float x[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        x[n] = fmaf(__uint_as_float((c & (15u << (4 * n))) | 0x4B000000u) - 8388608.f, scale * (1.f / (1 << (4 * n))), least);
+      w[2 * j] = half2_of(x[0], x[1]);
+      w[2 * j + 1] = half2_of(x[2], x[3]);
     }
     *reinterpret_cast<uint4*>(dst + t * DH) = make_uint4(w[0], w[1], w[2], w[3]);
   }

@@ -501,9 +501,10 @@ namespace {
 // One CTA does the bookkeeping of a small table and pool sooner: a block's
 // barrier is cheaper than a cluster's. Measured in us, 1 / 8 CTAs, at pages,
 // rows x columns: extend 2.4 / 3.8 (256, 8 x 32), 3.9 / 4.1 (8192, 128 x 64), 5.7 /
-// 4.6 (32768, 64 x 512); fork 3.8 / 5.2, 8.7 / 7.1, 17.1 / 16.3, and 7.1 / 8.1 (8192,
-// 64 x 128); compact 3.1 / 4.9, 12.2 / 7.0, 36 / 15, and 6.3 / 6.9 (4096, 32 x 128),
-// 7.3 / 6.5 (4096, 64 x 64). A row costs about as much as 64 entries.
+// 4.6 (32768, 64 x 512); fork 3.8 / 5.2, 8.7 / 7.1, 17.1 / 16.3, and 22.5 / 20.5
+// with its copies (3300, 96 x 33, 64 rows forked); compact 3.1 / 4.9, 12.2 / 7.0,
+// 36 / 15, and 6.3 / 6.9 (4096, 32 x 128), 7.3 / 6.5 (4096, 64 x 64). A row costs
+// about as much as 64 entries.
 template <typename F>
 int launch_book(const Meta& m, int most_pages, int64_t most_work, F launch) {
   const bool small = m.num_pages <= most_pages && (int64_t)m.B * (m.max_pages + 64) <= most_work;
@@ -543,7 +544,7 @@ extern "C" int mb_kv_pages_fork(void* const* pools, const int64_t* page_bytes, i
   if (rc) return rc;
   MB_REQUIRE(B == 0 || parent, "kv_pages_fork: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = launch_book(m, 8192, 12288, [&](auto c) {
+  rc = launch_book(m, 4096, 6144, [&](auto c) {
     MB_CUDA(mb::launch_pdl(kv_fork_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, s, m, parent));
     return MB_OK;
   });
