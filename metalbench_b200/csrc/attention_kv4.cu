@@ -1119,15 +1119,15 @@ int launch(const Args& a, int ctas, cudaStream_t s) {
 // page once a row tile of 16, expand the cache once to fp16 pages in the
 // workspace and run the tcgen05 prefill attention over those (the keys cut in
 // parts when the row tiles are too few for the SMs), where the times (us) that
-// expand_plan expects say so: 0.29 a page and row tile on one SM; or 1.2 a
-// 128-key tile and 4 a wave of CTAs, and the bytes at 5.5 TB/s. Measured in us,
+// expand_plan expects say so: 0.29 a page and row tile on one SM; or 1 a
+// 128-key tile and 3 a wave of CTAs, and the bytes at 5.5 TB/s. Measured in us,
 // expanded / unpacked:
-//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 69 / 84,
-//     128 rows 74 / 151, 512 rows 172 / 551;
-//   1 of 32768, 8, 4:  64 rows 134 / 146, 128 rows 128 / 277;
-//   16 of 2048, 8, 4:  64 rows 135 / 167, 128 rows 145 / 310;
-//   1 of 1024, 8, 1:  256 rows 20 / 13;  8 of 512, 8, 4:  64 rows 27 / 58;
-//   1 of 8192, 1, 8:  64 rows 27 / 17.
+//   2 sequences of 8192, 8 kv heads, 4 query heads each:  64 rows 58 / 83,
+//     128 rows 62 / 151, 512 rows 151 / 549;
+//   1 of 32768, 8, 4:  64 rows 118 / 145, 128 rows 107 / 276;
+//   16 of 2048, 8, 4:  64 rows 114 / 167, 128 rows 125 / 307;
+//   1 of 1024, 8, 1:  256 rows 18 / 13;  8 of 512, 8, 4:  64 rows 24 / 58;
+//   1 of 8192, 1, 8:  64 rows 25 / 17.
 constexpr int TC_ROWS = 64;
 constexpr size_t MOST_EXPANDED = size_t(6) << 30;  // workspace: a sequence of 1.3 million tokens of 8 heads
 
@@ -1154,7 +1154,7 @@ bool expand_plan(int B, int S, int Hq, int Hkv, int n_pages, Expand* e) {
   const double unpack = 9 + (pages + 8.0 * B * Hkv) * rt * 0.29 / sms;  // a unit's start and end: 8 pages
   const double calls = std::ceil((double)B / e->seqs), ctas = (double)e->seqs * Hq * ((S + 127) / 128) * sp;
   const double tiles = ((n_pages + 1) / 2 + sp - 1) / sp;
-  const double expand = 3 + calls * (4 + std::ceil(ctas / sms) * (4 + tiles * 1.2) + (sp > 1 ? 7 : 0)) +
+  const double expand = 3 + calls * (3 + std::ceil(ctas / sms) * (3 + tiles) + (sp > 1 ? 6 : 0)) +
                         pages * (BLOB + 2 * PAGE * DH * 2) / 5.5e6;
   return expand < unpack;
 }

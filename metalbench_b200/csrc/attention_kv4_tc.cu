@@ -21,7 +21,7 @@
 //               the port has to carry.
 //   warps 2-9   softmax, a thread a row (TMEM lane): four warps take the even
 //               tiles and four the odd ones, so that the exponentials of one
-//               (1024 cycles on the SFU) run while the other loads, masks and
+//               (900 cycles on the SFU) run while the other loads, masks and
 //               stores; both halves of one tile at once took 2460 cycles a tile,
 //               half of it with the SFU idle. First they take q, scale each row
 //               by its own power of two and store it as fp16. A row's
@@ -31,11 +31,15 @@
 // TMEM: S0 | S1 | O (128 columns each) | P0 | P1 (64 each). Shared memory: rings
 // of K and V, Q.
 //
-// Measured: 2 x 512 rows of 32 heads over 8192 keys of 8 in 172 us, 18 of them
-// the expansion, 2050 cycles a tile (218 us and 2850 with two threads a row on
-// one tile at a time and P in shared memory). The 64 KB of K and V that an SM
-// takes a tile are then 9 TB/s from L2, and a load of 32 KB takes 4000 cycles: that
-// bounds it now, before the SFU (1024 cycles) and the MMAs (1200).
+// Measured: 2 x 512 rows of 32 heads over 8192 keys of 8 in 151 us, 14 of them
+// the expansion, 1850 cycles a tile (218 us and 2850 with two threads a row on
+// one tile at a time and P in shared memory; 163 us with every exponential on the
+// SFU, 1 in 4 or 1 in 16 on the FMA pipe 164 and 155). The MMAs take 1024 cycles
+// of a tile, and the SFU 900; no unit is busy for more than 55 % of the time, loads
+// are not waited for (leaving them out changes nothing): what is left is the chain
+// S, softmax, P V of the two groups, which run in step since the one's reference
+// waits for the other's maximum. (Taking turns on the SFU: 3 % less before the
+// FMA pipe took its share. One warp for both products, or polling waits: more.)
 //
 // Few row tiles: `splits` CTAs share a row tile's keys and leave partials that
 // a second kernel joins. Every wait is bounded and reports through the device
@@ -110,6 +114,16 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x for x < 64 on the FMA pipe (x below -126: 2^-126; a NaN stays one). Cody and
+// Waite's reduction to f in [-1/2, 1/2], a polynomial of degree 4 there with the
+// smallest largest relative error (2.6e-6, fitted by Lawson's reweighting).
+__device__ __forceinline__ float ex2_fma(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
+  const float whole = x + 12582912.f;  // 1.5 * 2^23: the nearest whole number in its low bits
+  const float f = x - (whole - 12582912.f);
+  const float y = fmaf(fmaf(fmaf(fmaf(0.009570101f, f, 0.05591786f), f, 0.24024744f), f, 0.6931218f), f, 0.9999993f);
+  return y * __int_as_float((__float_as_int(whole) << 23) + 0x3F800000);
 }
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -357,7 +371,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows_kv4_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const float a = ex2(fmaf(__uint_as_float(s[4 * g + (i >> 3)][(2 * i) & 15]), scl[g], off));
-          const float c = ex2(fmaf(__uint_as_float(s[4 * g + (i >> 3)][(2 * i + 1) & 15]), scl[g], off));
+          const float y = fmaf(__uint_as_float(s[4 * g + (i >> 3)][(2 * i + 1) & 15]), scl[g], off);
+          const float c = (i & 3) == 1 ? ex2_fma(y) : ex2(y);  // 1 in 8 on the FMA pipe
           sm[(2 * i) & 3] += a;
           sm[(2 * i + 1) & 3] += c;
           w[32 * g + i] = half2_of(a, c);
@@ -400,6 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows_kv4_kernel(const __grid_
     const bool fin =
         ok && __all_sync(0xffffffffu, mbd::mbar_wait(ofinal, 0, status, MB_DEV_TIMEOUT_EPI, abort_flag));
     // both groups' sums, under the last reference, which is O's
+    if (m == -INFINITY && l == l) l = 0.f;  // no visible key: what ex2_fma makes of -inf is not 0
     // (in the quadrant's own rows of Q: every S has been made, and with no tile
     // the other quadrants may still be storing theirs)
     float2* ends = reinterpret_cast<float2*>(base + OFF_Q + quad * 4096) + lane;

@@ -244,7 +244,7 @@ def scaled_params(cache, at, exps):
 
 
 @pytest.mark.parametrize("q_exp, k_exp, v_lo, v_hi", [
-    (100, -100, 0, 1), (-100, 100, 0, 1), (0, 0, 100, 101), (0, 0, -100, -99), (0, 0, -12, 13), (30, -30, -40, 41),
+    (100, -100, 0, 1), (-100, 100, 0, 1), (0, 0, 100, 101), (0, 0, -100, -99), (0, 0, -12, 13), (0, 0, 24, 25), (0, 0, 12, 13), (30, -30, -40, 41),
 ])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("S, Hq", [(129, 4), (512, 8)])
