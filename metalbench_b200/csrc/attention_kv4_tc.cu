@@ -31,7 +31,7 @@
 // TMEM: S0 | S1 | O (128 columns each) | P0 | P1 (64 each). Shared memory: rings
 // of K and V, Q.
 //
-// Measured: 2 x 512 rows of 32 heads over 8192 keys of 8 in 151 us, 14 of them
+// Measured: 2 x 512 rows of 32 heads over 8192 keys of 8 in 151 us, 16 of them
 // the expansion, 1850 cycles a tile (218 us and 2850 with two threads a row on
 // one tile at a time and P in shared memory; 163 us with every exponential on the
 // SFU, 1 in 4 or 1 in 16 on the FMA pipe 164 and 155). The MMAs take 1024 cycles
