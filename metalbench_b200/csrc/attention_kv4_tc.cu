@@ -38,8 +38,8 @@
 // of a tile, and the SFU 900; no unit is busy for more than 55 % of the time, loads
 // are not waited for (leaving them out changes nothing): what is left is the chain
 // S, softmax, P V of the two groups, which run in step since the one's reference
-// waits for the other's maximum. (Taking turns on the SFU: 3 % less before the
-// FMA pipe took its share. One warp for both products, or polling waits: more.)
+// waits for the other's maximum. (Taking turns on the SFU: 160 us; one warp for
+// both products, or polling waits: more.)
 //
 // Few row tiles: `splits` CTAs share a row tile's keys and leave partials that
 // a second kernel joins. Every wait is bounded and reports through the device

@@ -288,6 +288,40 @@ def test_few_row_tiles_over_many_keys(ops, S, Hq, B, L, causal):
     assert status() == 0
 
 
+def test_prompts_on_two_streams_and_in_a_graph(ops):
+    """Both at once, each with its own workspace; then captured and replayed with other inputs."""
+    rng = np.random.default_rng(3)
+    sets = []
+    for S, L in ((300, 2000), (130, 3500)):
+        table, P = make_table(rng, np.array([L, L // 2]))
+        q = bf(rng.standard_normal((2, S, 8, 128)))
+        args = [q, torch.from_numpy(make_cache(rng, P, 2)).cuda(), i32(table), i32([L, L // 2]), i32([L - S, 0])]
+        sets.append((args, ops.attention_kv4(*args)))
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, (args, _) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(ops.attention_kv4(*args))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g, (_, want) in zip(got, sets))
+    graphs, outs = [], []
+    for args, _ in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.attention_kv4(*args))
+        graphs.append(g)
+    for args, _ in sets:
+        args[0].mul_(-1)
+        args[3].sub_(40)
+    want = [ops.attention_kv4(*args) for args, _ in sets]
+    for g in graphs + graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want)) and status() == 0
+
+
 @pytest.mark.parametrize("S, Hq, Hkv, lens, causal", [
     (512, 8, 2, [129, 400, 700], True), (512, 8, 2, [129, 400, 700], False), (128, 8, 2, [5000], True), (1, 32, 8, [3000, 7, 900], True),
 ])
