@@ -115,11 +115,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x for x < 64 on the FMA pipe (x below -126: 2^-126; a NaN stays one). Cody and
+// 2^x for x < 64 on the FMA pipe (x below -126.5: 0, whose exponent field the last
+// line makes of -127; a NaN stays one). Cody and
 // Waite's reduction to f in [-1/2, 1/2], a polynomial of degree 4 there with the
 // smallest largest relative error (2.6e-6, fitted by Lawson's reweighting).
 __device__ __forceinline__ float ex2_fma(float x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-127.f));
   const float whole = x + 12582912.f;  // 1.5 * 2^23: the nearest whole number in its low bits
   const float f = x - (whole - 12582912.f);
   const float y = fmaf(fmaf(fmaf(fmaf(0.009570101f, f, 0.05591786f), f, 0.24024744f), f, 0.6931218f), f, 0.9999993f);
@@ -415,7 +416,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows_kv4_kernel(const __grid_
     const bool fin =
         ok && __all_sync(0xffffffffu, mbd::mbar_wait(ofinal, 0, status, MB_DEV_TIMEOUT_EPI, abort_flag));
     // both groups' sums, under the last reference, which is O's
-    if (m == -INFINITY && l == l) l = 0.f;  // no visible key: what ex2_fma makes of -inf is not 0
     // (in the quadrant's own rows of Q: every S has been made, and with no tile
     // the other quadrants may still be storing theirs)
     float2* ends = reinterpret_cast<float2*>(base + OFF_Q + quad * 4096) + lane;

@@ -347,7 +347,12 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(
     const uint32_t par = pars[half][i * 16 + l];
     if (lo_bf(par) < INFINITY) most = fmaxf(most, fmaxf(fabsf(hi_bf(par)), fabsf(fmaf(lo_bf(par), 15.f, hi_bf(par)))));
   }
-  const int e = fp16_exp(max_of_16(most));
+  // values that are all zero must not raise the rows' references above what other
+  // pages need (any factor is right for them: a low one, far enough from fp32's end
+  // that the terms' sum, which takes 2^60 in return, stays finite)
+  constexpr int ZERO_VALUES = -60;
+  most = max_of_16(most);
+  const int e = half && most == 0.f ? ZERO_VALUES : fp16_exp(most);
   const float f = pow2i(-e);
   if (warp == 0 && l == 0) {
     int2* to_e = o.page_exp + to;

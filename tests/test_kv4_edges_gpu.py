@@ -1,0 +1,62 @@
+"""The 4-bit cache where its forms replace a number by another one: zeros and
+constants among the values, weights rounded to fp16, wide tables, a status that
+outlives its call. Against the plain 64-bit implementations (_kv4ref)."""
+import numpy as np
+import pytest
+import torch
+
+import _kv4ref as R
+from test_kv4_gpu import bf, clean_status, i32, make_cache, make_table, ops, status  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def held(ops, k, v, table, P):
+    """A cache of P pages with the tokens k, v [B, L, H, 128], as numpy."""
+    cache = ops.kv4_cache(P, k.shape[2])
+    ops.kv4_append(bf(k), bf(v), cache, i32(table), i32([0] * len(k)))
+    return cache.cpu().numpy()
+
+
+def attend(ops, q, cache, table, lens, first=None):
+    return ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(lens),
+                             start_pos=None if first is None else i32(first)).double().cpu().numpy()
+
+
+def near(got, ref, slack):
+    err, tol = np.abs(got - ref), slack + 2 ** -8 * (np.abs(ref) + slack)  # and the output's rounding to bf16
+    return float((err - tol).max()) <= 0
+
+
+# ---------------------------------------------------------------------------
+# values of zero, and values that are all alike
+# ---------------------------------------------------------------------------
+def strong_zeros(rng, where, octaves, B, L, Hkv, size, value=0.0):
+    """Keys and values of N(0, 1) and size * N(0, 1); the tokens `where` have all
+    dims of the value alike and scores about `octaves` above the others' mean, for
+    q of mean 1: a key of b in all its dims scores 128 b / sqrt(128) log2(e) = 16.3 b octaves."""
+    k, v = rng.standard_normal((B, L, Hkv, 128)), size * rng.standard_normal((B, L, Hkv, 128))
+    k[:, where], v[:, where] = octaves / 16.3, value
+    return R.bf16_round(k), R.bf16_round(v)
+
+
+PAGE0 = list(range(64))
+SOME = [0, 5, 63, 64, 130, 300, 511]
+MOST = list(range(0, 500))
+
+
+@pytest.mark.parametrize("size", [1.0, 0.1, 1e-3, 1e-6])
+@pytest.mark.parametrize("octaves", [0, 6, 12])
+@pytest.mark.parametrize("where", [PAGE0, SOME, MOST], ids=["page", "some", "most"])
+def test_prompts_over_zero_values(ops, where, octaves, size):
+    """Zeros count in the denominator and nowhere else: they must not take the
+    bits of the values that stand beside them."""
+    rng = np.random.default_rng(len(where) + octaves)
+    B, S, Hq, Hkv, lens = 2, 512, 4, 2, np.array([700, 600])
+    k, v = strong_zeros(rng, where, octaves, B, 700, Hkv, size)
+    table, P = make_table(rng, [700, 700])
+    cache = held(ops, k, v, table, P)
+    q = R.bf16_round(rng.standard_normal((B, S, Hq, 128)) + 1)
+    ref, _ = R.attention(q, cache, table, lens, lens - S)
+    assert near(attend(ops, q, cache, table, lens, lens - S), ref, R.prompt_slack(q, cache, table, lens, lens - S))
+    assert status() == 0
