@@ -267,7 +267,8 @@ int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv, const int* b
  * q, out: bf16 [B][S][Hq][128] with ldq / ldo elements between two positions'
  * rows (multiples of 8), the heads contiguous; out may be q. A row that sees no
  * key becomes zeros, one that sees a token read back as NaN becomes NaN. Good for
- * |q| below 2^111 and for a sequence's value scales within 2^90 of each other;
+ * |q| below 2^111 and for a sequence's value scales within 2^90 of each other
+ * (within 2^-50 .. 2^60 where values of zero stand beside them);
  * values stored with a scale below 2^-90 may count as up to 2^-86 more. Every
  * length is read on the device, so ragged batches balance and the call can be
  * captured. */

@@ -340,9 +340,13 @@ struct State {
       uint32_t k = *reinterpret_cast<const uint32_t*>(pg + K_PARAMS + key * 4);
       uint32_t v = *reinterpret_cast<const uint32_t*>(pg + V_PARAMS + key * 4);
       if (MASKED && key0 + key >= len) k = v = 0;  // what stands past the end may be anything
-      // a value scale of 0 (all dims alike, codes 0) must not enter the logarithm
-      // (scales below 2^-90 count as that: sums of 2^15 / s over 2^22 keys stay finite)
-      const float sv = lo_bf(v), s = sv == 0.f ? 1.f : fminf(fmaxf(sv, 0x1p-90f), 0x1p126f);
+      // A value scale of 0 (all dims alike, codes 0) must not enter the logarithm. Any
+      // other number gives the right sums, but one far above the true scales beside it
+      // would raise the reference and take the fp16 weights' bits: the minimum's own
+      // size, for zeros 2^-60 (their terms are still fp32 numbers beside scales of 2^60).
+      // (Scales below 2^-90 count as that: sums of 2^15 / s over 2^22 keys stay finite.)
+      const float sv = lo_bf(v), flat = fmaxf(fabsf(hi_bf(v)) * 0.125f, 0x1p-60f);
+      const float s = fminf(fmaxf(sv == 0.f ? flat : sv, 0x1p-90f), 0x1p126f);
       const float r = fast_rcp(s);
       // a key or value stored of what was no number or infinite has such a scale: it makes
       // the rows that see it NaN, by its score (a term of 0 * NaN would spread to all rows)

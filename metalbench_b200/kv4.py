@@ -83,8 +83,9 @@ def attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     1/sqrt(128) by default. max_kv_len: no kv_len is larger (longer ones are
     cut; by default the block table's width); give a bound near the longest
     length when the table is much wider. Good for |q| below 2^111 and for a
-    sequence's value scales within a factor of 2^90 of each other; values stored
-    with a scale below 2^-90 may count as up to 2^-86 more."""
+    sequence's value scales within a factor of 2^90 of each other (within 2^-50 ..
+    2^60 where values of zero stand beside them); values stored with a scale
+    below 2^-90 may count as up to 2^-86 more."""
     r = (_ext or _kv4()).attention(q, cache, block_table, kv_len, start_pos, scale, out, max_kv_len)
     if type(r) is int:
         _lib.check("mb_attention_kv4_bf16", r)

@@ -60,3 +60,72 @@ def test_prompts_over_zero_values(ops, where, octaves, size):
     ref, _ = R.attention(q, cache, table, lens, lens - S)
     assert near(attend(ops, q, cache, table, lens, lens - S), ref, R.prompt_slack(q, cache, table, lens, lens - S))
     assert status() == 0
+
+
+@pytest.mark.parametrize("size", [1.0, 0.1, 1e-3, 1e-6, 1e-10])
+@pytest.mark.parametrize("octaves", [0, 6, 12])
+@pytest.mark.parametrize("where", [PAGE0, SOME, MOST], ids=["page", "some", "most"])
+@pytest.mark.parametrize("B, S", [(1, 1), (2, 1), (2, 4)])
+def test_rows_over_zero_values(ops, B, S, where, octaves, size):
+    rng = np.random.default_rng(len(where) + octaves)
+    Hq, Hkv, lens = 8, 2, np.array([700, 600])[:B]
+    k, v = strong_zeros(rng, where, octaves, B, 700, Hkv, size)
+    table, P = make_table(rng, [700] * B)
+    cache = held(ops, k, v, table, P)
+    q = R.bf16_round(rng.standard_normal((B, S, Hq, 128)) + 1)
+    ref, slack = R.attention(q, cache, table, lens, lens - S)
+    assert near(attend(ops, q, cache, table, lens, lens - S), ref, slack)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("value", [2.0 ** -20, -0.375, 1e4])
+@pytest.mark.parametrize("octaves", [0, 8])
+@pytest.mark.parametrize("S, Hq", [(1, 8), (4, 8), (512, 4)])
+def test_constants_among_other_values(ops, S, Hq, octaves, value):
+    """All dims of some values alike (scale 0, codes 0, a minimum of its own)."""
+    rng = np.random.default_rng(octaves)
+    Hkv, lens = 2, np.array([700, 600])
+    k, v = strong_zeros(rng, SOME, octaves, 2, 700, Hkv, 0.5, value)
+    table, P = make_table(rng, [700, 700])
+    cache = held(ops, k, v, table, P)
+    q = R.bf16_round(rng.standard_normal((2, S, Hq, 128)) + 1)
+    ref, slack = R.attention(q, cache, table, lens, lens - S)
+    slack = R.prompt_slack(q, cache, table, lens, lens - S) if S >= 512 else slack
+    assert near(attend(ops, q, cache, table, lens, lens - S), ref, slack)
+
+
+def test_scales_of_zero_beside_scales_of_every_size(ops):
+    """Scales 2^-40 to 2^2 and, among them, scales of 0 with codes 0 and minima
+    of 0, of the neighbours' size and far below it."""
+    rng = np.random.default_rng(13)
+    table, P = make_table(rng, [300])
+    cache = make_cache(rng, P, 1)
+    s = np.exp2(rng.integers(-40, 3, (P, 1, 64)).astype(np.float64))
+    low = -7 * s
+    for p in range(P):
+        flat = rng.permutation(64)[:12]
+        s[p, 0, flat] = 0
+        low[p, 0, flat[4:8]] = 0
+        low[p, 0, flat[8:]] = 2.0 ** -30
+        codes = cache[p, 0, 4096: 8192].reshape(64, 64)
+        codes[flat] = 0
+    cache[..., 8448:] = np.stack([R.bf16_bits(s), R.bf16_bits(low)], -1).reshape(P, 1, 128).view(np.uint8)
+    for S in (1, 3):
+        q = R.bf16_round(rng.standard_normal((1, S, 8, 128)) * 4)
+        ref, slack = R.attention(q, cache, table, [300], None)
+        assert near(attend(ops, q, cache, table, [300]), ref, slack)
+
+
+@pytest.mark.parametrize("S, Hq", [(1, 8), (4, 8), (512, 4)])
+@pytest.mark.parametrize("exp", [-50, 60])
+def test_zeros_beside_very_small_and_very_large_values(ops, S, Hq, exp):
+    rng = np.random.default_rng(exp + 100)
+    lens = np.array([700, 600])
+    for where in (PAGE0, SOME, MOST):
+        k, v = strong_zeros(rng, where, 3, 2, 700, 2, 2.0 ** exp)
+        table, P = make_table(rng, [700, 700])
+        cache = held(ops, k, v, table, P)
+        q = R.bf16_round(rng.standard_normal((2, S, Hq, 128)) + 1)
+        ref, slack = R.attention(q, cache, table, lens, lens - S)
+        slack = R.prompt_slack(q, cache, table, lens, lens - S) if S >= 512 else slack
+        assert near(attend(ops, q, cache, table, lens, lens - S), ref, slack)
