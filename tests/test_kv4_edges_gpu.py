@@ -129,3 +129,27 @@ def test_zeros_beside_very_small_and_very_large_values(ops, S, Hq, exp):
         ref, slack = R.attention(q, cache, table, lens, lens - S)
         slack = R.prompt_slack(q, cache, table, lens, lens - S) if S >= 512 else slack
         assert near(attend(ops, q, cache, table, lens, lens - S), ref, slack)
+
+
+# ---------------------------------------------------------------------------
+# rounded weights
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("B, S, Hq, Hkv, L", [(1, 1, 8, 2, 700), (3, 1, 32, 8, 900), (2, 4, 8, 2, 300), (1, 1, 64, 8, 9000)])
+def test_equal_values_come_back_whatever_their_weights(ops, B, S, Hq, Hkv, L):
+    """Every token has the same value, so that the output is that value for any
+    weights: a weight's own rounding must go the same way in the numerator's
+    two parts (codes and minimum) and in the denominator. What may be off: n/16
+    accumulations of 2^-23 and n/32 of 2^-24 of scale * code + |minimum|, the
+    division and the reciprocal of the scale (2^-20 together), and weights
+    under 2^-22 of the largest, which fp16 holds to 2^-33 of that."""
+    rng = np.random.default_rng(L)
+    x = np.tile(np.arange(16) - 7.0, 8)  # scale 1, minimum -7: exact, many of them 0
+    lens = np.full(B, L)
+    table, P = make_table(rng, lens)
+    k = R.bf16_round(rng.standard_normal((B, L, Hkv, 128)))
+    cache = held(ops, k, np.broadcast_to(x, k.shape).copy(), table, P)
+    q = R.bf16_round(rng.standard_normal((B, S, Hq, 128)))
+    got = attend(ops, q, cache, table, lens)
+    size = x + 14  # scale * code + |minimum|
+    tol = size * (L / 16 * 2 ** -23 + L / 32 * 2 ** -24 + 2 ** -20 + L * 2 ** -33)
+    assert (np.abs(got - x) <= tol + 2 ** -8 * (np.abs(x) + tol)).all(), float(np.abs(got - x).max())
