@@ -52,7 +52,7 @@ using namespace kv4;
 template <int NT> struct Shape;
 template <> struct Shape<1> { static constexpr int NW = 12, ST = 2; };
 template <> struct Shape<2> { static constexpr int NW = 8, ST = 3; };
-constexpr int MAX_B = 512;  // sequences a launch: their page counts are planned in shared memory
+constexpr int MAX_B = 512;  // most sequences a launch: their page counts are planned in shared memory
 constexpr int UNIT_COST = 2;  // pages that starting and ending a unit cost
 
 struct Args {
@@ -1199,15 +1199,17 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
   MB_REQUIRE(max_kv_len > 0 && max_kv_len <= max_pages * PAGE, "attention kv4: max_kv_len must be in [1, max_pages*64]");
   const int pages = (max_kv_len + PAGE - 1) / PAGE;
   const Launch p = plan_launch(B, S, Hq, Hkv, pages);
-  MB_REQUIRE((int64_t)(B < MAX_B ? B : MAX_B) * Hkv * p.rt * ((int64_t)pages + UNIT_COST) < (1ll << 30),
-             "attention kv4: too many pages");
   MB_REQUIRE(workspace && workspace_bytes >= p.bytes && (uintptr_t)workspace % 16 == 0,
              "attention kv4: workspace of %zu bytes required, 16-byte aligned", p.bytes);
+  Expand e;
+  const bool expand = expand_plan(B, S, Hq, Hkv, pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
+                      mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo);
+  // sequences a launch of the other form: its flat list of pages is counted in 32 bits
+  const int64_t fit = ((1ll << 30) - 1) / ((int64_t)Hkv * p.rt * ((int64_t)pages + UNIT_COST));
+  MB_REQUIRE(expand || fit > 0, "attention kv4: too many pages for the rows of one sequence");
   uint32_t* status = mb::device_status_ptr();
   MB_REQUIRE(status, "attention kv4: no status word");
-  Expand e;
-  if (expand_plan(B, S, Hq, Hkv, pages, &e) && scale > 0.f && ldq < (1 << 30) && ldo < (1 << 30) &&
-      mb::attention_prefill_tc_ok(q, (int)ldq, nullptr, nullptr, out, (int)ldo)) {
+  if (expand) {
     MB_REQUIRE(workspace_bytes >= e.bytes, "attention kv4: workspace of %zu bytes required", e.bytes);
     uint8_t* w = static_cast<uint8_t*>(workspace);
     mb::Kv4Rows r;
@@ -1238,7 +1240,8 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
     }
     return MB_OK;
   }
-  for (int b = 0; b < B; b += MAX_B) {
+  const int step = (int)(fit < MAX_B ? fit : MAX_B);
+  for (int b = 0; b < B; b += step) {
     Args a;
     a.q = q + (int64_t)b * S * ldq;
     a.cache = cache;
@@ -1254,7 +1257,7 @@ extern "C" int mb_attention_kv4_bf16(const uint16_t* q, int64_t ldq, const uint8
     a.num_pages = num_pages;
     a.max_pages = max_pages;
     a.max_len = max_kv_len;
-    a.B = B - b < MAX_B ? B - b : MAX_B;
+    a.B = B - b < step ? B - b : step;
     a.S = S;
     a.Hkv = Hkv;
     a.G = Hq / Hkv;

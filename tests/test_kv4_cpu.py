@@ -98,6 +98,14 @@ def test_a_wide_table_does_not_ask_for_the_memory_of_expanded_pages(lib):
     assert 0 < most <= 6 << 30
 
 
+def test_one_sequence_of_too_many_rows_and_pages(lib):
+    """A negative scale takes the form whose row tiles and pages are counted in 32 bits."""
+    a = dict(q=FAKE, ldq=8192, cache=FAKE, num_pages=4, table=FAKE, max_pages=64, kv_len=FAKE, most=4096, start=None, B=3, S=1 << 22,
+             Hq=64, Hkv=8, Dh=128, scale=-0.1, out=FAKE, ldo=8192, ws=FAKE, ws_bytes=1 << 40)
+    rc = lib.mb_attention_kv4_bf16(*a.values(), None)
+    assert rc == -1 and "too many pages" in lib.mb_last_error().decode()
+
+
 def test_plain_quantiser_is_within_half_a_step():
     rng = np.random.default_rng(0)
     x = R.bf16_round(rng.standard_normal((64, 128)) * np.exp(rng.uniform(-20, 20, (64, 1))))

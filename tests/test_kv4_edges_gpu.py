@@ -153,3 +153,34 @@ def test_equal_values_come_back_whatever_their_weights(ops, B, S, Hq, Hkv, L):
     size = x + 14  # scale * code + |minimum|
     tol = size * (L / 16 * 2 ** -23 + L / 32 * 2 ** -24 + 2 ** -20 + L * 2 ** -33)
     assert (np.abs(got - x) <= tol + 2 ** -8 * (np.abs(x) + tol)).all(), float(np.abs(got - x).max())
+
+
+# ---------------------------------------------------------------------------
+# wide tables and bounds
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [128 ** -0.5, -(128 ** -0.5)])
+def test_many_sequences_under_a_wide_table(ops, scale):
+    """512 x 64 rows of 8 heads, 65536 columns: 2^30 pages of row tiles at the
+    table's width, far fewer in use. The expanded form (scale > 0) plans without
+    that list, the other one takes fewer sequences at a time."""
+    rng = np.random.default_rng(5)
+    B, S, Hq, M = 512, 64, 8, 65536
+    lens = np.zeros(B, dtype=np.int64)
+    lens[[0, 300, 510, 511]] = 130, 64, 1, 200
+    small, P = make_table(rng, lens)
+    table = torch.full((B, M), -1, dtype=torch.int32, device="cuda")
+    table[:, : small.shape[1]] = i32(small)
+    cache = make_cache(rng, P, 1)
+    c = torch.from_numpy(cache).cuda()
+    q = torch.randn(B, S, Hq, 128, device="cuda").to(torch.bfloat16)
+    got = ops.attention_kv4(q, c, table, i32(lens), start_pos=i32(lens - S), scale=scale)
+    for b in range(B):
+        if not lens[b]:
+            continue
+        # scale * q = |scale| * (+-q), exactly: the slack's term for a score's error is a multiple of the scale
+        # that it is given, and means its magnitude
+        x = np.sign(scale) * q[b: b + 1].double().cpu().numpy()
+        at = (cache, small[b: b + 1], lens[b: b + 1], lens[b: b + 1] - S, abs(scale))
+        ref, slack = R.attention(x, *at)
+        assert near(got[b: b + 1].double().cpu().numpy(), ref, np.maximum(slack, R.prompt_slack(x, *at)))
+    assert (got[torch.from_numpy(lens == 0).cuda()] == 0).all() and status() == 0
