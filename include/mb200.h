@@ -229,8 +229,9 @@ int mb_attention_prefill_bf16(const uint16_t* q, int ldq, const uint16_t* k_cach
  * Over the 128 dims x of a token and head: minimum = min(x), scale =
  * bf16((max(x) - min(x)) / 15), code = (x - minimum) / scale rounded to the
  * nearest whole number (ties to even), clamped to 0..15, and 0 where scale is 0;
- * a code stands for minimum + scale * code. A token with a NaN or an infinity
- * reads back as NaN (the others of its page do not change).
+ * a code stands for minimum + scale * code. A token with a NaN or an infinity,
+ * or whose max - min rounds to 2^128 or more in fp32 and so has no scale, reads
+ * back as NaN (the others of its page do not change).
  *
  * block_table [B][max_pages], kv_len, start_pos, new_len [B] are int32 in
  * device memory. A position outside the table, or a table entry outside

@@ -6,7 +6,10 @@
 //   m = min x,  s = bf16((max x - m) / 15),  u = clamp(rint((x - m) / s), 0, 15)
 // with u = 0 where s = 0; the stored value is m + s u. m is exact (x is bf16);
 // s is rounded to bf16 (2^-8 relative: at most 6 % of one code step at u = 15)
-// because its 2 bytes a token are read by every later step.
+// because its 2 bytes a token are read by every later step. Where max x - m is no
+// fp32 number (NaN, infinities, a range of 2^128) s is none either, and the token
+// reads as NaN; any other range gives finite values: 15 of half a step of s, 2^116 at
+// most, are less than what fp32 has above the largest bf16 number (2^120 - 2^104).
 #include "kv4.cuh"
 #include "kernels.h"
 

@@ -53,7 +53,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_tabl
     goes to position start_pos[b] + s of sequence b, unless that is kv_len[b] or
     past it: with the lengths that kv_pages_extend keeps there, nothing is stored
     for tokens that it found no pages for. Other slots of the cache stay as they
-    are."""
+    are. A token (and head) with a NaN or an infinity, or whose largest and smallest
+    number are 2^128 or more apart, reads back as NaN."""
     rc = (_ext or _kv4()).append(k, v, cache, block_table, start_pos, new_len, kv_len)
     if rc:
         _lib.check("mb_kv4_append_bf16", rc)

@@ -184,3 +184,30 @@ def test_many_sequences_under_a_wide_table(ops, scale):
         ref, slack = R.attention(x, *at)
         assert near(got[b: b + 1].double().cpu().numpy(), ref, np.maximum(slack, R.prompt_slack(x, *at)))
     assert (got[torch.from_numpy(lens == 0).cuda()] == 0).all() and status() == 0
+
+
+# ---------------------------------------------------------------------------
+# numbers at the end of the range
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("S", [7, 70])
+def test_a_range_that_overflows_reads_back_as_nan(ops, S):
+    """max - min is an fp32 number: from 2^128 on the token has no scale. Just
+    below, its largest code still stands for a finite number."""
+    big = 3.3895313892515355e38  # the largest bf16
+    x = np.zeros((1, S, 1, 128))
+    x[0, :, 0] = np.linspace(-1, 1, 128)
+    x[0, 1, 0, :2] = -big, big
+    x[0, 3, 0] = np.linspace(-big / 2, big / 2, 128)
+    x[0, 5, 0, :2] = -2.0 ** 126, big  # the range rounds to 2^128 and more
+    x = R.bf16_round(x)
+    cache = ops.kv4_cache(2, 1)
+    ops.kv4_append(bf(x), bf(-x), cache, i32([[0, 1]]), i32([0]))
+    for got, y in zip(ops.kv4_gather(cache, i32([[0, 1]]), i32([0]), S, i32([S])), (x, -x)):
+        got = got.cpu().numpy()[0, :, 0]
+        for s in range(S):
+            if s in (1, 5):
+                assert np.isnan(got[s]).all()
+            else:
+                u, sc, m = R.quantise(y[0, s, 0])
+                want = (m + sc * u).astype(np.float32)
+                assert np.isfinite(want).all() and np.array_equal(got[s], want)
