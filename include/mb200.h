@@ -121,7 +121,8 @@ const char* mb_kernel_names(void);
 int mb_run(const char* kernel, const mb_buf* bufs, int nbufs, const mb_scalar* scalars, int nsc,
            const char* config_json, int warmup, int iters, mb_timing* out);
 
-/* Status word that bounded device waits write on timeout; 0 = clean. There is
+/* Status word that bounded device waits write on timeout, and calls on a paged
+ * 4-bit cache when they skip a page index out of range (0x8); 0 = clean. There is
  * one word per device; both calls act on the current device. Reading it
  * synchronises the device. mb_clear_device_status resets it. The value also
  * includes the word mb_sqr_mm_f32_noalloc falls back to on a device that has
@@ -237,7 +238,8 @@ int mb_attention_prefill_bf16(const uint16_t* q, int ldq, const uint16_t* k_cach
  * device memory. A position outside the table, or a table entry outside
  * 0..num_pages-1, is never accessed: it is not stored, is read back as zeros,
  * leaves the attention rows of its sequence unspecified, and is recorded in the
- * device status word (0x8, until mb_clear_device_status). */
+ * device status word (0x8, until mb_clear_device_status; mb_run does not take it
+ * for a fault of its own). */
 
 /* Bytes of one page of all Hkv heads. */
 size_t mb_kv4_page_bytes(int Hkv);

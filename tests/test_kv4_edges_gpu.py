@@ -211,3 +211,17 @@ def test_a_range_that_overflows_reads_back_as_nan(ops, S):
                 u, sc, m = R.quantise(y[0, s, 0])
                 want = (m + sc * u).astype(np.float32)
                 assert np.isfinite(want).all() and np.array_equal(got[s], want)
+
+
+# ---------------------------------------------------------------------------
+# one caller's mistake
+# ---------------------------------------------------------------------------
+def test_a_bad_page_stays_its_callers(ops):
+    """The mark that a table entry out of range leaves is there until it is
+    cleared; other kernels of the device go on."""
+    from metalbench_b200 import harness
+    ops.attention_kv4(torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16, device="cuda"), ops.kv4_cache(1, 1), i32([[7]]), i32([5]))
+    assert status() == 8
+    name = next(n for n in sorted(harness.registry_all()) if "transpose" in n)
+    assert harness.evaluate(name, warmup=1, iters=2, ref_warmup=0, ref_iters=1)["correct"]
+    assert status() == 8
