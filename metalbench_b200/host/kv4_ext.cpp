@@ -304,9 +304,13 @@ Pools pools(PyObject* o, const char* name, const Pages& p) {
     const int64_t size = p.P ? (int64_t)t.nbytes() / p.P : 16;
     if (size == 0 || size % 16 || !aligned(t))
       bad_shape(name, "a pool whose pages are a multiple of 16 bytes and 16-byte aligned", t);
-    for (void* q : r.ptr)
-      if (q == t.data_ptr() && p.P) refuse(PyExc_ValueError, name, "the same pool twice");
-    r.ptr.push_back(t.data_ptr());
+    uint8_t* at = static_cast<uint8_t*>(t.data_ptr());
+    for (size_t k = 0; k < r.ptr.size(); ++k) {
+      uint8_t* q = static_cast<uint8_t*>(r.ptr[k]);
+      if (p.P && at < q + p.P * r.bytes[k] && q < at + t.nbytes())
+        refuse(PyExc_ValueError, name, "the same pool twice, or pools that overlap");
+    }
+    r.ptr.push_back(at);
     r.bytes.push_back(size);
   }
   return r;

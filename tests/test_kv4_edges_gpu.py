@@ -225,3 +225,19 @@ def test_a_bad_page_stays_its_callers(ops):
     name = next(n for n in sorted(harness.registry_all()) if "transpose" in n)
     assert harness.evaluate(name, warmup=1, iters=2, ref_warmup=0, ref_iters=1)["correct"]
     assert status() == 8
+
+
+# ---------------------------------------------------------------------------
+# pools of other types and sizes
+# ---------------------------------------------------------------------------
+def test_pools_that_overlap_are_refused(ops):
+    """A page moved in one would be another page of the other."""
+    both = torch.zeros(5, 64, dtype=torch.uint8, device="cuda")
+    t, n, r = i32([[0, 1]]), i32([70]), i32([1, 1, 0, 0])
+    for pools in ([both[:4], both[1:]], [both[1:], both[:4]]):
+        with pytest.raises(ValueError, match="pool"):
+            ops.kv_pages_fork(pools, t, n, r, i32([0]))
+        with pytest.raises(ValueError, match="pool"):
+            ops.kv_pages_compact(pools, t, n, r)
+    halves = torch.zeros(8, 64, dtype=torch.uint8, device="cuda")
+    assert int(ops.kv_pages_fork([halves[:4], halves[4:]], t, n, r, i32([0]))) == 0
