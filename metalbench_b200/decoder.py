@@ -193,8 +193,11 @@ class DecoderLayer:
         X = x.unsqueeze(0) if squeeze else x
         ops._cuda(X, "DecoderLayer.forward(x)", (torch.bfloat16,))
         B, S, D = X.shape
-        if start_pos.dtype != torch.int32 or not start_pos.is_cuda or start_pos.numel() != B:
-            raise ValueError("start_pos must be an int32 CUDA tensor with one entry per sequence")
+        for nm, t in (("start_pos", start_pos), ("kv_len", kv_len), ("new_len", new_len)):
+            if t is not None and (t.dtype != torch.int32 or t.device != X.device or t.numel() != B
+                                  or not t.is_contiguous()):
+                raise ValueError(f"{nm} must be a contiguous int32 CUDA tensor with one entry per sequence, "
+                                 "on x's device")
         kv4 = isinstance(cache, KV4Layer)
         if kv4:
             own, pool = cache.owner, cache.owner.pools[cache.index]
@@ -202,9 +205,6 @@ class DecoderLayer:
                 raise ValueError("the 4-bit cache has another batch, number of kv heads or device")
             if kv_len is None:
                 kv_len = own.seq_len
-            if new_len is not None and (new_len.dtype != torch.int32 or new_len.device != X.device
-                                        or tuple(new_len.shape) != (B,) or not new_len.is_contiguous()):
-                raise ValueError("new_len must be an int32 tensor with one entry per sequence")
             if max_kv_len is None:
                 max_kv_len = own.max_pages * PAGE  # the lengths are on the device
             ws_bytes = _lib.lib().mb_decoder_layer_workspace_bytes_kv4(self._h, B, S, max_kv_len)

@@ -241,3 +241,24 @@ def test_pools_that_overlap_are_refused(ops):
             ops.kv_pages_compact(pools, t, n, r)
     halves = torch.zeros(8, 64, dtype=torch.uint8, device="cuda")
     assert int(ops.kv_pages_fork([halves[:4], halves[4:]], t, n, r, i32([0]))) == 0
+
+
+# ---------------------------------------------------------------------------
+# the decoder layer's lengths
+# ---------------------------------------------------------------------------
+def test_lengths_that_are_no_int32_of_the_device_are_refused(ops):
+    """Their addresses go to the kernels as they are."""
+    from metalbench_b200.decoder import PagedKV4Cache, PagedKVCache
+    from test_decoder_gpu import _layer, _weights
+    rng = np.random.default_rng(3)
+    layer = _layer(torch, _weights(rng, 512, 4, 2, 512), 512, 4, 2, 512, 10000.0)
+    x = bf(rng.standard_normal((2, 1, 512)))
+    pairs = i32([[0, 9], [1, 9]])
+    for cache in (PagedKV4Cache(2, 64, 2).layer(0), PagedKVCache(2, 64, 2)):
+        for bad in (torch.tensor([1, 1]), torch.tensor([1, 1], dtype=torch.int32), i32([1, 1]).long(), i32([1]), i32([1, 1, 1]), pairs[:, 0]):
+            with pytest.raises(ValueError, match="kv_len"):
+                layer(x, cache, i32([0, 0]), kv_len=bad, max_kv_len=64)
+            with pytest.raises(ValueError, match="start_pos"):
+                layer(x, cache, bad, max_kv_len=64)
+    with pytest.raises(ValueError, match="new_len"):
+        layer(x, PagedKV4Cache(2, 64, 2).layer(0), i32([0, 0]), new_len=pairs[:, 1])
