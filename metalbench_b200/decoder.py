@@ -75,9 +75,12 @@ class PagedKV4Cache:
     A step is ``start = cache.extend(new_len)``, then for every layer either
     ``layer(x, cache.layer(i), start, ...)`` or ``append`` and ``attend``. Nothing is
     read back by the host, so steps can be captured in a CUDA graph;
-    ``cache.status`` tells, when the program next looks, whether the last page
-    operation was served (0), or how many pages were lacking (then it changed
-    nothing, and the tokens that had no room are not stored)."""
+    ``cache.status`` tells, when the program next looks, whether every page
+    operation since ``clear_status`` was served (0), replayed ones too. One that
+    was not changed nothing, and the tokens that had no room are not stored: the
+    status is then the number of pages that were lacking (after several such
+    operations the bits of their numbers together), or -1 for a length, parent or
+    table entry out of range."""
 
     def __init__(self, batch: int, max_len: int, n_kv_heads: int, n_layers: int = 1,
                  num_pages: int | None = None, device=None):
@@ -95,16 +98,23 @@ class PagedKV4Cache:
 
     def extend(self, new_len: torch.Tensor) -> torch.Tensor:
         """Room for new_len[b] more tokens a sequence; the positions of the first of them."""
-        start, self.status = ops.kv_pages_extend(self.block_table, self.seq_len, self.page_refs, new_len)
+        start, status = ops.kv_pages_extend(self.block_table, self.seq_len, self.page_refs, new_len)
+        self.status.bitwise_or_(status)
         return start
 
     def fork(self, parent: torch.Tensor) -> None:
         """Row b becomes a fork of row parent[b] (its own number: stays; -1: is freed)."""
-        self.status = ops.kv_pages_fork(self.pools, self.block_table, self.seq_len, self.page_refs, parent)
+        self.status.bitwise_or_(ops.kv_pages_fork(self.pools, self.block_table, self.seq_len, self.page_refs,
+                                                  parent))
 
     def compact(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Move the pages in use to the front of every pool: (new numbers, pages in use)."""
-        return ops.kv_pages_compact(self.pools, self.block_table, self.seq_len, self.page_refs)
+        remap, live = ops.kv_pages_compact(self.pools, self.block_table, self.seq_len, self.page_refs)
+        self.status.bitwise_or_(live.clamp(max=0))
+        return remap, live
+
+    def clear_status(self) -> None:
+        self.status.zero_()
 
     def append(self, i: int, k: torch.Tensor, v: torch.Tensor, start_pos: torch.Tensor,
                new_len: torch.Tensor | None = None) -> None:

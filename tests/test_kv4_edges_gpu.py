@@ -262,3 +262,36 @@ def test_lengths_that_are_no_int32_of_the_device_are_refused(ops):
                 layer(x, cache, bad, max_kv_len=64)
     with pytest.raises(ValueError, match="new_len"):
         layer(x, PagedKV4Cache(2, 64, 2).layer(0), i32([0, 0]), new_len=pairs[:, 1])
+
+
+# ---------------------------------------------------------------------------
+# the cache's status
+# ---------------------------------------------------------------------------
+def test_the_status_keeps_what_a_replayed_step_lacked(ops):
+    """Two pages, 64 tokens a step: the third replay finds none, whatever ran between."""
+    from metalbench_b200.decoder import PagedKV4Cache
+    cache = PagedKV4Cache(1, 256, 1, num_pages=2)
+    full, none = i32([64]), i32([0])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        cache.extend(none)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.extend(full)
+        cache.fork(none)  # a second operation of the step, served
+    for length, lacking in ((64, 0), (128, 0), (128, 1), (128, 1)):
+        g.replay()
+        cache.extend(none)
+        cache.compact()
+        assert cache.seq_len.tolist() == [length] and int(cache.status) == lacking
+    cache.clear_status()
+    cache.extend(none)
+    assert int(cache.status) == 0
+    cache.block_table[0, 1] = 9
+    cache.compact()
+    cache.extend(none)
+    assert int(cache.status) == -1
+    g.replay()
+    assert int(cache.status) == -1
