@@ -84,8 +84,13 @@ class DecoderStack:
         if self.kv4 is not None:
             dev = self.kv4.block_table.device
             g = torch.Generator(device=dev).manual_seed(seed + 7919 * self.tp_rank)
-            start = self.kv4.extend(torch.full((self.batch,), length, dtype=torch.int32, device=dev) -
-                                    self.kv4.seq_len)
+            own = self.kv4
+            new = torch.full((self.batch,), length, dtype=torch.int32, device=dev) - own.seq_len
+            start, status = ops.kv_pages_extend(own.block_table, own.seq_len, own.page_refs, new)
+            lack = int(status)  # (set-up code: it may wait)
+            if lack:
+                raise ValueError(f"fill_cache_random: the 4-bit cache lacks {lack} page(s)" if lack > 0 else
+                                 f"fill_cache_random: a sequence is longer than {length}, or that is past max_len")
             zero = torch.zeros_like(start)
             Hkv = self.kv4.pools[0].shape[1]
             for i in range(self.n_layers):

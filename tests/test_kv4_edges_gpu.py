@@ -295,3 +295,20 @@ def test_the_status_keeps_what_a_replayed_step_lacked(ops):
     assert int(cache.status) == -1
     g.replay()
     assert int(cache.status) == -1
+
+
+def test_filling_a_cache_that_is_too_small_is_an_error(ops):
+    from metalbench_b200.decoder import DecoderConfig
+    from metalbench_b200.stack import DecoderStack
+    from test_decoder_gpu import _weights
+    rng = np.random.default_rng(3)
+    W = [[bf(w) for w in _weights(rng, 512, 4, 2, 512)]]
+    st = DecoderStack(DecoderConfig(512, 4, 2, 512), 1, 3, 256, weights=W, kv_bits=4, num_pages=5)
+    with pytest.raises(ValueError, match="lacks 1"):
+        st.fill_cache_random(100)
+    assert st.kv4.seq_len.tolist() == [0, 0, 0]
+    st.fill_cache_random(64)
+    assert st.kv4.seq_len.tolist() == [64] * 3
+    with pytest.raises(ValueError, match="longer"):
+        st.fill_cache_random(50)
+    st.close()
