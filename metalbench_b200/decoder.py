@@ -43,7 +43,7 @@ class PagedKVCache:
 
     def __init__(self, batch: int, max_len: int, n_kv_heads: int, head_dim: int = 128,
                  device=None, block_table: torch.Tensor | None = None):
-        device = device or torch.device("cuda", torch.cuda.current_device())
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         self.batch = batch
         self.max_pages = (max_len + PAGE - 1) // PAGE
         n_pages = batch * self.max_pages
@@ -84,7 +84,7 @@ class PagedKV4Cache:
 
     def __init__(self, batch: int, max_len: int, n_kv_heads: int, n_layers: int = 1,
                  num_pages: int | None = None, device=None):
-        device = device or torch.device("cuda", torch.cuda.current_device())
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         if batch < 1 or max_len < 1 or n_layers < 1:
             raise ValueError("PagedKV4Cache: batch, max_len and n_layers must be at least 1")
         self.batch, self.n_layers = batch, n_layers

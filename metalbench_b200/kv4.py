@@ -39,7 +39,7 @@ def kv4_cache(num_pages: int, n_kv_heads: int, device=None) -> torch.Tensor:
     """An empty 4-bit cache: uint8 [num_pages, n_kv_heads, 8704] (head dim 128)."""
     if num_pages < 1 or n_kv_heads < 1:
         raise ValueError("kv4_cache: needs at least one page and one head")
-    device = device or torch.device("cuda", torch.cuda.current_device())
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     return torch.zeros((num_pages, n_kv_heads, PAGE_HEAD_BYTES), dtype=torch.uint8, device=device)
 
 

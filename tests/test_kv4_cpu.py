@@ -35,6 +35,22 @@ def test_host_tensors_are_refused():
         ops.kv_pages_compact([], i32(1, 1), i32(1), i32(2))
 
 
+def test_device_zero_is_a_device(monkeypatch):
+    """And not the current one."""
+    ops, asked = _ops(), []
+    from metalbench_b200.decoder import PagedKV4Cache
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for name in ("zeros", "full"):
+        real = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, real=real, device=None, **k: asked.append(torch.device(device)) or real(*a, **k))
+    ops.kv4_cache(1, 1, 0)
+    PagedKV4Cache(1, 64, 1, device=0)
+    assert asked and set(asked) == {torch.device("cuda", 0)}
+    asked.clear()
+    ops.kv4_cache(1, 1)
+    assert asked == [torch.device("cuda", 3)]
+
+
 @pytest.fixture(scope="module")
 def lib():
     _ops()
