@@ -539,7 +539,7 @@ int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
                          const uint16_t* v_cache, const int* block_table, int max_pages,
                          const int* start_pos, const int* kv_len, int B, int S, int Hq, int Hkv,
                          int causal, uint16_t* out, int ldo, cudaStream_t stream, int splits,
-                         int max_kv_len, float* part_o, float* part_ml, float scale) {
+                         int max_kv_len, float* part_o, float* part_ml) {
   MB_REQUIRE(splits == 1 || (!causal && part_o && part_ml && max_kv_len > 0),
              "attention: split-KV needs a non-causal call, max_kv_len and partial buffers");
   AttnTcParams p;
@@ -562,7 +562,7 @@ int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
   p.G = Hq / Hkv;
   p.causal = causal;
   p.n_qt = (S + TQ - 1) / TQ;
-  p.scale_log2 = 1.4426950408889634f * scale;
+  p.scale_log2 = 1.4426950408889634f / sqrtf((float)DHT);
   p.out = out;
   p.ldo = ldo;
   p.splits = splits;

@@ -99,8 +99,7 @@ int attention_prefill_tc(const uint16_t* q, int ldq, const uint16_t* k_cache,
                          const uint16_t* v_cache, const int* block_table, int max_pages,
                          const int* start_pos, const int* kv_len, int B, int S, int Hq, int Hkv,
                          int causal, uint16_t* out, int ldo, cudaStream_t stream, int splits = 1,
-                         int max_kv_len = 0, float* part_o = nullptr, float* part_ml = nullptr,
-                         float scale = 0.08838834764831845f /* 1 / sqrt(128); > 0 */);
+                         int max_kv_len = 0, float* part_o = nullptr, float* part_ml = nullptr);
 int attention_split_plan(int64_t B, int64_t S, int64_t Hq, int64_t kv_len);
 // kv4.cu: the pages of B sequences of at most max_len tokens of a 4-bit cache in
 // fp16: k 2^-x and v 2^-y [B][Hkv][pages][64][128] with a page's (x, y) in
