@@ -186,6 +186,18 @@ def test_many_sequences_under_a_wide_table(ops, scale):
     assert (got[torch.from_numpy(lens == 0).cuda()] == 0).all() and status() == 0
 
 
+@pytest.mark.parametrize("S", [1, 3, 80])
+@pytest.mark.parametrize("most", [None, 130, 1000])
+def test_every_bound_gives_the_defined_rows(ops, S, most):
+    rng = np.random.default_rng(18)
+    table = np.arange(300, dtype=np.int32).reshape(2, 150)
+    cache = make_cache(rng, 300, 2)
+    q, n = R.bf16_round(rng.standard_normal((2, S, 8, 128))), [130, 100]
+    got = ops.attention_kv4(bf(q), torch.from_numpy(cache).cuda(), i32(table), i32(n), max_kv_len=most).double().cpu().numpy()
+    ref, slack = R.attention(q, cache, table, n, None)
+    assert near(got, ref, np.maximum(slack, R.prompt_slack(q, cache, table, n, None)))
+
+
 # ---------------------------------------------------------------------------
 # numbers at the end of the range
 # ---------------------------------------------------------------------------
@@ -230,6 +242,33 @@ def test_a_bad_page_stays_its_callers(ops):
 # ---------------------------------------------------------------------------
 # pools of other types and sizes
 # ---------------------------------------------------------------------------
+def test_pages_of_the_bf16_cache_and_of_real_size(ops):
+    """Forks and a compaction of bf16 key and value pages [pages, heads, 64, 128],
+    of 68 KiB 4-bit pages (five pieces of the copy) and of 8.5 KiB ones together."""
+    rng = np.random.default_rng(31)
+    B, M, P = 5, 6, 30
+    ref = R.Pages(np.full((B, M), -1, np.int32), np.zeros(B, np.int32), np.zeros(P, np.int32))
+    pools = [torch.randn(P, 2, 64, 128, device="cuda").to(torch.bfloat16), torch.randn(P, 3, 64, 128, device="cuda").to(torch.bfloat16),
+             torch.randint(0, 256, (P, 8, R.BLOB), dtype=torch.uint8, device="cuda"),
+             torch.randint(0, 256, (P, 1, R.BLOB), dtype=torch.uint8, device="cuda")]
+    data = [p.view(torch.uint8).cpu().numpy().copy() for p in pools]
+    table, lens, refs = i32(ref.table), i32(ref.lens), i32(ref.refs)
+
+    def same():
+        for a, b in ((table, ref.table), (lens, ref.lens), (refs, ref.refs), *zip((p.view(torch.uint8) for p in pools), data)):
+            assert np.array_equal(a.cpu().numpy(), b)
+
+    new = [300, 130, 64, 7, 0]
+    assert int(ops.kv_pages_extend(table, lens, refs, i32(new))[1]) == ref.extend(new) == 0
+    for parent in ([0, 0, 1, 3, 0], [1, 1, -1, 0, 4], [-1, 1, 1, 3, 3], [0, -1, 2, 3, 3]):
+        assert int(ops.kv_pages_fork(pools, table, lens, refs, i32(parent))) == ref.fork(parent, data) == 0
+        same()
+        live, remap = ref.compact(data)
+        got, n = ops.kv_pages_compact(pools, table, lens, refs)
+        assert int(n) == live and np.array_equal(got.cpu().numpy(), remap)
+        same()
+
+
 def test_pools_that_overlap_are_refused(ops):
     """A page moved in one would be another page of the other."""
     both = torch.zeros(5, 64, dtype=torch.uint8, device="cuda")
