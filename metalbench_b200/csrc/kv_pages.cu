@@ -499,17 +499,26 @@ int check_pools(const char* what, void* const* pools, const int64_t* bytes, int 
 
 namespace {
 // One CTA does the bookkeeping of a small table and pool sooner: a block's
-// barrier is cheaper than a cluster's. Measured in us, 1 / 8 CTAs, at pages,
-// rows x columns: extend 2.4 / 3.8 (256, 8 x 32), 3.9 / 4.1 (8192, 128 x 64), 5.7 /
-// 4.6 (32768, 64 x 512); fork 3.8 / 5.2, 8.7 / 7.1, 17.1 / 16.3, and 22.5 / 20.5
-// with its copies (3300, 96 x 33, 64 rows forked); compact 3.1 / 4.9, 12.2 / 7.0,
-// 36 / 15, and 6.3 / 6.9 (4096, 32 x 128), 7.3 / 6.5 (4096, 64 x 64). A row costs
-// about as much as 64 entries.
+// barrier is cheaper than a cluster's. Measured in us, 1 / 8 CTAs, in graphs:
+//   pages, rows x columns    extend      fork (a quarter of the rows)   compact
+//     256,   8 x 32        2.5 / 3.7        3.7 / 5.3        3.2 / 4.7
+//    2048,  64 x 32        3.1 / 3.9        5.1 / 5.9        5.3 / 5.7
+//    2048,  96 x 33        3.4 / 3.8        6.4 / 6.0        6.3 / 5.8
+//    4096,  32 x 128       2.8 / 3.9        5.6 / 7.4        6.3 / 7.0
+//    4096,  64 x 64        3.1 / 4.0        5.7 / 6.6        7.3 / 6.5
+//    4096, 128 x 32        3.9 / 4.0        6.9 / 6.0        8.1 / 5.8
+//    8192,  16 x 512       3.1 / 3.9       11.8 / 14.1      10.3 / 11.7
+//    8192,  64 x 128       3.4 / 4.2        7.4 / 8.2       10.5 / 7.6
+//    8192, 128 x 64        4.2 / 4.2        8.9 / 7.3       12.3 / 7.0
+//   16384,  64 x 128       4.2 / 4.0        9.0 / 9.0       13.9 / 8.2
+//   32768,  64 x 512       5.7 / 4.4       17.5 / 16.2      36.3 / 14.5
+// A fork's time goes by its rows (32 warps take one each); a row of a compaction
+// costs about as much as 64 entries.
 template <typename F>
-int launch_book(const Meta& m, int most_pages, int64_t most_work, F launch) {
-  const bool small = m.num_pages <= most_pages && (int64_t)m.B * (m.max_pages + 64) <= most_work;
+int launch_book(bool small, F launch) {
   return small ? launch(std::integral_constant<int, 1>()) : launch(std::integral_constant<int, 8>());
 }
+int64_t book_work(const Meta& m) { return (int64_t)m.B * (m.max_pages + 64); }
 }  // namespace
 
 extern "C" size_t mb_kv_pages_workspace_bytes(int B, int max_pages, int num_pages) {
@@ -526,7 +535,7 @@ extern "C" int mb_kv_pages_extend(int* block_table, int* seq_len, int* page_refs
                      status, false, workspace, workspace_bytes);
   if (rc) return rc;
   MB_REQUIRE(B == 0 || (new_len && start_pos), "kv_pages_extend: null pointer");
-  return launch_book(m, 8192, 16384, [&](auto c) {
+  return launch_book(num_pages <= 8192 && book_work(m) <= 16384, [&](auto c) {
     MB_CUDA(mb::launch_pdl(kv_extend_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, static_cast<cudaStream_t>(stream), m,
                            new_len, start_pos));
     return MB_OK;
@@ -544,7 +553,7 @@ extern "C" int mb_kv_pages_fork(void* const* pools, const int64_t* page_bytes, i
   if (rc) return rc;
   MB_REQUIRE(B == 0 || parent, "kv_pages_fork: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = launch_book(m, 4096, 6144, [&](auto c) {
+  rc = launch_book(num_pages <= 8192 && B <= 64, [&](auto c) {
     MB_CUDA(mb::launch_pdl(kv_fork_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, s, m, parent));
     return MB_OK;
   });
@@ -563,7 +572,7 @@ extern "C" int mb_kv_pages_compact(void* const* pools, const int64_t* page_bytes
   if (rc) return rc;
   MB_REQUIRE(num_pages == 0 || remap, "kv_pages_compact: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = launch_book(m, 4096, 6144, [&](auto c) {
+  rc = launch_book(num_pages <= 4096 && book_work(m) <= 6144, [&](auto c) {
     MB_CUDA(mb::launch_pdl(kv_compact_kernel<c()>, dim3(c()), dim3(THREADS<c()>), 0, s, m, remap));
     return MB_OK;
   });
