@@ -455,11 +455,10 @@ struct State {
       }
     }
 
-    // ---- weights and O^T += V^T P^T, 16 keys at a time ----
-    const uint32_t pg_s = mbd::smem_u32(pg);
+    // ---- weights, 16 keys at a time ----
+    uint32_t pf[NT][4][2];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      uint32_t pf[NT][2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = mt * 16 + gid + 8 * r;
@@ -474,14 +473,31 @@ struct State {
             l[t][c] = fmaf(p[c], rv, l[t][c]);
             om[t][c] = fmaf(p[c], mv, om[t][c]);
           }
-          pf[t][r] = transpose8x8(pack_h2(p[0], p[1]));
+          pf[t][mt][r] = transpose8x8(pack_h2(p[0], p[1]));
         }
       }
-      const int key = mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-      const uint32_t rowp = pg_s + V_CODES + key * ROW;
-      const int sw = (key >> 1) & 3;
+    }
+
+    // ---- O^T += V^T P^T ----
+    // A page's products start from 0 and are added to the running sum with rounding:
+    // the matrix unit cuts off what lies below its accumulator's last bits, and for one
+    // that holds a long share's sum of codes, all of one sign, that is a bias which
+    // grows with the share (30 x 131075 keys, 16 heads of 1: error of the result
+    // 0.0028, here 0.0018, of 0.0016 that the output's own rounding makes; 64 x 8193
+    // 118.7 -> 121.1 us).
+    const uint32_t pg_s = mbd::smem_u32(pg);
 #pragma unroll
-      for (int p = 0; p < 4; p += 2) {
+    for (int p = 0; p < 4; p += 2) {
+      float acc[NT][2][2][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i >> 3][(i >> 2) & 1][i & 3] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const int key = mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+        const uint32_t rowp = pg_s + V_CODES + key * ROW;
+        const int sw = (key >> 1) & 3;
         uint32_t v[4];  // octets 0, 1 of piece p, then of piece p + 1
         ldsm_x4_t(v, rowp + (((p + (lane >> 4)) ^ sw) << 4));
 #pragma unroll
@@ -491,11 +507,15 @@ struct State {
           spread(v[2 * j + 1], e1);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_f16_16816(o[t][p + j][0], e0[0], e0[1], e1[0], e1[1], pf[t][0], pf[t][1]);
-            mma_f16_16816(o[t][p + j][1], e0[2], e0[3], e1[2], e1[3], pf[t][0], pf[t][1]);
+            mma_f16_16816(acc[t][j][0], e0[0], e0[1], e1[0], e1[1], pf[t][mt][0], pf[t][mt][1]);
+            mma_f16_16816(acc[t][j][1], e0[2], e0[3], e1[2], e1[3], pf[t][mt][0], pf[t][mt][1]);
           }
         }
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][p + (i >> 3)][(i >> 2) & 1][i & 3] += acc[t][i >> 3][(i >> 2) & 1][i & 3];
     }
   }
 };

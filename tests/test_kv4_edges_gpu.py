@@ -155,6 +155,26 @@ def test_equal_values_come_back_whatever_their_weights(ops, B, S, Hq, Hkv, L):
     assert (np.abs(got - x) <= tol + 2 ** -8 * (np.abs(x) + tol)).all(), float(np.abs(got - x).max())
 
 
+def test_a_long_share_has_no_bias(ops):
+    """About 100 pages a warp of equal values, the minimum -7 and codes of 7: what the
+    matrix unit cuts off of 16 products and its accumulator (less than 2^-24 of it
+    each) may bias a page's four sums, 4 * 17 * 2^-24 of the codes' part in all, but
+    not add up over the pages; sums with rounding have no mean error. (Sequences name
+    the same few pages over and over.)"""
+    rng = np.random.default_rng(8)
+    B, Hq, P, M = 64, 8, 50, 2800
+    x = np.tile(np.arange(16) - 7.0, 8)
+    k = R.bf16_round(rng.standard_normal((1, P * 64, 1, 128)))
+    cache = held(ops, k, np.broadcast_to(x, k.shape).copy(), np.arange(P, dtype=np.int32)[None], P)
+    q = R.bf16_round(rng.standard_normal((B, 1, Hq, 128)))
+    for n in (8, 3):  # query rows a sequence: one column tile, two
+        rows = q if n == 8 else np.repeat(q, 3, 1)
+        got = attend(ops, rows, cache, rng.integers(0, P, (B, M)).astype(np.int32), np.full(B, M * 64))
+        bias = got[..., x == 0].mean() / 7
+        print("bias", bias)
+        assert abs(bias) <= 4 * 17 * 2 ** -24, bias
+
+
 # ---------------------------------------------------------------------------
 # wide tables and bounds
 # ---------------------------------------------------------------------------
