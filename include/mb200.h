@@ -272,7 +272,10 @@ int mb_kv4_gather_f32(const uint8_t* cache, int num_pages, int Hkv, const int* b
  * key becomes zeros, one that sees a token read back as NaN becomes NaN. Good for
  * |q| below 2^111 and for a sequence's value scales within 2^90 of each other
  * (within 2^-50 .. 2^60 where values of zero stand beside them);
- * values stored with a scale below 2^-90 may count as up to 2^-86 more. Every
+ * values stored with a scale below 2^-90 may count as up to 2^-86 more.
+ * Sums are fp32. Up to about 64 rows a sequence the codes are multiplied as they
+ * are, with q and the softmax weights in 11 bits (fp16, powers of two taken out);
+ * for more, where that is sooner, keys and values are rounded to 11 bits too. Every
  * length is read on the device, so ragged batches balance and the call can be
  * captured. */
 size_t mb_attention_kv4_workspace_bytes(int B, int S, int Hq, int Hkv, int max_kv_len);

@@ -47,8 +47,9 @@ namespace {
 using namespace kv4;
 
 // Warps of a CTA and pages in a warp's ring, for NT column tiles of 8 rows: as
-// many warps as the registers of an SM hold (168 and 255 a thread), and as many
-// pages in flight as its shared memory does.
+// many warps as the registers of an SM hold (168 and 255 a thread; two column tiles
+// use all 255, of which the compiler spills 24 bytes), and as many pages in flight
+// as its shared memory does.
 template <int NT> struct Shape;
 template <> struct Shape<1> { static constexpr int NW = 12, ST = 2; };
 template <> struct Shape<2> { static constexpr int NW = 8, ST = 3; };
@@ -110,7 +111,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // A weight cut to fp16's 11 bits before it goes into any sum: the terms of codes and
 // minimum cancel in the output, and with the codes' weight alone rounded its error
 // counts as often as the code is larger than the value (64 x 8193: error of the result
-// 0.00179, here 0.00172, of 0.00166 that the output's own rounding makes; no time).
+// 0.00179 then, 0.00172 so, of 0.00166 that the output's own rounding makes; no time).
 // Cutting takes one operation, rounding two. Half a step, the mean of what is cut off,
 // is a factor of every weight alike and drops out of the quotient; from there an error
 // is at most half a step.
@@ -796,7 +797,7 @@ __global__ void __launch_bounds__(Shape<NT>::NW * 32) attn_kv4_kernel(const Args
 // One sequence (B = 1): every length is the same, so a cluster of CTAs takes a
 // unit, its pages split evenly over the warps, and joins it over distributed
 // shared memory: nothing to plan, no partials in memory and no second kernel.
-// (8 kv heads: 517 keys 8.7 -> 7.5 us, 16000 keys 16.6 -> 11.3 us.)
+// (8 kv heads: 517 keys 9.2 -> 6.6 us, 16000 keys 16.0 -> 12.5 us.)
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -1090,12 +1091,18 @@ int resident_clusters(int size) {
   return known[dev][slot] - 1;
 }
 
-// Cluster size for one sequence, 0: the kernel for many. Expected times in us
-// (measured with 1, 2 and 8 kv heads and 60 to 64000 keys): 5.3 and 0.7 for
-// every doubling of the cluster up to four, 0.2 a page and warp rounds of
-// pages of its unit, against 13 and 0.18 a page on every SM. (8 heads: 517 keys
-// 7.5 and 8.7, 4000 keys 8.0 and 12.1, 16000 keys 12.2 and 16.6, 64000 keys 30
-// and 26.)
+// Cluster size for one sequence, 0: the kernel for many. Expected times in us:
+// 5.3, 0.3 more for a cluster of two and 0.6 for a larger one, and 0.2 for every
+// page of a CTA's part of its unit; against 13, and 0.18 for every page of an SM's
+// part of all units. Measured in graphs, the kernel for many / clusters of 1, 4, 8, 16:
+//   8 kv heads,   517 keys    9.2 /   6.6   7.0   7.4  15.4
+//                4000        10.4 /  17.5   9.0   7.4  15.4
+//               16000        16.0 /  49.9  17.7  12.5  19.3
+//               64000        24.2 / 182.0  50.9  29.9  37.5
+//              131075        36.3 / 366.2  97.8  54.5  62.1
+//   1 kv head,  16000        13.3 /  49.0  16.8  11.0   9.1
+//               64000        14.8 / 180.7  50.1  28.3  18.4
+// (Seven clusters of 16 run at a time: eight units take two rounds.)
 template <int NT>
 int one_cluster(int units, int pages) {
   const double flat = 13 + 0.18 * (double)units * pages / mb::num_sms();

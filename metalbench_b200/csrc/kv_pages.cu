@@ -357,9 +357,10 @@ __global__ void __cluster_dims__(CTAS) __launch_bounds__(THREADS<CTAS>)
 // writes free pages, a compaction moves pages above `live` below it). A CTA is
 // one warp, whose first lane moves pieces of up to 16 KB through a ring in
 // shared memory with bulk copies in both directions: no registers and no
-// instructions a byte, and pieces on their way in while others go out. (1843
-// pages of 4 pools of 68 KB, 1.0 GB read and written: 193 us with 16-byte loads
-// and stores by 256 threads and 8 CTAs an SM, 177 us here, 6.4 TB/s.)
+// instructions a byte, and pieces on their way in while others go out. (2036
+// pages of 4 pools of 68 KiB, 1.13 GB read and written: 193 us with 16-byte loads
+// and stores by 256 threads and 8 CTAs an SM, 177 us here, 6.4 TB/s. Smaller pages
+// cost as much a piece and have not been measured.)
 constexpr int PIECE = 16384;
 constexpr int RING = 6, LAG = 2;  // pieces; a piece's place is filled again LAG pieces after it went out
 constexpr int COPY_SMEM = RING * PIECE + RING * 8;

@@ -86,7 +86,9 @@ def attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     length when the table is much wider. Good for |q| below 2^111 and for a
     sequence's value scales within a factor of 2^90 of each other (within 2^-50 ..
     2^60 where values of zero stand beside them); values stored with a scale
-    below 2^-90 may count as up to 2^-86 more."""
+    below 2^-90 may count as up to 2^-86 more. Sums are fp32; q and the softmax
+    weights have 11 bits, and where many rows (64 or more a sequence) take the
+    tcgen05 form the keys and values too."""
     r = (_ext or _kv4()).attention(q, cache, block_table, kv_len, start_pos, scale, out, max_kv_len)
     if type(r) is int:
         _lib.check("mb_attention_kv4_bf16", r)
